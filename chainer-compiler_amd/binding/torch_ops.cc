@@ -86,6 +86,7 @@ struct Operand {
         describe(t, &desc);
         ptr = &desc;
     }
+    Operand(const Operand&) = delete;
 };
 
 double number(PyObject* o) {
@@ -415,6 +416,175 @@ PyObject* plan_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- float layers of a language model ----
+
+// Their operands lie on the device whose stream the call goes to.
+const at::Tensor& on_device(PyObject* o, const char* name) {
+    const at::Tensor& t = tensor(o);
+    if (!t.is_cuda() || t.get_device() != c10::hip::current_device()) {
+        PyErr_Format(PyExc_ValueError, "%s is not a tensor on the current device", name);
+        throw PythonError();
+    }
+    return t;
+}
+
+PyObject* optional_on_device(PyObject* o, const char* name) {
+    if (o != Py_None) on_device(o, name);
+    return o;
+}
+
+// A given result, or a new one.
+at::Tensor result(PyObject* out, at::IntArrayRef shape, const at::TensorOptions& options) {
+    return out == Py_None ? at::empty(shape, options) : on_device(out, "out");
+}
+
+// New results, None in the place of one that was not asked for.
+PyObject* tuple_of(std::initializer_list<at::Tensor> results) {
+    PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(results.size()));
+    if (!t) throw PythonError();
+    Py_ssize_t i = 0;
+    for (const at::Tensor& r : results) {
+        PyObject* o = r.defined() ? THPVariable_Wrap(r) : Py_None;
+        if (!r.defined()) Py_INCREF(o);
+        if (!o) {
+            Py_DECREF(t);
+            throw PythonError();
+        }
+        PyTuple_SET_ITEM(t, i++, o);
+    }
+    return t;
+}
+
+// linear_plan(w, w_scale or None, b or None) -> address of the plan
+PyObject* linear_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 3);
+        Operand w(on_device(a[0], "w")), scale(optional_on_device(a[1], "w_scale")), b(optional_on_device(a[2], "b"));
+        chx_hip_linear_plan* plan = nullptr;
+        void* s = current_stream();
+        checked([&] { return chx_hip_linear_plan_create(w.ptr, scale.ptr, b.ptr, s, &plan); });
+        return PyLong_FromLongLong(static_cast<long long>(reinterpret_cast<intptr_t>(plan)));
+    });
+}
+
+// linear_run(plan, columns of the result, x, activation, r or None, dtype or None, out or None)
+PyObject* linear_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 7);
+        const chx_hip_linear_plan* plan = reinterpret_cast<const chx_hip_linear_plan*>(integer(a[0]));
+        const at::Tensor& x = on_device(a[2], "x");
+        const int32_t activation = static_cast<int32_t>(integer(a[3]));
+        if (x.dim() < 1) fail(PyExc_ValueError, "x needs an axis");
+        c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = integer(a[1]);
+        const at::Tensor y = result(a[6], shape, a[5] == Py_None ? x.options() : x.options().dtype(scalar_type(a[5])));
+        Operand xd(x), rd(optional_on_device(a[4], "r")), yd(y);
+        void* s = current_stream();
+        checked([&] { return chx_hip_linear_plan_run(plan, xd.ptr, activation, rd.ptr, yd.ptr, s); });
+        return wrapped(a[6], y);
+    });
+}
+
+// linear_run_experts(plan, columns of the result, x, order, offsets, activation, dtype or None, out or None)
+PyObject* linear_run_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 8);
+        const chx_hip_linear_plan* plan = reinterpret_cast<const chx_hip_linear_plan*>(integer(a[0]));
+        const at::Tensor &x = on_device(a[2], "x"), &order = on_device(a[3], "order"), &offsets = on_device(a[4], "offsets");
+        const int32_t activation = static_cast<int32_t>(integer(a[5]));
+        const at::Tensor y = result(a[7], {order.numel(), integer(a[1])}, a[6] == Py_None ? x.options() : x.options().dtype(scalar_type(a[6])));
+        Operand xd(x), od(order), fd(offsets), yd(y);
+        void* s = current_stream();
+        checked([&] { return chx_hip_linear_plan_run_experts(plan, xd.ptr, od.ptr, fd.ptr, activation, yd.ptr, s); });
+        return wrapped(a[7], y);
+    });
+}
+
+// Scratch memory of a call, from torch's allocator: it stays valid in the order of the stream, and inside a recording too.
+at::Tensor scratch(size_t bytes, const at::Tensor& like) {
+    return bytes ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// expert_routing(logits, k, bias or None, sigmoid, groups, top_groups, group_best, normalize, scale) -> (experts, weights, order, offsets)
+PyObject* expert_routing(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 9);
+        const at::Tensor& logits = on_device(a[0], "logits");
+        if (logits.dim() != 2) fail(PyExc_ValueError, "logits must be a matrix");
+        const int64_t T = logits.size(0), E = logits.size(1), k = integer(a[1]);
+        if (k < 1) fail(PyExc_ValueError, "at least one expert is chosen");
+        Operand ld(logits), bd(optional_on_device(a[2], "bias"));
+        const int32_t sigmoid = static_cast<int32_t>(integer(a[3])), groups = static_cast<int32_t>(integer(a[4])), top_groups = static_cast<int32_t>(integer(a[5]));
+        const int32_t group_best = static_cast<int32_t>(integer(a[6])), normalize = static_cast<int32_t>(integer(a[7]));
+        const float scale = static_cast<float>(number(a[8]));
+        size_t bytes = 0;
+        checked([&] { return chx_hip_expert_routing_workspace(T, E, &bytes); });
+        const at::TensorOptions ints = logits.options().dtype(at::kInt);
+        const at::Tensor experts = at::empty({T, k}, ints), weights = at::empty({T, k}, ints.dtype(at::kFloat)), order = at::empty({T * k}, ints);
+        const at::Tensor offsets = at::empty({E + 1}, ints), space = scratch(bytes, logits);
+        Operand ed(experts), wd(weights), od(order), fd(offsets);
+        void* s = current_stream();
+        checked([&] {
+            return chx_hip_expert_routing(ld.ptr, bd.ptr, sigmoid, groups, top_groups, group_best, normalize, scale, ed.ptr, wd.ptr, od.ptr, fd.ptr,
+                                          bytes ? space.data_ptr() : nullptr, bytes, s);
+        });
+        return tuple_of({experts, weights, order, offsets});
+    });
+}
+
+// expert_combine(x, weights, r or None, out or None)
+PyObject* expert_combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 4);
+        const at::Tensor &x = on_device(a[0], "x"), &weights = on_device(a[1], "weights");
+        if (x.dim() != 2 || weights.dim() != 2) fail(PyExc_ValueError, "x and weights must be matrices");
+        const at::Tensor y = result(a[3], {weights.size(0), x.size(1)}, x.options());
+        Operand xd(x), wd(weights), rd(optional_on_device(a[2], "r")), yd(y);
+        void* s = current_stream();
+        checked([&] { return chx_hip_expert_combine(xd.ptr, wd.ptr, rd.ptr, yd.ptr, s); });
+        return wrapped(a[3], y);
+    });
+}
+
+// token_logprobs(logits, tokens or None, top) -> (log probabilities or None, entropy, top log probabilities, top tokens)
+PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 3);
+        at::Tensor logits = on_device(a[0], "logits");
+        const bool given = a[1] != Py_None;
+        const int64_t top = integer(a[2]);
+        if (logits.dim() < 1 || top < 0) fail(PyExc_ValueError, "logits need an axis, and no less than 0 alternatives can be asked for");
+        c10::SmallVector<int64_t, 8> rows(logits.sizes().begin(), logits.sizes().end() - 1), best = rows;
+        best.push_back(top);
+        at::Tensor tokens;
+        if (given) {
+            tokens = on_device(a[1], "tokens");
+            if (tokens.sizes() != at::IntArrayRef(rows)) fail(PyExc_ValueError, "a token for each row of the logits is expected");
+        }
+        const at::TensorOptions floats = logits.options().dtype(at::kFloat);
+        const at::Tensor entropy = at::empty(rows, floats), top_logprobs = at::empty(best, floats), top_tokens = at::empty(best, floats.dtype(at::kLong));
+        const at::Tensor logprobs = given ? at::empty(rows, floats) : at::Tensor();
+        const int64_t V = logits.size(-1), R = entropy.numel();
+        // (views; the library takes a matrix and vectors)
+        if (logits.dim() != 2) logits = logits.view({R, V});
+        const at::Tensor flat_top = top_logprobs.view({R, top}), flat_best = top_tokens.view({R, top}), flat_entropy = entropy.view({R});
+        size_t bytes = 0;
+        checked([&] { return chx_hip_token_logprobs_workspace(R, V, top, &bytes); });
+        const at::Tensor space = scratch(bytes, logits);
+        Operand ld(logits), ed(flat_entropy), td(flat_top), bd(flat_best);
+        void* s = current_stream();
+        void* memory = bytes ? space.data_ptr() : nullptr;
+        if (given) {
+            const at::Tensor flat_tokens = tokens.view({R}), flat_logprobs = logprobs.view({R});
+            Operand kd(flat_tokens), pd(flat_logprobs);
+            checked([&] { return chx_hip_token_logprobs(ld.ptr, kd.ptr, pd.ptr, ed.ptr, td.ptr, bd.ptr, memory, bytes, s); });
+        } else {
+            checked([&] { return chx_hip_token_logprobs(ld.ptr, nullptr, nullptr, ed.ptr, td.ptr, bd.ptr, memory, bytes, s); });
+        }
+        return tuple_of({logprobs, entropy, top_logprobs, top_tokens});
+    });
+}
+
 // ---- runs of the virtual machine (chxvm.py); its library is loaded by the caller, who hands the entry points over ----
 struct Machine {
     decltype(&chxvm_program_run_to_host) run;
@@ -532,6 +702,12 @@ PyMethodDef methods[] = {
         {"matmul_integer", fast(matmul_integer), METH_FASTCALL, nullptr},
         {"qlinear_matmul", fast(qlinear_matmul), METH_FASTCALL, nullptr},
         {"plan_run", fast(plan_run), METH_FASTCALL, nullptr},
+        {"linear_plan", fast(linear_plan), METH_FASTCALL, nullptr},
+        {"linear_run", fast(linear_run), METH_FASTCALL, nullptr},
+        {"linear_run_experts", fast(linear_run_experts), METH_FASTCALL, nullptr},
+        {"expert_routing", fast(expert_routing), METH_FASTCALL, nullptr},
+        {"expert_combine", fast(expert_combine), METH_FASTCALL, nullptr},
+        {"token_logprobs", fast(token_logprobs), METH_FASTCALL, nullptr},
         {"vm_init", fast(vm_init), METH_FASTCALL, nullptr},
         {"vm_run", fast(vm_run), METH_FASTCALL, nullptr},
         {"vm_outputs", vm_outputs, METH_O, nullptr},

@@ -101,6 +101,29 @@ inline bool is_contiguous(const chx_hip_tensor& t) {
     return true;
 }
 
+// Whether the bytes between the first and the last element of one array meet those of the other; both with elements.
+inline bool arrays_overlap(const chx_hip_tensor& a, const chx_hip_tensor& b) {
+    intptr_t lo[2], hi[2];
+    const chx_hip_tensor* t[2] = {&a, &b};
+    for (int i = 0; i < 2; ++i) {
+        lo[i] = reinterpret_cast<intptr_t>(t[i]->data);
+        hi[i] = lo[i] + dtype_size(t[i]->dtype);
+        for (int d = 0; d < t[i]->ndim; ++d) {
+            const int64_t span = (t[i]->shape[d] - 1) * t[i]->strides[d];
+            (span < 0 ? lo : hi)[i] += span;
+        }
+    }
+    return lo[0] < hi[1] && lo[1] < hi[0];
+}
+
+// One array given twice.
+inline bool same_array(const chx_hip_tensor& a, const chx_hip_tensor& b) {
+    if (a.data != b.data || a.dtype != b.dtype || !same_shape(a, b)) return false;
+    for (int i = 0; i < a.ndim; ++i)
+        if (a.shape[i] != 1 && a.strides[i] != b.strides[i]) return false;
+    return true;
+}
+
 // NCHW-shaped view of channels-last memory: strides (H*W*C', 1, W*C', C') in
 // elements, where C' >= C is the allocated channel pitch.
 inline bool is_channels_last(const chx_hip_tensor& t, int64_t* channel_pitch) {

@@ -1,0 +1,51 @@
+// Products with an epilogue from a plan (linear_plan.hip): what the host hands to the kernels, and the order of the laid-out weights.
+#pragma once
+
+#include "chx_internal.h"
+
+namespace chx {
+
+enum LinearType { kHalfHalf = 0, kHalfInt8 = 1, kFloatFloat = 2 };  // x and w
+
+// Weights [N, K] are laid out in groups of 64 rows, along k in units of 64 bytes of a row, a unit as four fragments of 1 KB: the operand of
+// one matrix instruction (16 rows, a lane's 16 bytes together; two instructions' for int8, four for float32).
+//   float16  32 k a unit: lane l holds k = 8 (l / 16) + j
+//   int8     64 k a unit: bytes 8 s + j of lane l hold k = 32 s + 8 (l / 16) + j, so that x is read as for float16
+//   float32  16 k a unit: k = 4 (l / 16) + j; instruction j of the unit takes the k that are j modulo 4
+// Row r of fragment f is row 16 (r / 4) + 4 f + r % 4 of the group: a lane of the result then holds 16 neighbouring columns, 32 bytes of
+// float16, and four lanes a whole line.  K is filled up with zeros to whole steps (128 bytes of x), N to whole groups.
+constexpr int kGroupRows = 64, kFragment = 1024, kUnit = 4 * kFragment;
+
+__host__ __device__ inline int group_row(int fragment, int r) {
+    return 16 * (r >> 2) + 4 * fragment + (r & 3);
+}
+
+struct LinearArgs {
+    const char* x;
+    const char* w;
+    const float* scale;  // of int8 rows, [N], or null
+    const float* bias;   // [N] or null
+    const char* r;       // residual or null
+    char* y;
+    int64_t x_row, x_col, r_row, r_col, y_row, y_col;  // bytes
+    int64_t w_group, w_expert;                          // bytes from one group, one expert, to the next
+    int32_t M, N, K, units;                             // units: of laid-out weights along k
+    int32_t activation, y_half;                         // y_half: y and r are float16
+    int32_t vector_y, vector_r;                         // 16 bytes of neighbouring columns at a time
+    int32_t tiles_m, tiles_n;
+    // rows that a routing has sent to experts: M of them
+    const int32_t* order;
+    const int32_t* offsets;
+    int32_t experts, fan, n_padded;
+};
+
+// The kernels, by the types of x and w (linear_half.hip, linear_int8.hip, linear_float.hip).  `rows`: few rows, weights straight into
+// registers; `tile`: both operands through LDS.  `direct`: rows of x can be copied in whole 16-byte pieces.
+enum LinearTile { kTile256 = 0, kTile128 = 1 };
+template <LinearType kType>
+struct LinearKernels {
+    static int rows(const LinearArgs& a, int row_tiles, int fragments, bool direct, hipStream_t s);
+    static int tile(const LinearArgs& a, LinearTile t, bool direct, hipStream_t s);
+};
+
+}  // namespace chx

@@ -1,0 +1,330 @@
+// Matrix products with bias, activation and residual in their epilogue, from weights that are laid out once: the host side and the
+// layout (linear_plan.h); the kernels are in linear_kernel.h.
+#include <algorithm>
+#include <cstring>
+#include <new>
+
+#include "linear_plan.h"
+
+struct chx_hip_linear_plan {
+    chx::LinearType type = chx::kHalfHalf;
+    char* w = nullptr;       // laid out; then scales and biases, each float32 [experts][n_padded]
+    float* scale = nullptr;
+    float* bias = nullptr;
+    int64_t w_group = 0, w_expert = 0;
+    int32_t N = 0, K = 0, units = 0, experts = 0, n_padded = 0;  // experts 0: a plan without
+    int device = 0;
+};
+
+namespace chx {
+namespace {
+
+struct LayoutArgs {
+    const char* w;
+    int64_t ws_e, ws_n, ws_k;  // bytes
+    char* out;
+    int32_t N, K, units, groups, type;
+    int64_t fragments;  // of all
+};
+
+// One lane writes 16 bytes, a wavefront a fragment.  Runs once per layer; w is read through its strides.
+__global__ __launch_bounds__(256) void linear_layout_kernel(LayoutArgs a) {
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= a.fragments) return;
+    const int lane = threadIdx.x & 63, fragment = (int)(at & 3);
+    const int64_t unit = (at >> 2) % a.units, group = (at >> 2) / a.units % a.groups, expert = (at >> 2) / a.units / a.groups;
+    const int64_t n = group * kGroupRows + group_row(fragment, lane & 15);
+    const char* row = a.w + expert * a.ws_e + n * a.ws_n;
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (n < a.N) {
+        if (a.type == kHalfHalf) {
+            for (int j = 0; j < 8; ++j) {
+                const int64_t k = unit * 32 + (lane >> 4) * 8 + j;
+                if (k < a.K) v[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + k * a.ws_k) << (16 * (j & 1));
+            }
+        } else if (a.type == kHalfInt8) {
+            for (int j = 0; j < 16; ++j) {
+                const int64_t k = unit * 64 + (j >> 3) * 32 + (lane >> 4) * 8 + (j & 7);
+                if (k < a.K) v[j / 4] |= (uint32_t)*reinterpret_cast<const uint8_t*>(row + k * a.ws_k) << (8 * (j & 3));
+            }
+        } else {
+            for (int j = 0; j < 4; ++j) {
+                const int64_t k = unit * 16 + (lane >> 4) * 4 + j;
+                if (k < a.K) v[j] = *reinterpret_cast<const uint32_t*>(row + k * a.ws_k);
+            }
+        }
+    }
+    *reinterpret_cast<uint4*>(a.out + at * kFragment + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+struct VectorArgs {
+    const char* v;
+    int64_t s_e, s_n;  // bytes
+    float* out;
+    int32_t N, n_padded, half;
+    int64_t total;
+};
+
+__global__ __launch_bounds__(256) void linear_vector_kernel(VectorArgs a) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= a.total) return;
+    const int64_t e = at / a.n_padded, n = at % a.n_padded;
+    const char* p = a.v + e * a.s_e + n * a.s_n;
+    a.out[at] = n >= a.N ? 0.f : a.half ? (float)*reinterpret_cast<const _Float16*>(p) : *reinterpret_cast<const float*>(p);
+}
+
+// The axes before the last as one run of rows.
+bool as_rows(const chx_hip_tensor& t, int64_t* rows, int64_t* row_stride) {
+    int64_t count = 1, st = 0;
+    bool first = true;
+    for (int d = t.ndim - 2; d >= 0; --d) {
+        if (t.shape[d] == 1) continue;
+        if (first) {
+            st = t.strides[d];
+            first = false;
+        } else if (t.strides[d] != st * count) {
+            return false;
+        }
+        count *= t.shape[d];
+    }
+    *rows = count;
+    *row_stride = st;
+    return true;
+}
+
+// Distances and address that are whole elements: the kernels load by element where they cannot load more.
+int check_elements(const chx_hip_tensor& t, const char* name) {
+    const int64_t es = dtype_size(t.dtype);
+    CHX_REQUIRE(aligned(t.data, (size_t)es), "linear plan: %s does not begin at an element's address", name);
+    for (int d = 0; d < t.ndim; ++d) CHX_REQUIRE(t.strides[d] % es == 0, "linear plan: a stride of %s is not a number of whole elements", name);
+    return CHX_HIP_OK;
+}
+
+bool aligned_rows(const void* p, int64_t row_stride, int64_t rows, int64_t bytes) {
+    return aligned(p, (size_t)bytes) && (rows == 1 || row_stride % bytes == 0);
+}
+
+struct Call {
+    LinearArgs a;
+    bool direct;
+};
+
+int prepare_call(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, Call* c) {
+    CHX_REQUIRE(plan != nullptr, "linear plan: null plan");
+    CHX_PROPAGATE(check_tensor(x, "linear plan x"));
+    CHX_PROPAGATE(check_tensor(y, "linear plan y"));
+    const int32_t type = plan->type == kFloatFloat ? CHX_HIP_FLOAT32 : CHX_HIP_FLOAT16;
+    CHX_REQUIRE(x->dtype == type, "linear plan: x must be %s for these weights, not %s", dtype_name(type), dtype_name(x->dtype));
+    CHX_REQUIRE(y->dtype == CHX_HIP_FLOAT32 || (y->dtype == CHX_HIP_FLOAT16 && type == CHX_HIP_FLOAT16), "linear plan: y must be float32%s, not %s",
+                type == CHX_HIP_FLOAT16 ? " or float16" : "", dtype_name(y->dtype));
+    CHX_REQUIRE(activation >= CHX_HIP_ACT_NONE && activation <= CHX_HIP_ACT_SILU, "linear plan: unknown activation %d", activation);
+    CHX_REQUIRE(x->ndim >= 1 && x->shape[x->ndim - 1] == plan->K, "linear plan: the last axis of x must have %d elements", plan->K);
+    CHX_REQUIRE(y->ndim >= 1 && y->shape[y->ndim - 1] == plan->N, "linear plan: the last axis of y must have %d elements", plan->N);
+    CHX_PROPAGATE(check_elements(*x, "x"));
+    CHX_PROPAGATE(check_elements(*y, "y"));
+    int device = 0;
+    CHX_HIP_CALL(hipGetDevice(&device));
+    CHX_REQUIRE(device == plan->device, "linear plan: created on device %d, run on device %d", plan->device, device);
+    LinearArgs& a = c->a;
+    memset(&a, 0, sizeof(a));
+    int64_t x_rows = 0, y_rows = 0;
+    CHX_REQUIRE(as_rows(*x, &x_rows, &a.x_row), "linear plan: the leading axes of x are not one run of rows");
+    CHX_REQUIRE(as_rows(*y, &y_rows, &a.y_row), "linear plan: the leading axes of y are not one run of rows");
+    CHX_REQUIRE(y_rows < (int64_t(1) << 31) && x_rows < (int64_t(1) << 31), "linear plan: 2^31 rows or more");
+    const int64_t xe = dtype_size(x->dtype), ye = dtype_size(y->dtype);
+    a.x = static_cast<const char*>(x->data);
+    a.y = static_cast<char*>(y->data);
+    a.x_col = plan->K == 1 ? xe : x->strides[x->ndim - 1];
+    a.y_col = plan->N == 1 ? ye : y->strides[y->ndim - 1];
+    a.y_half = y->dtype == CHX_HIP_FLOAT16;
+    a.vector_y = a.y_col == ye && aligned_rows(a.y, a.y_row, y_rows, 4 * ye);
+    if (r != nullptr) {
+        CHX_PROPAGATE(check_tensor(r, "linear plan r"));
+        CHX_REQUIRE(r->dtype == y->dtype && same_shape(*r, *y), "linear plan: r must have the type and shape of y");
+        CHX_PROPAGATE(check_elements(*r, "r"));
+        int64_t r_rows = 0;
+        CHX_REQUIRE(as_rows(*r, &r_rows, &a.r_row), "linear plan: the leading axes of r are not one run of rows");
+        a.r = static_cast<const char*>(r->data);
+        a.r_col = plan->N == 1 ? ye : r->strides[r->ndim - 1];
+        a.vector_r = a.r_col == ye && aligned_rows(a.r, a.r_row, r_rows, 4 * ye);
+    }
+    if (numel(*y) > 0) {
+        CHX_REQUIRE(numel(*x) == 0 || !arrays_overlap(*x, *y), "linear plan: x and y overlap");
+        CHX_REQUIRE(r == nullptr || same_array(*r, *y) || !arrays_overlap(*r, *y), "linear plan: r and y overlap and are not the same array");
+    }
+    a.w = plan->w;
+    a.scale = plan->scale;
+    a.bias = plan->bias;
+    a.w_group = plan->w_group;
+    a.w_expert = plan->w_expert;
+    a.M = (int32_t)y_rows;
+    a.N = plan->N;
+    a.K = plan->K;
+    a.units = plan->units;
+    a.n_padded = plan->n_padded;
+    a.activation = activation;
+    a.fan = 1;
+    // rows that can be copied in pieces of 16 bytes, addressed with 32 bits from a tile's first one
+    c->direct = a.x_col == xe && aligned_rows(a.x, a.x_row, x_rows, 16) && a.x_row >= 0 && a.x_row < (int64_t(1) << 23);
+    return CHX_HIP_OK;
+}
+
+template <LinearType kType>
+int launch(LinearArgs& a, bool direct, hipStream_t s) {
+    // The most tiles of rows there can be: experts' tiles begin anew with each of them.
+    auto tiles = [&](int32_t height) {
+        if (!a.order) return (a.M + height - 1) / height;
+        return a.M / height + std::min(a.M, a.experts);
+    };
+    const int32_t groups = (a.N + kGroupRows - 1) / kGroupRows;
+    const int64_t rows_each = a.order ? (a.M + a.experts - 1) / a.experts : a.M;
+    if (rows_each <= 64) {
+        const int row_tiles = rows_each <= 16 ? 1 : rows_each <= 32 ? 2 : 4;
+        a.tiles_m = tiles(16 * row_tiles);
+        const int64_t wide = (int64_t)a.tiles_m * groups;
+        const int fragments = wide >= 512 ? 4 : wide >= 256 ? 2 : 1;
+        a.tiles_n = groups * (4 / fragments);
+        CHX_REQUIRE((int64_t)a.tiles_m * a.tiles_n < (int64_t(1) << 31), "linear plan: too many results");
+        const bool whole = direct && a.K % (kType == kFloatFloat ? 32 : 64) == 0;
+        return LinearKernels<kType>::rows(a, row_tiles, fragments, whole, s);
+    }
+    const int64_t large = (int64_t)tiles(256) * ((a.N + 255) / 256);
+    const bool t256 = large >= 200;
+    a.tiles_m = tiles(t256 ? 256 : 128);
+    a.tiles_n = t256 ? (a.N + 255) / 256 : (a.N + 127) / 128;
+    CHX_REQUIRE((int64_t)a.tiles_m * a.tiles_n < (int64_t(1) << 31), "linear plan: too many results");
+    return LinearKernels<kType>::tile(a, t256 ? kTile256 : kTile128, direct, s);
+}
+
+int launch_of(const chx_hip_linear_plan* plan, Call& c, hipStream_t s) {
+    if (c.a.M == 0 || c.a.N == 0) return CHX_HIP_OK;
+    switch (plan->type) {
+        case kHalfHalf: return launch<kHalfHalf>(c.a, c.direct, s);
+        case kHalfInt8: return launch<kHalfInt8>(c.a, c.direct, s);
+        default: return launch<kFloatFloat>(c.a, c.direct, s);
+    }
+}
+
+}  // namespace
+}  // namespace chx
+
+using namespace chx;
+
+extern "C" int chx_hip_linear_plan_create(
+        const chx_hip_tensor* w, const chx_hip_tensor* w_scale, const chx_hip_tensor* b, void* stream, chx_hip_linear_plan** out) {
+    CHX_REQUIRE(out != nullptr, "linear plan: null output");
+    *out = nullptr;
+    CHX_PROPAGATE(check_tensor(w, "linear plan w"));
+    CHX_REQUIRE(w->dtype == CHX_HIP_FLOAT16 || w->dtype == CHX_HIP_FLOAT32 || w->dtype == CHX_HIP_INT8, "linear plan: w must be float16, float32 or int8, not %s",
+                dtype_name(w->dtype));
+    CHX_REQUIRE(w->ndim == 2 || w->ndim == 3, "linear plan: w must be [N, K] or [experts, N, K]");
+    CHX_PROPAGATE(check_elements(*w, "w"));
+    const int lead = w->ndim - 2;
+    const int64_t E = lead ? w->shape[0] : 1, N = w->shape[lead], K = w->shape[lead + 1];
+    CHX_REQUIRE(E >= 1 && N >= 1 && K >= 1, "linear plan: w has no elements");
+    CHX_REQUIRE(E <= 65536 && N <= (1 << 24) && K <= (1 << 24), "linear plan: more than 65536 experts, or more than 2^24 rows or columns of w");
+    CHX_REQUIRE((w->dtype == CHX_HIP_INT8) == (w_scale != nullptr), "linear plan: int8 weights have a w_scale, others have none");
+    auto check_vector = [&](const chx_hip_tensor* t, const char* name) -> int {
+        CHX_PROPAGATE(check_tensor(t, name));
+        CHX_REQUIRE(t->dtype == CHX_HIP_FLOAT32 || (t->dtype == CHX_HIP_FLOAT16 && t == b), "linear plan: the type of %s", name);
+        CHX_REQUIRE(t->ndim == lead + 1 && t->shape[lead] == N && (lead == 0 || t->shape[0] == E), "linear plan: %s must be [N], or [experts, N]", name);
+        return check_elements(*t, name);
+    };
+    if (w_scale) CHX_PROPAGATE(check_vector(w_scale, "w_scale"));
+    if (b) CHX_PROPAGATE(check_vector(b, "b"));
+    chx_hip_linear_plan p;
+    p.type = w->dtype == CHX_HIP_FLOAT16 ? kHalfHalf : w->dtype == CHX_HIP_INT8 ? kHalfInt8 : kFloatFloat;
+    const int64_t step = p.type == kFloatFloat ? 32 : 64, units_of_step = p.type == kHalfInt8 ? 1 : 2;
+    const int64_t groups = (N + kGroupRows - 1) / kGroupRows;
+    p.units = (int32_t)((K + step - 1) / step * units_of_step);
+    p.N = (int32_t)N;
+    p.K = (int32_t)K;
+    p.experts = lead ? (int32_t)E : 0;
+    p.n_padded = (int32_t)(groups * kGroupRows);
+    p.w_group = (int64_t)p.units * kUnit;
+    p.w_expert = groups * p.w_group;
+    // (a tile's groups are addressed with 32 bits)
+    CHX_REQUIRE(p.w_group < (int64_t(1) << 29), "linear plan: a row of w is too long");
+    CHX_HIP_CALL(hipGetDevice(&p.device));
+    const int64_t vector_bytes = E * p.n_padded * 4, bytes = E * p.w_expert + (w_scale ? vector_bytes : 0) + (b ? vector_bytes : 0);
+    void* memory = nullptr;
+    CHX_PROPAGATE(spare_memory(&memory, (size_t)bytes, "linear plan"));
+    p.w = static_cast<char*>(memory);
+    char* next = p.w + E * p.w_expert;
+    LayoutArgs l = {static_cast<const char*>(w->data), lead ? w->strides[0] : 0, w->strides[lead], w->strides[lead + 1], p.w, p.N, p.K, p.units,
+                    (int32_t)groups, (int32_t)p.type, E * groups * p.units * 4};
+    int rc = CHX_HIP_OK;
+    const int64_t blocks = (l.fragments + 3) / 4;
+    if (blocks >= (int64_t(1) << 31)) {
+        set_error("linear plan: too many weights");
+        rc = CHX_HIP_EINVAL;
+    } else {
+        linear_layout_kernel<<<(unsigned)blocks, 256, 0, as_stream(stream)>>>(l);
+        rc = launch_check("linear_layout_kernel");
+    }
+    auto vector = [&](const chx_hip_tensor* t) {
+        float* out_v = reinterpret_cast<float*>(next);
+        next += vector_bytes;
+        if (rc != CHX_HIP_OK) return out_v;
+        VectorArgs v = {static_cast<const char*>(t->data), lead ? t->strides[0] : 0, t->strides[lead], out_v, p.N, p.n_padded, t->dtype == CHX_HIP_FLOAT16, E * p.n_padded};
+        linear_vector_kernel<<<(unsigned)((v.total + 255) / 256), 256, 0, as_stream(stream)>>>(v);
+        rc = launch_check("linear_vector_kernel");
+        return out_v;
+    };
+    if (w_scale) p.scale = vector(w_scale);
+    if (b) p.bias = vector(b);
+    // (later calls may come on any stream)
+    if (rc == CHX_HIP_OK && hipStreamSynchronize(as_stream(stream)) != hipSuccess) {
+        set_error("linear plan: the stream is in error, or being recorded");
+        rc = CHX_HIP_ERUNTIME;
+    }
+    chx_hip_linear_plan* made = rc == CHX_HIP_OK ? new (std::nothrow) chx_hip_linear_plan(p) : nullptr;
+    if (made == nullptr) {
+        (void)hipFree(memory);
+        if (rc == CHX_HIP_OK) CHX_FAIL(CHX_HIP_ERUNTIME, "linear plan: no memory on the host");
+        return rc;
+    }
+    *out = made;
+    return CHX_HIP_OK;
+}
+
+extern "C" void chx_hip_linear_plan_destroy(chx_hip_linear_plan* plan) {
+    if (!plan) return;
+    (void)hipFree(plan->w);
+    delete plan;
+}
+
+extern "C" int chx_hip_linear_plan_run(
+        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, void* stream) {
+    Call c;
+    CHX_PROPAGATE(prepare_call(plan, x, activation, r, y, &c));
+    CHX_REQUIRE(plan->experts == 0, "linear plan: the weights are experts': run_experts takes them");
+    CHX_REQUIRE(x->ndim == y->ndim, "linear plan: x and y differ in their number of axes");
+    for (int d = 0; d + 1 < x->ndim; ++d) CHX_REQUIRE(x->shape[d] == y->shape[d], "linear plan: x and y differ on axis %d", d);
+    return launch_of(plan, c, as_stream(stream));
+}
+
+extern "C" int chx_hip_linear_plan_run_experts(
+        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, const chx_hip_tensor* order, const chx_hip_tensor* offsets, int32_t activation,
+        chx_hip_tensor* y, void* stream) {
+    Call c;
+    CHX_PROPAGATE(prepare_call(plan, x, activation, nullptr, y, &c));
+    CHX_REQUIRE(plan->experts > 0, "linear plan: the weights have no experts: run takes them");
+    CHX_PROPAGATE(check_tensor(order, "linear plan order"));
+    CHX_PROPAGATE(check_tensor(offsets, "linear plan offsets"));
+    CHX_REQUIRE(x->ndim == 2 && y->ndim == 2, "linear plan: x and y must be matrices for experts");
+    CHX_REQUIRE(order->dtype == CHX_HIP_INT32 && is_contiguous(*order) && numel(*order) == y->shape[0], "linear plan: order must be int32, contiguous, a number for each row of y");
+    CHX_REQUIRE(offsets->dtype == CHX_HIP_INT32 && is_contiguous(*offsets) && numel(*offsets) == plan->experts + 1, "linear plan: offsets must be int32, contiguous, %d numbers",
+                plan->experts + 1);
+    CHX_REQUIRE(aligned(order->data, 4) && aligned(offsets->data, 4), "linear plan: order and offsets must begin at an element's address");
+    if (y->shape[0] == 0) return CHX_HIP_OK;
+    CHX_REQUIRE(x->shape[0] > 0 && y->shape[0] % x->shape[0] == 0, "linear plan: the rows of y must be a multiple of those of x");
+    CHX_REQUIRE(!arrays_overlap(*order, *y) && !arrays_overlap(*offsets, *y), "linear plan: y overlaps order or offsets");
+    c.a.order = static_cast<const int32_t*>(order->data);
+    c.a.offsets = static_cast<const int32_t*>(offsets->data);
+    c.a.experts = plan->experts;
+    c.a.fan = (int32_t)(y->shape[0] / x->shape[0]);
+    // rows are gathered: all of x within 32 bits
+    c.direct = c.direct && c.a.x_row * x->shape[0] < (int64_t(1) << 32);
+    return launch_of(plan, c, as_stream(stream));
+}

@@ -323,6 +323,63 @@ class QLinearConvPlan(object):
             pass
 
 
+class LinearPlan(object):
+    """The weights of a layer, laid out once (chx_hip_linear_plan): w [N, K], or [experts, N, K]; float16, float32, or int8 with
+    w_scale float32 [N] / [experts, N]; b float16 or float32 likewise.  Tensors passed here are not needed afterwards."""
+
+    def __init__(self, w, b=None, w_scale=None):
+        self.out_features = int(w.shape[-2]) if w.dim() >= 2 else 0
+        self._plan = capi.native().linear_plan(w, w_scale, b)
+
+    def run(self, x, activation="", r=None, dtype=None, out=None):
+        """act(x . w^T * w_scale + b) + r over the last axis of x; the result has the type of x, or `dtype`.  activation: "",
+        "relu", "gelu", "gelu_tanh" or "silu".  r may be `out`."""
+        return capi.native().linear_run(self._handle(), self.out_features, x, capi.ACTIVATIONS[activation], r, dtype, out)
+
+    def run_experts(self, x, order, offsets, activation="", dtype=None, out=None):
+        """The products of an expert layer: for p = order[i], offsets[e] <= i < offsets[e + 1], row p of the result is
+        act(x[p // (P // R)] . w[e]^T * w_scale[e] + b[e]), with P = len(order) and R = len(x); order and offsets as
+        ExpertRouting gives them.  Rows that no place names are left as they are (undefined in a new result)."""
+        return capi.native().linear_run_experts(self._handle(), self.out_features, x, order, offsets, capi.ACTIVATIONS[activation], dtype, out)
+
+    def _handle(self):
+        if self._plan is None:
+            raise ValueError("the plan is closed")
+        return self._plan
+
+    def close(self):
+        plan, self._plan = self._plan, None
+        if plan is not None:
+            capi.lib().chx_hip_linear_plan_destroy(ctypes.c_void_p(plan))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def ExpertRouting(logits, k, bias=None, score="softmax", groups=1, top_groups=None, group_best=1, normalize=True, scale=1.0):
+    """chx_hip_expert_routing: (experts int32 [T, k], weights float32 [T, k], order int32 [T k], offsets int32 [E + 1]) for logits
+    [T, E].  score: "softmax" or "sigmoid"; bias float32 [E] is added to the scores for the choice alone; the experts of
+    the top_groups (by default all) best of `groups` groups can be chosen, a group's score being the sum of its group_best (1 or
+    2) best; the weights are divided by their sum if `normalize`, and multiplied by `scale`."""
+    return capi.native().expert_routing(logits, k, bias, ("softmax", "sigmoid").index(score), groups, groups if top_groups is None else top_groups,
+                                        group_best, 1 if normalize else 0, scale)
+
+
+def ExpertCombine(x, weights, r=None, out=None):
+    """chx_hip_expert_combine: sum_j weights[t, j] * x[t k + j] + r[t] for x [T k, N] and weights float32 [T, k], as
+    LinearPlan.run_experts and ExpertRouting give them.  r may be `out`."""
+    return capi.native().expert_combine(x, weights, r, out)
+
+
+def TokenLogProbs(logits, tokens=None, top=0):
+    """chx_hip_token_logprobs over the last axis of logits [.., V]: (log probabilities of `tokens` [..] or None, entropy [..], the
+    `top` best log probabilities [.., top], their tokens int64 [.., top])."""
+    return capi.native().token_logprobs(logits, tokens, top)
+
+
 def _pool_out(in_dim, p0, p1, k, s, cover_all):
     if cover_all:
         return (in_dim + p0 + p1 - k + s - 1) // s + 1

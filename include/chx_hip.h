@@ -438,6 +438,82 @@ int chx_hip_conv_f32(
  * inside ChainerX's Softmax is not in the reference tree.) */
 int chx_hip_softmax_f32(const chx_hip_tensor* x, int32_t axis, int32_t is_onnx_semantics, chx_hip_tensor* y, void* stream);
 
+/* ---- float layers of a language model --------------------------------------------------- */
+
+/* No entry point below allocates device memory or waits for the device, except where it says so, so that all of them can be
+ * recorded into graphs; scratch memory is the caller's (`workspace`, of at least the bytes that the entry point's _workspace
+ * function gives; two calls that may run at the same time need one each).  No counterpart in the reference, whose op set has no
+ * such layers (the closest are Linear, runtime/ops/connection.cc:12-15, and Softmax, runtime/ops/activation.cc:66-95).
+ * What lies in device memory (orders, offsets, tokens) is checked by the kernels: places outside their range are left out. */
+
+/* What an epilogue applies to a sum v.  GELU: v Phi(v), Phi the normal distribution; GELU_TANH: its approximation
+ * 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))); SILU: v / (1 + exp(-v)). */
+enum { CHX_HIP_ACT_NONE = 0, CHX_HIP_ACT_RELU = 1, CHX_HIP_ACT_GELU = 2, CHX_HIP_ACT_GELU_TANH = 3, CHX_HIP_ACT_SILU = 4 };
+
+/* The weights of a layer, laid out once for its products:
+ *   w        [N, K], or [E, N, K] for a layer with E experts: float16, float32 or int8, any strides
+ *   w_scale  float32 [N] / [E, N] of int8 weights (a weight is w * w_scale), else NULL
+ *   b        float16 or float32 [N] / [E, N], or NULL
+ * create() copies all of them and waits for the stream.  A plan belongs to the device it was created on and may be used by
+ * several threads and streams at once; it must outlive the graphs that its runs were recorded into. */
+typedef struct chx_hip_linear_plan chx_hip_linear_plan;
+int chx_hip_linear_plan_create(
+        const chx_hip_tensor* w, const chx_hip_tensor* w_scale, const chx_hip_tensor* b, void* stream, chx_hip_linear_plan** plan);
+void chx_hip_linear_plan_destroy(chx_hip_linear_plan* plan);
+
+/* y[.., n] = act(w_scale[n] * sum_k x[.., k] w[n, k] + b[n]) + r[.., n], for a plan without experts.
+ *   x  [.., K], float16 for float16 and int8 weights, float32 for float32 ones; any alignment and strides whose leading axes are
+ *      one run of rows
+ *   y  [.., N] likewise, float16 or float32 (float32 only for float32 x)
+ *   r  NULL, or of y's shape and type; may be y itself
+ * Sums and epilogue are float32, in an order that depends on the sizes alone; the result is rounded once.  y must not overlap x,
+ * nor r unless it is r. */
+int chx_hip_linear_plan_run(
+        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, void* stream);
+
+/* The same with experts, over P rows: places offsets[e] <= i < offsets[e + 1] of `order` are expert e's, and for p = order[i]
+ *   y[p, n] = act(w_scale[e, n] * sum_k x[p / (P / R), k] w[e, n, k] + b[e, n])
+ *   x        [R, K], R a divisor of P (a row's results are next to each other where it goes to several experts)
+ *   order    int32 [P], offsets int32 [E + 1], contiguous, as chx_hip_expert_routing gives them: each row at most once
+ *   y        [P, N]; rows that no place names are left as they are */
+int chx_hip_linear_plan_run_experts(
+        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, const chx_hip_tensor* order, const chx_hip_tensor* offsets, int32_t activation,
+        chx_hip_tensor* y, void* stream);
+
+/* Routing rows to experts.  logits [T, E], float16 or float32; per row, in 64 bits where that decides:
+ *   s = softmax(logits), or 1 / (1 + exp(-logits)) with `sigmoid`;  key = s + bias (float32 [E], or NULL)
+ *   the E experts are `groups` groups of neighbours; a group's score is the sum of its `group_best` (1 or 2) best keys, and only
+ *   the top_groups best groups' experts can be chosen
+ *   the k = experts->shape[1] largest keys are chosen, largest first; of equal ones (groups likewise) the lower index first
+ *   weight = s of the chosen (not the key), over the sum of the chosen if `normalize` (0 where that sum is 0), times `scale`
+ * A NaN logit counts as -inf, +inf as the largest finite number; an expert with -inf has s = 0 and is chosen only when the others run out.
+ *   experts int32 [T, k];  weights float32 [T, k]
+ *   order   int32 [T k]: the places t k + j, those of expert 0 first, of one expert in ascending order
+ *   offsets int32 [E + 1]: where each expert's places begin in order
+ * E at most 1024, k and groups at most 64.  All results are dense and overlap nothing; workspace: aligned to 4. */
+int chx_hip_expert_routing_workspace(int64_t rows, int64_t experts, size_t* bytes);
+int chx_hip_expert_routing(
+        const chx_hip_tensor* logits, const chx_hip_tensor* bias, int32_t sigmoid, int32_t groups, int32_t top_groups, int32_t group_best,
+        int32_t normalize, float scale, chx_hip_tensor* experts, chx_hip_tensor* weights, chx_hip_tensor* order, chx_hip_tensor* offsets,
+        void* workspace, size_t workspace_bytes, void* stream);
+
+/* y[t, n] = sum_j weights[t, j] * x[t k + j, n] + r[t, n]: what k experts made of a row, weighted; sums in float32.  x [T k, N] and y,
+ * r [T, N] float16 or float32, of one type, any strides; weights float32 [T, k], contiguous.  A row whose weight is 0 adds nothing,
+ * whatever it holds.  r: NULL, or y itself, or an array that does not overlap y. */
+int chx_hip_expert_combine(const chx_hip_tensor* x, const chx_hip_tensor* weights, const chx_hip_tensor* r, chx_hip_tensor* y, void* stream);
+
+/* What a network answers: over each row of logits [R, V] (float16 or float32, any strides), in float32,
+ *   logprobs[r]     the log probability of tokens[r] (int32 or int64 [R]); 0 for a negative token (a place without one), NaN for one of V or more
+ *   entropy[r]      -sum p log p
+ *   top_logprobs, top_tokens [R, top]: the largest logits' log probabilities and (int64) indexes, best first; of equal logits the lower
+ *                   index first, a NaN before all others
+ * logprobs, entropy and top_logprobs float32.  tokens and logprobs may be NULL, `top` 0.  A row of nothing but -inf has entropy 0 and log probabilities -inf;
+ * one with a NaN or +inf has NaN.  top at most 64 and V.  All results are dense and overlap nothing; workspace: aligned to 16. */
+int chx_hip_token_logprobs_workspace(int64_t rows, int64_t logits, int64_t top, size_t* bytes);
+int chx_hip_token_logprobs(
+        const chx_hip_tensor* logits, const chx_hip_tensor* tokens, chx_hip_tensor* logprobs, chx_hip_tensor* entropy, chx_hip_tensor* top_logprobs,
+        chx_hip_tensor* top_tokens, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- pooling on quantized tensors ------------------------------------------------------ */
 
 /* MaxPoolOp::RunImpl, runtime/ops/pooling.cc:47-61, as it occurs in a quantized
