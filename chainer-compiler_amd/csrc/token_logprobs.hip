@@ -3,12 +3,16 @@
 //   m = max x;  s = sum exp(x - m);  t = sum (x - m) exp(x - m)          over a row's V logits
 //   log p(token) = x[token] - m - log s;   entropy = log s - t / s;      alternatives: the `top` largest logits, the lower index first
 //
-// Bound by the bytes of the logits: one pass with a running maximum, four loads of 16 bytes a lane under way, in float32.  Where rows are few, work-groups
-// share a row and a second launch joins their parts, in one order.
+// Bound by the bytes of the logits: one pass with a running maximum, four loads of 16 bytes a lane under way.  Where rows are few, work-groups share a row and
+// a second launch joins their parts, in one order; where they are many and short, each wavefront has a row of its own.
 //
-// The alternatives are found in the same pass.  A wavefront keeps a threshold below which nothing can be among its `top` best, first from the
-// maxima of its lanes (the top-th largest of 64 of them has top logits at or above it), later from what it has gathered; a block of 32 logits a lane is
-// compared by its maximum alone, and what passes goes to a list in LDS that is cut to its best when it is full.
+// The arithmetic is what comes next: a float16 logit takes 8 issue slots of a lane (4 of them the exponential), which keep the vector
+// units busy for 60 us of 4096 rows of 65,536.  Their sums are therefore kept relative to a number M in units of log 2, the rounded m log2(e): y = x log2(e) - M is one fused
+// multiply-add that also converts x, exact to its own rounding, and M drops out at the end.  (float32 logits may be too large for that product: x - m first.)
+//
+// The alternatives are found in the same pass.  What is below a threshold cannot be among the `top` best: the top-th largest of the maxima that the
+// lanes found in their first 32 logits has top logits at or above it.  32 logits of a lane are compared by their maximum alone; what
+// passes goes to a list in LDS, and the lists are ranked at the end by counting, for every entry, those before it.
 #include <cfloat>
 #include <cmath>
 #include <cstring>
@@ -19,11 +23,13 @@ namespace chx {
 namespace {
 
 constexpr int kMostTop = 64, kWaves = 4;
-constexpr int kKept = 256, kList = kKept + 512;  // entries of a list: it is cut when there are more than kKept, and 512 more may come in between
-constexpr int kLoads = 4;               // of 16 bytes (float16), 32 (float32): 8 logits each
-constexpr int kBlock = 64 * 8 * kLoads; // logits of a wavefront's step
+constexpr int kKept = 256, kList = kKept + 512;  // entries of a wavefront's list: it is cut when there are more than kKept, and 512 more may come in between
+constexpr int kLoads = 4;                        // of 16 bytes (float16), 32 (float32): 8 logits each
+constexpr int kBlock = 64 * 8 * kLoads;          // logits of a wavefront's step
 constexpr int kMostParts = 64;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+
+struct Sums;
 
 struct LogprobArgs {
     const char* logits;
@@ -37,8 +43,8 @@ struct LogprobArgs {
     float* entropy;
     float* top_logprob;
     int64_t* top_token;
-    float* sums;     // of the parts: [row][part][4]
-    uint64_t* lists; // [row][part][top], best first
+    Sums* sums;  // of the parts: [row][part]
+    uint64_t* lists;    // [row][part][top], best first, zeros where a part has none
 };
 
 __device__ __forceinline__ uint32_t sortable(float v) {
@@ -53,208 +59,276 @@ __device__ __forceinline__ uint64_t entry_of(float v, int32_t index) {
     return (uint64_t)sortable(v) << 32 | (uint32_t)~index;
 }
 
+// Sums of 2^y and y 2^y over logits x: y = x log2(e) - m for float16, (x - m) log2(e) for float32.
 struct Sums {
-    float m, s, t;  // t in units of log 2: sum (x - m) log2(e) exp(x - m)
+    float m, s, t;
 };
-// The sums over both, relative to the larger maximum.
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m);
-    const float ya = (a.m - m) * kLog2e, yb = (b.m - m) * kLog2e;
-    const float fa = a.s == 0.f ? 0.f : __builtin_amdgcn_exp2f(ya), fb = b.s == 0.f ? 0.f : __builtin_amdgcn_exp2f(yb);
-    Sums r;
-    r.m = m;
-    r.s = a.s * fa + b.s * fb;
-    r.t = (fa == 0.f ? 0.f * a.s : (a.t + ya * a.s) * fa) + (fb == 0.f ? 0.f * b.s : (b.t + yb * b.s) * fb);
-    return r;
+constexpr float kNoMaximum[2] = {-FLT_MAX, -1e6f};  // [kHalf]: below every m, and its differences are finite or give 0
+
+template <bool kHalf>
+__device__ __forceinline__ float log2_of(float x, float m) {
+    return kHalf ? __builtin_fmaf(x, kLog2e, -m) : (x - m) * kLog2e;
+}
+template <bool kHalf>
+__device__ __forceinline__ float maximum_of(float x) {
+    return kHalf ? x * kLog2e : x;
 }
 
-// The `top` best of `count` entries of one wavefront, kept at the front of its list; returns how many there are, and the least of them (0: all are).
-__device__ int32_t cut_list(uint64_t* list, int32_t count, int32_t top, uint64_t* least_kept) {
-    const int lane = threadIdx.x & 63;
-    *least_kept = 0;
-    if (count <= top) return count;
-    uint64_t mine[kList / 64];
+// x - m as a natural logarithm.
+template <bool kHalf>
+__device__ __forceinline__ float log_of(float x, float m) {
+    return kHalf ? log2_of<true>(x, m) * kLn2 : x - m;
+}
+
+// The sums relative to a larger maximum.
+template <bool kHalf>
+__device__ __forceinline__ void move_to(Sums& z, float m) {
+    const float y = kHalf ? z.m - m : (z.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(y);
+    z.t = f == 0.f ? 0.f * z.s : (z.t + y * z.s) * f;  // (y may be -inf; a NaN stays one)
+    z.s = z.s * f;
+    z.m = m;
+}
+
+// Of all lanes, in every lane.
+template <bool kHalf>
+__device__ __forceinline__ void join_lanes(Sums& z) {
+    float m = z.m;
 #pragma unroll
-    for (int i = 0; i < kList / 64; ++i) mine[i] = 64 * i + lane < count ? list[64 * i + lane] : 0;
+    for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+    move_to<kHalf>(z, m);
+#pragma unroll
+    for (int d = 32; d; d /= 2) {
+        z.s += __shfl_xor(z.s, d);
+        z.t += __shfl_xor(z.t, d);
+    }
+}
+
+// The `top` best of more than that many entries of one wavefront, kept at the front of its list; returns the least of them.  kKept entries are held in
+// registers; more of them, which takes logits that rise for thousands, are read again and again, so that the loop over the logits
+// does not pay for registers that it hardly ever needs.
+template <bool kFew>
+__device__ __forceinline__ uint64_t cut_list(uint64_t* list, int32_t count, int32_t top) {
+    constexpr int kHeld = kFew ? kKept / 64 : 1;
+    const int lane = threadIdx.x & 63;
+    uint64_t mine[kHeld];
+    if constexpr (kFew) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) mine[i] = 64 * i + lane < count ? list[64 * i + lane] : 0;
+    }
     // the top-th largest, bit by bit: no two entries are equal
     uint64_t least = 0;
     for (int b = 63; b >= 0; --b) {
         const uint64_t try_at = least | 1ull << b;
         int n = 0;
+        if constexpr (kFew) {
 #pragma unroll
-        for (int i = 0; i < kList / 64; ++i) {
-            if (64 * i >= count) break;
-            n += __popcll(__builtin_amdgcn_ballot_w64(mine[i] >= try_at));
+            for (int i = 0; i < kHeld; ++i) n += __popcll(__builtin_amdgcn_ballot_w64(mine[i] >= try_at));
+        } else {
+            for (int i = lane; i - lane < count; i += 64) n += __popcll(__builtin_amdgcn_ballot_w64(i < count && list[i] >= try_at));
         }
         if (n >= top) least = try_at;
     }
     int32_t at = 0;
+    auto keep = [&](uint64_t entry, bool there) {
+        const uint64_t kept = __builtin_amdgcn_ballot_w64(there && entry >= least);
+        if ((kept >> lane) & 1) list[at + __popcll(kept & ((1ull << lane) - 1))] = entry;
+        at += __popcll(kept);
+    };
+    if constexpr (kFew) {
 #pragma unroll
-    for (int i = 0; i < kList / 64; ++i) {
-        const uint64_t keep = __builtin_amdgcn_ballot_w64(mine[i] >= least);
-        if ((keep >> lane) & 1) list[at + __popcll(keep & ((1ull << lane) - 1))] = mine[i];
-        at += __popcll(keep);
+        for (int i = 0; i < kHeld; ++i) keep(mine[i], mine[i] != 0);
+    } else {
+        for (int i = lane; i - lane < count; i += 64) keep(i < count ? list[i] : 0, i < count);  // (never ahead of what is read)
     }
-    *least_kept = least;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    return at;
+    return least;
 }
 
-// entries[0, count), count <= 64, of one wavefront: best first, zeros behind them up to `top`.
-__device__ void sort_list(uint64_t* list, int32_t count, int32_t top) {
-    const int lane = threadIdx.x & 63;
-    const uint64_t mine = lane < count ? list[lane] : 0;
-    int rank = 0;
-    for (int i = 0; i < count; ++i) rank += __shfl(mine, i) > mine;
-    __builtin_amdgcn_wave_barrier();
-    if (lane < top) list[lane < count ? rank : lane] = mine;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+// How many of a list's entries come before `mine`.
+__device__ __forceinline__ int32_t before_in(const uint64_t* list, int32_t count, uint64_t mine) {
+    int32_t n = 0;
+#pragma unroll 8
+    for (int32_t i = 0; i < count; ++i) n += list[i] > mine;
+    return n;
 }
 
-// The best `top` of `lists` sorted lists of `top` entries, `stride` entries apart; the lanes of one wavefront, lists <= 64.  Lane j gets the j-th.
-__device__ uint64_t merge_lists(const uint64_t* list, int32_t lists, int32_t stride, int32_t top) {
-    const int lane = threadIdx.x & 63;
-    int32_t next = 0;
-    uint64_t head = lane < lists && top > 0 ? list[(int64_t)lane * stride] : 0, got = 0;
-    for (int j = 0; j < top; ++j) {
-        uint64_t best = head;
-#pragma unroll
-        for (int d = 32; d; d /= 2) {
-            const uint64_t other = __shfl_xor(best, d);
-            best = other > best ? other : best;
-        }
-        if (lane == j) got = best;
-        if (head == best && best != 0) {
-            ++next;
-            head = next < top ? list[(int64_t)lane * stride + next] : 0;
-        }
-    }
-    return got;
+// A row's token and its logit: two loads one after the other, asked for before the sums are there.
+struct Given {
+    float logit, in_place_of;  // in_place_of: 0 without a token, NaN for one that the row does not have, else 1
+};
+template <bool kHalf>
+__device__ __forceinline__ Given given(const LogprobArgs& a, int64_t row) {
+    if (!a.logprob) return {0.f, 0.f};
+    const char* p = a.tokens + row * a.token_col;
+    const int64_t token = a.token64 ? *reinterpret_cast<const int64_t*>(p) : *reinterpret_cast<const int32_t*>(p);
+    if (token < 0 || token >= a.V) return {0.f, token < 0 ? 0.f : NAN};
+    const char* q = a.logits + row * a.row + token * a.col;
+    return {kHalf ? (float)*reinterpret_cast<const _Float16*>(q) : *reinterpret_cast<const float*>(q), 1.f};
 }
 
-// What is reported for a row, by one wavefront; `best` as from merge_lists.
-__device__ void report(const LogprobArgs& a, int64_t row, const Sums& z, uint64_t best) {
-    const int lane = threadIdx.x & 63;
+// What is reported for a row: of its token and its entropy by one lane, of an alternative by whoever has it.
+template <bool kHalf>
+__device__ __forceinline__ void report_row(const LogprobArgs& a, int64_t row, const Sums& z, const Given& g) {
     // (no logit above -inf: no token has a probability)
     const bool none = z.s == 0.f;
     const float log_s = none ? 0.f : logf(z.s);
-    if (lane == 0) {
-        if (a.logprob) {
-            const char* p = a.tokens + row * a.token_col;
-            const int64_t token = a.token64 ? *reinterpret_cast<const int64_t*>(p) : *reinterpret_cast<const int32_t*>(p);
-            float v = 0.f;
-            if (token >= a.V) {
-                v = NAN;
-            } else if (token >= 0) {
-                const char* q = a.logits + row * a.row + token * a.col;
-                v = none ? -INFINITY : (a.half ? (float)*reinterpret_cast<const _Float16*>(q) : *reinterpret_cast<const float*>(q)) - z.m - log_s;
-            }
-            a.logprob[row] = v;
-        }
-        a.entropy[row] = none ? 0.f : log_s - kLn2 * z.t / z.s;
-    }
-    if (lane < a.top) {
-        const float x = of_sortable((uint32_t)(best >> 32));
-        a.top_logprob[row * a.top + lane] = none ? -INFINITY : x - z.m - log_s;
-        a.top_token[row * a.top + lane] = (int64_t)(uint32_t)~(uint32_t)best;
-    }
+    if (a.logprob) a.logprob[row] = g.in_place_of != 1.f ? g.in_place_of : none ? -INFINITY : log_of<kHalf>(g.logit, z.m) - log_s;
+    a.entropy[row] = none ? 0.f : log_s - kLn2 * z.t / z.s;
 }
 
+template <bool kHalf>
+__device__ __forceinline__ void report_best(const LogprobArgs& a, int64_t row, const Sums& z, int32_t rank, uint64_t entry) {
+    const bool none = z.s == 0.f;
+    a.top_logprob[row * a.top + rank] = none ? -INFINITY : log_of<kHalf>(of_sortable((uint32_t)(entry >> 32)), z.m) - logf(z.s);
+    a.top_token[row * a.top + rank] = (int64_t)(uint32_t)~(uint32_t)entry;
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 
-// Eight logits from index i on; -inf from `end` on.
+// Eight logits as they lie in memory, from index i on; -inf from `end` on.
 template <bool kHalf>
-__device__ __forceinline__ void load8(const char* row, int64_t col, int32_t i, int32_t end, float* x) {
-    constexpr int kElement = kHalf ? 2 : 4;
-    if (col == kElement && i + 8 <= end) {
-        const u32x4_any* p = reinterpret_cast<const u32x4_any*>(row + (int64_t)i * kElement);
-        if constexpr (kHalf) {
-            const half8 h = __builtin_bit_cast(half8, p[0]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = (float)h[j];
-        } else {
-            const u32x4_any lo = p[0], hi = p[1];
-            __builtin_memcpy(x, &lo, 16);
-            __builtin_memcpy(x + 4, &hi, 16);
-        }
-        return;
+struct Eight {
+    u32x4 v[kHalf ? 1 : 2];
+    __device__ __forceinline__ void load(const char* p) {
+        v[0] = reinterpret_cast<const u32x4_any*>(p)[0];
+        if constexpr (!kHalf) v[1] = reinterpret_cast<const u32x4_any*>(p)[1];
     }
+    __device__ __forceinline__ void load_some(const char* row, int64_t col, int32_t i, int32_t end) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = -INFINITY;
-        if (i + j < end) {
+        for (int j = 0; j < 8; ++j) {
             const char* p = row + (int64_t)(i + j) * col;
-            if constexpr (kHalf) x[j] = (float)*reinterpret_cast<const _Float16*>(p);
-            else x[j] = *reinterpret_cast<const float*>(p);
+            if constexpr (kHalf) {
+                const uint32_t h = i + j < end ? *reinterpret_cast<const uint16_t*>(p) : 0xfc00u;
+                v[0][j / 2] = j & 1 ? v[0][j / 2] | h << 16 : h;
+            } else {
+                v[j / 4][j & 3] = i + j < end ? *reinterpret_cast<const uint32_t*>(p) : 0xff800000u;
+            }
         }
     }
-}
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (kHalf) return (float)__builtin_bit_cast(half8, v[0])[j];
+        else return __builtin_bit_cast(float4v, v[j / 4])[j & 3];
+    }
+    // What was made of these is made again where it is asked for next, and takes no registers until then.
+    __device__ __forceinline__ void forget() {
+        asm volatile("" : "+v"(v[0]));
+        if constexpr (!kHalf) asm volatile("" : "+v"(v[1]));
+    }
+    // (a NaN may go unnoticed)
+    __device__ __forceinline__ float maximum() const {
+        if constexpr (kHalf) {
+            const half8 h = __builtin_bit_cast(half8, v[0]);
+            half2v m = {h[0], h[1]};
+#pragma unroll
+            for (int j = 2; j < 8; j += 2) m = __builtin_elementwise_max(m, half2v{h[j], h[j + 1]});
+            return (float)(m[0] > m[1] ? m[0] : m[1]);
+        } else {
+            float m = at(0);
+#pragma unroll
+            for (int j = 1; j < 8; ++j) m = fmaxf(m, at(j));
+            return m;
+        }
+    }
+};
 
-template <bool kHalf>
+// kTeam wavefronts to a row: 4, or 1 where rows are many and short (no parts then).
+template <bool kHalf, int kTeam>
 __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs a) {
     __shared__ uint64_t lists[kWaves][kList];
+    __shared__ int32_t counts[kWaves];
     __shared__ Sums sums[kWaves];
+    __shared__ uint32_t maxima[kTeam > 1 ? kWaves : 1][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = blockIdx.x / a.parts;
-    const int32_t part = blockIdx.x % a.parts;
+    const int member = kTeam > 1 ? wave : 0;
+    int64_t row = kTeam > 1 ? blockIdx.x / a.parts : (int64_t)blockIdx.x * kWaves + wave;
+    const int32_t part = kTeam > 1 ? blockIdx.x % a.parts : 0;
+    if (kTeam == 1 && row >= a.R) return;
     const int32_t begin = part * a.part, end = min(begin + a.part, a.V);
     const char* logits = a.logits + row * a.row;
     uint64_t* list = lists[wave];
-    // (a maximum of the lowest number to begin with: its differences are finite)
-    Sums z = {-FLT_MAX, 0.f, 0.f};
+    constexpr int kElement = kHalf ? 2 : 4;
+    const bool dense = a.col == kElement;
+    Sums z = {kNoMaximum[kHalf], 0.f, 0.f};
     int32_t count = 0;
-    float below = NAN;  // what is not above it cannot be among the best; NaN: not known yet
-    for (int32_t b = begin + wave * kBlock; b < end; b += kWaves * kBlock) {
-        float x[kLoads * 8];
+    float below = NAN;  // what is not above it cannot be among the best; a NaN lets everything pass
+    bool first = true;
+    for (int32_t b = begin + member * kBlock; first || b < end; b += kTeam * kBlock) {
+        Eight<kHalf> x[kLoads];
+        if (dense && b + kBlock <= end) {
+            const char* p = logits + (int64_t)(b + lane * 8) * kElement;
 #pragma unroll
-        for (int l = 0; l < kLoads; ++l) load8<kHalf>(logits, a.col, b + (l * 64 + lane) * 8, end, x + l * 8);
-        float most = x[0];
+            for (int l = 0; l < kLoads; ++l) x[l].load(p + l * 64 * 8 * kElement);
+        } else {
 #pragma unroll
-        for (int j = 1; j < kLoads * 8; ++j) most = fmaxf(most, x[j]);
-        const float m = fmaxf(z.m, most);
-        {
-            const float y = (z.m - m) * kLog2e, f = __builtin_amdgcn_exp2f(y);
-            z.t = f == 0.f ? 0.f * z.s : (z.t + y * z.s) * f;
-            z.s *= f;
-            z.m = m;
+            for (int l = 0; l < kLoads; ++l) {
+                const int32_t i = b + (l * 64 + lane) * 8;
+                if (dense && i + 8 <= end) x[l].load(logits + (int64_t)i * kElement);
+                else x[l].load_some(logits, a.col, i, end);
+            }
         }
+        float best[kLoads];
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) best[l] = x[l].maximum();
+        const float most = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+        move_to<kHalf>(z, fmaxf(z.m, maximum_of<kHalf>(most)));
         float s = 0.f, t = 0.f;
 #pragma unroll
         for (int j = 0; j < kLoads * 8; ++j) {
-            const float y = (x[j] - m) * kLog2e, e = __builtin_amdgcn_exp2f(y);
+            const float y = log2_of<kHalf>(x[j / 8].at(j & 7), z.m), e = __builtin_amdgcn_exp2f(y);
             s += e;
             t = __builtin_fmaf(fmaxf(y, -16384.f), e, t);  // (0, not NaN, for a logit of -inf)
         }
         z.s += s;
         z.t += t;
-        if (a.top == 0) continue;
-        if (below != below) {
-            // the top-th largest of the lanes' maxima has `top` logits at or above it
-            const uint32_t mine = sortable(most);
-            int before = 0;
-            for (int i = 0; i < 64; ++i) {
-                const uint32_t other = __shfl(mine, i);
-                before += other > mine || (other == mine && i < lane);
+        if (a.top == 0) {
+            first = false;
+            continue;
+        }
+        if (first) {
+            // the top-th largest of the lanes' maxima, of all wavefronts of the row, or of the maxima of its loads in one: its upper 20 bits, which is
+            // a little below
+            first = false;
+            constexpr int kMaxima = 4;
+            static_assert(kTeam == 1 ? kLoads == kMaxima : kTeam == kMaxima, "as many to a lane");
+            uint32_t mine[kMaxima];
+            if constexpr (kTeam > 1) {
+                maxima[wave][lane] = sortable(most);
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < kMaxima; ++w) mine[w] = maxima[w][lane];
+            } else {
+#pragma unroll
+                for (int l = 0; l < kMaxima; ++l) mine[l] = sortable(best[l]);
             }
-            const uint64_t at = __builtin_amdgcn_ballot_w64(before == a.top - 1);
-            const uint32_t key = __builtin_amdgcn_readlane(mine, __builtin_ctzll(at));
-            // (what lies next below: below 0 not -0, which equals it; below -inf a NaN, so that everything passes)
-            below = of_sortable(key == 0x80000000u ? key - 2 : key - 1);
+            uint32_t least = 0;
+            for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1) {
+                int n = 0;
+#pragma unroll
+                for (int w = 0; w < kMaxima; ++w) n += __popcll(__builtin_amdgcn_ballot_w64(mine[w] >= (least | bit)));
+                if (n >= a.top) least |= bit;
+            }
+            // (what lies next below: below 0 not -0, which equals it; below -inf a NaN)
+            below = of_sortable(least == 0x80000000u ? least - 2 : least - 1);
         }
         // (a sum that has become NaN may hide one from the maximum)
         if (__builtin_amdgcn_ballot_w64(!(most <= below) || z.s != z.s)) {
             uint64_t least = 0;
-#pragma unroll 1
+#pragma unroll
             for (int l = 0; l < kLoads; ++l) {
-                if (count > kKept) count = cut_list(list, count, a.top, &least);
+                if (__builtin_amdgcn_ballot_w64(!(best[l] <= below) || z.s != z.s) == 0) continue;
+                if (count > kKept) {
+                    least = cut_list<false>(list, count, a.top);
+                    count = a.top;
+                }
+                x[l].forget();
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float v = x[j];
-#pragma unroll
-                    for (int q = 1; q < kLoads; ++q) v = q == l ? x[q * 8 + j] : v;
+                    const float v = x[l].at(j);
                     const int32_t index = b + (l * 64 + lane) * 8 + j;
                     const uint64_t pass = __builtin_amdgcn_ballot_w64(index < end && !(v <= below));
                     if (pass == 0) continue;
@@ -268,52 +342,83 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
             if (least != 0) below = of_sortable((uint32_t)(least >> 32));
         }
     }
-    // lanes, then wavefronts, in one order
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        Sums o = {__shfl_xor(z.m, d), __shfl_xor(z.s, d), __shfl_xor(z.t, d)};
-        z = joined(z, o);
+    Given g;
+    if (lane == 0 && member == 0 && a.parts == 1) g = given<kHalf>(a, row);
+    join_lanes<kHalf>(z);
+    if (count > 64) {
+        if (count <= kKept) cut_list<true>(list, count, a.top);
+        else cut_list<false>(list, count, a.top);
+        count = a.top;
     }
-    if (lane == 0) sums[wave] = z;
-    if (a.top > 0) {
-        uint64_t least;
-        count = cut_list(list, count, a.top, &least);
-        sort_list(list, count, a.top);
-    }
-    __syncthreads();
-    if (wave != 0) return;
-    z = sums[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) z = joined(z, sums[w]);
-    const uint64_t best = merge_lists(&lists[0][0], kWaves, kList, a.top);
-    if (a.parts == 1) {
-        report(a, row, z, best);
+    if constexpr (kTeam == 1) {
+        if (lane == 0) report_row<kHalf>(a, row, z, g);
+        const uint64_t mine = lane < count ? list[lane] : 0;
+        const int32_t rank = before_in(list, count, mine);
+        if (lane < count && rank < a.top) report_best<kHalf>(a, row, z, rank, mine);
         return;
     }
-    float* to = a.sums + (row * a.parts + part) * 4;
     if (lane == 0) {
-        to[0] = z.m;
-        to[1] = z.s;
-        to[2] = z.t;
+        sums[wave] = z;
+        counts[wave] = count;
     }
-    if (lane < a.top) a.lists[(row * a.parts + part) * a.top + lane] = best;
+    __syncthreads();
+    z = lane < kTeam ? sums[lane] : Sums{kNoMaximum[kHalf], 0.f, 0.f};
+    join_lanes<kHalf>(z);
+    const bool whole = a.parts == 1;
+    if (threadIdx.x == 0) {
+        if (whole) report_row<kHalf>(a, row, z, g);
+        else a.sums[blockIdx.x] = z;
+    }
+    if (a.top == 0) return;
+    const uint64_t mine = lane < count ? list[lane] : 0;
+    int32_t rank = 0;
+#pragma unroll
+    for (int w = 0; w < kTeam; ++w) rank += before_in(lists[w], counts[w], mine);
+    if (lane < count && rank < a.top) {
+        if (whole) report_best<kHalf>(a, row, z, rank, mine);
+        else a.lists[(int64_t)blockIdx.x * a.top + rank] = mine;
+    }
+    if (!whole) {  // a part may have fewer logits than alternatives
+        int32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kTeam; ++w) all += counts[w];
+        if ((int32_t)threadIdx.x >= all && (int32_t)threadIdx.x < a.top) a.lists[(int64_t)blockIdx.x * a.top + threadIdx.x] = 0;
+    }
 }
 
-// The parts of a row, by one wavefront.
-__global__ __launch_bounds__(64) void token_logprobs_join_kernel(LogprobArgs a) {
-    const int lane = threadIdx.x;
+// The parts of a row.  The largest of their last entries is a bound for what can be among the best.
+template <bool kHalf>
+__global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogprobArgs a) {
+    __shared__ uint64_t list[kMostParts * kMostTop];
+    __shared__ unsigned long long bound;
+    __shared__ int32_t count;
+    const int lane = threadIdx.x & 63;
     const int64_t row = blockIdx.x;
-    Sums z = {-FLT_MAX, 0.f, 0.f};
-    if (lane < a.parts) {
-        const float* from = a.sums + (row * a.parts + lane) * 4;
-        z = {from[0], from[1], from[2]};
+    const uint64_t* from = a.lists + row * a.parts * a.top;
+    const int32_t all = a.parts * a.top;
+    Sums z = lane < a.parts ? a.sums[row * a.parts + lane] : Sums{kNoMaximum[kHalf], 0.f, 0.f};
+    const uint64_t last = a.top > 0 && lane < a.parts ? from[(lane + 1) * a.top - 1] : 0, first = (int32_t)threadIdx.x < all ? from[threadIdx.x] : 0;
+    Given g;
+    if (threadIdx.x == 0) {
+        g = given<kHalf>(a, row);
+        bound = 1;
+        count = 0;
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        Sums o = {__shfl_xor(z.m, d), __shfl_xor(z.s, d), __shfl_xor(z.t, d)};
-        z = joined(z, o);
+    __syncthreads();
+    if (threadIdx.x < 64 && last != 0) atomicMax(&bound, (unsigned long long)last);
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < all; i += 256) {
+        const uint64_t e = i == (int32_t)threadIdx.x ? first : from[i];
+        if (e >= bound) list[atomicAdd(&count, 1)] = e;  // (in any order: they are ranked)
     }
-    report(a, row, z, merge_lists(a.lists + row * a.parts * a.top, a.parts, a.top, a.top));
+    join_lanes<kHalf>(z);
+    if (threadIdx.x == 0) report_row<kHalf>(a, row, z, g);
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < count; i += 256) {
+        const uint64_t mine = list[i];
+        const int32_t rank = before_in(list, count, mine);
+        if (rank < a.top) report_best<kHalf>(a, row, z, rank, mine);
+    }
 }
 
 // Parts of a row: as many as give each compute unit four work-groups, each of at least a step of all its wavefronts.
@@ -330,7 +435,22 @@ void split(int64_t R, int64_t V, int32_t* parts, int32_t* part) {
 int64_t workspace_of(int64_t R, int64_t V, int64_t top) {
     int32_t parts, part;
     split(R, V, &parts, &part);
-    return parts == 1 ? 0 : R * parts * (16 + 8 * top);
+    return parts == 1 ? 0 : R * parts * (16 + 8 * top);  // (Sums are 12 bytes)
+}
+
+template <bool kHalf>
+int launch(const LogprobArgs& a, hipStream_t s) {
+    // One wavefront to a row of one or two steps.  us as four / as one, 8192 rows of float16 with 5 alternatives: 1000 logits 57 / 17, 4096 59 / 26, 8192 53 / 44
+    // (but 66 / 62 with 20, 81 / 150 with 64); 1024 rows of 4096 10.0 / 10.0 (14.8 / 16.4 with 64).
+    if (a.V <= kBlock || (a.V <= 2 * kBlock && a.R >= 2048)) {
+        token_logprobs_kernel<kHalf, 1><<<(unsigned)((a.R + kWaves - 1) / kWaves), 64 * kWaves, 0, s>>>(a);
+        return launch_check("token_logprobs_kernel");
+    }
+    token_logprobs_kernel<kHalf, kWaves><<<(unsigned)(a.R * a.parts), 64 * kWaves, 0, s>>>(a);
+    CHX_PROPAGATE(launch_check("token_logprobs_kernel"));
+    if (a.parts == 1) return CHX_HIP_OK;
+    token_logprobs_join_kernel<kHalf><<<(unsigned)a.R, 256, 0, s>>>(a);
+    return launch_check("token_logprobs_join_kernel");
 }
 
 int check_sizes(int64_t R, int64_t V, int64_t top) {
@@ -404,14 +524,7 @@ extern "C" int chx_hip_token_logprobs(
     a.entropy = static_cast<float*>(entropy->data);
     a.top_logprob = static_cast<float*>(top_logprobs->data);
     a.top_token = static_cast<int64_t*>(top_tokens->data);
-    a.sums = static_cast<float*>(workspace);
+    a.sums = static_cast<Sums*>(workspace);
     a.lists = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + R * a.parts * 16);
-    const hipStream_t s = as_stream(stream);
-    const unsigned blocks = (unsigned)(R * a.parts);
-    if (a.half) token_logprobs_kernel<true><<<blocks, 64 * kWaves, 0, s>>>(a);
-    else token_logprobs_kernel<false><<<blocks, 64 * kWaves, 0, s>>>(a);
-    CHX_PROPAGATE(launch_check("token_logprobs_kernel"));
-    if (a.parts == 1) return CHX_HIP_OK;
-    token_logprobs_join_kernel<<<(unsigned)R, 64, 0, s>>>(a);
-    return launch_check("token_logprobs_join_kernel");
+    return a.half ? launch<true>(a, as_stream(stream)) : launch<false>(a, as_stream(stream));
 }
