@@ -7,9 +7,11 @@
 //
 // A wavefront takes a row, its lanes the experts lane + 64 i.  Without a bias and groups the choice is made on the logits themselves, of which the
 // keys are a monotonic function; else the keys are 64-bit numbers, so that which expert is chosen does not hang on how exp
-// rounds.  Bound by latency: chains of 6 steps across the lanes, one for each of the k.
+// rounds.  Bound by latency: k times the largest of 64 lanes, which takes some 80 cycles through the lanes' data paths (DPP) where six exchanges through
+// LDS take 400.
 #include <cfloat>
 #include <cstring>
+#include <type_traits>
 
 #include "chx_internal.h"
 
@@ -17,9 +19,12 @@ namespace chx {
 namespace {
 
 constexpr int kMostExperts = 1024, kMostChosen = 64, kMostGroups = 64;
-constexpr int kBlockWaves = 4;    // of a launch with many rows
-constexpr int kSingleWaves = 16;  // of the one work-group that takes few
-constexpr int kMostChunks = 256, kSingleRows = 32;
+// Wavefronts of a work-group (with 16 experts to a lane and keys in 64 bits, sixteen would have to spill registers)
+constexpr int waves_of(int per) {
+    return per > 8 ? 8 : 16;
+}
+// Rows that one launch takes: us for one / two launches over 256 experts with k = 8 and a bias, 16 rows 9.4 / 10.8 (host 7 / 10.6), 32 rows 16.1 / 10.8.
+constexpr int kMostChunks = 256, kSingleRows = 16;
 
 struct RoutingArgs {
     const char* logits;
@@ -46,20 +51,49 @@ __device__ __forceinline__ uint64_t sortable(double v) {
     return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) v = fmaxf(v, __shfl_xor(v, d));
+// Reductions over the wavefront: within rows of 16 lanes, then from row to row; lane 63 has them all.
+template <int kControl, int kRows>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kControl, kRows, 0xf, false);  // (0 where no lane is)
+}
+template <int kControl, int kRows>
+__device__ __forceinline__ float moved(float v) {
+    return __builtin_bit_cast(float, moved<kControl, kRows>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int kControl, int kRows>
+__device__ __forceinline__ double moved(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)moved<kControl, kRows>((uint32_t)(b >> 32)) << 32 | moved<kControl, kRows>((uint32_t)b));
+}
+constexpr int kShift1 = 0x111, kShift2 = 0x112, kShift4 = 0x114, kShift8 = 0x118, kToNextRow = 0x142, kToUpperHalf = 0x143;
+
+// (of numbers from 0 on)
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, moved<kShift1, 0xf>(v));
+    v = max(v, moved<kShift2, 0xf>(v));
+    v = max(v, moved<kShift4, 0xf>(v));
+    v = max(v, moved<kShift8, 0xf>(v));
+    v = max(v, moved<kToNextRow, 0xa>(v));
+    v = max(v, moved<kToUpperHalf, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+// What the lanes up to this one have together.
+template <typename T>
+__device__ __forceinline__ T sum_up_to(T v) {
+    v += moved<kShift1, 0xf>(v);
+    v += moved<kShift2, 0xf>(v);
+    v += moved<kShift4, 0xf>(v);
+    v += moved<kShift8, 0xf>(v);
+    v += moved<kToNextRow, 0xa>(v);
+    v += moved<kToUpperHalf, 0xc>(v);
     return v;
 }
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
-    return v;
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+    return __shfl(sum_up_to(v), 63);
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
-    return v;
+__device__ __forceinline__ float of_sortable(uint32_t k) {
+    return __builtin_bit_cast(float, k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
 
 // The choice for one row; lane j holds the j-th expert and its weight afterwards (j < k).  keys: LDS for E numbers of this wavefront.
@@ -68,7 +102,7 @@ __device__ void route(const RoutingArgs& a, int32_t t, double* keys, int32_t* ex
     const int lane = threadIdx.x & 63;
     const char* row = a.logits + (int64_t)t * a.row;
     float x[kPer];
-    float most = -INFINITY;
+    uint32_t most_key = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int e = lane + 64 * i;
@@ -78,12 +112,13 @@ __device__ void route(const RoutingArgs& a, int32_t t, double* keys, int32_t* ex
             const float v = a.half ? (float)*reinterpret_cast<const _Float16*>(p) : *reinterpret_cast<const float*>(p);
             x[i] = v != v ? -INFINITY : fminf(v, FLT_MAX);
         }
-        most = fmaxf(most, x[i]);
+        most_key = max(most_key, sortable(x[i]));
     }
-    most = wave_max(most);
+    const float most = of_sortable(wave_max(most_key));
     // (a row of nothing but -inf: no expert has a score)
     const float base = most == -INFINITY ? 0.f : most;
-    uint64_t key[kPer];  // 0: not to be had (any more)
+    typedef typename std::conditional<kExact, uint64_t, uint32_t>::type Key;
+    Key key[kPer];  // 0: not to be had (any more)
     double score[kExact ? kPer : 1];
     if constexpr (kExact) {
         double sum = 0.0;
@@ -116,6 +151,7 @@ __device__ void route(const RoutingArgs& a, int32_t t, double* keys, int32_t* ex
             const int size = a.E / a.groups;
             double first = -INFINITY, second = -INFINITY;
             if (lane < a.groups) {
+#pragma unroll 8
                 for (int i = 0; i < size; ++i) {
                     const double o = keys[lane * size + i];
                     second = fmax(second, fmin(first, o));
@@ -127,60 +163,59 @@ __device__ void route(const RoutingArgs& a, int32_t t, double* keys, int32_t* ex
             const uint64_t mine = lane < a.groups ? sortable(of_group) : 0;
             int before = 0;
             for (int g = 0; g < a.groups; ++g) {
-                const uint64_t other = __shfl(mine, g);
+                const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), g) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, g);
                 before += other > mine || (other == mine && g < lane);
             }
             taken = __builtin_amdgcn_ballot_w64(lane < a.groups && before < a.top_groups);
             __builtin_amdgcn_wave_barrier();
+            const float of_size = 1.f / (float)size;  // (e / size, exactly: (e + 0.5) / size is 0.5 / size or more from a border, the product off by 2^-22 of itself)
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int e = lane + 64 * i;
-                key[i] = e < a.E && ((taken >> (e / size)) & 1) ? sortable(v[i]) : 0;
+                key[i] = e < a.E && ((taken >> (int)(((float)e + 0.5f) * of_size)) & 1) ? sortable(v[i]) : 0;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) key[i] = lane + 64 * i < a.E ? sortable(v[i]) : 0;
         }
     } else {
-        // (the index below the logit: equal ones are found lowest first)
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = lane + 64 * i;
-            key[i] = e < a.E ? (uint64_t)sortable(x[i]) << 32 | (uint32_t)~e : 0;
-        }
+        for (int i = 0; i < kPer; ++i) key[i] = lane + 64 * i < a.E ? sortable(x[i]) : 0;
     }
     int32_t chosen = 0;
     float of_chosen = 0.f;  // logit, or score
     for (int j = 0; j < a.k; ++j) {
-        uint64_t best = 0;
-        int32_t at = kMostExperts;
-        float value = 0.f;
+        // this lane's best, the largest of all, and the lowest index among those that have it
+        Key best = key[0];
+        int32_t at = lane;
+        float value = kExact ? (float)score[0] : x[0];
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) {
+            const bool better = key[i] > best;
+            best = better ? key[i] : best;
+            at = better ? lane + 64 * i : at;
+            value = better ? (kExact ? (float)score[kExact ? i : 0] : x[i]) : value;
+        }
+        const uint32_t upper = kExact ? (uint32_t)((uint64_t)best >> 32) : (uint32_t)best;
+        const uint32_t most_upper = wave_max(upper);
+        uint64_t with = __builtin_amdgcn_ballot_w64(upper == most_upper);
+        if (with & (with - 1)) {
+            bool mine = upper == most_upper;
+            if constexpr (kExact) {
+                const uint32_t most_lower = wave_max(mine ? (uint32_t)best : 0);
+                mine = mine && (uint32_t)best == most_lower;
+            }
+            const uint32_t lowest = wave_max(mine ? (uint32_t)~at : 0);
+            with = __builtin_amdgcn_ballot_w64(mine && (uint32_t)~at == lowest);
+        }
+        const int from = __builtin_ctzll(with);
+        const int32_t which = __builtin_amdgcn_readlane(at, from);
+        const float of_which = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, value), from));
+        chosen = lane == j ? which : chosen;
+        of_chosen = lane == j ? of_which : of_chosen;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            if (key[i] > best) {
-                best = key[i];
-                at = lane + 64 * i;
-                if constexpr (kExact) value = (float)score[i];
-                else value = x[i];
-            }
-#pragma unroll
-        for (int d = 32; d; d /= 2) {
-            const uint64_t other = __shfl_xor(best, d);
-            const int32_t other_at = __shfl_xor(at, d);
-            const float other_value = __shfl_xor(value, d);
-            if (other > best || (other == best && other_at < at)) {
-                best = other;
-                at = other_at;
-                value = other_value;
-            }
-        }
-        if (lane == j) {
-            chosen = at;
-            of_chosen = value;
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (lane + 64 * i == at) key[i] = 0;
+            if (lane + 64 * i == which) key[i] = 0;
     }
     float w = 0.f;
     if constexpr (kExact) {
@@ -233,14 +268,9 @@ __device__ void sums_before(int32_t* counts, int32_t E, int32_t* total) {
     int32_t carry = 0;
     for (int32_t e0 = 0; e0 < E; e0 += 64) {
         const int32_t n = e0 + lane < E ? counts[e0 + lane] : 0;
-        int32_t upto = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int32_t o = __shfl_up(upto, d);
-            if (lane >= d) upto += o;
-        }
+        const int32_t upto = (int32_t)sum_up_to((uint32_t)n);
         if (e0 + lane < E) counts[e0 + lane] = carry + upto - n;
-        carry += __shfl(upto, 63);
+        carry += __builtin_amdgcn_readlane(upto, 63);
     }
     *total = carry;
 }
@@ -251,14 +281,14 @@ __device__ __forceinline__ int32_t bits_of(int32_t E) {
 
 // Few rows: everything in one work-group.
 template <int kPer, bool kExact>
-__global__ __launch_bounds__(64 * kSingleWaves) void routing_single_kernel(RoutingArgs a) {
-    __shared__ double keys[kSingleWaves][kExact ? 64 * kPer : 1];
+__global__ __launch_bounds__(64 * waves_of(kPer)) void routing_single_kernel(RoutingArgs a) {
+    __shared__ double keys[waves_of(kPer)][kExact ? 64 * kPer : 1];
     __shared__ int32_t counts[64 * kPer];
     __shared__ int32_t chosen[kSingleRows * kMostChosen];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int e = threadIdx.x; e < a.E; e += 64 * kSingleWaves) counts[e] = 0;
+    for (int e = threadIdx.x; e < a.E; e += 64 * waves_of(kPer)) counts[e] = 0;
     __syncthreads();
-    for (int32_t t = wave; t < a.T; t += kSingleWaves) {
+    for (int32_t t = wave; t < a.T; t += waves_of(kPer)) {
         int32_t e;
         float w;
         route<kPer, kExact>(a, t, keys[wave], &e, &w);
@@ -282,14 +312,14 @@ __global__ __launch_bounds__(64 * kSingleWaves) void routing_single_kernel(Routi
 
 // Many rows: a chunk of them to a work-group, which counts how many went to each expert ...
 template <int kPer, bool kExact>
-__global__ __launch_bounds__(64 * kBlockWaves) void routing_kernel(RoutingArgs a) {
-    __shared__ double keys[kBlockWaves][kExact ? 64 * kPer : 1];
+__global__ __launch_bounds__(64 * waves_of(kPer)) void routing_kernel(RoutingArgs a) {
+    __shared__ double keys[waves_of(kPer)][kExact ? 64 * kPer : 1];
     __shared__ int32_t counts[64 * kPer];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int e = threadIdx.x; e < a.E; e += 64 * kBlockWaves) counts[e] = 0;
+    for (int e = threadIdx.x; e < a.E; e += 64 * waves_of(kPer)) counts[e] = 0;
     __syncthreads();
     const int32_t begin = blockIdx.x * a.chunk, end = min(begin + a.chunk, a.T);
-    for (int32_t t = begin + wave; t < end; t += kBlockWaves) {
+    for (int32_t t = begin + wave; t < end; t += waves_of(kPer)) {
         int32_t e;
         float w;
         route<kPer, kExact>(a, t, keys[wave], &e, &w);
@@ -300,28 +330,27 @@ __global__ __launch_bounds__(64 * kBlockWaves) void routing_kernel(RoutingArgs a
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += 64 * kBlockWaves) a.counts[(int64_t)blockIdx.x * a.E + e] = counts[e];
+    for (int e = threadIdx.x; e < a.E; e += 64 * waves_of(kPer)) a.counts[(int64_t)blockIdx.x * a.E + e] = counts[e];
 }
 
 // ... and one that adds up what the chunks before its own have, and puts its places in order.
-__global__ __launch_bounds__(256) void routing_order_kernel(RoutingArgs a) {
+__global__ __launch_bounds__(1024) void routing_order_kernel(RoutingArgs a) {
     __shared__ int32_t at[kMostExperts], before[kMostExperts];
-    for (int e = threadIdx.x; e < a.E; e += 256) at[e] = before[e] = 0;
+    for (int e = threadIdx.x; e < a.E; e += 1024) at[e] = before[e] = 0;
     __syncthreads();
     const int chunks = gridDim.x;
-    // (several threads to an expert where there are fewer experts than threads)
-    const int share = max(1, 256 / a.E), e0 = share > 1 ? threadIdx.x % a.E : threadIdx.x, part = share > 1 ? threadIdx.x / a.E : 0;
+    // (several threads to an expert, eight loads of each under way)
+    const int share = 1024 / a.E, e = threadIdx.x % a.E, part = threadIdx.x / a.E;
     if (part < share) {
-        for (int e = e0; e < a.E; e += 256) {
-            int32_t all = 0, earlier = 0;
-            for (int c = part; c < chunks; c += share) {
-                const int32_t n = a.counts[(int64_t)c * a.E + e];
-                all += n;
-                if (c < (int)blockIdx.x) earlier += n;
-            }
-            atomicAdd(&at[e], all);
-            atomicAdd(&before[e], earlier);
+        int32_t all = 0, earlier = 0;
+#pragma unroll 8
+        for (int c = part; c < chunks; c += share) {
+            const int32_t n = a.counts[(int64_t)c * a.E + e];
+            all += n;
+            earlier += c < (int)blockIdx.x ? n : 0;
         }
+        atomicAdd(&at[e], all);
+        atomicAdd(&before[e], earlier);
     }
     __syncthreads();
     if (threadIdx.x >= 64) return;
@@ -343,18 +372,18 @@ __global__ __launch_bounds__(256) void routing_order_kernel(RoutingArgs a) {
 template <int kPer>
 void launch_routing(const RoutingArgs& a, bool exact, int32_t chunks, hipStream_t s) {
     if (chunks == 0) {
-        if (exact) routing_single_kernel<kPer, true><<<1, 64 * kSingleWaves, 0, s>>>(a);
-        else routing_single_kernel<kPer, false><<<1, 64 * kSingleWaves, 0, s>>>(a);
+        if (exact) routing_single_kernel<kPer, true><<<1, 64 * waves_of(kPer), 0, s>>>(a);
+        else routing_single_kernel<kPer, false><<<1, 64 * waves_of(kPer), 0, s>>>(a);
         return;
     }
-    if (exact) routing_kernel<kPer, true><<<(unsigned)chunks, 64 * kBlockWaves, 0, s>>>(a);
-    else routing_kernel<kPer, false><<<(unsigned)chunks, 64 * kBlockWaves, 0, s>>>(a);
+    if (exact) routing_kernel<kPer, true><<<(unsigned)chunks, 64 * waves_of(kPer), 0, s>>>(a);
+    else routing_kernel<kPer, false><<<(unsigned)chunks, 64 * waves_of(kPer), 0, s>>>(a);
 }
 
-// Rows to a chunk: as many chunks as there may be, whole wavefronts' shares.
+// Rows to a chunk: as many chunks as there may be, of 4 rows at least.
 int32_t rows_of_chunk(int64_t T) {
     const int64_t rows = (T + kMostChunks - 1) / kMostChunks;
-    return (int32_t)((rows + kBlockWaves - 1) / kBlockWaves * kBlockWaves);
+    return (int32_t)((rows + 3) / 4 * 4);
 }
 
 int64_t workspace_of(int64_t T, int64_t E) {
@@ -514,7 +543,7 @@ extern "C" int chx_hip_expert_routing(
     else launch_routing<16>(a, exact, chunks, s);
     CHX_PROPAGATE(launch_check("routing_kernel"));
     if (chunks == 0) return CHX_HIP_OK;
-    routing_order_kernel<<<(unsigned)chunks, 256, 0, s>>>(a);
+    routing_order_kernel<<<(unsigned)chunks, 1024, 0, s>>>(a);
     return launch_check("routing_order_kernel");
 }
 

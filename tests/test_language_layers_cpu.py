@@ -138,10 +138,10 @@ def routing(host):
                            ((5, 16, 2), {"weights": T("float16", (5, 2))}, "weights must be")]:
         refused(host, run(*args, **kw), text)
     assert lib.chx_hip_expert_routing_workspace(ctypes.c_int64(5), ctypes.c_int64(0), ctypes.byref(ctypes.c_size_t())) == host.capi.EINVAL
-    host.check(run(32, 16, 2))
+    host.check(run(16, 16, 2))
     assert len(host.launches()) == 1
     host.clear()
-    host.check(run(33, 1024, 64))
+    host.check(run(17, 1024, 64))
     assert len(host.launches()) == 2
 
 
