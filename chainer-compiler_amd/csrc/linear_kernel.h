@@ -6,6 +6,8 @@
 // rounded once.  w is the first operand of an instruction, so that a lane's results are neighbouring columns of one row of y.
 #pragma once
 
+#include <type_traits>
+
 #include "linear_plan.h"
 
 namespace chx {
@@ -20,11 +22,11 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // 
 template <LinearType kType>
 struct Of {
     static constexpr bool kFloat = kType == kFloatFloat;
-    static constexpr int kElement = kFloat ? 4 : 2;                 // bytes of an element of x
-    static constexpr int kChunk = 16 / kElement;                    // elements in 16 bytes
-    static constexpr int kStep = 128 / kElement;                    // k of a step: 128 bytes of a row of x
-    static constexpr int kUnits = kType == kHalfInt8 ? 1 : 2;       // units of w in a step
-    static constexpr int kSteps = kType == kHalfInt8 ? 2 : 1;       // fragments of x (64 bytes of each of 16 rows) to a unit of w
+    static constexpr int kElement = kFloat ? 4 : 2;          // bytes of an element of x
+    static constexpr int kChunk = 16 / kElement;             // elements in 16 bytes
+    static constexpr int kUnitK = unit_k(kType), kUnit = unit_bytes(kType);
+    static constexpr int kPieces = kUnit / 1024;             // of 16 bytes a lane that a unit's four fragments are
+    static constexpr int kFragmentsOf = 4 / kPieces;         // fragments in a piece
 };
 
 // Eight weights of 8 bits as float16.  0x6400 + b is the float16 1024 + b for a byte b; with the sign bit flipped, b is w + 128,
@@ -42,7 +44,7 @@ __device__ __forceinline__ u32x4 halves_of_bytes(uint32_t lo, uint32_t hi) {
     return r;
 }
 
-// One fragment of w (for int8 its part `s`) times one of x.
+// One fragment of w times one of x.
 template <LinearType kType>
 __device__ __forceinline__ f32x4 product(u32x4 w, u32x4 x, f32x4 acc) {
     if constexpr (kType == kFloatFloat) {
@@ -55,10 +57,11 @@ __device__ __forceinline__ f32x4 product(u32x4 w, u32x4 x, f32x4 acc) {
     }
 }
 
+// Fragment f of the pieces that hold it.
 template <LinearType kType>
-__device__ __forceinline__ u32x4 operand(u32x4 w, int s) {
-    if constexpr (kType == kHalfInt8) return halves_of_bytes(w[2 * s], w[2 * s + 1]);
-    return w;
+__device__ __forceinline__ u32x4 fragment_of(const u32x4* pieces, int f) {
+    if constexpr (kType == kHalfInt8) return halves_of_bytes(pieces[f / 2][2 * (f & 1)], pieces[f / 2][2 * (f & 1) + 1]);
+    else return pieces[f];
 }
 
 // 16 bytes of a row of x from element k on, zeros from K on (0 * inf would be NaN); any alignment, any distance between elements.
@@ -77,9 +80,9 @@ __device__ __forceinline__ u32x4 chunk_of(const char* row, int64_t col, int32_t 
     return v;
 }
 
-// gelu(v) = v Phi(v).  For float16 results Phi(-z) = exp(-z^2 / 2) P(t), t = 1 / (1 + 0.4 z), with P fitted by least squares to the relative
-// error over 0 <= z <= 9: 2.6e-6, where rounding the result to float16 takes 4.9e-4.  Some 15 instructions; the library's erff takes three
-// times as many, which a work-group that has its compute unit for itself hides under nothing.
+// gelu(v) = v Phi(v) = max(v, 0) - z Phi(-z), z = |v|.  For float16 results Phi(-z) = exp(-z^2 / 2) P(t), t = 1 / (1 + 0.4 z), with P fitted by least
+// squares to the relative error over 0 <= z <= 9: 2.6e-6, where rounding the result to float16 takes 4.9e-4.  Some 15 instructions; the
+// library's erff takes three times as many.
 __device__ __forceinline__ float gelu_short(float v) {
     const float z = __builtin_fabsf(v);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f, z, 1.0f));
@@ -90,47 +93,44 @@ __device__ __forceinline__ float gelu_short(float v) {
     p = __builtin_fmaf(p, t, 1.9333978946e-01f);
     p = __builtin_fmaf(p, t, 1.5472590493e-01f);
     p = __builtin_fmaf(p, t, 2.8555855905e-04f);
-    const float tail = p * __builtin_amdgcn_exp2f(-0.72134752f * z * z);  // Phi(-z)
-    return v * (v > 0.f ? 1.f - tail : tail);
+    const float tail = p * __builtin_amdgcn_exp2f(-0.72134752f * z * z);  // Phi(-z); a NaN stays one
+    return __builtin_fmaf(-fminf(z, 64.f), tail, fmaxf(v, 0.f));           // (infinite z: 0 of it)
 }
 
-template <LinearType kType>
-__device__ __forceinline__ float activated(float v, int32_t act) {
+template <LinearType kType, int kCount>
+__device__ __forceinline__ void activate(float (&v)[kCount], int32_t act) {
+    constexpr bool kFloat = Of<kType>::kFloat;
     switch (act) {
-        case CHX_HIP_ACT_RELU: return v < 0.f ? 0.f : v;  // (a NaN stays)
+        case CHX_HIP_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // (a NaN stays)
+            break;
         case CHX_HIP_ACT_GELU:
-            if constexpr (kType == kFloatFloat) return 0.5f * v * erfcf(-0.70710678f * v);
-            else return gelu_short(v);
-        case CHX_HIP_ACT_GELU_TANH: {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) v[i] = kFloat ? 0.5f * v[i] * erfcf(-0.70710678f * v[i]) : gelu_short(v[i]);
+            break;
+        case CHX_HIP_ACT_GELU_TANH:
             // 0.5 v (1 + tanh u) = v / (1 + exp(-2 u))
-            const float u = 0.7978845608f * __builtin_fmaf(0.044715f * v * v, v, v);
-            if constexpr (kType == kFloatFloat) return v / (1.f + expf(-2.f * u));
-            else return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.8853901f * u));
-        }
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) {
+                const float u = 0.7978845608f * __builtin_fmaf(0.044715f * v[i] * v[i], v[i], v[i]);
+                v[i] = kFloat ? v[i] / (1.f + expf(-2.f * u)) : v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.8853901f * u));
+            }
+            break;
         case CHX_HIP_ACT_SILU:
-            if constexpr (kType == kFloatFloat) return v / (1.f + expf(-v));
-            else return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950f * v));
-        default: return v;
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) v[i] = kFloat ? v[i] / (1.f + expf(-v[i])) : v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950f * v[i]));
+            break;
+        default: break;
     }
 }
 
 // kCount neighbouring columns (a multiple of 4, from a multiple of 4 on) of one row of the result.
 template <LinearType kType, int kCount>
-__device__ __forceinline__ void finish(const LinearArgs& a, float* v, int64_t row, int32_t n, const float* scale, const float* bias) {
+__device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[kCount], int64_t row, int32_t n) {
     if (n >= a.N) return;
     const bool whole = n + kCount <= a.N;
-    if (scale) {
-#pragma unroll
-        for (int i = 0; i < kCount; ++i) v[i] *= scale[i];
-    }
-    if (bias) {
-#pragma unroll
-        for (int i = 0; i < kCount; ++i) v[i] += bias[i];
-    }
-    if (a.activation != CHX_HIP_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < kCount; ++i) v[i] = activated<kType>(v[i], a.activation);
-    }
+    activate<kType, kCount>(v, a.activation);
     if (a.r) {
         const char* p = a.r + row * a.r_row + (int64_t)n * a.r_col;
         if (whole && a.vector_r) {
@@ -225,7 +225,8 @@ __device__ __forceinline__ int32_t row_at(const LinearArgs& a, const Rows& t, in
 template <LinearType kType, int kRowTiles, int kFragments, int kWaves, bool kDirect, bool kExperts>
 __global__ __launch_bounds__(64 * kWaves) void linear_rows_kernel(LinearArgs a) {
     using O = Of<kType>;
-    constexpr int kDeep = kRowTiles * kFragments >= 8 ? 2 : 4;
+    static_assert(kFragments % O::kFragmentsOf == 0, "whole pieces");
+    constexpr int kDeep = kRowTiles * kFragments >= 8 ? 2 : 4, kPieces = kFragments / O::kFragmentsOf;
     extern __shared__ f32x4 rows_sums[];  // [wave][row tile][fragment][lane]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t columns = blockIdx.x % a.tiles_n, tile = blockIdx.x / a.tiles_n;
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_rows_kernel(LinearArgs a) 
         t = {0, tile * 16 * kRowTiles, min(a.M - tile * 16 * kRowTiles, 16 * kRowTiles)};
     }
     const int32_t fragment = columns * kFragments;  // of all: 4 to a group
-    const char* w = a.w + t.expert * a.w_expert + (int64_t)(fragment >> 2) * a.w_group + (fragment & 3) * kFragment + lane * 16;
+    const char* w = a.w + t.expert * a.w_expert + (int64_t)(fragment >> 2) * a.w_group + (fragment & 3) / O::kFragmentsOf * 1024 + lane * 16;
     const char* x[kRowTiles];
 #pragma unroll
     for (int i = 0; i < kRowTiles; ++i) {
@@ -252,30 +253,26 @@ __global__ __launch_bounds__(64 * kWaves) void linear_rows_kernel(LinearArgs a) 
         for (int f = 0; f < kFragments; ++f) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     struct Unit {
-        u32x4 w[kFragments];
-        u32x4 x[kRowTiles][O::kSteps];
+        u32x4 w[kPieces];
+        u32x4 x[kRowTiles];
     };
     auto load = [&](Unit& u, int32_t unit) {
 #pragma unroll
-        for (int f = 0; f < kFragments; ++f) u.w[f] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w + (int64_t)unit * kUnit + f * kFragment));
+        for (int p = 0; p < kPieces; ++p) u.w[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w + (int64_t)unit * O::kUnit + p * 1024));
+        const int32_t k = unit * O::kUnitK + chunk;
 #pragma unroll
-        for (int i = 0; i < kRowTiles; ++i)
-#pragma unroll
-            for (int s = 0; s < O::kSteps; ++s) {
-                const int32_t k = (unit * O::kSteps + s) * 4 * O::kChunk + chunk;
-                if constexpr (kDirect) u.x[i][s] = *reinterpret_cast<const u32x4*>(x[i] + (int64_t)k * O::kElement);
-                else u.x[i][s] = chunk_of<kType>(x[i], a.x_col, k, a.K);
-            }
+        for (int i = 0; i < kRowTiles; ++i) {
+            if constexpr (kDirect) u.x[i] = *reinterpret_cast<const u32x4*>(x[i] + (int64_t)k * O::kElement);
+            else u.x[i] = chunk_of<kType>(x[i], a.x_col, k, a.K);
+        }
     };
     auto multiply = [&](const Unit& u) {
 #pragma unroll
-        for (int s = 0; s < O::kSteps; ++s)
+        for (int f = 0; f < kFragments; ++f) {
+            const u32x4 o = fragment_of<kType>(u.w, f);
 #pragma unroll
-            for (int f = 0; f < kFragments; ++f) {
-                const u32x4 o = operand<kType>(u.w[f], s);
-#pragma unroll
-                for (int i = 0; i < kRowTiles; ++i) acc[i][f] = product<kType>(o, u.x[i][s], acc[i][f]);
-            }
+            for (int i = 0; i < kRowTiles; ++i) acc[i][f] = product<kType>(o, u.x[i], acc[i][f]);
+        }
     };
     Unit ring[kDeep];
     const int32_t mine = a.units > wave ? (a.units - wave + kWaves - 1) / kWaves : 0;
@@ -304,27 +301,44 @@ __global__ __launch_bounds__(64 * kWaves) void linear_rows_kernel(LinearArgs a) 
         if (row < 0) continue;
         float v[4] = {sum[0], sum[1], sum[2], sum[3]};
         const int64_t at_n = (int64_t)t.expert * a.n_padded + n;
-        finish<kType, 4>(a, v, row, n, kType == kHalfInt8 ? a.scale + at_n : nullptr, a.bias ? a.bias + at_n : nullptr);
+        // (scales and biases are filled up to whole groups)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (kType == kHalfInt8) v[j] *= a.scale[at_n + j];
+            if (a.bias) v[j] += a.bias[at_n + j];
+        }
+        finish<kType, 4>(a, v, row, n);
     }
 }
 
 // ---- tiles -------------------------------------------------------------------------------------------
 //
-// Both operands of a step (128 bytes of every row) are brought into LDS while the step before it is multiplied.  A row of x is eight pieces of
-// 16 bytes; piece c of row r lies at place c ^ (r & 7), so that the sixteen rows that a fragment is read from do not meet in one bank.
+// A work-group of kWavesM x kWavesN wavefronts, each 16 kRowFragments rows and 64 columns.  w comes into a ring of three units in LDS, x into one of
+// three blocks of two units (a block is 128 bytes of every row: of half a line at a time, the other half was fetched again where the
+// rows lie a power of two apart: 435 us instead of 419 for 4096 x 4096 x 16384), by asynchronous copies two and three units ahead.  While a unit
+// is multiplied from registers, the next one's fragments come from LDS into others, so its place in the ring is free a unit early.
+// A row of x in a block is eight pieces of 16 bytes; piece c of row r lies at place c ^ (r & 7): the sixteen rows that a fragment is
+// read from then do not meet in one bank.
 __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 
+template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN>
+struct TileShape {
+    static constexpr int kThreads = 64 * kWavesM * kWavesN, kRows = kWavesM * kRowFragments * 16, kGroups = kWavesN, kRing = 3;
+    static constexpr int kBlock = kRows * 128, kUnits = kGroups * unit_bytes(kType);  // bytes of x, of w
+    static constexpr int kCopiesX = kBlock / 16 / kThreads, kCopiesW = kUnits / 16 / kThreads;
+    static constexpr int kAtW = kRing * kBlock, kAtRows = kAtW + kRing * kUnits, kLds = kAtRows + kRows * 4;
+    static_assert(kBlock % (32 * kThreads) == 0 && kUnits % (16 * kThreads) == 0, "whole copies");
+};
+
 template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN, bool kDirect, bool kExperts>
-__global__ __launch_bounds__(64 * kWavesM * kWavesN) void linear_tile_kernel(LinearArgs a) {
+__global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(LinearArgs a) {
     using O = Of<kType>;
-    constexpr int kThreads = 64 * kWavesM * kWavesN;
-    constexpr int kBM = kWavesM * kRowFragments * 16, kGroups = kWavesN;
-    constexpr int kBytesX = kBM * 128, kBytesW = kGroups * O::kUnits * kUnit, kStage = kBytesX + kBytesW;
-    constexpr int kCopiesX = kBytesX / 16 / kThreads, kCopiesW = kBytesW / 16 / kThreads;
+    using S = TileShape<kType, kRowFragments, kWavesM, kWavesN>;
+    constexpr int kThreads = S::kThreads, kBM = S::kRows, kGroups = S::kGroups, kCopiesX = S::kCopiesX, kCopiesW = S::kCopiesW;
     extern __shared__ __attribute__((aligned(128))) char tile_lds[];
-    int32_t* rows = reinterpret_cast<int32_t*>(tile_lds + 2 * kStage);  // of the result
+    int32_t* rows = reinterpret_cast<int32_t*>(tile_lds + S::kAtRows);  // of the result
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / kWavesN, wn = wave % kWavesN;
     // Work-groups that follow each other run on different XCDs, each with its own L2: an eighth of the tiles to each, in blocks
@@ -347,53 +361,49 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void linear_tile_kernel(Lin
     }
     for (int i = threadIdx.x; i < kBM; i += kThreads) rows[i] = row_at<kExperts>(a, t, i);
 
-    // x: this thread's pieces of a step
-    uint32_t x_at[kCopiesX];
-    const char* x_row[kCopiesX];
-    int32_t x_chunk[kCopiesX];
+    // x: this thread's pieces of a block, as offsets from the tile's first row (experts: from x); the same piece of every row
     const char* x_base = a.x + (kExperts ? 0 : (int64_t)t.first * a.x_row);
+    const int32_t x_chunk = (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7);
+    auto row_of = [&](int i) __attribute__((always_inline)) -> int64_t {
+        const int32_t row = max(row_at<kExperts>(a, t, min((i * kThreads + (int)threadIdx.x) >> 3, t.count - 1)), 0);
+        return kExperts ? (int64_t)(row / a.fan) * a.x_row : (int64_t)(row - t.first) * a.x_row;
+    };
+    typedef typename std::conditional<kDirect, uint32_t, int64_t>::type Offset;
+    Offset x_at[kCopiesX];
 #pragma unroll
-    for (int i = 0; i < kCopiesX; ++i) {
-        const int slot = i * kThreads + threadIdx.x, r = slot >> 3;
-        const int32_t row = max(row_at<kExperts>(a, t, min(r, t.count - 1)), 0);
-        const int64_t off = kExperts ? (int64_t)(row / a.fan) * a.x_row : (int64_t)(row - t.first) * a.x_row;
-        x_chunk[i] = (slot & 7) ^ (r & 7);
-        x_row[i] = x_base + off;
-        x_at[i] = (uint32_t)off + x_chunk[i] * 16;
-    }
-    // w: whole units, in the order in which they lie
-    uint32_t w_at[kCopiesW];
+    for (int i = 0; i < kCopiesX; ++i) x_at[i] = (Offset)row_of(i) + (kDirect ? x_chunk * 16 : 0);
+    // w: a unit of one group after the other, in the order in which it lies
     const char* w_base = a.w + t.expert * a.w_expert + (int64_t)tn * kGroups * a.w_group;
     const int32_t last_group = (a.N + kGroupRows - 1) / kGroupRows - 1 - tn * kGroups;
+    uint32_t w_at[kCopiesW];
 #pragma unroll
     for (int i = 0; i < kCopiesW; ++i) {
-        const int at = (i * kThreads + threadIdx.x) * 16, g = at / (O::kUnits * kUnit);
-        w_at[i] = (uint32_t)(min(g, last_group) * a.w_group) + at % (O::kUnits * kUnit);
+        const int at = (i * kThreads + threadIdx.x) * 16, g = at / O::kUnit;
+        w_at[i] = (uint32_t)(min(g, last_group) * a.w_group) + at % O::kUnit;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile_lds + wave * 1024;
-    const int32_t steps = (a.K + O::kStep - 1) / O::kStep;
 
+    constexpr int kBlockK = 2 * O::kUnitK;
     u32x4 staged[kCopiesX];
-    auto is_direct = [&](int32_t step) { return kDirect && (step + 1) * O::kStep <= a.K; };
-    auto copy = [&](int32_t step, int buffer) {
-        const uint32_t lds = lds0 + buffer * kStage;
-        if (is_direct(step)) {
-            const char* base = x_base + (int64_t)step * 128;
+    auto load_pieces = [&](int32_t block) __attribute__((always_inline)) {
+        if (a.x_col == O::kElement && (block + 1) * kBlockK <= a.K) {
 #pragma unroll
-            for (int i = 0; i < kCopiesX; ++i) copy_to_lds(x_at[i], base, lds + i * kThreads * 16);
+            for (int i = 0; i < kCopiesX; ++i)
+                staged[i] = *reinterpret_cast<const u32x4_any*>(x_base + x_at[i] + (int64_t)block * 128 + (kDirect ? 0 : x_chunk * 16));
         } else {
 #pragma unroll
-            for (int i = 0; i < kCopiesX; ++i) staged[i] = chunk_of<kType>(x_row[i], a.x_col, step * O::kStep + x_chunk[i] * O::kChunk, a.K);
+            for (int i = 0; i < kCopiesX; ++i) staged[i] = chunk_of<kType>(x_base + x_at[i] - (kDirect ? x_chunk * 16 : 0), a.x_col, block * kBlockK + x_chunk * O::kChunk, a.K);
         }
-        const char* base = w_base + (int64_t)step * (O::kUnits * kUnit);
-#pragma unroll
-        for (int i = 0; i < kCopiesW; ++i) copy_to_lds(w_at[i], base, lds + kBytesX + i * kThreads * 16);
     };
-    auto settle = [&](int32_t step, int buffer) {
-        if (!is_direct(step)) {
+    auto store_pieces = [&](int place) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < kCopiesX; ++i) *reinterpret_cast<u32x4*>(tile_lds + buffer * kStage + (i * kThreads + threadIdx.x) * 16) = staged[i];
-        }
+        for (int i = 0; i < kCopiesX; ++i) *reinterpret_cast<u32x4*>(tile_lds + place * S::kBlock + (i * kThreads + threadIdx.x) * 16) = staged[i];
+    };
+    auto copy_w = [&](int c, int32_t unit, int place) __attribute__((always_inline)) {
+        copy_to_lds(w_at[c], w_base + (int64_t)unit * O::kUnit, lds0 + S::kAtW + place * S::kUnits + c * kThreads * 16);
+    };
+    auto copy_x = [&](int c, int32_t block, int place) __attribute__((always_inline)) {
+        copy_to_lds((uint32_t)x_at[c], x_base + (int64_t)block * 128, lds0 + place * S::kBlock + c * kThreads * 16);
     };
 
     f32x4 acc[kRowFragments][4];
@@ -401,60 +411,161 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void linear_tile_kernel(Lin
     for (int i = 0; i < kRowFragments; ++i)
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int x_lane = (wm * kRowFragments * 16 + (lane & 15)) * 128, x_swizzle = lane & 7, x_quarter = lane >> 4;
-    const int w_lane = kBytesX + wn * O::kUnits * kUnit + lane * 16;
+    const int x_lane = (wm * kRowFragments * 16 + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+    const int w_lane = S::kAtW + wn * O::kUnit + lane * 16;
+    struct Unit {
+        u32x4 w[O::kPieces], x[kRowFragments];
+    };
+    // (half: which of its block's two units)
+    auto read_w = [&](Unit& r, int p, int place) __attribute__((always_inline)) { r.w[p] = *reinterpret_cast<const u32x4*>(tile_lds + place * S::kUnits + w_lane + p * 1024); };
+    auto read_x = [&](Unit& r, int i, int place, int half) __attribute__((always_inline)) {
+        r.x[i] = *reinterpret_cast<const u32x4*>(tile_lds + place * S::kBlock + (x_lane ^ (half * 64)) + i * 2048);
+    };
+    auto read_unit = [&](Unit& r, int place_x, int half, int place_w) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < O::kPieces; ++p) read_w(r, p, place_w);
+#pragma unroll
+        for (int i = 0; i < kRowFragments; ++i) read_x(r, i, place_x, half);
+    };
+    auto multiply = [&](const u32x4 (&w)[4], const Unit& r, int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[i][f] = product<kType>(w[f], r.x[i], acc[i][f]);
+    };
+    auto fragments_of = [&](u32x4 (&w)[4], const Unit& r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) w[f] = fragment_of<kType>(r.w, f);
+    };
+    Unit even, odd;
 
-    copy(0, 0);
-    settle(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int32_t step = 0; step < steps; ++step) {
-        const int now = step & 1;
-        if (step + 1 < steps) copy(step + 1, now ^ 1);
-        const char* at = tile_lds + now * kStage;
+    // A last block of fewer k (one unit, or two) comes first, by itself.
+    const int32_t blocks = a.K / kBlockK, left = a.units - 2 * blocks;
+    if (left > 0) {
+        load_pieces(blocks);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            u32x4 w[4];
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                if constexpr (kType == kHalfInt8) w[f] = operand<kType>(*reinterpret_cast<const u32x4*>(at + w_lane + f * kFragment), half);
-                else w[f] = *reinterpret_cast<const u32x4*>(at + w_lane + half * kUnit + f * kFragment);
-            }
-#pragma unroll
-            for (int i = 0; i < kRowFragments; ++i) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(at + x_lane + i * 16 * 128 + (((half * 4 + x_quarter) ^ x_swizzle) << 4));
-#pragma unroll
-                for (int f = 0; f < 4; ++f) acc[i][f] = product<kType>(w[f], x, acc[i][f]);
-            }
+        for (int c = 0; c < kCopiesW; ++c) {
+            copy_w(c, 2 * blocks, 0);
+            copy_w(c, a.units - 1, 1);
         }
-        if (step + 1 < steps) settle(step + 1, now ^ 1);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        store_pieces(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        for (int h = 0; h < left; ++h) {
+            read_unit(even, 0, h, h);
+            u32x4 w[4];
+            fragments_of(w, even);
+#pragma unroll
+            for (int i = 0; i < kRowFragments; ++i) multiply(w, even, i);
+        }
         __syncthreads();
     }
-
-    const int32_t n = (tn * kGroups + wn) * kGroupRows + (lane >> 4) * 16;
-    const int64_t at_n = (int64_t)t.expert * a.n_padded + n;
-    float scale[16], bias[16];
-    if (n < a.N) {  // (both are filled up to whole groups)
-        if constexpr (kType == kHalfInt8) {
+    if (blocks > 0) {
+        // (copies behind the last block bring it again, to a place that nobody reads any more: no step has a condition in it)
+        const int32_t last = blocks - 1;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) scale[i] = a.scale[at_n + i];
-        }
-        if (a.bias) {
+        for (int b = 0; b < S::kRing; ++b) {
+            if constexpr (kDirect) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) bias[i] = a.bias[at_n + i];
+                for (int c = 0; c < kCopiesX; ++c) copy_x(c, min(b, last), b);
+            } else {
+                load_pieces(min(b, last));
+                if (b + 1 < S::kRing) store_pieces(b);  // (the last one's are stored in the loop)
+            }
+#pragma unroll
+            for (int c = 0; c < kCopiesW; ++c) copy_w(c, min(b, 2 * blocks - 1), b);
         }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        read_unit(even, 0, 0, 0);
+        int here_x = 0, here_w = 0;  // places in the rings of this block and unit
+        auto behind = [](int place) __attribute__((always_inline)) { return place + 1 == S::kRing ? 0 : place + 1; };
+        // One unit, the block's first or second, from `now`, with the next one's fragments into `then`.
+        auto step = [&](int32_t block, auto second, const Unit& now, Unit& then) __attribute__((always_inline)) {
+            constexpr bool kSecond = decltype(second)::value;
+            const int next_x = behind(here_x), next_w = behind(here_w), before_x = behind(next_x);
+            // The copies that the next unit needs are there, of w from two steps ago, of x from three or more; and this wavefront has read this unit.
+            if constexpr (kDirect) {
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kCopiesX + kCopiesW) : "memory");
+            } else if constexpr (kSecond) {
+                store_pieces(before_x);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kCopiesX + kCopiesW) : "memory");
+            }
+            __builtin_amdgcn_s_barrier();
+            // ahead: half of the block three behind this one, in its place when both its units are read; else the other half of the one before
+            const int32_t ahead = min(block + (kSecond ? 3 : 2), last), ahead_w = min(2 * block + (kSecond ? 1 : 0) + 3, 2 * blocks - 1);
+            if constexpr (!kDirect && kSecond) load_pieces(ahead);
+            // What is read for the next unit and copied ahead goes between the products: copies one behind the other would keep the
+            // wavefront from its products until the last of them is under way.
+            u32x4 w[4];
+            fragments_of(w, now);
+            constexpr int kHalf = kDirect ? kCopiesX / 2 : 0, kCopies = kCopiesW + kHalf;
+#pragma unroll
+            for (int i = 0; i < kRowFragments; ++i) {
+                if (i < O::kPieces) read_w(then, i, next_w);
+                read_x(then, i, kSecond ? next_x : here_x, kSecond ? 0 : 1);
+#pragma unroll
+                for (int c = i * kCopies / kRowFragments; c < (i + 1) * kCopies / kRowFragments; ++c) {
+                    if (c < kCopiesW) copy_w(c, ahead_w, here_w);
+                    else copy_x(c - kCopiesW + (kSecond ? 0 : kHalf), ahead, kSecond ? here_x : before_x);
+                }
+                multiply(w, now, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            here_w = next_w;
+            if constexpr (kSecond) here_x = next_x;
+        };
+        for (int32_t block = 0; block < blocks; ++block) {
+            step(block, std::false_type(), even, odd);
+            step(block, std::true_type(), odd, even);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+
+    // The results go through LDS, 32 rows of a wavefront at a time, so that the epilogue is a loop over eight columns of a lane: written out over the
+    // accumulators it is 60 KB of code, which each tile fetched anew (a tenth of the time).  Piece c of 16 bytes of a row lies at place c ^ (row & 15).
+    __syncthreads();
+    constexpr int kPassRows = 32;
+    static_assert(kWavesM * kWavesN * kPassRows * 256 <= S::kAtRows, "the rings hold them");
+    char* mine = tile_lds + wave * kPassRows * 256;
+    const int32_t n = (tn * kGroups + wn) * kGroupRows + (lane & 7) * 8;
+    const int64_t at_n = (int64_t)t.expert * a.n_padded + (n < a.n_padded ? n : 0);
+    // (scales and biases are filled up to whole groups)
+    float scale[8], bias[8];
 #pragma unroll
-    for (int i = 0; i < kRowFragments; ++i) {
-        const int32_t row = rows[(wm * kRowFragments + i) * 16 + (lane & 15)];
-        if (row < 0) continue;
-        float v[16];
+    for (int j = 0; j < 8; ++j) {
+        scale[j] = kType == kHalfInt8 ? a.scale[at_n + j] : 1.f;
+        bias[j] = a.bias ? a.bias[at_n + j] : 0.f;
+    }
+#pragma unroll 1
+    for (int pass = 0; pass < kRowFragments / 2; ++pass) {
 #pragma unroll
-        for (int f = 0; f < 4; ++f)
+        for (int i0 = 0; i0 < kRowFragments; i0 += 2) {
+            if (pass != i0 / 2) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[f * 4 + j] = acc[i][f][j];
-        finish<kType, 16>(a, v, row, n, kType == kHalfInt8 ? scale : nullptr, a.bias ? bias : nullptr);
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+                    *reinterpret_cast<f32x4*>(mine + (i * 16 + (lane & 15)) * 256 + ((((lane >> 4) * 4 + f) ^ (lane & 15)) << 4)) = acc[i0 + i][f];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+        for (int i = 0; i < kPassRows / 8; ++i) {
+            const int r = i * 8 + (lane >> 3), row = rows[(wm * kRowFragments + pass * 2) * 16 + r];
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((lane & 7) * 2 ^ (r & 15)) << 4));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((lane & 7) * 2 + 1) ^ (r & 15)) * 16);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = j < 4 ? lo[j & 3] : hi[j & 3];
+                if constexpr (kType == kHalfInt8) v[j] *= scale[j];
+                v[j] += bias[j];
+            }
+            if (row >= 0) finish<kType, 8>(a, v, row, n);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -470,12 +581,11 @@ int launch_rows(const LinearArgs& a, hipStream_t s) {
 
 template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN, bool kDirect, bool kExperts>
 int launch_tile(const LinearArgs& a, hipStream_t s) {
-    constexpr int kBM = kWavesM * kRowFragments * 16;
-    constexpr int kLds = 2 * (kBM * 128 + kWavesN * Of<kType>::kUnits * kUnit) + kBM * 4;
+    using S = TileShape<kType, kRowFragments, kWavesM, kWavesN>;
     auto kernel = linear_tile_kernel<kType, kRowFragments, kWavesM, kWavesN, kDirect, kExperts>;
-    if constexpr (kLds > 65536)  // (has to be asked for, on every device)
-        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-    kernel<<<(unsigned)(a.tiles_m * a.tiles_n), 64 * kWavesM * kWavesN, kLds, s>>>(a);
+    if constexpr (S::kLds > 65536)  // (has to be asked for, on every device)
+        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
+    kernel<<<(unsigned)(a.tiles_m * a.tiles_n), S::kThreads, S::kLds, s>>>(a);
     return launch_check("linear_tile_kernel");
 }
 
@@ -496,14 +606,18 @@ int tile_of(const LinearArgs& a, bool direct, hipStream_t s) {
 
 template <LinearType kType>
 int LinearKernels<kType>::rows(const LinearArgs& a, int row_tiles, int fragments, bool direct, hipStream_t s) {
+    if constexpr (kType != kHalfInt8) {  // (two of its fragments are one piece)
+        if (fragments == 1) {
+            if (row_tiles == 1) return rows_of<kType, 1, 1>(a, direct, s);
+            if (row_tiles == 2) return rows_of<kType, 2, 1>(a, direct, s);
+            return rows_of<kType, 4, 1>(a, direct, s);
+        }
+    }
     switch (row_tiles * 8 + fragments) {
-        case 8 + 1: return rows_of<kType, 1, 1>(a, direct, s);
         case 8 + 2: return rows_of<kType, 1, 2>(a, direct, s);
         case 8 + 4: return rows_of<kType, 1, 4>(a, direct, s);
-        case 16 + 1: return rows_of<kType, 2, 1>(a, direct, s);
         case 16 + 2: return rows_of<kType, 2, 2>(a, direct, s);
         case 16 + 4: return rows_of<kType, 2, 4>(a, direct, s);
-        case 32 + 1: return rows_of<kType, 4, 1>(a, direct, s);
         case 32 + 2: return rows_of<kType, 4, 2>(a, direct, s);
         default: return rows_of<kType, 4, 4>(a, direct, s);
     }

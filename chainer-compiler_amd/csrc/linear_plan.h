@@ -7,14 +7,21 @@ namespace chx {
 
 enum LinearType { kHalfHalf = 0, kHalfInt8 = 1, kFloatFloat = 2 };  // x and w
 
-// Weights [N, K] are laid out in groups of 64 rows, along k in units of 64 bytes of a row, a unit as four fragments of 1 KB: the operand of
-// one matrix instruction (16 rows, a lane's 16 bytes together; two instructions' for int8, four for float32).
-//   float16  32 k a unit: lane l holds k = 8 (l / 16) + j
-//   int8     64 k a unit: bytes 8 s + j of lane l hold k = 32 s + 8 (l / 16) + j, so that x is read as for float16
+// Weights [N, K] are laid out in groups of 64 rows, along k in units that belong to 64 bytes of a row of x, a unit as four fragments: the
+// operand of one matrix instruction (16 rows; four instructions' for float32), a lane's bytes together.
+//   float16  32 k a unit: 16 bytes of lane l hold k = 8 (l / 16) + j;  a fragment is 1 KB
 //   float32  16 k a unit: k = 4 (l / 16) + j; instruction j of the unit takes the k that are j modulo 4
+//   int8     32 k a unit, as for float16 with 8 bytes; those of fragments 2 p and 2 p + 1 are next to each other, 16 bytes of a lane
 // Row r of fragment f is row 16 (r / 4) + 4 f + r % 4 of the group: a lane of the result then holds 16 neighbouring columns, 32 bytes of
-// float16, and four lanes a whole line.  K is filled up with zeros to whole steps (128 bytes of x), N to whole groups.
-constexpr int kGroupRows = 64, kFragment = 1024, kUnit = 4 * kFragment;
+// float16, and four lanes a whole line.  K is filled up with zeros to whole units, N to whole groups.
+constexpr int kGroupRows = 64;
+
+__host__ __device__ constexpr int unit_bytes(LinearType t) {
+    return t == kHalfInt8 ? 2048 : 4096;
+}
+__host__ __device__ constexpr int unit_k(LinearType t) {
+    return t == kFloatFloat ? 16 : 32;
+}
 
 __host__ __device__ inline int group_row(int fragment, int r) {
     return 16 * (r >> 2) + 4 * fragment + (r & 3);

@@ -24,37 +24,35 @@ struct LayoutArgs {
     int64_t ws_e, ws_n, ws_k;  // bytes
     char* out;
     int32_t N, K, units, groups, type;
-    int64_t fragments;  // of all
+    int64_t w_group;
+    int64_t kilobytes;  // of all
 };
 
-// One lane writes 16 bytes, a wavefront a fragment.  Runs once per layer; w is read through its strides.
+// One lane writes 16 bytes, a wavefront 1 KB: a fragment, or two of int8.  Runs once per layer; w is read through its strides.
 __global__ __launch_bounds__(256) void linear_layout_kernel(LayoutArgs a) {
     const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= a.fragments) return;
-    const int lane = threadIdx.x & 63, fragment = (int)(at & 3);
-    const int64_t unit = (at >> 2) % a.units, group = (at >> 2) / a.units % a.groups, expert = (at >> 2) / a.units / a.groups;
-    const int64_t n = group * kGroupRows + group_row(fragment, lane & 15);
-    const char* row = a.w + expert * a.ws_e + n * a.ws_n;
+    if (at >= a.kilobytes) return;
+    const int lane = threadIdx.x & 63, each = a.type == kHalfInt8 ? 2 : 4;
+    const int part = (int)(at % each);
+    const int64_t unit = at / each % a.units, group = at / each / a.units % a.groups, expert = at / each / a.units / a.groups;
+    const char* first = a.w + expert * a.ws_e + group * kGroupRows * a.ws_n;
     uint32_t v[4] = {0, 0, 0, 0};
-    if (n < a.N) {
-        if (a.type == kHalfHalf) {
-            for (int j = 0; j < 8; ++j) {
-                const int64_t k = unit * 32 + (lane >> 4) * 8 + j;
-                if (k < a.K) v[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + k * a.ws_k) << (16 * (j & 1));
-            }
-        } else if (a.type == kHalfInt8) {
-            for (int j = 0; j < 16; ++j) {
-                const int64_t k = unit * 64 + (j >> 3) * 32 + (lane >> 4) * 8 + (j & 7);
-                if (k < a.K) v[j / 4] |= (uint32_t)*reinterpret_cast<const uint8_t*>(row + k * a.ws_k) << (8 * (j & 3));
-            }
-        } else {
-            for (int j = 0; j < 4; ++j) {
-                const int64_t k = unit * 16 + (lane >> 4) * 4 + j;
-                if (k < a.K) v[j] = *reinterpret_cast<const uint32_t*>(row + k * a.ws_k);
-            }
-        }
+    const int64_t k0 = unit * (a.type == kFloatFloat ? 16 : 32) + (lane >> 4) * (a.type == kFloatFloat ? 4 : 8);
+    auto element = [&](int fragment, int j) -> const char* {
+        const int r = group_row(fragment, lane & 15);
+        return group * kGroupRows + r < a.N && k0 + j < a.K ? first + r * a.ws_n + (k0 + j) * a.ws_k : nullptr;
+    };
+    if (a.type == kHalfHalf) {
+        for (int j = 0; j < 8; ++j)
+            if (const char* p = element(part, j)) v[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(p) << (16 * (j & 1));
+    } else if (a.type == kHalfInt8) {
+        for (int j = 0; j < 16; ++j)
+            if (const char* p = element(2 * part + (j >> 3), j & 7)) v[j / 4] |= (uint32_t)*reinterpret_cast<const uint8_t*>(p) << (8 * (j & 3));
+    } else {
+        for (int j = 0; j < 4; ++j)
+            if (const char* p = element(part, j)) v[j] = *reinterpret_cast<const uint32_t*>(p);
     }
-    *reinterpret_cast<uint4*>(a.out + at * kFragment + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<uint4*>(a.out + (expert * a.groups + group) * a.w_group + (unit * each + part) * 1024 + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 struct VectorArgs {
@@ -182,10 +180,10 @@ int launch(LinearArgs& a, bool direct, hipStream_t s) {
         const int row_tiles = rows_each <= 16 ? 1 : rows_each <= 32 ? 2 : 4;
         a.tiles_m = tiles(16 * row_tiles);
         const int64_t wide = (int64_t)a.tiles_m * groups;
-        const int fragments = wide >= 512 ? 4 : wide >= 256 ? 2 : 1;
+        const int fragments = wide >= 512 ? 4 : wide >= 256 || kType == kHalfInt8 ? 2 : 1;
         a.tiles_n = groups * (4 / fragments);
         CHX_REQUIRE((int64_t)a.tiles_m * a.tiles_n < (int64_t(1) << 31), "linear plan: too many results");
-        const bool whole = direct && a.K % (kType == kFloatFloat ? 32 : 64) == 0;
+        const bool whole = direct && a.K % unit_k(kType) == 0;
         return LinearKernels<kType>::rows(a, row_tiles, fragments, whole, s);
     }
     const int64_t large = (int64_t)tiles(256) * ((a.N + 255) / 256);
@@ -234,14 +232,13 @@ extern "C" int chx_hip_linear_plan_create(
     if (b) CHX_PROPAGATE(check_vector(b, "b"));
     chx_hip_linear_plan p;
     p.type = w->dtype == CHX_HIP_FLOAT16 ? kHalfHalf : w->dtype == CHX_HIP_INT8 ? kHalfInt8 : kFloatFloat;
-    const int64_t step = p.type == kFloatFloat ? 32 : 64, units_of_step = p.type == kHalfInt8 ? 1 : 2;
     const int64_t groups = (N + kGroupRows - 1) / kGroupRows;
-    p.units = (int32_t)((K + step - 1) / step * units_of_step);
+    p.units = (int32_t)((K + unit_k(p.type) - 1) / unit_k(p.type));
     p.N = (int32_t)N;
     p.K = (int32_t)K;
     p.experts = lead ? (int32_t)E : 0;
     p.n_padded = (int32_t)(groups * kGroupRows);
-    p.w_group = (int64_t)p.units * kUnit;
+    p.w_group = (int64_t)p.units * unit_bytes(p.type);
     p.w_expert = groups * p.w_group;
     // (a tile's groups are addressed with 32 bits)
     CHX_REQUIRE(p.w_group < (int64_t(1) << 29), "linear plan: a row of w is too long");
@@ -252,9 +249,9 @@ extern "C" int chx_hip_linear_plan_create(
     p.w = static_cast<char*>(memory);
     char* next = p.w + E * p.w_expert;
     LayoutArgs l = {static_cast<const char*>(w->data), lead ? w->strides[0] : 0, w->strides[lead], w->strides[lead + 1], p.w, p.N, p.K, p.units,
-                    (int32_t)groups, (int32_t)p.type, E * groups * p.units * 4};
+                    (int32_t)groups, (int32_t)p.type, p.w_group, E * groups * p.units * unit_bytes(p.type) / 1024};
     int rc = CHX_HIP_OK;
-    const int64_t blocks = (l.fragments + 3) / 4;
+    const int64_t blocks = (l.kilobytes + 3) / 4;
     if (blocks >= (int64_t(1) << 31)) {
         set_error("linear plan: too many weights");
         rc = CHX_HIP_EINVAL;
