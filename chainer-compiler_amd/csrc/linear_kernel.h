@@ -179,31 +179,38 @@ struct Rows {
     int32_t expert, first, count;  // count 0: no such tile
 };
 
-// Tile `index` of the experts' tiles of `height` rows each, counted from expert 0 on.  Every wavefront finds it by itself, 64 experts at a time.
+// Tile `index` of the experts' tiles of `height` rows each.  kWholeFirst: first the whole ones of expert 0 on, then what is left of each expert's rows, so that
+// the shorter ones come last; else those of expert 0, of expert 1 and so on (one search instead of two, for tiles that take a few us).
+// Every wavefront finds it by itself, 64 experts at a time.
+template <bool kWholeFirst>
 __device__ __forceinline__ Rows expert_rows(const LinearArgs& a, int32_t index, int32_t height) {
     const int lane = threadIdx.x & 63;
-    for (int32_t e0 = 0; e0 < a.experts; e0 += 64) {
-        const int32_t e = e0 + lane;
-        int32_t lo = 0, hi = 0;
-        if (e < a.experts) {  // (offsets from device memory: kept inside the order whatever they say)
-            lo = min(max(a.offsets[e], 0), a.M);
-            hi = min(max(a.offsets[e + 1], lo), a.M);
-        }
-        const int32_t tiles = (hi - lo + height - 1) / height;
-        int32_t upto = tiles;
+#pragma unroll 1
+    for (int pass = 0; pass < (kWholeFirst ? 2 : 1); ++pass) {
+        for (int32_t e0 = 0; e0 < a.experts; e0 += 64) {
+            const int32_t e = e0 + lane;
+            int32_t lo = 0, hi = 0;
+            if (e < a.experts) {  // (offsets from device memory: kept inside the order whatever they say)
+                lo = min(max(a.offsets[e], 0), a.M);
+                hi = min(max(a.offsets[e + 1], lo), a.M);
+            }
+            const int32_t whole = (hi - lo) / height, more = (hi - lo) % height != 0;
+            const int32_t tiles = !kWholeFirst ? whole + more : pass == 0 ? whole : more;
+            int32_t upto = tiles;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int32_t v = __shfl_up(upto, d);
-            if (lane >= d) upto += v;
+            for (int d = 1; d < 64; d *= 2) {
+                const int32_t v = __shfl_up(upto, d);
+                if (lane >= d) upto += v;
+            }
+            const uint64_t past = __builtin_amdgcn_ballot_w64(upto > index);
+            if (past) {
+                const int at = __builtin_ctzll(past);
+                const int32_t first = __builtin_amdgcn_readlane(lo, at), count = __builtin_amdgcn_readlane(hi, at) - first;
+                const int32_t t = pass == 1 ? count / height : index - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(tiles, at));
+                return {e0 + at, first + t * height, min(count - t * height, height)};
+            }
+            index -= __builtin_amdgcn_readlane(upto, 63);
         }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > index);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            const int32_t first = __builtin_amdgcn_readlane(lo, at), end = __builtin_amdgcn_readlane(hi, at);
-            const int32_t t = index - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(tiles, at));
-            return {e0 + at, first + t * height, min(end - first - t * height, height)};
-        }
-        index -= __builtin_amdgcn_readlane(upto, 63);
     }
     return {0, 0, 0};
 }
@@ -217,85 +224,163 @@ __device__ __forceinline__ int32_t row_at(const LinearArgs& a, const Rows& t, in
     return p >= 0 && p < a.M ? p : -1;  // (from device memory)
 }
 
+// An asynchronous copy of 16 bytes a lane into LDS: lane i's to lds + 16 i (the same for all lanes), counted like a load.
+__device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
+}
+
 // ---- few rows ---------------------------------------------------------------------------------------
 //
 // Bound by the bytes of w, each read once.  A work-group takes kFragments fragments' columns (16 each) and all k, its kWaves wavefronts every
-// kWaves-th unit of k: fragments go from memory straight into registers, kDeep units ahead of the products, and the wavefronts' sums
-// are added in LDS, in one order.  x comes from the caches as fragments (rows that are not there repeat the last one; their results are dropped).
-template <LinearType kType, int kRowTiles, int kFragments, int kWaves, bool kDirect, bool kExperts>
-__global__ __launch_bounds__(64 * kWaves) void linear_rows_kernel(LinearArgs a) {
+// kWaves-th block of two units: w goes from memory straight into registers, kDeep blocks ahead of the products, and the wavefronts' sums
+// are added in LDS, in one order.  x comes from the caches.  Up to 16 rows are loaded as fragments; of more, a block (128 bytes of every row) is copied
+// into LDS of the wavefront's own, because lanes next to each other that load from different rows take a cache access each: 64 rows x 4096 x
+// 16384 36 us instead of 48.  Rows that are not there repeat the last one; their results are dropped.
+template <LinearType kType, int kRowTiles, int kFragments>
+struct RowsShape {
+    static constexpr int kWaves = 8, kPieces = kFragments / Of<kType>::kFragmentsOf;
+    static constexpr bool kInLds = kRowTiles > 1;       // x
+    static constexpr int kDeep = 2;
+    static constexpr int kBlock = kInLds ? kRowTiles * 2048 : 0;  // bytes of x in LDS
+    static constexpr int kOfBlocks = kWaves * kDeep * kBlock, kOfSums = kWaves * kRowTiles * kFragments * 1024;
+    static constexpr int kLds = kOfBlocks > kOfSums ? kOfBlocks : kOfSums;
+};
+
+// kStream: w is more than the caches are likely to hold from one call to the next, and goes by them (launch_rows).
+template <LinearType kType, int kRowTiles, int kFragments, bool kDirect, bool kExperts, bool kStream>
+__global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWaves)) void linear_rows_kernel(LinearArgs a) {
     using O = Of<kType>;
+    using S = RowsShape<kType, kRowTiles, kFragments>;
+    constexpr int kWaves = S::kWaves, kDeep = S::kDeep, kPieces = S::kPieces;
+    constexpr int kRows = S::kInLds ? 2 * kRowTiles : 1;  // that a lane has pieces of
+    constexpr bool kCopied = S::kInLds && kDirect;
     static_assert(kFragments % O::kFragmentsOf == 0, "whole pieces");
-    constexpr int kDeep = kRowTiles * kFragments >= 8 ? 2 : 4, kPieces = kFragments / O::kFragmentsOf;
-    extern __shared__ f32x4 rows_sums[];  // [wave][row tile][fragment][lane]
+    extern __shared__ __attribute__((aligned(128))) char rows_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t columns = blockIdx.x % a.tiles_n, tile = blockIdx.x / a.tiles_n;
     Rows t;
     if constexpr (kExperts) {
-        t = expert_rows(a, tile, 16 * kRowTiles);
+        t = expert_rows<false>(a, tile, 16 * kRowTiles);
         if (t.count <= 0) return;
     } else {
         t = {0, tile * 16 * kRowTiles, min(a.M - tile * 16 * kRowTiles, 16 * kRowTiles)};
     }
     const int32_t fragment = columns * kFragments;  // of all: 4 to a group
     const char* w = a.w + t.expert * a.w_expert + (int64_t)(fragment >> 2) * a.w_group + (fragment & 3) / O::kFragmentsOf * 1024 + lane * 16;
-    const char* x[kRowTiles];
+    // x: this lane's piece of every eighth row of a block (registers: its pieces of one row), as offsets from the tile's first row (experts: from x)
+    const char* x_base = a.x + (kExperts ? 0 : (int64_t)t.first * a.x_row);
+    const int32_t x_chunk = S::kInLds ? (lane & 7) ^ (lane >> 3) : lane >> 4;
+    typedef typename std::conditional<kDirect, uint32_t, int64_t>::type Offset;
+    Offset x_at[kRows];
 #pragma unroll
-    for (int i = 0; i < kRowTiles; ++i) {
-        const int32_t row = max(row_at<kExperts>(a, t, min(16 * i + (lane & 15), t.count - 1)), 0);
-        x[i] = a.x + (int64_t)(kExperts ? row / a.fan : row) * a.x_row;
+    for (int i = 0; i < kRows; ++i) {
+        const int32_t row = max(row_at<kExperts>(a, t, min(S::kInLds ? 8 * i + (lane >> 3) : lane & 15, t.count - 1)), 0);
+        x_at[i] = (Offset)(kExperts ? (int64_t)(row / a.fan) * a.x_row : (int64_t)(row - t.first) * a.x_row) + (kDirect ? x_chunk * 16 : 0);
     }
-    const int32_t chunk = (lane >> 4) * O::kChunk;
+    char* blocks = rows_lds + wave * kDeep * S::kBlock;  // this wavefront's
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)blocks;
     f32x4 acc[kRowTiles][kFragments];
 #pragma unroll
     for (int i = 0; i < kRowTiles; ++i)
 #pragma unroll
         for (int f = 0; f < kFragments; ++f) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    struct Unit {
-        u32x4 w[kPieces];
-        u32x4 x[kRowTiles];
+    struct Block {
+        u32x4 w[2][kPieces];
+        u32x4 x[S::kInLds ? kRows : 2];
     };
-    auto load = [&](Unit& u, int32_t unit) {
+    auto load = [&](Block& r, int place, int32_t block) __attribute__((always_inline)) {
+        if constexpr (kCopied) {
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p) u.w[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w + (int64_t)unit * O::kUnit + p * 1024));
-        const int32_t k = unit * O::kUnitK + chunk;
+            for (int i = 0; i < kRows; ++i) copy_to_lds((uint32_t)x_at[i], x_base + (int64_t)block * 128, lds0 + place * S::kBlock + i * 1024);
+        } else if constexpr (S::kInLds) {
 #pragma unroll
-        for (int i = 0; i < kRowTiles; ++i) {
-            if constexpr (kDirect) u.x[i] = *reinterpret_cast<const u32x4*>(x[i] + (int64_t)k * O::kElement);
-            else u.x[i] = chunk_of<kType>(x[i], a.x_col, k, a.K);
+            for (int i = 0; i < kRows; ++i) r.x[i] = chunk_of<kType>(x_base + x_at[i], a.x_col, block * 2 * O::kUnitK + x_chunk * O::kChunk, a.K);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if constexpr (kDirect) r.x[u] = *reinterpret_cast<const u32x4*>(x_base + (int64_t)block * 128 + u * 64 + x_at[0]);
+                else r.x[u] = chunk_of<kType>(x_base + x_at[0], a.x_col, (block * 2 + u) * O::kUnitK + x_chunk * O::kChunk, a.K);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+                const u32x4* from = reinterpret_cast<const u32x4*>(w + (int64_t)min(2 * block + u, a.units - 1) * O::kUnit + p * 1024);
+                if constexpr (kStream) r.w[u][p] = __builtin_nontemporal_load(from);
+                else r.w[u][p] = *from;
+            }
     };
-    auto multiply = [&](const Unit& u) {
+    // younger: whether the loads of kDeep - 1 blocks behind this one are under way
+    auto multiply = [&](Block& r, int place, int32_t block, auto younger) __attribute__((always_inline)) {
+        u32x4 x[2][kRowTiles];
+        if constexpr (S::kInLds) {
+            char* at = blocks + place * S::kBlock;
+            if constexpr (!kCopied) {
 #pragma unroll
-        for (int f = 0; f < kFragments; ++f) {
-            const u32x4 o = fragment_of<kType>(u.w, f);
+                for (int i = 0; i < kRows; ++i) *reinterpret_cast<u32x4*>(at + i * 1024 + lane * 16) = r.x[i];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            } else if constexpr (decltype(younger)::value) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kDeep - 1) * (kRows + 2 * kPieces)) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
 #pragma unroll
-            for (int i = 0; i < kRowTiles; ++i) acc[i][f] = product<kType>(o, u.x[i], acc[i][f]);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < kRowTiles; ++i)
+                    x[u][i] = *reinterpret_cast<const u32x4*>(at + (i * 16 + (lane & 15)) * 128 + (((u * 4 + (lane >> 4)) ^ (lane & 7)) << 4));
+        } else {
+            x[0][0] = r.x[0];
+            x[1][0] = r.x[1];
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (2 * block + u >= a.units) break;  // (the last block may be one unit)
+#pragma unroll
+            for (int f = 0; f < kFragments; ++f) {
+                const u32x4 o = fragment_of<kType>(r.w[u], f);
+#pragma unroll
+                for (int i = 0; i < kRowTiles; ++i) acc[i][f] = product<kType>(o, x[u][i], acc[i][f]);
+            }
+        }
+        // (what is read from this place is there before anything is copied to it)
+        if constexpr (S::kInLds) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
-    Unit ring[kDeep];
-    const int32_t mine = a.units > wave ? (a.units - wave + kWaves - 1) / kWaves : 0;
+    Block ring[kDeep];
+    const int32_t all = (a.units + 1) / 2, mine = all > wave ? (all - wave + kWaves - 1) / kWaves : 0;
 #pragma unroll
     for (int d = 0; d < kDeep; ++d)
-        if (d < mine) load(ring[d], wave + d * kWaves);
-    for (int32_t j = 0; j < mine; j += kDeep) {
+        if (d < mine) load(ring[d], d, wave + d * kWaves);
+    int32_t j = 0;
+    for (; j + 2 * kDeep <= mine; j += kDeep) {  // (without conditions, so that each product waits for its own loads alone)
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            if (j + d < mine) multiply(ring[d]);
-            if (j + d + kDeep < mine) load(ring[d], wave + (j + d + kDeep) * kWaves);
+            multiply(ring[d], d, wave + (j + d) * kWaves, std::true_type());
+            load(ring[d], d, wave + (j + d + kDeep) * kWaves);
         }
     }
+    for (; j < mine; j += kDeep) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            if (j + d < mine) multiply(ring[d], d, wave + (j + d) * kWaves, std::false_type());
+            if (j + d + kDeep < mine) load(ring[d], d, wave + (j + d + kDeep) * kWaves);
+        }
+    }
+    f32x4* sums = reinterpret_cast<f32x4*>(rows_lds);  // [wave][row tile][fragment][lane]
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kRowTiles; ++i)
 #pragma unroll
-        for (int f = 0; f < kFragments; ++f) rows_sums[((wave * kRowTiles + i) * kFragments + f) * 64 + lane] = acc[i][f];
+        for (int f = 0; f < kFragments; ++f) sums[((wave * kRowTiles + i) * kFragments + f) * 64 + lane] = acc[i][f];
     __syncthreads();
     for (int at = threadIdx.x; at < kRowTiles * kFragments * 64; at += 64 * kWaves) {
         const int l = at & 63, f = (at >> 6) % kFragments, i = (at >> 6) / kFragments;
-        f32x4 sum = rows_sums[at];
+        f32x4 sum = sums[at];
 #pragma unroll
-        for (int v = 1; v < kWaves; ++v) sum += rows_sums[v * kRowTiles * kFragments * 64 + at];
+        for (int v = 1; v < kWaves; ++v) sum += sums[v * kRowTiles * kFragments * 64 + at];
         const int32_t row = row_at<kExperts>(a, t, 16 * i + (l & 15));
         const int32_t n = ((fragment + f) >> 2) * kGroupRows + group_row((fragment + f) & 3, (l >> 4) * 4);
         if (row < 0) continue;
@@ -303,9 +388,9 @@ __global__ __launch_bounds__(64 * kWaves) void linear_rows_kernel(LinearArgs a) 
         const int64_t at_n = (int64_t)t.expert * a.n_padded + n;
         // (scales and biases are filled up to whole groups)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (kType == kHalfInt8) v[j] *= a.scale[at_n + j];
-            if (a.bias) v[j] += a.bias[at_n + j];
+        for (int j4 = 0; j4 < 4; ++j4) {
+            if constexpr (kType == kHalfInt8) v[j4] *= a.scale[at_n + j4];
+            if (a.bias) v[j4] += a.bias[at_n + j4];
         }
         finish<kType, 4>(a, v, row, n);
     }
@@ -319,9 +404,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_rows_kernel(LinearArgs a) 
 // is multiplied from registers, the next one's fragments come from LDS into others, so its place in the ring is free a unit early.
 // A row of x in a block is eight pieces of 16 bytes; piece c of row r lies at place c ^ (r & 7): the sixteen rows that a fragment is
 // read from then do not meet in one bank.
-__device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
-}
+constexpr int32_t kPieceColumns = 4;
 
 template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN>
 struct TileShape {
@@ -342,19 +425,25 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / kWavesN, wn = wave % kWavesN;
     // Work-groups that follow each other run on different XCDs, each with its own L2: an eighth of the tiles to each, in blocks
-    // of 8 tiles of rows, so that what a block reads stays there.
-    const int32_t all = a.tiles_m * a.tiles_n;
-    int32_t id = blockIdx.x;
-    {
-        const int32_t q = all >> 3, rest = all & 7, xcd = id & 7;
-        id = xcd * q + min(xcd, rest) + (id >> 3);
+    // of 8 tiles of rows, so that what a block reads stays there.  Experts' tiles, of which there may be fewer than the grid has, are dealt out to the XCDs in
+    // pieces of 2 x kPieceColumns, so that the last XCD is not left with those that are not there.
+    int32_t tm, tn;
+    if constexpr (kExperts) {
+        const int32_t across = (a.tiles_n + kPieceColumns - 1) / kPieceColumns, at = blockIdx.x >> 3, inside = at % (2 * kPieceColumns);
+        const int32_t piece = at / (2 * kPieceColumns) * 8 + (blockIdx.x & 7);
+        tm = piece / across * 2 + (inside & 1);
+        tn = piece % across * kPieceColumns + (inside >> 1);
+        if (tn >= a.tiles_n) return;
+    } else {
+        const int32_t all = a.tiles_m * a.tiles_n, q = all >> 3, rest = all & 7, xcd = blockIdx.x & 7, id = xcd * q + min(xcd, rest) + ((int32_t)blockIdx.x >> 3);
+        constexpr int32_t kBlock = 8;
+        const int32_t block = id / (kBlock * a.tiles_n), height = min(a.tiles_m - block * kBlock, kBlock), inside = id - block * kBlock * a.tiles_n;
+        tm = block * kBlock + inside % height;
+        tn = inside / height;
     }
-    constexpr int32_t kBlock = 8;
-    const int32_t block = id / (kBlock * a.tiles_n), height = min(a.tiles_m - block * kBlock, kBlock), inside = id - block * kBlock * a.tiles_n;
-    const int32_t tm = block * kBlock + inside % height, tn = inside / height;
     Rows t;
     if constexpr (kExperts) {
-        t = expert_rows(a, tm, kBM);
+        t = expert_rows<true>(a, tm, kBM);
         if (t.count <= 0) return;
     } else {
         t = {0, tm * kBM, min(a.M - tm * kBM, kBM)};
@@ -475,12 +564,12 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __syncthreads();
-        read_unit(even, 0, 0, 0);
         int here_x = 0, here_w = 0;  // places in the rings of this block and unit
         auto behind = [](int place) __attribute__((always_inline)) { return place + 1 == S::kRing ? 0 : place + 1; };
-        // One unit, the block's first or second, from `now`, with the next one's fragments into `then`.
-        auto step = [&](int32_t block, auto second, const Unit& now, Unit& then) __attribute__((always_inline)) {
-            constexpr bool kSecond = decltype(second)::value;
+        // One unit, the block's first or second, from `now`, with the next one's fragments into `then`.  A wavefront without rows takes part in the copies alone: half a
+        // tile at the end of an expert's rows.
+        auto step = [&](int32_t block, auto second, auto has_rows, const Unit& now, Unit& then) __attribute__((always_inline)) {
+            constexpr bool kSecond = decltype(second)::value, kHasRows = decltype(has_rows)::value;
             const int next_x = behind(here_x), next_w = behind(here_w), before_x = behind(next_x);
             // The copies that the next unit needs are there, of w from two steps ago, of x from three or more; and this wavefront has read this unit.
             if constexpr (kDirect) {
@@ -498,27 +587,34 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
             // What is read for the next unit and copied ahead goes between the products: copies one behind the other would keep the
             // wavefront from its products until the last of them is under way.
             u32x4 w[4];
-            fragments_of(w, now);
+            if constexpr (kHasRows) fragments_of(w, now);
             constexpr int kHalf = kDirect ? kCopiesX / 2 : 0, kCopies = kCopiesW + kHalf;
 #pragma unroll
             for (int i = 0; i < kRowFragments; ++i) {
-                if (i < O::kPieces) read_w(then, i, next_w);
-                read_x(then, i, kSecond ? next_x : here_x, kSecond ? 0 : 1);
+                if constexpr (kHasRows) {
+                    if (i < O::kPieces) read_w(then, i, next_w);
+                    read_x(then, i, kSecond ? next_x : here_x, kSecond ? 0 : 1);
+                }
 #pragma unroll
                 for (int c = i * kCopies / kRowFragments; c < (i + 1) * kCopies / kRowFragments; ++c) {
                     if (c < kCopiesW) copy_w(c, ahead_w, here_w);
                     else copy_x(c - kCopiesW + (kSecond ? 0 : kHalf), ahead, kSecond ? here_x : before_x);
                 }
-                multiply(w, now, i);
+                if constexpr (kHasRows) multiply(w, now, i);
                 __builtin_amdgcn_sched_barrier(0);
             }
             here_w = next_w;
             if constexpr (kSecond) here_x = next_x;
         };
-        for (int32_t block = 0; block < blocks; ++block) {
-            step(block, std::false_type(), even, odd);
-            step(block, std::true_type(), odd, even);
-        }
+        auto all_steps = [&](auto has_rows) __attribute__((always_inline)) {
+            if constexpr (decltype(has_rows)::value) read_unit(even, 0, 0, 0);
+            for (int32_t block = 0; block < blocks; ++block) {
+                step(block, std::false_type(), has_rows, even, odd);
+                step(block, std::true_type(), has_rows, odd, even);
+            }
+        };
+        if (wm * kRowFragments * 16 < t.count) all_steps(std::true_type());
+        else all_steps(std::false_type());
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
@@ -573,9 +669,15 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
 
 template <LinearType kType, int kRowTiles, int kFragments, bool kDirect, bool kExperts>
 int launch_rows(const LinearArgs& a, hipStream_t s) {
-    constexpr int kWaves = kRowTiles * kFragments >= 8 ? 4 : 8;
-    constexpr int kLds = kWaves * kRowTiles * kFragments * 1024;
-    linear_rows_kernel<kType, kRowTiles, kFragments, kWaves, kDirect, kExperts><<<(unsigned)(a.tiles_m * a.tiles_n), 64 * kWaves, kLds, s>>>(a);
+    using S = RowsShape<kType, kRowTiles, kFragments>;
+    // From 32 MB of weights on past the caches, in us with / without them, eight layers in turn: 134 MB of one row 25.9 / 22.9, 400 MB of 64 experts 50.6 / 44.5,
+    // 67 MB of int8 14.8 / 13.6; 33 MB 8.5 / 8.4; but 17 MB of int8 6.1 / 7.3, 25 MB 10.9 / 13.8.
+    const int64_t bytes = a.order ? a.w_expert * a.experts : (int64_t)a.n_padded / kGroupRows * a.w_group;
+    auto kernel = kDirect && bytes >= (int64_t(32) << 20) ? linear_rows_kernel<kType, kRowTiles, kFragments, kDirect, kExperts, kDirect>
+                                                           : linear_rows_kernel<kType, kRowTiles, kFragments, kDirect, kExperts, false>;
+    if constexpr (S::kLds > 65536)  // (has to be asked for, on every device)
+        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
+    kernel<<<(unsigned)(a.tiles_m * a.tiles_n), 64 * S::kWaves, S::kLds, s>>>(a);
     return launch_check("linear_rows_kernel");
 }
 
@@ -585,7 +687,13 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
     auto kernel = linear_tile_kernel<kType, kRowFragments, kWavesM, kWavesN, kDirect, kExperts>;
     if constexpr (S::kLds > 65536)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
-    kernel<<<(unsigned)(a.tiles_m * a.tiles_n), S::kThreads, S::kLds, s>>>(a);
+    int64_t grid = (int64_t)a.tiles_m * a.tiles_n;
+    if (kExperts) {  // (whole pieces, the same number for each XCD)
+        const int64_t pieces = (int64_t)((a.tiles_m + 1) / 2) * ((a.tiles_n + kPieceColumns - 1) / kPieceColumns);
+        grid = (pieces + 7) / 8 * 8 * 2 * kPieceColumns;
+        CHX_REQUIRE(grid < (int64_t(1) << 31), "linear plan: too many results");
+    }
+    kernel<<<(unsigned)grid, S::kThreads, S::kLds, s>>>(a);
     return launch_check("linear_tile_kernel");
 }
 
@@ -606,21 +714,20 @@ int tile_of(const LinearArgs& a, bool direct, hipStream_t s) {
 
 template <LinearType kType>
 int LinearKernels<kType>::rows(const LinearArgs& a, int row_tiles, int fragments, bool direct, hipStream_t s) {
-    if constexpr (kType != kHalfInt8) {  // (two of its fragments are one piece)
-        if (fragments == 1) {
-            if (row_tiles == 1) return rows_of<kType, 1, 1>(a, direct, s);
-            if (row_tiles == 2) return rows_of<kType, 2, 1>(a, direct, s);
-            return rows_of<kType, 4, 1>(a, direct, s);
-        }
-    }
+    // (the grid is made for these numbers: any others are refused)
     switch (row_tiles * 8 + fragments) {
+        case 8 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 1, 1>(a, direct, s); else break;  // (two fragments of int8 are one piece)
+        case 16 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 2, 1>(a, direct, s); else break;
+        case 32 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 4, 1>(a, direct, s); else break;
         case 8 + 2: return rows_of<kType, 1, 2>(a, direct, s);
         case 8 + 4: return rows_of<kType, 1, 4>(a, direct, s);
         case 16 + 2: return rows_of<kType, 2, 2>(a, direct, s);
         case 16 + 4: return rows_of<kType, 2, 4>(a, direct, s);
         case 32 + 2: return rows_of<kType, 4, 2>(a, direct, s);
-        default: return rows_of<kType, 4, 4>(a, direct, s);
+        case 32 + 4: return rows_of<kType, 4, 4>(a, direct, s);
+        default: break;
     }
+    CHX_FAIL(CHX_HIP_EUNSUPPORTED, "linear plan: no kernel for %d tiles of rows and %d fragments", row_tiles, fragments);
 }
 
 template <LinearType kType>

@@ -167,31 +167,71 @@ int prepare_call(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32
     return CHX_HIP_OK;
 }
 
+// What runs a product: work-groups of 16 row_tiles rows and 16 fragments columns (linear_rows_kernel), or, with fragments 0, a tile.
+struct Choice {
+    int row_tiles, fragments;
+    LinearTile tile;
+};
+
+// The kernel for M rows that are all multiplied with the same weights: the smallest of its sizes that does not need more work-groups than there are compute
+// units.  All sizes were timed over 7 weights from 1024 x 1024 to 4096 x 16384, 12 numbers of rows and the three types, recorded, three layers in turn.
+// us in float16 of the one chosen, and of the next smaller and larger ones:
+//   K x N            rows   16 x 16   32 x 16   32 x 32   32 x 64   64 x 64   128 x 128   256 x 256
+//   4096 x 4096        32     16.0     [10.7]     13.6      17.6      19.3       28.4
+//                      64     28.9      18.4     [13.3]     17.1      21.5       29.1
+//                     128     54.4      34.0      22.7     [16.9]     20.8       29.3
+//                     256                         43.5      29.8     [21.0]      29.2        73
+//                     512                                   59.6      40.0      [30.0]       73
+//                    2048                                            158.9      [64.7]       84
+//   4096 x 16384     1024                                            414.7      147.3      [111]
+// Where the tiles of 128 are too few, products of int8 and float32 lose more by that (512 rows of 4096 x 4096: 39.5 and 28.2, 242 and 155).
+// Up to 8 rows x is not copied into LDS (16 x 16, 16 x 32 and 16 x 64).
+Choice choose(int64_t M, int64_t N, LinearType type) {
+    const int64_t most = 256;
+    auto groups = [&](int64_t rows, int64_t columns) { return (M + rows - 1) / rows * ((N + columns - 1) / columns); };
+    const int first = type == kHalfInt8 ? 2 : 1;  // (two fragments of int8 are one piece)
+    const int row_tiles = M <= 8 ? 1 : 2;
+    for (int fragments = first; fragments <= 4; fragments *= 2)
+        if (groups(16 * row_tiles, 16 * fragments) <= most) return {row_tiles, fragments, kTile128};
+    if (M <= 32) return {row_tiles, 4, kTile128};
+    const int64_t tiles = groups(128, 128);
+    if (M <= 64 || groups(64, 64) <= most || (type != kHalfHalf && tiles < 200)) return {4, 4, kTile128};
+    return {0, 0, tiles > 2 * most && type != kFloatFloat ? kTile256 : kTile128};
+}
+
+// The same for experts, by the rows that each has on the average.  us with 16 x 64 / 32 x 64 / 64 x 64 / tiles of 128 / of 256, float16, experts' loads
+// as uneven as their normally distributed scores make them:
+//   64 experts of 1536 x 2048:  rows each  2    46.6 /  46.7 /  60.8 /  70.6 /  92.9
+//                                         16    78.3 /  65.8 /  77.4 /  82.2 / 116.8
+//   64 experts of 1024 x 2048:            64   123.3 /  93.7 /  93.5 /  80.5 /  99.1
+//   32 experts of 2048 x 4096:           128   479.3 / 315.5 / 242.0 / 167.4 / 184.5
+//                                        512                   784.9 / 378.4 / 313.4
+// (int8: 8 rows each 34.5 / 36.9, 512 rows each over 8 experts 167.5 and 186.4 in tiles; float32: 64 rows each 331 / 249 / 286 / 357, 128 rows 868 / 807 / 927.)
+Choice choose_for_experts(int64_t M, int64_t experts, int64_t N, LinearType type) {
+    const int64_t each = (M + experts - 1) / experts;
+    int row_tiles = each <= (type == kHalfHalf ? 4 : 8) ? 1 : 2;
+    if (each > (type == kFloatFloat ? 64 : 48)) {
+        if (type != kFloatFloat || each > 128) return {0, 0, each >= 256 && type == kHalfHalf ? kTile256 : kTile128};
+        row_tiles = 4;
+    }
+    const int64_t wide = (M / (16 * row_tiles) + std::min(M, experts)) * ((N + kGroupRows - 1) / kGroupRows);
+    return {row_tiles, wide >= 256 ? 4 : wide >= 128 || type == kHalfInt8 ? 2 : 1, kTile128};
+}
+
 template <LinearType kType>
 int launch(LinearArgs& a, bool direct, hipStream_t s) {
+    const Choice c = a.order ? choose_for_experts(a.M, a.experts, a.N, kType) : choose(a.M, a.N, kType);
+    const int32_t height = c.fragments > 0 ? 16 * c.row_tiles : c.tile == kTile256 ? 256 : 128;
+    const int32_t width = c.fragments > 0 ? 16 * c.fragments : height;
     // The most tiles of rows there can be: experts' tiles begin anew with each of them.
-    auto tiles = [&](int32_t height) {
-        if (!a.order) return (a.M + height - 1) / height;
-        return a.M / height + std::min(a.M, a.experts);
-    };
-    const int32_t groups = (a.N + kGroupRows - 1) / kGroupRows;
-    const int64_t rows_each = a.order ? (a.M + a.experts - 1) / a.experts : a.M;
-    if (rows_each <= 64) {
-        const int row_tiles = rows_each <= 16 ? 1 : rows_each <= 32 ? 2 : 4;
-        a.tiles_m = tiles(16 * row_tiles);
-        const int64_t wide = (int64_t)a.tiles_m * groups;
-        const int fragments = wide >= 512 ? 4 : wide >= 256 || kType == kHalfInt8 ? 2 : 1;
-        a.tiles_n = groups * (4 / fragments);
-        CHX_REQUIRE((int64_t)a.tiles_m * a.tiles_n < (int64_t(1) << 31), "linear plan: too many results");
-        const bool whole = direct && a.K % unit_k(kType) == 0;
-        return LinearKernels<kType>::rows(a, row_tiles, fragments, whole, s);
-    }
-    const int64_t large = (int64_t)tiles(256) * ((a.N + 255) / 256);
-    const bool t256 = large >= 200;
-    a.tiles_m = tiles(t256 ? 256 : 128);
-    a.tiles_n = t256 ? (a.N + 255) / 256 : (a.N + 127) / 128;
-    CHX_REQUIRE((int64_t)a.tiles_m * a.tiles_n < (int64_t(1) << 31), "linear plan: too many results");
-    return LinearKernels<kType>::tile(a, t256 ? kTile256 : kTile128, direct, s);
+    const int64_t tiles_m = a.order ? a.M / height + std::min(a.M, a.experts) : (a.M + height - 1) / height;
+    // (those of few rows take all fragments of whole groups)
+    const int64_t tiles_n = c.fragments > 0 ? (int64_t)a.n_padded / width : (a.N + width - 1) / width;
+    CHX_REQUIRE(tiles_m * tiles_n < (int64_t(1) << 31), "linear plan: too many results");
+    a.tiles_m = (int32_t)tiles_m;
+    a.tiles_n = (int32_t)tiles_n;
+    if (c.fragments == 0) return LinearKernels<kType>::tile(a, c.tile, direct, s);
+    return LinearKernels<kType>::rows(a, c.row_tiles, c.fragments, direct && a.K % (2 * unit_k(kType)) == 0, s);
 }
 
 int launch_of(const chx_hip_linear_plan* plan, Call& c, hipStream_t s) {

@@ -114,7 +114,7 @@ def another_device(host):
 
 def no_memory(host):
     w = host.tensor("float16", (64, 32))
-    host.hh.hh_no_memory(ctypes.c_size_t(64 * 64 * 2))
+    host.hh.hh_no_memory(ctypes.c_size_t(64 * 32 * 2))
     refused(host, make(host, w)[0], "hipMalloc", host.capi.EUNSUPPORTED)
 
 
@@ -191,7 +191,7 @@ def launches(host):
     T, lib = host.tensor, host.lib
     for kind, w_kind in (("float16", "float16"), ("float16", "int8"), ("float32", "float32")):
         plan = make(host, T(w_kind, (256, 96)), T("float32", (256,)) if w_kind == "int8" else None)[1]
-        for rows, name in ((1, "linear_rows_kernel"), (16, "linear_rows_kernel"), (1000, "linear_tile_kernel")):
+        for rows, name in ((1, "linear_rows_kernel"), (16, "linear_rows_kernel"), (20000, "linear_tile_kernel")):
             host.clear()
             host.check(lib.chx_hip_linear_plan_run(plan, ref(T(kind, (rows, 96))), 0, None, ref(T(kind, (rows, 256))), None))
             assert len(host.launches()) == 1 and name in host.launches()[0], host.launches()
