@@ -282,6 +282,9 @@ extern "C" int chx_hip_linear_plan_create(
     p.w_expert = groups * p.w_group;
     // (a tile's groups are addressed with 32 bits)
     CHX_REQUIRE(p.w_group < (int64_t(1) << 29), "linear plan: a row of w is too long");
+    CHX_REQUIRE((double)E * (double)p.w_expert < 0x1p46, "linear plan: too many weights");
+    // (memory is allocated and the stream waited for: neither can be recorded)
+    if (stream_is_capturing(as_stream(stream))) CHX_FAIL(CHX_HIP_EUNSUPPORTED, "linear plan: cannot be created while the stream is being captured into a graph");
     CHX_HIP_CALL(hipGetDevice(&p.device));
     const int64_t vector_bytes = E * p.n_padded * 4, bytes = E * p.w_expert + (w_scale ? vector_bytes : 0) + (b ? vector_bytes : 0);
     void* memory = nullptr;
@@ -361,7 +364,7 @@ extern "C" int chx_hip_linear_plan_run_experts(
     c.a.offsets = static_cast<const int32_t*>(offsets->data);
     c.a.experts = plan->experts;
     c.a.fan = (int32_t)(y->shape[0] / x->shape[0]);
-    // rows are gathered: all of x within 32 bits
-    c.direct = c.direct && c.a.x_row * x->shape[0] < (int64_t(1) << 32);
+    // rows are gathered: all of x, and a block of 128 bytes behind its last row's beginning, within 32 bits
+    c.direct = c.direct && c.a.x_row * x->shape[0] + 128 < (int64_t(1) << 32);
     return launch_of(plan, c, as_stream(stream));
 }

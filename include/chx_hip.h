@@ -454,7 +454,7 @@ enum { CHX_HIP_ACT_NONE = 0, CHX_HIP_ACT_RELU = 1, CHX_HIP_ACT_GELU = 2, CHX_HIP
  *   w        [N, K], or [E, N, K] for a layer with E experts: float16, float32 or int8, any strides
  *   w_scale  float32 [N] / [E, N] of int8 weights (a weight is w * w_scale), else NULL
  *   b        float16 or float32 [N] / [E, N], or NULL
- * create() copies all of them and waits for the stream.  A plan belongs to the device it was created on and may be used by
+ * create() copies all of them and waits for the stream (CHX_HIP_EUNSUPPORTED on one that is being captured).  A plan belongs to the device it was created on and may be used by
  * several threads and streams at once; it must outlive the graphs that its runs were recorded into. */
 typedef struct chx_hip_linear_plan chx_hip_linear_plan;
 int chx_hip_linear_plan_create(
@@ -474,7 +474,7 @@ int chx_hip_linear_plan_run(
 /* The same with experts, over P rows: places offsets[e] <= i < offsets[e + 1] of `order` are expert e's, and for p = order[i]
  *   y[p, n] = act(w_scale[e, n] * sum_k x[p / (P / R), k] w[e, n, k] + b[e, n])
  *   x        [R, K], R a divisor of P (a row's results are next to each other where it goes to several experts)
- *   order    int32 [P], offsets int32 [E + 1], contiguous, as chx_hip_expert_routing gives them: each row at most once
+ *   order    int32 [P], offsets int32 [E + 1], contiguous, as chx_hip_expert_routing gives them: each row at most once, offsets that do not decrease
  *   y        [P, N]; rows that no place names are left as they are */
 int chx_hip_linear_plan_run_experts(
         const chx_hip_linear_plan* plan, const chx_hip_tensor* x, const chx_hip_tensor* order, const chx_hip_tensor* offsets, int32_t activation,

@@ -116,6 +116,9 @@ def test_layouts(g, kind, m):
                 check(y, *want, k)
                 y.fill_(7.0)
                 assert bool((out == 7.0).all())
+    plan = g.ops.LinearPlan(w, b=b)
+    check(plan.run(x[0]).reshape(1, n), *formula(x[:1], w, None, b, "", None), k)               # one axis
+    check(plan.run(x[:1].expand(m, k)), *formula(x[:1].expand(m, k), w, None, b, "", None), k)   # one row again and again
     x3 = normal(12, (3, 4, k), kind)
     y3 = g.ops.LinearPlan(w).run(x3)
     assert y3.shape == (3, 4, n)
@@ -170,6 +173,32 @@ def test_recorded_and_on_two_streams(g, kind):
         also = [plan.run(small) for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[0]) for y in got) and all(torch.equal(y, want[1]) for y in also)
+
+
+def test_a_plan_is_not_created_inside_a_recording(g):
+    w, x = normal(35, (64, 64), HALF), normal(36, (4, 64), HALF)
+    plan = g.ops.LinearPlan(w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(g.capi.ChxHipError) as e:
+            g.ops.LinearPlan(w)
+        y = plan.run(x)
+    assert e.value.code == g.capi.EUNSUPPORTED
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, plan.run(x))
+
+
+def test_tensors_that_are_not_on_the_device(g):
+    w, x = normal(37, (64, 64), HALF), normal(38, (4, 64), HALF)
+    plan = g.ops.LinearPlan(w)
+    for call in (lambda: g.ops.LinearPlan(w.cpu()), lambda: plan.run(x.cpu()), lambda: plan.run(x, r=x.cpu()), lambda: plan.run(x, out=x.cpu())):
+        with pytest.raises(ValueError):
+            call()
+    plan.close()
+    with pytest.raises(ValueError):
+        plan.run(x)
 
 
 # ---- experts -------------------------------------------------------------------------------------------
