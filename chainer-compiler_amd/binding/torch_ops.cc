@@ -455,6 +455,11 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> results) {
     return t;
 }
 
+// Scratch memory of a call, from torch's allocator: it stays valid in the order of the stream, and inside a recording too.
+at::Tensor scratch(size_t bytes, const at::Tensor& like) {
+    return bytes ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
 // linear_plan(w, w_scale or None, b or None) -> address of the plan
 PyObject* linear_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -479,8 +484,11 @@ PyObject* linear_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
         shape.back() = integer(a[1]);
         const at::Tensor y = result(a[6], shape, a[5] == Py_None ? x.options() : x.options().dtype(scalar_type(a[5])));
         Operand xd(x), rd(optional_on_device(a[4], "r")), yd(y);
+        size_t bytes = 0;
+        checked([&] { return chx_hip_linear_plan_workspace(plan, xd.ptr, x.numel() / std::max<int64_t>(x.size(-1), 1), &bytes); });
+        const at::Tensor space = scratch(bytes, x);
         void* s = current_stream();
-        checked([&] { return chx_hip_linear_plan_run(plan, xd.ptr, activation, rd.ptr, yd.ptr, s); });
+        checked([&] { return chx_hip_linear_plan_run(plan, xd.ptr, activation, rd.ptr, yd.ptr, bytes ? space.data_ptr() : nullptr, bytes, s); });
         return wrapped(a[6], y);
     });
 }
@@ -494,15 +502,13 @@ PyObject* linear_run_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int32_t activation = static_cast<int32_t>(integer(a[5]));
         const at::Tensor y = result(a[7], {order.numel(), integer(a[1])}, a[6] == Py_None ? x.options() : x.options().dtype(scalar_type(a[6])));
         Operand xd(x), od(order), fd(offsets), yd(y);
+        size_t bytes = 0;
+        checked([&] { return chx_hip_linear_plan_workspace(plan, xd.ptr, order.numel(), &bytes); });
+        const at::Tensor space = scratch(bytes, x);
         void* s = current_stream();
-        checked([&] { return chx_hip_linear_plan_run_experts(plan, xd.ptr, od.ptr, fd.ptr, activation, yd.ptr, s); });
+        checked([&] { return chx_hip_linear_plan_run_experts(plan, xd.ptr, od.ptr, fd.ptr, activation, yd.ptr, bytes ? space.data_ptr() : nullptr, bytes, s); });
         return wrapped(a[7], y);
     });
-}
-
-// Scratch memory of a call, from torch's allocator: it stays valid in the order of the stream, and inside a recording too.
-at::Tensor scratch(size_t bytes, const at::Tensor& like) {
-    return bytes ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : at::Tensor();
 }
 
 // expert_routing(logits, k, bias or None, sigmoid, groups, top_groups, group_best, normalize, scale) -> (experts, weights, order, offsets)

@@ -307,7 +307,7 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int p = 0; p < kPieces; ++p) {
-                const u32x4* from = reinterpret_cast<const u32x4*>(w + (int64_t)min(2 * block + u, a.units - 1) * O::kUnit + p * 1024);
+                const u32x4* from = reinterpret_cast<const u32x4*>(w + (int64_t)(2 * block + u) * O::kUnit + p * 1024);
                 if constexpr (kStream) r.w[u][p] = __builtin_nontemporal_load(from);
                 else r.w[u][p] = *from;
             }
@@ -338,7 +338,6 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            if (2 * block + u >= a.units) break;  // (the last block may be one unit)
 #pragma unroll
             for (int f = 0; f < kFragments; ++f) {
                 const u32x4 o = fragment_of<kType>(r.w[u], f);
@@ -350,7 +349,7 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
         if constexpr (S::kInLds) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
     Block ring[kDeep];
-    const int32_t all = (a.units + 1) / 2, mine = all > wave ? (all - wave + kWaves - 1) / kWaves : 0;
+    const int32_t all = a.units / 2, mine = all > wave ? (all - wave + kWaves - 1) / kWaves : 0;
 #pragma unroll
     for (int d = 0; d < kDeep; ++d)
         if (d < mine) load(ring[d], d, wave + d * kWaves);
@@ -398,6 +397,8 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
 
 // ---- tiles -------------------------------------------------------------------------------------------
 //
+// x lies in rows of whole blocks, in 16-byte pieces (others are brought into such first, linear_plan.hip: loaded through registers here, 4096 rows of
+// 4097 x 16384 took 636 us instead of 443).
 // A work-group of kWavesM x kWavesN wavefronts, each 16 kRowFragments rows and 64 columns.  w comes into a ring of three units in LDS, x into one of
 // three blocks of two units (a block is 128 bytes of every row: of half a line at a time, the other half was fetched again where the
 // rows lie a power of two apart: 435 us instead of 419 for 4096 x 4096 x 16384), by asynchronous copies two and three units ahead.  While a unit
@@ -415,7 +416,7 @@ struct TileShape {
     static_assert(kBlock % (32 * kThreads) == 0 && kUnits % (16 * kThreads) == 0, "whole copies");
 };
 
-template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN, bool kDirect, bool kExperts>
+template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN, bool kExperts>
 __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(LinearArgs a) {
     using O = Of<kType>;
     using S = TileShape<kType, kRowFragments, kWavesM, kWavesN>;
@@ -457,10 +458,9 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
         const int32_t row = max(row_at<kExperts>(a, t, min((i * kThreads + (int)threadIdx.x) >> 3, t.count - 1)), 0);
         return kExperts ? (int64_t)(row / a.fan) * a.x_row : (int64_t)(row - t.first) * a.x_row;
     };
-    typedef typename std::conditional<kDirect, uint32_t, int64_t>::type Offset;
-    Offset x_at[kCopiesX];
+    uint32_t x_at[kCopiesX];
 #pragma unroll
-    for (int i = 0; i < kCopiesX; ++i) x_at[i] = (Offset)row_of(i) + (kDirect ? x_chunk * 16 : 0);
+    for (int i = 0; i < kCopiesX; ++i) x_at[i] = (uint32_t)row_of(i) + x_chunk * 16;
     // w: a unit of one group after the other, in the order in which it lies
     const char* w_base = a.w + t.expert * a.w_expert + (int64_t)tn * kGroups * a.w_group;
     const int32_t last_group = (a.N + kGroupRows - 1) / kGroupRows - 1 - tn * kGroups;
@@ -472,27 +472,11 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile_lds + wave * 1024;
 
-    constexpr int kBlockK = 2 * O::kUnitK;
-    u32x4 staged[kCopiesX];
-    auto load_pieces = [&](int32_t block) __attribute__((always_inline)) {
-        if (a.x_col == O::kElement && (block + 1) * kBlockK <= a.K) {
-#pragma unroll
-            for (int i = 0; i < kCopiesX; ++i)
-                staged[i] = *reinterpret_cast<const u32x4_any*>(x_base + x_at[i] + (int64_t)block * 128 + (kDirect ? 0 : x_chunk * 16));
-        } else {
-#pragma unroll
-            for (int i = 0; i < kCopiesX; ++i) staged[i] = chunk_of<kType>(x_base + x_at[i] - (kDirect ? x_chunk * 16 : 0), a.x_col, block * kBlockK + x_chunk * O::kChunk, a.K);
-        }
-    };
-    auto store_pieces = [&](int place) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < kCopiesX; ++i) *reinterpret_cast<u32x4*>(tile_lds + place * S::kBlock + (i * kThreads + threadIdx.x) * 16) = staged[i];
-    };
     auto copy_w = [&](int c, int32_t unit, int place) __attribute__((always_inline)) {
         copy_to_lds(w_at[c], w_base + (int64_t)unit * O::kUnit, lds0 + S::kAtW + place * S::kUnits + c * kThreads * 16);
     };
     auto copy_x = [&](int c, int32_t block, int place) __attribute__((always_inline)) {
-        copy_to_lds((uint32_t)x_at[c], x_base + (int64_t)block * 128, lds0 + place * S::kBlock + c * kThreads * 16);
+        copy_to_lds(x_at[c], x_base + (int64_t)block * 128, lds0 + place * S::kBlock + c * kThreads * 16);
     };
 
     f32x4 acc[kRowFragments][4];
@@ -526,39 +510,14 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     };
     Unit even, odd;
 
-    // A last block of fewer k (one unit, or two) comes first, by itself.
-    const int32_t blocks = a.K / kBlockK, left = a.units - 2 * blocks;
-    if (left > 0) {
-        load_pieces(blocks);
-#pragma unroll
-        for (int c = 0; c < kCopiesW; ++c) {
-            copy_w(c, 2 * blocks, 0);
-            copy_w(c, a.units - 1, 1);
-        }
-        store_pieces(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();
-        for (int h = 0; h < left; ++h) {
-            read_unit(even, 0, h, h);
-            u32x4 w[4];
-            fragments_of(w, even);
-#pragma unroll
-            for (int i = 0; i < kRowFragments; ++i) multiply(w, even, i);
-        }
-        __syncthreads();
-    }
-    if (blocks > 0) {
+    const int32_t blocks = a.units / 2;
+    {
         // (copies behind the last block bring it again, to a place that nobody reads any more: no step has a condition in it)
         const int32_t last = blocks - 1;
 #pragma unroll
         for (int b = 0; b < S::kRing; ++b) {
-            if constexpr (kDirect) {
 #pragma unroll
-                for (int c = 0; c < kCopiesX; ++c) copy_x(c, min(b, last), b);
-            } else {
-                load_pieces(min(b, last));
-                if (b + 1 < S::kRing) store_pieces(b);  // (the last one's are stored in the loop)
-            }
+            for (int c = 0; c < kCopiesX; ++c) copy_x(c, min(b, last), b);
 #pragma unroll
             for (int c = 0; c < kCopiesW; ++c) copy_w(c, min(b, 2 * blocks - 1), b);
         }
@@ -572,23 +531,15 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
             constexpr bool kSecond = decltype(second)::value, kHasRows = decltype(has_rows)::value;
             const int next_x = behind(here_x), next_w = behind(here_w), before_x = behind(next_x);
             // The copies that the next unit needs are there, of w from two steps ago, of x from three or more; and this wavefront has read this unit.
-            if constexpr (kDirect) {
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kCopiesX + kCopiesW) : "memory");
-            } else if constexpr (kSecond) {
-                store_pieces(before_x);
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            } else {
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kCopiesX + kCopiesW) : "memory");
-            }
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kCopiesX + kCopiesW) : "memory");
             __builtin_amdgcn_s_barrier();
             // ahead: half of the block three behind this one, in its place when both its units are read; else the other half of the one before
             const int32_t ahead = min(block + (kSecond ? 3 : 2), last), ahead_w = min(2 * block + (kSecond ? 1 : 0) + 3, 2 * blocks - 1);
-            if constexpr (!kDirect && kSecond) load_pieces(ahead);
             // What is read for the next unit and copied ahead goes between the products: copies one behind the other would keep the
             // wavefront from its products until the last of them is under way.
             u32x4 w[4];
             if constexpr (kHasRows) fragments_of(w, now);
-            constexpr int kHalf = kDirect ? kCopiesX / 2 : 0, kCopies = kCopiesW + kHalf;
+            constexpr int kHalf = kCopiesX / 2, kCopies = kCopiesW + kHalf;
 #pragma unroll
             for (int i = 0; i < kRowFragments; ++i) {
                 if constexpr (kHasRows) {
@@ -681,10 +632,10 @@ int launch_rows(const LinearArgs& a, hipStream_t s) {
     return launch_check("linear_rows_kernel");
 }
 
-template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN, bool kDirect, bool kExperts>
+template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN, bool kExperts>
 int launch_tile(const LinearArgs& a, hipStream_t s) {
     using S = TileShape<kType, kRowFragments, kWavesM, kWavesN>;
-    auto kernel = linear_tile_kernel<kType, kRowFragments, kWavesM, kWavesN, kDirect, kExperts>;
+    auto kernel = linear_tile_kernel<kType, kRowFragments, kWavesM, kWavesN, kExperts>;
     if constexpr (S::kLds > 65536)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
     int64_t grid = (int64_t)a.tiles_m * a.tiles_n;
@@ -704,10 +655,8 @@ int rows_of(const LinearArgs& a, bool direct, hipStream_t s) {
 }
 
 template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN>
-int tile_of(const LinearArgs& a, bool direct, hipStream_t s) {
-    if (a.order)
-        return direct ? launch_tile<kType, kRowFragments, kWavesM, kWavesN, true, true>(a, s) : launch_tile<kType, kRowFragments, kWavesM, kWavesN, false, true>(a, s);
-    return direct ? launch_tile<kType, kRowFragments, kWavesM, kWavesN, true, false>(a, s) : launch_tile<kType, kRowFragments, kWavesM, kWavesN, false, false>(a, s);
+int tile_of(const LinearArgs& a, hipStream_t s) {
+    return a.order ? launch_tile<kType, kRowFragments, kWavesM, kWavesN, true>(a, s) : launch_tile<kType, kRowFragments, kWavesM, kWavesN, false>(a, s);
 }
 
 }  // namespace
@@ -731,8 +680,8 @@ int LinearKernels<kType>::rows(const LinearArgs& a, int row_tiles, int fragments
 }
 
 template <LinearType kType>
-int LinearKernels<kType>::tile(const LinearArgs& a, LinearTile t, bool direct, hipStream_t s) {
-    return t == kTile256 ? tile_of<kType, 8, 2, 4>(a, direct, s) : tile_of<kType, 4, 2, 2>(a, direct, s);
+int LinearKernels<kType>::tile(const LinearArgs& a, LinearTile t, hipStream_t s) {
+    return t == kTile256 ? tile_of<kType, 8, 2, 4>(a, s) : tile_of<kType, 4, 2, 2>(a, s);
 }
 
 }  // namespace chx

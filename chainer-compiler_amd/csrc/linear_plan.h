@@ -13,7 +13,7 @@ enum LinearType { kHalfHalf = 0, kHalfInt8 = 1, kFloatFloat = 2 };  // x and w
 //   float32  16 k a unit: k = 4 (l / 16) + j; instruction j of the unit takes the k that are j modulo 4
 //   int8     32 k a unit, as for float16 with 8 bytes; those of fragments 2 p and 2 p + 1 are next to each other, 16 bytes of a lane
 // Row r of fragment f is row 16 (r / 4) + 4 f + r % 4 of the group: a lane of the result then holds 16 neighbouring columns, 32 bytes of
-// float16, and four lanes a whole line.  K is filled up with zeros to whole units, N to whole groups.
+// float16, and four lanes a whole line.  K is filled up with zeros to whole blocks of two units (128 bytes of x), N to whole groups.
 constexpr int kGroupRows = 64;
 
 __host__ __device__ constexpr int unit_bytes(LinearType t) {
@@ -36,7 +36,7 @@ struct LinearArgs {
     char* y;
     int64_t x_row, x_col, r_row, r_col, y_row, y_col;  // bytes
     int64_t w_group, w_expert;                          // bytes from one group, one expert, to the next
-    int32_t M, N, K, units;                             // units: of laid-out weights along k
+    int32_t M, N, K, units;                             // units: of laid-out weights along k, an even number
     int32_t activation, y_half;                         // y_half: y and r are float16
     int32_t vector_y, vector_r;                         // 16 bytes of neighbouring columns at a time
     int32_t tiles_m, tiles_n;
@@ -47,12 +47,13 @@ struct LinearArgs {
 };
 
 // The kernels, by the types of x and w (linear_half.hip, linear_int8.hip, linear_float.hip).  `rows`: few rows, weights straight into
-// registers; `tile`: both operands through LDS.  `direct`: rows of x can be copied in whole 16-byte pieces.
+// registers; `tile`: both operands through LDS.  `direct`: x lies in rows of whole blocks that can be
+// copied in 16-byte pieces (for tiles it does).
 enum LinearTile { kTile256 = 0, kTile128 = 1 };
 template <LinearType kType>
 struct LinearKernels {
     static int rows(const LinearArgs& a, int row_tiles, int fragments, bool direct, hipStream_t s);
-    static int tile(const LinearArgs& a, LinearTile t, bool direct, hipStream_t s);
+    static int tile(const LinearArgs& a, LinearTile t, hipStream_t s);
 };
 
 }  // namespace chx

@@ -71,6 +71,32 @@ __global__ __launch_bounds__(256) void linear_vector_kernel(VectorArgs a) {
     a.out[at] = n >= a.N ? 0.f : a.half ? (float)*reinterpret_cast<const _Float16*>(p) : *reinterpret_cast<const float*>(p);
 }
 
+// x in rows of whole blocks of 16-byte pieces, with zeros behind K, for the tiles: one lane a piece.
+struct RowsArgs {
+    const char* x;
+    int64_t x_row, x_col;  // bytes
+    char* out;
+    int64_t pitch, pieces;  // bytes of a row; 16-byte pieces of all
+    int32_t K;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void linear_pieces_kernel(RowsArgs a) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= a.pieces) return;
+    constexpr int kCount = 16 / sizeof(T);
+    const int64_t row = at / (a.pitch / 16), k0 = at % (a.pitch / 16) * kCount;
+    const char* p = a.x + row * a.x_row + k0 * a.x_col;
+    T v[kCount];
+    if (a.x_col == sizeof(T) && k0 + kCount <= a.K) {
+        __builtin_memcpy(v, __builtin_assume_aligned(p, sizeof(T)), 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) v[j] = k0 + j < a.K ? *reinterpret_cast<const T*>(p + j * a.x_col) : T(0);
+    }
+    __builtin_memcpy(__builtin_assume_aligned(a.out + at * 16, 16), v, 16);
+}
+
 // The axes before the last as one run of rows.
 bool as_rows(const chx_hip_tensor& t, int64_t* rows, int64_t* row_stride) {
     int64_t count = 1, st = 0;
@@ -104,8 +130,19 @@ bool aligned_rows(const void* p, int64_t row_stride, int64_t rows, int64_t bytes
 
 struct Call {
     LinearArgs a;
+    int64_t x_rows;
     bool direct;
 };
+
+// Bytes of a row of x in whole pieces, as the tiles take it.
+int64_t pitch_of(int32_t K, LinearType type) {
+    return ((int64_t)K * (type == kFloatFloat ? 4 : 2) + 127) / 128 * 128;
+}
+
+// Whether a tile can address rows of x that are `pitch` bytes apart: 32 bits from its first one, or from x for experts.
+bool within_reach(int64_t pitch, int64_t x_rows, bool experts) {
+    return pitch < (int64_t(1) << 23) && (!experts || pitch * x_rows + 128 < (int64_t(1) << 32));
+}
 
 int prepare_call(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, Call* c) {
     CHX_REQUIRE(plan != nullptr, "linear plan: null plan");
@@ -162,8 +199,9 @@ int prepare_call(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32
     a.n_padded = plan->n_padded;
     a.activation = activation;
     a.fan = 1;
-    // rows that can be copied in pieces of 16 bytes, addressed with 32 bits from a tile's first one
-    c->direct = a.x_col == xe && aligned_rows(a.x, a.x_row, x_rows, 16) && a.x_row >= 0 && a.x_row < (int64_t(1) << 23);
+    c->x_rows = x_rows;
+    // whole blocks that can be copied in pieces of 16 bytes, addressed with 32 bits from a tile's first row
+    c->direct = a.K % (2 * unit_k(plan->type)) == 0 && a.x_col == xe && aligned_rows(a.x, a.x_row, x_rows, 16) && a.x_row >= 0 && within_reach(a.x_row, x_rows, false);
     return CHX_HIP_OK;
 }
 
@@ -218,9 +256,24 @@ Choice choose_for_experts(int64_t M, int64_t experts, int64_t N, LinearType type
     return {row_tiles, wide >= 256 ? 4 : wide >= 128 || type == kHalfInt8 ? 2 : 1, kTile128};
 }
 
+// The kernel for a call: experts 0 without experts; x of x_rows rows.
+Choice choice_of(int64_t M, int64_t experts, int64_t x_rows, int64_t N, int32_t K, LinearType type) {
+    const Choice c = experts ? choose_for_experts(M, experts, N, type) : choose(M, N, type);
+    // (rows that a tile cannot address: the other kernel has 64 bits for them)
+    if (c.fragments == 0 && !within_reach(pitch_of(K, type), x_rows, experts > 0)) return {4, 4, kTile128};
+    return c;
+}
+
+// Whether x is brought into whole blocks first: for tiles always, for the other kernel where the launch that this takes (2 to 3 us) is made up for by copies instead of
+// loads through registers (512 rows of 2047 x 4096: int8 31 us and 23 with the launch, float32 91 and 85; below some 256 rows that is what it costs).
+bool into_pieces(const Choice& c, bool direct, int64_t x_rows, int32_t K, bool experts, LinearType type) {
+    return !direct && (c.fragments == 0 || (c.row_tiles > 1 && x_rows > 256 && within_reach(pitch_of(K, type), x_rows, experts)));
+}
+
 template <LinearType kType>
-int launch(LinearArgs& a, bool direct, hipStream_t s) {
-    const Choice c = a.order ? choose_for_experts(a.M, a.experts, a.N, kType) : choose(a.M, a.N, kType);
+int launch(Call& call, void* workspace, size_t workspace_bytes, hipStream_t s) {
+    LinearArgs& a = call.a;
+    const Choice c = choice_of(a.M, a.experts, call.x_rows, a.N, a.K, kType);
     const int32_t height = c.fragments > 0 ? 16 * c.row_tiles : c.tile == kTile256 ? 256 : 128;
     const int32_t width = c.fragments > 0 ? 16 * c.fragments : height;
     // The most tiles of rows there can be: experts' tiles begin anew with each of them.
@@ -230,16 +283,30 @@ int launch(LinearArgs& a, bool direct, hipStream_t s) {
     CHX_REQUIRE(tiles_m * tiles_n < (int64_t(1) << 31), "linear plan: too many results");
     a.tiles_m = (int32_t)tiles_m;
     a.tiles_n = (int32_t)tiles_n;
-    if (c.fragments == 0) return LinearKernels<kType>::tile(a, c.tile, direct, s);
-    return LinearKernels<kType>::rows(a, c.row_tiles, c.fragments, direct && a.K % (2 * unit_k(kType)) == 0, s);
+    if (into_pieces(c, call.direct, call.x_rows, a.K, a.order != nullptr, kType)) {
+        RowsArgs r = {a.x, a.x_row, a.x_col, static_cast<char*>(workspace), pitch_of(a.K, kType), 0, a.K};
+        CHX_REQUIRE(workspace != nullptr && aligned(workspace, 16) && (int64_t)workspace_bytes >= r.pitch * call.x_rows,
+                    "linear plan: a workspace of %lld bytes, aligned to 16, is needed for rows like these", (long long)(r.pitch * call.x_rows));
+        r.pieces = r.pitch / 16 * call.x_rows;
+        CHX_REQUIRE(r.pieces < (int64_t(1) << 38), "linear plan: too many rows");
+        const unsigned blocks = (unsigned)((r.pieces + 255) / 256);
+        if (kType == kFloatFloat) linear_pieces_kernel<uint32_t><<<blocks, 256, 0, s>>>(r);
+        else linear_pieces_kernel<uint16_t><<<blocks, 256, 0, s>>>(r);
+        CHX_PROPAGATE(launch_check("linear_pieces_kernel"));
+        a.x = r.out;
+        a.x_row = r.pitch;
+        a.x_col = kType == kFloatFloat ? 4 : 2;
+        call.direct = true;
+    }
+    return c.fragments > 0 ? LinearKernels<kType>::rows(a, c.row_tiles, c.fragments, call.direct, s) : LinearKernels<kType>::tile(a, c.tile, s);
 }
 
-int launch_of(const chx_hip_linear_plan* plan, Call& c, hipStream_t s) {
+int launch_of(const chx_hip_linear_plan* plan, Call& c, void* workspace, size_t workspace_bytes, hipStream_t s) {
     if (c.a.M == 0 || c.a.N == 0) return CHX_HIP_OK;
     switch (plan->type) {
-        case kHalfHalf: return launch<kHalfHalf>(c.a, c.direct, s);
-        case kHalfInt8: return launch<kHalfInt8>(c.a, c.direct, s);
-        default: return launch<kFloatFloat>(c.a, c.direct, s);
+        case kHalfHalf: return launch<kHalfHalf>(c, workspace, workspace_bytes, s);
+        case kHalfInt8: return launch<kHalfInt8>(c, workspace, workspace_bytes, s);
+        default: return launch<kFloatFloat>(c, workspace, workspace_bytes, s);
     }
 }
 
@@ -273,7 +340,7 @@ extern "C" int chx_hip_linear_plan_create(
     chx_hip_linear_plan p;
     p.type = w->dtype == CHX_HIP_FLOAT16 ? kHalfHalf : w->dtype == CHX_HIP_INT8 ? kHalfInt8 : kFloatFloat;
     const int64_t groups = (N + kGroupRows - 1) / kGroupRows;
-    p.units = (int32_t)((K + unit_k(p.type) - 1) / unit_k(p.type));
+    p.units = (int32_t)((K + 2 * unit_k(p.type) - 1) / (2 * unit_k(p.type)) * 2);
     p.N = (int32_t)N;
     p.K = (int32_t)K;
     p.experts = lead ? (int32_t)E : 0;
@@ -334,19 +401,35 @@ extern "C" void chx_hip_linear_plan_destroy(chx_hip_linear_plan* plan) {
     delete plan;
 }
 
+extern "C" int chx_hip_linear_plan_workspace(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int64_t y_rows, size_t* bytes) {
+    CHX_REQUIRE(bytes != nullptr, "linear plan: null output");
+    *bytes = 0;
+    CHX_REQUIRE(plan != nullptr, "linear plan: null plan");
+    CHX_PROPAGATE(check_tensor(x, "linear plan x"));
+    int64_t rows = 0, row_stride = 0;
+    // (what a run refuses needs none)
+    if (x->ndim < 1 || y_rows < 1 || x->shape[x->ndim - 1] != plan->K || !as_rows(*x, &rows, &row_stride) || rows < 1) return CHX_HIP_OK;
+    const Choice c = choice_of(y_rows, plan->experts, rows, plan->N, plan->K, plan->type);
+    const int64_t xe = plan->type == kFloatFloat ? 4 : 2;
+    const bool direct = plan->K % (2 * unit_k(plan->type)) == 0 && x->strides[x->ndim - 1] == xe && aligned_rows(x->data, row_stride, rows, 16) && row_stride >= 0 && within_reach(row_stride, rows, plan->experts > 0);
+    if (into_pieces(c, direct, rows, plan->K, plan->experts > 0, plan->type)) *bytes = (size_t)(pitch_of(plan->K, plan->type) * rows);
+    return CHX_HIP_OK;
+}
+
 extern "C" int chx_hip_linear_plan_run(
-        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, void* stream) {
+        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, void* workspace,
+        size_t workspace_bytes, void* stream) {
     Call c;
     CHX_PROPAGATE(prepare_call(plan, x, activation, r, y, &c));
     CHX_REQUIRE(plan->experts == 0, "linear plan: the weights are experts': run_experts takes them");
     CHX_REQUIRE(x->ndim == y->ndim, "linear plan: x and y differ in their number of axes");
     for (int d = 0; d + 1 < x->ndim; ++d) CHX_REQUIRE(x->shape[d] == y->shape[d], "linear plan: x and y differ on axis %d", d);
-    return launch_of(plan, c, as_stream(stream));
+    return launch_of(plan, c, workspace, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int chx_hip_linear_plan_run_experts(
         const chx_hip_linear_plan* plan, const chx_hip_tensor* x, const chx_hip_tensor* order, const chx_hip_tensor* offsets, int32_t activation,
-        chx_hip_tensor* y, void* stream) {
+        chx_hip_tensor* y, void* workspace, size_t workspace_bytes, void* stream) {
     Call c;
     CHX_PROPAGATE(prepare_call(plan, x, activation, nullptr, y, &c));
     CHX_REQUIRE(plan->experts > 0, "linear plan: the weights have no experts: run takes them");
@@ -364,7 +447,7 @@ extern "C" int chx_hip_linear_plan_run_experts(
     c.a.offsets = static_cast<const int32_t*>(offsets->data);
     c.a.experts = plan->experts;
     c.a.fan = (int32_t)(y->shape[0] / x->shape[0]);
-    // rows are gathered: all of x, and a block of 128 bytes behind its last row's beginning, within 32 bits
-    c.direct = c.direct && c.a.x_row * x->shape[0] + 128 < (int64_t(1) << 32);
-    return launch_of(plan, c, as_stream(stream));
+    // (rows are gathered: all of x, and a block of 128 bytes behind its last row's beginning, within 32 bits)
+    c.direct = c.direct && within_reach(c.a.x_row, x->shape[0], true);
+    return launch_of(plan, c, workspace, workspace_bytes, as_stream(stream));
 }

@@ -467,9 +467,11 @@ void chx_hip_linear_plan_destroy(chx_hip_linear_plan* plan);
  *   y  [.., N] likewise, float16 or float32 (float32 only for float32 x)
  *   r  NULL, or of y's shape and type; may be y itself
  * Sums and epilogue are float32, in an order that depends on the sizes alone; the result is rounded once.  y must not overlap x,
- * nor r unless it is r. */
+ * nor r unless it is r.  workspace: for many rows that are not whole 16-byte pieces, aligned to 16; y_rows: rows of y. */
+int chx_hip_linear_plan_workspace(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int64_t y_rows, size_t* bytes);
 int chx_hip_linear_plan_run(
-        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, void* stream);
+        const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, void* workspace,
+        size_t workspace_bytes, void* stream);
 
 /* The same with experts, over P rows: places offsets[e] <= i < offsets[e + 1] of `order` are expert e's, and for p = order[i]
  *   y[p, n] = act(w_scale[e, n] * sum_k x[p / (P / R), k] w[e, n, k] + b[e, n])
@@ -478,7 +480,7 @@ int chx_hip_linear_plan_run(
  *   y        [P, N]; rows that no place names are left as they are */
 int chx_hip_linear_plan_run_experts(
         const chx_hip_linear_plan* plan, const chx_hip_tensor* x, const chx_hip_tensor* order, const chx_hip_tensor* offsets, int32_t activation,
-        chx_hip_tensor* y, void* stream);
+        chx_hip_tensor* y, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Routing rows to experts.  logits [T, E], float16 or float32; per row, in 64 bits where that decides:
  *   s = softmax(logits), or 1 / (1 + exp(-logits)) with `sigmoid`;  key = s + bias (float32 [E], or NULL)

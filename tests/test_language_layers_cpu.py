@@ -59,7 +59,7 @@ def runs(host):
     host.clear()
 
     def run(plan, x, y, r=None, act=0):
-        return lib.chx_hip_linear_plan_run(plan, ref(x), act, ref(r), ref(y), None)
+        return lib.chx_hip_linear_plan_run(plan, ref(x), act, ref(r), ref(y), None, ctypes.c_size_t(0), None)
 
     x, y = T("float16", (5, 32)), T("float16", (5, 64))
     both = T("float16", (5, 100))
@@ -90,7 +90,7 @@ def experts(host):
     x, order, offsets, y = T("float16", (4, 32)), T("int32", (8,)), T("int32", (4,)), T("float16", (8, 64))
 
     def run(p, x, o, f, y):
-        return lib.chx_hip_linear_plan_run_experts(p, ref(x), ref(o), ref(f), 0, ref(y), None)
+        return lib.chx_hip_linear_plan_run_experts(p, ref(x), ref(o), ref(f), 0, ref(y), None, ctypes.c_size_t(0), None)
 
     for args, text in [((plain, x, order, offsets, y), "no experts"), ((plan, x, None, offsets, y), "null tensor"), ((plan, x, order, None, y), "null tensor"),
                        ((plan, x, T("int32", (7,)), offsets, y), "order must be"), ((plan, x, T("int32", (8,), [2]), offsets, y), "order must be"),
@@ -109,12 +109,12 @@ def another_device(host):
     plan = make(host, T("float16", (64, 32)))[1]
     host.clear()
     host.check(host.lib.chx_hip_init(1))
-    refused(host, host.lib.chx_hip_linear_plan_run(plan, ref(T("float16", (5, 32))), 0, None, ref(T("float16", (5, 64))), None), "created on device 0, run on device 1")
+    refused(host, host.lib.chx_hip_linear_plan_run(plan, ref(T("float16", (5, 32))), 0, None, ref(T("float16", (5, 64))), None, ctypes.c_size_t(0), None), "created on device 0, run on device 1")
 
 
 def no_memory(host):
     w = host.tensor("float16", (64, 32))
-    host.hh.hh_no_memory(ctypes.c_size_t(64 * 32 * 2))
+    host.hh.hh_no_memory(ctypes.c_size_t(64 * 64 * 2))
     refused(host, make(host, w)[0], "hipMalloc", host.capi.EUNSUPPORTED)
 
 
@@ -190,11 +190,22 @@ def launches(host):
     """Few rows take the kernel that streams weights, many the tiles; every type has both."""
     T, lib = host.tensor, host.lib
     for kind, w_kind in (("float16", "float16"), ("float16", "int8"), ("float32", "float32")):
-        plan = make(host, T(w_kind, (256, 96)), T("float32", (256,)) if w_kind == "int8" else None)[1]
+        plan = make(host, T(w_kind, (256, 128)), T("float32", (256,)) if w_kind == "int8" else None)[1]
         for rows, name in ((1, "linear_rows_kernel"), (16, "linear_rows_kernel"), (20000, "linear_tile_kernel")):
             host.clear()
-            host.check(lib.chx_hip_linear_plan_run(plan, ref(T(kind, (rows, 96))), 0, None, ref(T(kind, (rows, 256))), None))
+            host.check(lib.chx_hip_linear_plan_run(plan, ref(T(kind, (rows, 128))), 0, None, ref(T(kind, (rows, 256))), None, ctypes.c_size_t(0), None))
             assert len(host.launches()) == 1 and name in host.launches()[0], host.launches()
+        # many rows that are not whole pieces are brought into such first, in the caller's memory
+        x, y, size = T(kind, (20000, 128), [129, 1]), T(kind, (20000, 256)), ctypes.c_size_t()
+        host.check(lib.chx_hip_linear_plan_workspace(plan, ref(x), ctypes.c_int64(20000), ctypes.byref(size)))
+        assert size.value == 20000 * (512 if kind == "float32" else 256)
+        host.clear()
+        refused(host, lib.chx_hip_linear_plan_run(plan, ref(x), 0, None, ref(y), ctypes.c_void_p(host.malloc(size.value)), ctypes.c_size_t(size.value - 1), None), "workspace")
+        host.check(lib.chx_hip_linear_plan_run(plan, ref(x), 0, None, ref(y), ctypes.c_void_p(host.malloc(size.value)), size, None))
+        assert len(host.launches()) == 2 and "linear_pieces_kernel" in host.launches()[0] and "linear_tile_kernel" in host.launches()[1], host.launches()
+        for few in (T(kind, (8, 128), [129, 1]), T(kind, (20000, 128))):
+            host.check(lib.chx_hip_linear_plan_workspace(plan, ref(few), ctypes.c_int64(few.shape[0]), ctypes.byref(size)))
+            assert size.value == 0
 
 
 if __name__ == "__main__":
