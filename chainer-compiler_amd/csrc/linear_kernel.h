@@ -235,7 +235,7 @@ __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, u
 // kWaves-th block of two units: w goes from memory straight into registers, kDeep blocks ahead of the products, and the wavefronts' sums
 // are added in LDS, in one order.  x comes from the caches.  Up to 16 rows are loaded as fragments; of more, a block (128 bytes of every row) is copied
 // into LDS of the wavefront's own, because lanes next to each other that load from different rows take a cache access each: 64 rows x 4096 x
-// 16384 36 us instead of 48.  Rows that are not there repeat the last one; their results are dropped.
+// 16384, 32 columns to a work-group, 36 us instead of 48 (with 64 columns it takes 27).  Rows that are not there repeat the last one; their results are dropped.
 template <LinearType kType, int kRowTiles, int kFragments>
 struct RowsShape {
     static constexpr int kWaves = 8, kPieces = kFragments / Of<kType>::kFragmentsOf;
@@ -539,11 +539,12 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
             // wavefront from its products until the last of them is under way.
             u32x4 w[4];
             if constexpr (kHasRows) fragments_of(w, now);
-            constexpr int kHalf = kCopiesX / 2, kCopies = kCopiesW + kHalf;
+            constexpr int kHalf = kCopiesX / 2, kCopies = kCopiesW + kHalf, kPiecesEach = (O::kPieces + kRowFragments - 1) / kRowFragments;
 #pragma unroll
             for (int i = 0; i < kRowFragments; ++i) {
                 if constexpr (kHasRows) {
-                    if (i < O::kPieces) read_w(then, i, next_w);
+#pragma unroll
+                    for (int p = i * kPiecesEach; p < O::kPieces && p < (i + 1) * kPiecesEach; ++p) read_w(then, p, next_w);
                     read_x(then, i, kSecond ? next_x : here_x, kSecond ? 0 : 1);
                 }
 #pragma unroll
@@ -681,7 +682,9 @@ int LinearKernels<kType>::rows(const LinearArgs& a, int row_tiles, int fragments
 
 template <LinearType kType>
 int LinearKernels<kType>::tile(const LinearArgs& a, LinearTile t, hipStream_t s) {
-    return t == kTile256 ? tile_of<kType, 8, 2, 4>(a, s) : tile_of<kType, 4, 2, 2>(a, s);
+    if (t == kTile64) return tile_of<kType, 2, 2, 2>(a, s);
+    if constexpr (kType != kFloatFloat) return t == kTile256 ? tile_of<kType, 8, 2, 4>(a, s) : tile_of<kType, 4, 2, 2>(a, s);
+    CHX_FAIL(CHX_HIP_EUNSUPPORTED, "linear plan: no kernel for tiles of 128 rows of float32");
 }
 
 }  // namespace chx

@@ -49,7 +49,7 @@ struct LinearArgs {
 // The kernels, by the types of x and w (linear_half.hip, linear_int8.hip, linear_float.hip).  `rows`: few rows, weights straight into
 // registers; `tile`: both operands through LDS.  `direct`: x lies in rows of whole blocks that can be
 // copied in 16-byte pieces (for tiles it does).
-enum LinearTile { kTile256 = 0, kTile128 = 1 };
+enum LinearTile { kTile256 = 0, kTile128 = 1, kTile64 = 2 };  // 256 x 256, 128 x 128, 64 x 128 (rows x columns); float32 has the last one alone
 template <LinearType kType>
 struct LinearKernels {
     static int rows(const LinearArgs& a, int row_tiles, int fragments, bool direct, hipStream_t s);

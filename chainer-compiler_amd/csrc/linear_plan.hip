@@ -211,18 +211,49 @@ struct Choice {
     LinearTile tile;
 };
 
+// float32, M > 32: the kernel with the least time, where one of 256 compute units has the most work-groups to do.  us of a work-group each, by K = 4096 (512 rows of
+// 4096 x 4096: 205 us in 32 x 32, 185 in 32 x 64, 168 in 64 x 32, 152 in 64 x 64, 131 in tiles of 64 x 128; 2048 rows 829, 755, 667, 598 and 472):
+// the first that fits instead cost up to half as much again where a few work-groups were left over.  us of each in this order, and of a library's product alone:
+//   690 x 10880 x 1560 rows x K x N   320   344   304   366   334   213
+//   91 x 3648 x 9760                   95    87   112   132   117    62
+//   699 x 3328 x 13056                800   726   642   574   476   452
+//   1782 x 5248 x 867                 180   207   193   183   169   139
+//   300 x 1024 x 1024                16.7  15.5  15.3  25.7  37.9  23.4
+Choice choose_float(int64_t M, int64_t N) {
+    static const struct {
+        Choice c;
+        int rows, columns;
+        float first, next;
+    } kernels[] = {{{2, 2, kTile64}, 32, 32, 25.5f, 25.5f}, {{2, 4, kTile64}, 32, 64, 46.f, 46.f}, {{4, 2, kTile64}, 64, 32, 42.f, 42.f},
+                   {{4, 4, kTile64}, 64, 64, 76.f, 76.f},   {{0, 0, kTile64}, 64, 128, 131.f, 115.f}};
+    Choice best = kernels[0].c;
+    float least = 0.f;
+    for (const auto& k : kernels) {
+        const int64_t each = ((M + k.rows - 1) / k.rows * ((N + k.columns - 1) / k.columns) + 255) / 256;
+        const float us = k.first + (float)(each - 1) * k.next;
+        if (least == 0.f || us < least) {
+            least = us;
+            best = k.c;
+        }
+    }
+    return best;
+}
+
 // The kernel for M rows that are all multiplied with the same weights: the smallest of its sizes that does not need more work-groups than there are compute
 // units.  All sizes were timed over 7 weights from 1024 x 1024 to 4096 x 16384, 12 numbers of rows and the three types, recorded, three layers in turn.
 // us in float16 of the one chosen, and of the next smaller and larger ones:
-//   K x N            rows   16 x 16   32 x 16   32 x 32   32 x 64   64 x 64   128 x 128   256 x 256
-//   4096 x 4096        32     16.0     [10.7]     13.6      17.6      19.3       28.4
-//                      64     28.9      18.4     [13.3]     17.1      21.5       29.1
-//                     128     54.4      34.0      22.7     [16.9]     20.8       29.3
-//                     256                         43.5      29.8     [21.0]      29.2        73
-//                     512                                   59.6      40.0      [30.0]       73
-//                    2048                                            158.9      [64.7]       84
-//   4096 x 16384     1024                                            414.7      147.3      [111]
-// Where the tiles of 128 are too few, products of int8 and float32 lose more by that (512 rows of 4096 x 4096: 39.5 and 28.2, 242 and 155).
+//  K x N            rows   16 x 16   32 x 16   32 x 32   32 x 64   64 x 64   64 x 128   128 x 128   256 x 256
+//  4096 x 4096        32     16.0     [10.7]     13.6      17.6      19.3                  28.4
+//                     64     28.9      18.4     [13.3]     17.1      21.5                  29.1
+//                    128     54.4      34.0      22.7     [16.9]     20.8                  29.3
+//                    256                         43.5      29.8     [21.0]      29.0       33.4        77
+//                    512                                   62.0      41.8      [30.3]      33.6        78
+//                   1024                                             80.1       43.1      [40.1]       78
+//                   2048                                            158.1       84.1      [68.2]       80
+//  4096 x 16384     1024                                            414.7                 147.3      [111]
+// Where the tiles of 128 are too few, products of int8 lose more by that (512 rows of 4096 x 4096: 42.2 in 128 x 128, 33.0 in 64 x 128 and 29.2 in 64 x 64).
+// Tiles of 64 x 128 take the place of those of 128 x 128 where a compute unit has less than twice as many of them to do: 436 rows of 8448 x 9056
+// 81.5 instead of 102.4 (int8 91.6 and 97.2), 2048 of 1024 x 1024 11.6 instead of 15.2.
 // Up to 8 rows x is not copied into LDS (16 x 16, 16 x 32 and 16 x 64).
 Choice choose(int64_t M, int64_t N, LinearType type) {
     const int64_t most = 256;
@@ -230,37 +261,40 @@ Choice choose(int64_t M, int64_t N, LinearType type) {
     const int first = type == kHalfInt8 ? 2 : 1;  // (two fragments of int8 are one piece)
     const int row_tiles = M <= 8 ? 1 : 2;
     for (int fragments = first; fragments <= 4; fragments *= 2)
-        if (groups(16 * row_tiles, 16 * fragments) <= most) return {row_tiles, fragments, kTile128};
-    if (M <= 32) return {row_tiles, 4, kTile128};
+        if (groups(16 * row_tiles, 16 * fragments) <= most) return {row_tiles, fragments, kTile64};
+    if (M <= 32) return {row_tiles, 4, kTile64};
+    if (type == kFloatFloat) return choose_float(M, N);
     const int64_t tiles = groups(128, 128);
-    if (M <= 64 || groups(64, 64) <= most || (type != kHalfHalf && tiles < 200)) return {4, 4, kTile128};
-    return {0, 0, tiles > 2 * most && type != kFloatFloat ? kTile256 : kTile128};
+    if (M <= 64 || groups(64, 64) <= most || (type == kHalfInt8 && tiles < 160)) return {4, 4, kTile64};
+    if (tiles > 2 * most) return {0, 0, kTile256};
+    return {0, 0, (groups(64, 128) + most - 1) / most < 2 * ((tiles + most - 1) / most) ? kTile64 : kTile128};
 }
 
-// The same for experts, by the rows that each has on the average.  us with 16 x 64 / 32 x 64 / 64 x 64 / tiles of 128 / of 256, float16, experts' loads
+// The same for experts, by the rows that each has on the average.  us with 16 x 64 / 32 x 64 / 64 x 64 / tiles of 64 x 128 / of 128 / of 256, experts' loads
 // as uneven as their normally distributed scores make them:
-//   64 experts of 1536 x 2048:  rows each  2    46.6 /  46.7 /  60.8 /  70.6 /  92.9
-//                                         16    78.3 /  65.8 /  77.4 /  82.2 / 116.8
-//   64 experts of 1024 x 2048:            64   123.3 /  93.7 /  93.5 /  80.5 /  99.1
-//   32 experts of 2048 x 4096:           128   479.3 / 315.5 / 242.0 / 167.4 / 184.5
-//                                        512                   784.9 / 378.4 / 313.4
-// (int8: 8 rows each 34.5 / 36.9, 512 rows each over 8 experts 167.5 and 186.4 in tiles; float32: 64 rows each 331 / 249 / 286 / 357, 128 rows 868 / 807 / 927.)
+//   64 experts of 1536 x 2048:  rows each  2   float16   47 /   46 /   62 /   59 /   73 /   78   int8    32 /   31 /   52 /   30 /   49 /   64
+//                                          8             58 /   52 /   65 /   66 /   78 /   82           41 /   35 /   62 /   37 /   54 /   70
+//                                         16             80 /   66 /   79 /   74 /   83 /   89           56 /   45 /   62 /   40 /   59 /   71
+//                                         32            123 /   94 /  102 /   90 /   89 /   96           87 /   62 /   77 /   50 /   63 /   81
+//   64 experts of 1024 x 2048:            64            128 /   94 /   95 /   76 /   78 /   87          101 /   65 /   75 /   46 /   56 /   68
+//   32 experts of 2048 x 4096:           128            497 /  321 /  241 /  185 /  163 /  176          318 /  189 /  181 /  123 /  121 /  157
+//                                        512           1849 / 1095 /  777 /  484 /  383 /  307         1192 /  648 /  585 /  355 /  312 /  297
+//   8 experts of 4096 x 4096:            512           1028 /  620 /  433 /  229 /  186 /  179          681 /  357 /  310 /  177 /  164 /  175
+// (float32, the first four: 8 rows each 136 / 142 / 234 / 183, 32 rows 307 / 235 / 283 / 278, 64 rows 358 / 246 / 278 / 243, 128 rows 1364 / 850 / 784 / 659.)
 Choice choose_for_experts(int64_t M, int64_t experts, int64_t N, LinearType type) {
     const int64_t each = (M + experts - 1) / experts;
-    int row_tiles = each <= (type == kHalfHalf ? 4 : 8) ? 1 : 2;
-    if (each > (type == kFloatFloat ? 64 : 48)) {
-        if (type != kFloatFloat || each > 128) return {0, 0, each >= 256 && type == kHalfHalf ? kTile256 : kTile128};
-        row_tiles = 4;
-    }
+    if (each > (type == kFloatFloat ? 64 : type == kHalfHalf ? 24 : 12))
+        return {0, 0, type == kFloatFloat || each <= 96 ? kTile64 : each >= 256 && type == kHalfHalf ? kTile256 : kTile128};
+    const int row_tiles = each <= (type == kFloatFloat ? 8 : 4) ? 1 : 2;
     const int64_t wide = (M / (16 * row_tiles) + std::min(M, experts)) * ((N + kGroupRows - 1) / kGroupRows);
-    return {row_tiles, wide >= 256 ? 4 : wide >= 128 || type == kHalfInt8 ? 2 : 1, kTile128};
+    return {row_tiles, wide >= 256 ? 4 : wide >= 128 || type == kHalfInt8 ? 2 : 1, kTile64};
 }
 
 // The kernel for a call: experts 0 without experts; x of x_rows rows.
 Choice choice_of(int64_t M, int64_t experts, int64_t x_rows, int64_t N, int32_t K, LinearType type) {
     const Choice c = experts ? choose_for_experts(M, experts, N, type) : choose(M, N, type);
     // (rows that a tile cannot address: the other kernel has 64 bits for them)
-    if (c.fragments == 0 && !within_reach(pitch_of(K, type), x_rows, experts > 0)) return {4, 4, kTile128};
+    if (c.fragments == 0 && !within_reach(pitch_of(K, type), x_rows, experts > 0)) return {4, 4, kTile64};
     return c;
 }
 
@@ -274,8 +308,8 @@ template <LinearType kType>
 int launch(Call& call, void* workspace, size_t workspace_bytes, hipStream_t s) {
     LinearArgs& a = call.a;
     const Choice c = choice_of(a.M, a.experts, call.x_rows, a.N, a.K, kType);
-    const int32_t height = c.fragments > 0 ? 16 * c.row_tiles : c.tile == kTile256 ? 256 : 128;
-    const int32_t width = c.fragments > 0 ? 16 * c.fragments : height;
+    const int32_t height = c.fragments > 0 ? 16 * c.row_tiles : c.tile == kTile256 ? 256 : c.tile == kTile128 ? 128 : 64;
+    const int32_t width = c.fragments > 0 ? 16 * c.fragments : std::max(height, 128);
     // The most tiles of rows there can be: experts' tiles begin anew with each of them.
     const int64_t tiles_m = a.order ? a.M / height + std::min(a.M, a.experts) : (a.M + height - 1) / height;
     // (those of few rows take all fragments of whole groups)

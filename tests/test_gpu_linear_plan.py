@@ -67,6 +67,7 @@ TYPES = [(HALF, HALF), (HALF, torch.int8), (FLOAT, FLOAT)]
     (1, 1, 1), (1, 64, 16), (3, 130, 65), (16, 512, 64), (17, 63, 100), (33, 256, 33),         # few rows: one, two, four tiles of 16
     (64, 1000, 130), (65, 64, 64), (129, 96, 200), (300, 330, 17),                             # the bounds of both kernels, ragged steps
     (2000, 128, 6600),                                                                         # the large tiles
+    (150, 72, 10300), (300, 130, 9000), (90, 200, 9700),                                       # tiles of 64 x 128, of 128 x 128; more than one round of few rows
     (1, 0x1200, 0x900),
 ])
 def test_sizes(g, kind, w_kind, m, k, n):
@@ -217,6 +218,7 @@ def routed(seed, places, experts, empty=()):
 @pytest.mark.parametrize("places,experts,fan,k,n", [
     (1, 1, 1, 64, 64), (8, 70, 2, 130, 48), (96, 130, 8, 64, 200),                 # a row or none to an expert, more than 64 experts
     (640, 3, 2, 100, 130), (3000, 20, 1, 64, 96), (9000, 3, 3, 128, 1100),         # tiles of 128 and of 256 rows
+    (600, 18, 2, 200, 150), (700, 9, 1, 96, 90),                                   # tiles of 64 rows
 ])
 def test_experts(g, kind, w_kind, places, experts, fan, k, n):
     chosen, order, offsets = routed(21, places, experts, empty=(0,) if experts > 1 else ())
