@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <cstdlib>
 #include <string>
 
 #include "chx_hip.h"
@@ -114,6 +115,22 @@ inline bool arrays_overlap(const chx_hip_tensor& a, const chx_hip_tensor& b) {
         }
     }
     return lo[0] < hi[1] && lo[1] < hi[0];
+}
+
+// Whether no two elements of an array share bytes: along each axis, taken by distance, more than what lies inside.
+inline bool elements_apart(const chx_hip_tensor& t) {
+    bool done[CHX_HIP_MAX_NDIM] = {};
+    int64_t inside = dtype_size(t.dtype);
+    for (int i = 0; i < t.ndim; ++i) {
+        int at = -1;
+        for (int d = 0; d < t.ndim; ++d)
+            if (!done[d] && t.shape[d] > 1 && (at < 0 || std::abs(t.strides[d]) < std::abs(t.strides[at]))) at = d;
+        if (at < 0) break;
+        done[at] = true;
+        if (std::abs(t.strides[at]) < inside) return false;
+        inside += (t.shape[at] - 1) * std::abs(t.strides[at]);
+    }
+    return true;
 }
 
 // One array given twice.

@@ -562,6 +562,7 @@ extern "C" int chx_hip_expert_combine(const chx_hip_tensor* x, const chx_hip_ten
         CHX_REQUIRE(r->dtype == y->dtype && same_shape(*r, *y), "%s: r must have the type and shape of y", op);
     }
     if (T == 0 || N == 0) return CHX_HIP_OK;
+    CHX_REQUIRE(elements_apart(*y), "%s: elements of y overlap", op);
     CHX_REQUIRE(!arrays_overlap(*x, *y) && !arrays_overlap(*weights, *y), "%s: y overlaps x or weights", op);
     CHX_REQUIRE(r == nullptr || same_array(*r, *y) || !arrays_overlap(*r, *y), "%s: r and y overlap and are not the same array", op);
     CombineArgs a;

@@ -184,6 +184,7 @@ int prepare_call(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32
         a.vector_r = a.r_col == ye && aligned_rows(a.r, a.r_row, r_rows, 4 * ye);
     }
     if (numel(*y) > 0) {
+        CHX_REQUIRE(elements_apart(*y), "linear plan: elements of y overlap");
         CHX_REQUIRE(numel(*x) == 0 || !arrays_overlap(*x, *y), "linear plan: x and y overlap");
         CHX_REQUIRE(r == nullptr || same_array(*r, *y) || !arrays_overlap(*r, *y), "linear plan: r and y overlap and are not the same array");
     }

@@ -455,7 +455,8 @@ enum { CHX_HIP_ACT_NONE = 0, CHX_HIP_ACT_RELU = 1, CHX_HIP_ACT_GELU = 2, CHX_HIP
  *   w_scale  float32 [N] / [E, N] of int8 weights (a weight is w * w_scale), else NULL
  *   b        float16 or float32 [N] / [E, N], or NULL
  * create() copies all of them and waits for the stream (CHX_HIP_EUNSUPPORTED on one that is being captured).  A plan belongs to the device it was created on and may be used by
- * several threads and streams at once; it must outlive the graphs that its runs were recorded into. */
+ * several threads and streams at once; it must outlive the graphs that its runs were recorded into.  destroy() waits for the device and is not for use while a stream is
+ * being captured. */
 typedef struct chx_hip_linear_plan chx_hip_linear_plan;
 int chx_hip_linear_plan_create(
         const chx_hip_tensor* w, const chx_hip_tensor* w_scale, const chx_hip_tensor* b, void* stream, chx_hip_linear_plan** plan);
@@ -466,7 +467,7 @@ void chx_hip_linear_plan_destroy(chx_hip_linear_plan* plan);
  *      one run of rows
  *   y  [.., N] likewise, float16 or float32 (float32 only for float32 x)
  *   r  NULL, or of y's shape and type; may be y itself
- * Sums and epilogue are float32, in an order that depends on the sizes alone; the result is rounded once.  y must not overlap x,
+ * Sums and epilogue are float32, in an order that depends on the sizes alone; the result is rounded once.  y must not overlap x, itself,
  * nor r unless it is r.  workspace: for many rows that are not whole 16-byte pieces, aligned to 16; y_rows: rows of y. */
 int chx_hip_linear_plan_workspace(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int64_t y_rows, size_t* bytes);
 int chx_hip_linear_plan_run(
@@ -488,7 +489,7 @@ int chx_hip_linear_plan_run_experts(
  *   the top_groups best groups' experts can be chosen
  *   the k = experts->shape[1] largest keys are chosen, largest first; of equal ones (groups likewise) the lower index first
  *   weight = s of the chosen (not the key), over the sum of the chosen if `normalize` (0 where that sum is 0), times `scale`
- * A NaN logit counts as -inf, +inf as the largest finite number; an expert with -inf has s = 0 and is chosen only when the others run out.
+ * A NaN logit counts as -inf, +inf as the largest finite number; an expert with -inf has s = 0 (without bias and groups it is chosen only when the others run out).
  *   experts int32 [T, k];  weights float32 [T, k]
  *   order   int32 [T k]: the places t k + j, those of expert 0 first, of one expert in ascending order
  *   offsets int32 [E + 1]: where each expert's places begin in order
@@ -500,7 +501,7 @@ int chx_hip_expert_routing(
         void* workspace, size_t workspace_bytes, void* stream);
 
 /* y[t, n] = sum_j weights[t, j] * x[t k + j, n] + r[t, n]: what k experts made of a row, weighted; sums in float32.  x [T k, N] and y,
- * r [T, N] float16 or float32, of one type, any strides; weights float32 [T, k], contiguous.  A row whose weight is 0 adds nothing,
+ * r [T, N] float16 or float32, of one type, any strides (y's elements apart); weights float32 [T, k], contiguous.  A row whose weight is 0 adds nothing,
  * whatever it holds.  r: NULL, or y itself, or an array that does not overlap y. */
 int chx_hip_expert_combine(const chx_hip_tensor* x, const chx_hip_tensor* weights, const chx_hip_tensor* r, chx_hip_tensor* y, void* stream);
 

@@ -73,6 +73,8 @@ def runs(host):
                        ((half, shifted(x, 1), y), "address"), ((half, x, shifted(y, 1)), "address"),
                        ((half, inside, T("float16", (5, 64), [100, 1], base=both.data)), "x and y overlap"),
                        ((half, x, y, shifted(y, 2)), "r and y overlap"),
+                       ((half, x, T("float16", (5, 64), [0, 1])), "elements of y overlap"), ((half, x, T("float16", (5, 64), [63, 1])), "elements of y overlap"),
+                       ((half, x, T("float16", (5, 64), [1, 4])), "elements of y overlap"),
                        ((half, T("float16", (1 << 31, 32), [0, 1]), T("float16", (1 << 31, 64), [0, 1])), "2^31 rows")]:
         refused(host, run(*args), text)
     odd = T("float16", (5, 32))
@@ -155,7 +157,7 @@ def combine(host):
     for args, text in [((None, w, y), "null tensor"), ((T("int8", (6, 32)), w, y), "float16 or float32"), ((x, T("float16", (3, 2)), y), "weights must be"), ((x, T("float32", (2, 2)), y), "must have 4 rows"),
                        ((x, T("float32", (3, 2), [4, 1]), y), "weights must be"), ((x, w, T("float32", (3, 32))), "of the type of x"), ((x, w, T("float16", (3, 31))), "y must be"),
                        ((x, w, y, T("float16", (2, 32))), "r must have"), ((x, w, T("float16", (3, 32), base=x.data)), "overlaps x"), ((x, w, y, shifted(y, 2)), "not the same array"),
-                       ((shifted(x, 1), w, y), "whole elements")]:
+                       ((shifted(x, 1), w, y), "whole elements"), ((x, w, T("float16", (3, 32), [0, 1])), "elements of y overlap")]:
         refused(host, run(*args), text)
     host.check(run(x, w, y, y))
     assert len(host.launches()) == 1
