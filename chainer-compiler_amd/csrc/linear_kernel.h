@@ -179,38 +179,36 @@ struct Rows {
     int32_t expert, first, count;  // count 0: no such tile
 };
 
-// Tile `index` of the experts' tiles of `height` rows each.  kWholeFirst: first the whole ones of expert 0 on, then what is left of each expert's rows, so that
-// the shorter ones come last; else those of expert 0, of expert 1 and so on (one search instead of two, for tiles that take a few us).
-// Every wavefront finds it by itself, 64 experts at a time.
-template <bool kWholeFirst>
+// Tile `index` of the experts' tiles of up to `height` rows: those of expert 0, of expert 1 and so on, each expert's of one size, a multiple of `grain` (a divisor of
+// height).  With whole tiles first and what is left of each expert's rows behind them, tiles of few rows were bound by their weights, which came a second time: 4096 rows to 4 of
+// 32 experts of 4096 x 2048 took 313 us instead of 296, 2048 rows to 8 of 128 experts of 2048 x 768 200 instead of 188.  (384 rows to each of the 32, 256 and 128 of
+// them to a tile, took as long as 512.)  Every
+// wavefront finds its tile by itself, 64 experts at a time.
+template <int kGrain>
 __device__ __forceinline__ Rows expert_rows(const LinearArgs& a, int32_t index, int32_t height) {
     const int lane = threadIdx.x & 63;
-#pragma unroll 1
-    for (int pass = 0; pass < (kWholeFirst ? 2 : 1); ++pass) {
-        for (int32_t e0 = 0; e0 < a.experts; e0 += 64) {
-            const int32_t e = e0 + lane;
-            int32_t lo = 0, hi = 0;
-            if (e < a.experts) {  // (offsets from device memory: kept inside the order whatever they say)
-                lo = min(max(a.offsets[e], 0), a.M);
-                hi = min(max(a.offsets[e + 1], lo), a.M);
-            }
-            const int32_t whole = (hi - lo) / height, more = (hi - lo) % height != 0;
-            const int32_t tiles = !kWholeFirst ? whole + more : pass == 0 ? whole : more;
-            int32_t upto = tiles;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const int32_t v = __shfl_up(upto, d);
-                if (lane >= d) upto += v;
-            }
-            const uint64_t past = __builtin_amdgcn_ballot_w64(upto > index);
-            if (past) {
-                const int at = __builtin_ctzll(past);
-                const int32_t first = __builtin_amdgcn_readlane(lo, at), count = __builtin_amdgcn_readlane(hi, at) - first;
-                const int32_t t = pass == 1 ? count / height : index - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(tiles, at));
-                return {e0 + at, first + t * height, min(count - t * height, height)};
-            }
-            index -= __builtin_amdgcn_readlane(upto, 63);
+    for (int32_t e0 = 0; e0 < a.experts; e0 += 64) {
+        const int32_t e = e0 + lane;
+        int32_t lo = 0, hi = 0;
+        if (e < a.experts) {  // (offsets from device memory: kept inside the order whatever they say)
+            lo = min(max(a.offsets[e], 0), a.M);
+            hi = min(max(a.offsets[e + 1], lo), a.M);
         }
+        const int32_t tiles = (hi - lo) / height + ((hi - lo) % height != 0);
+        int32_t upto = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int32_t v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > index);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            const int32_t first = __builtin_amdgcn_readlane(lo, at), count = __builtin_amdgcn_readlane(hi, at) - first, of = __builtin_amdgcn_readlane(tiles, at);
+            const int32_t t = index - (__builtin_amdgcn_readlane(upto, at) - of), each = ((count + of - 1) / of + kGrain - 1) / kGrain * kGrain;
+            return {e0 + at, first + t * each, min(count - t * each, each)};
+        }
+        index -= __builtin_amdgcn_readlane(upto, 63);
     }
     return {0, 0, 0};
 }
@@ -260,7 +258,7 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
     const int32_t columns = blockIdx.x % a.tiles_n, tile = blockIdx.x / a.tiles_n;
     Rows t;
     if constexpr (kExperts) {
-        t = expert_rows<false>(a, tile, 16 * kRowTiles);
+        t = expert_rows<16>(a, tile, 16 * kRowTiles);
         if (t.count <= 0) return;
     } else {
         t = {0, tile * 16 * kRowTiles, min(a.M - tile * 16 * kRowTiles, 16 * kRowTiles)};
@@ -399,13 +397,13 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
 //
 // x lies in rows of whole blocks, in 16-byte pieces (others are brought into such first, linear_plan.hip: loaded through registers here, 4096 rows of
 // 4097 x 16384 took 636 us instead of 443).
-// A work-group of kWavesM x kWavesN wavefronts, each 16 kRowFragments rows and 64 columns.  w comes into a ring of three units in LDS, x into one of
+// A work-group of kWavesM x kWavesN wavefronts, each 16 kRowFragments rows (every kWavesM-th 16 of the tile's) and 64 columns.  w comes into a ring of three units in LDS, x into one of
 // three blocks of two units (a block is 128 bytes of every row: of half a line at a time, the other half was fetched again where the
 // rows lie a power of two apart: 435 us instead of 419 for 4096 x 4096 x 16384), by asynchronous copies two and three units ahead.  While a unit
 // is multiplied from registers, the next one's fragments come from LDS into others, so its place in the ring is free a unit early.
 // A row of x in a block is eight pieces of 16 bytes; piece c of row r lies at place c ^ (r & 7): the sixteen rows that a fragment is
 // read from then do not meet in one bank.
-constexpr int32_t kPieceColumns = 4;
+constexpr int32_t kPieceRows = 2, kPieceColumns = 4;
 
 template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN>
 struct TileShape {
@@ -427,13 +425,13 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     const int wm = wave / kWavesN, wn = wave % kWavesN;
     // Work-groups that follow each other run on different XCDs, each with its own L2: an eighth of the tiles to each, in blocks
     // of 8 tiles of rows, so that what a block reads stays there.  Experts' tiles, of which there may be fewer than the grid has, are dealt out to the XCDs in
-    // pieces of 2 x kPieceColumns, so that the last XCD is not left with those that are not there.
+    // pieces of kPieceRows x kPieceColumns, so that the last XCD is not left with those that are not there.
     int32_t tm, tn;
     if constexpr (kExperts) {
-        const int32_t across = (a.tiles_n + kPieceColumns - 1) / kPieceColumns, at = blockIdx.x >> 3, inside = at % (2 * kPieceColumns);
-        const int32_t piece = at / (2 * kPieceColumns) * 8 + (blockIdx.x & 7);
-        tm = piece / across * 2 + (inside & 1);
-        tn = piece % across * kPieceColumns + (inside >> 1);
+        const int32_t across = (a.tiles_n + kPieceColumns - 1) / kPieceColumns, at = blockIdx.x >> 3, inside = at % (kPieceRows * kPieceColumns);
+        const int32_t piece = at / (kPieceRows * kPieceColumns) * 8 + (blockIdx.x & 7);
+        tm = piece / across * kPieceRows + inside % kPieceRows;
+        tn = piece % across * kPieceColumns + inside / kPieceRows;
         if (tn >= a.tiles_n) return;
     } else {
         const int32_t all = a.tiles_m * a.tiles_n, q = all >> 3, rest = all & 7, xcd = blockIdx.x & 7, id = xcd * q + min(xcd, rest) + ((int32_t)blockIdx.x >> 3);
@@ -444,7 +442,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     }
     Rows t;
     if constexpr (kExperts) {
-        t = expert_rows<true>(a, tm, kBM);
+        t = expert_rows<16 * kWavesM>(a, tm, kBM);
         if (t.count <= 0) return;
     } else {
         t = {0, tm * kBM, min(a.M - tm * kBM, kBM)};
@@ -484,7 +482,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     for (int i = 0; i < kRowFragments; ++i)
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int x_lane = (wm * kRowFragments * 16 + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+    const int x_lane = (wm * 16 + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
     const int w_lane = S::kAtW + wn * O::kUnit + lane * 16;
     struct Unit {
         u32x4 w[O::kPieces], x[kRowFragments];
@@ -492,7 +490,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     // (half: which of its block's two units)
     auto read_w = [&](Unit& r, int p, int place) __attribute__((always_inline)) { r.w[p] = *reinterpret_cast<const u32x4*>(tile_lds + place * S::kUnits + w_lane + p * 1024); };
     auto read_x = [&](Unit& r, int i, int place, int half) __attribute__((always_inline)) {
-        r.x[i] = *reinterpret_cast<const u32x4*>(tile_lds + place * S::kBlock + (x_lane ^ (half * 64)) + i * 2048);
+        r.x[i] = *reinterpret_cast<const u32x4*>(tile_lds + place * S::kBlock + (x_lane ^ (half * 64)) + i * kWavesM * 2048);
     };
     auto read_unit = [&](Unit& r, int place_x, int half, int place_w) __attribute__((always_inline)) {
 #pragma unroll
@@ -525,10 +523,12 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
         __syncthreads();
         int here_x = 0, here_w = 0;  // places in the rings of this block and unit
         auto behind = [](int place) __attribute__((always_inline)) { return place + 1 == S::kRing ? 0 : place + 1; };
-        // One unit, the block's first or second, from `now`, with the next one's fragments into `then`.  A wavefront without rows takes part in the copies alone: half a
-        // tile at the end of an expert's rows.
-        auto step = [&](int32_t block, auto second, auto has_rows, const Unit& now, Unit& then) __attribute__((always_inline)) {
-            constexpr bool kSecond = decltype(second)::value, kHasRows = decltype(has_rows)::value;
+        const int32_t fragments = (t.count - wm * 16 + 16 * kWavesM - 1) / (16 * kWavesM);  // of this wavefront's that have rows
+        // One unit, the block's first or second, from `now`, with the next one's fragments into `then`.  `whole`: with all of this wavefront's
+        // fragments; else with those that have rows, each behind a branch (an expert's tile, of which a quarter or more is missing: 296 us for 4096 rows to 4 of 32 experts of 4096 x
+        // 2048 instead of 310; but 600 rows of 4096 x 4096, the last 88 rows of which are a tile, 37.5 instead of 31.8).
+        auto step = [&](int32_t block, auto second, auto whole, const Unit& now, Unit& then) __attribute__((always_inline)) {
+            constexpr bool kSecond = decltype(second)::value, kWhole = decltype(whole)::value;
             const int next_x = behind(here_x), next_w = behind(here_w), before_x = behind(next_x);
             // The copies that the next unit needs are there, of w from two steps ago, of x from three or more; and this wavefront has read this unit.
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kCopiesX + kCopiesW) : "memory");
@@ -538,34 +538,33 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
             // What is read for the next unit and copied ahead goes between the products: copies one behind the other would keep the
             // wavefront from its products until the last of them is under way.
             u32x4 w[4];
-            if constexpr (kHasRows) fragments_of(w, now);
+            fragments_of(w, now);
             constexpr int kHalf = kCopiesX / 2, kCopies = kCopiesW + kHalf, kPiecesEach = (O::kPieces + kRowFragments - 1) / kRowFragments;
 #pragma unroll
             for (int i = 0; i < kRowFragments; ++i) {
-                if constexpr (kHasRows) {
 #pragma unroll
-                    for (int p = i * kPiecesEach; p < O::kPieces && p < (i + 1) * kPiecesEach; ++p) read_w(then, p, next_w);
-                    read_x(then, i, kSecond ? next_x : here_x, kSecond ? 0 : 1);
-                }
+                for (int p = i * kPiecesEach; p < O::kPieces && p < (i + 1) * kPiecesEach; ++p) read_w(then, p, next_w);
+                if (kWhole || i < fragments) read_x(then, i, kSecond ? next_x : here_x, kSecond ? 0 : 1);
 #pragma unroll
                 for (int c = i * kCopies / kRowFragments; c < (i + 1) * kCopies / kRowFragments; ++c) {
                     if (c < kCopiesW) copy_w(c, ahead_w, here_w);
                     else copy_x(c - kCopiesW + (kSecond ? 0 : kHalf), ahead, kSecond ? here_x : before_x);
                 }
-                if constexpr (kHasRows) multiply(w, now, i);
+                if (kWhole || i < fragments) multiply(w, now, i);
                 __builtin_amdgcn_sched_barrier(0);
             }
             here_w = next_w;
             if constexpr (kSecond) here_x = next_x;
         };
-        auto all_steps = [&](auto has_rows) __attribute__((always_inline)) {
-            if constexpr (decltype(has_rows)::value) read_unit(even, 0, 0, 0);
+        auto all_steps = [&](auto whole) __attribute__((always_inline)) {
+            read_unit(even, 0, 0, 0);
             for (int32_t block = 0; block < blocks; ++block) {
-                step(block, std::false_type(), has_rows, even, odd);
-                step(block, std::true_type(), has_rows, odd, even);
+                step(block, std::false_type(), whole, even, odd);
+                step(block, std::true_type(), whole, odd, even);
             }
         };
-        if (wm * kRowFragments * 16 < t.count) all_steps(std::true_type());
+        if constexpr (!kExperts) all_steps(std::true_type());
+        else if (fragments * 4 > kRowFragments * 3) all_steps(std::true_type());
         else all_steps(std::false_type());
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -600,7 +599,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 2
         for (int i = 0; i < kPassRows / 8; ++i) {
-            const int r = i * 8 + (lane >> 3), row = rows[(wm * kRowFragments + pass * 2) * 16 + r];
+            const int r = i * 8 + (lane >> 3), row = rows[((pass * 2 + (r >> 4)) * kWavesM + wm) * 16 + (r & 15)];
             const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((lane & 7) * 2 ^ (r & 15)) << 4));
             const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((lane & 7) * 2 + 1) ^ (r & 15)) * 16);
             float v[8];
@@ -641,8 +640,8 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
     int64_t grid = (int64_t)a.tiles_m * a.tiles_n;
     if (kExperts) {  // (whole pieces, the same number for each XCD)
-        const int64_t pieces = (int64_t)((a.tiles_m + 1) / 2) * ((a.tiles_n + kPieceColumns - 1) / kPieceColumns);
-        grid = (pieces + 7) / 8 * 8 * 2 * kPieceColumns;
+        const int64_t pieces = (int64_t)((a.tiles_m + kPieceRows - 1) / kPieceRows) * ((a.tiles_n + kPieceColumns - 1) / kPieceColumns);
+        grid = (pieces + 7) / 8 * 8 * kPieceRows * kPieceColumns;
         CHX_REQUIRE(grid < (int64_t(1) << 31), "linear plan: too many results");
     }
     kernel<<<(unsigned)grid, S::kThreads, S::kLds, s>>>(a);

@@ -273,18 +273,19 @@ Choice choose(int64_t M, int64_t N, LinearType type) {
 
 // The same for experts, by the rows that each has on the average.  us with 16 x 64 / 32 x 64 / 64 x 64 / tiles of 64 x 128 / of 128 / of 256, experts' loads
 // as uneven as their normally distributed scores make them:
-//   64 experts of 1536 x 2048:  rows each  2   float16   47 /   46 /   62 /   59 /   73 /   78   int8    32 /   31 /   52 /   30 /   49 /   64
-//                                          8             58 /   52 /   65 /   66 /   78 /   82           41 /   35 /   62 /   37 /   54 /   70
-//                                         16             80 /   66 /   79 /   74 /   83 /   89           56 /   45 /   62 /   40 /   59 /   71
-//                                         32            123 /   94 /  102 /   90 /   89 /   96           87 /   62 /   77 /   50 /   63 /   81
-//   64 experts of 1024 x 2048:            64            128 /   94 /   95 /   76 /   78 /   87          101 /   65 /   75 /   46 /   56 /   68
-//   32 experts of 2048 x 4096:           128            497 /  321 /  241 /  185 /  163 /  176          318 /  189 /  181 /  123 /  121 /  157
-//                                        512           1849 / 1095 /  777 /  484 /  383 /  307         1192 /  648 /  585 /  355 /  312 /  297
-//   8 experts of 4096 x 4096:            512           1028 /  620 /  433 /  229 /  186 /  179          681 /  357 /  310 /  177 /  164 /  175
-// (float32, the first four: 8 rows each 136 / 142 / 234 / 183, 32 rows 307 / 235 / 283 / 278, 64 rows 358 / 246 / 278 / 243, 128 rows 1364 / 850 / 784 / 659.)
+//   64 experts of 1536 x 2048:  rows each  2   float16   47 /   46 /   63 /   58 /   72 /   76   int8    32 /   32 /   54 /   30 /   51 /   68
+//                                          8             58 /   52 /   67 /   65 /   77 /   81           41 /   36 /   65 /   37 /   55 /   70
+//                                         16             80 /   66 /   79 /   73 /   82 /   87           56 /   46 /   66 /   40 /   60 /   72
+//                                         32            123 /   94 /  103 /   90 /   88 /   93           87 /   63 /   78 /   51 /   64 /   79
+//   64 experts of 1024 x 2048:            64            128 /   94 /   94 /   74 /   76 /   86          101 /   65 /   78 /   46 /   56 /   75
+//   32 experts of 2048 x 4096:           128            497 /  320 /  241 /  167 /  152 /  159          318 /  190 /  184 /  121 /  124 /  157
+//                                        512           1849 / 1093 /  780 /  433 /  345 /  295         1192 /  658 /  588 /  356 /  308 /  297
+//   8 experts of 4096 x 4096:            512           1028 /  621 /  434 /  206 /  178 /  180          681 /  357 /  310 /  180 /  165 /  183
+// (float32, the first four: 8 rows each 136 / 141 / 233 / 138, 32 rows 307 / 242 / 281 / 221, 64 rows 358 / 242 / 276 / 194, 128 rows 1364 / 853 / 784 / 631; 32 rows each
+// of 1024 x 2048 202 / 155 / 198 / 162.)
 Choice choose_for_experts(int64_t M, int64_t experts, int64_t N, LinearType type) {
     const int64_t each = (M + experts - 1) / experts;
-    if (each > (type == kFloatFloat ? 64 : type == kHalfHalf ? 24 : 12))
+    if (each > (type == kFloatFloat ? 32 : type == kHalfHalf ? 24 : 12))
         return {0, 0, type == kFloatFloat || each <= 96 ? kTile64 : each >= 256 && type == kHalfHalf ? kTile256 : kTile128};
     const int row_tiles = each <= (type == kFloatFloat ? 8 : 4) ? 1 : 2;
     const int64_t wide = (M / (16 * row_tiles) + std::min(M, experts)) * ((N + kGroupRows - 1) / kGroupRows);

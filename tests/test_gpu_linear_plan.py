@@ -219,6 +219,7 @@ def routed(seed, places, experts, empty=()):
     (1, 1, 1, 64, 64), (8, 70, 2, 130, 48), (96, 130, 8, 64, 200),                 # a row or none to an expert, more than 64 experts
     (640, 3, 2, 100, 130), (3000, 20, 1, 64, 96), (9000, 3, 3, 128, 1100),         # tiles of 128 and of 256 rows
     (600, 18, 2, 200, 150), (700, 9, 1, 96, 90),                                   # tiles of 64 rows
+    (1100, 4, 1, 96, 300), (600, 5, 1, 130, 140),                                  # an expert's rows over two tiles that they do not fill
 ])
 def test_experts(g, kind, w_kind, places, experts, fan, k, n):
     chosen, order, offsets = routed(21, places, experts, empty=(0,) if experts > 1 else ())
