@@ -205,7 +205,7 @@ __device__ __forceinline__ Rows expert_rows(const LinearArgs& a, int32_t index, 
         if (past) {
             const int at = __builtin_ctzll(past);
             const int32_t first = __builtin_amdgcn_readlane(lo, at), count = __builtin_amdgcn_readlane(hi, at) - first, of = __builtin_amdgcn_readlane(tiles, at);
-            const int32_t t = index - (__builtin_amdgcn_readlane(upto, at) - of), each = ((count + of - 1) / of + kGrain - 1) / kGrain * kGrain;
+            const int32_t t = index - (__builtin_amdgcn_readlane(upto, at) - of), each = (int32_t)((((uint32_t)count + of - 1) / of + kGrain - 1) / kGrain * kGrain);
             return {e0 + at, first + t * each, min(count - t * each, each)};
         }
         index -= __builtin_amdgcn_readlane(upto, 63);
@@ -403,7 +403,14 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
 // is multiplied from registers, the next one's fragments come from LDS into others, so its place in the ring is free a unit early.
 // A row of x in a block is eight pieces of 16 bytes; piece c of row r lies at place c ^ (r & 7): the sixteen rows that a fragment is
 // read from then do not meet in one bank.
+// The tiles of experts that one XCD takes together: kPieceRows of rows times kPieceColumns, or of so many columns less that as few as may be are missing
+// from the last piece (work-groups without a tile, a quarter of all where three columns were counted as four: 2048 rows to 8 of 128 experts of 2048 x 768 164 us instead of
+// 188, 4096 rows to 8 of 64 of 2048 x 1280 217 instead of 269).
 constexpr int32_t kPieceRows = 2, kPieceColumns = 4;
+__host__ __device__ inline int32_t piece_columns(int32_t tiles_n) {
+    const int32_t across = (tiles_n + kPieceColumns - 1) / kPieceColumns;
+    return (tiles_n + across - 1) / across;
+}
 
 template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN>
 struct TileShape {
@@ -425,13 +432,13 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void linear_tile_kernel(
     const int wm = wave / kWavesN, wn = wave % kWavesN;
     // Work-groups that follow each other run on different XCDs, each with its own L2: an eighth of the tiles to each, in blocks
     // of 8 tiles of rows, so that what a block reads stays there.  Experts' tiles, of which there may be fewer than the grid has, are dealt out to the XCDs in
-    // pieces of kPieceRows x kPieceColumns, so that the last XCD is not left with those that are not there.
+    // pieces, so that the last XCD is not left with those that are not there.
     int32_t tm, tn;
     if constexpr (kExperts) {
-        const int32_t across = (a.tiles_n + kPieceColumns - 1) / kPieceColumns, at = blockIdx.x >> 3, inside = at % (kPieceRows * kPieceColumns);
-        const int32_t piece = at / (kPieceRows * kPieceColumns) * 8 + (blockIdx.x & 7);
+        const int32_t wide = piece_columns(a.tiles_n), across = (a.tiles_n + wide - 1) / wide, at = blockIdx.x >> 3, inside = at % (kPieceRows * wide);
+        const int32_t piece = at / (kPieceRows * wide) * 8 + (blockIdx.x & 7);
         tm = piece / across * kPieceRows + inside % kPieceRows;
-        tn = piece % across * kPieceColumns + inside / kPieceRows;
+        tn = piece % across * wide + inside / kPieceRows;
         if (tn >= a.tiles_n) return;
     } else {
         const int32_t all = a.tiles_m * a.tiles_n, q = all >> 3, rest = all & 7, xcd = blockIdx.x & 7, id = xcd * q + min(xcd, rest) + ((int32_t)blockIdx.x >> 3);
@@ -640,8 +647,9 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
     int64_t grid = (int64_t)a.tiles_m * a.tiles_n;
     if (kExperts) {  // (whole pieces, the same number for each XCD)
-        const int64_t pieces = (int64_t)((a.tiles_m + kPieceRows - 1) / kPieceRows) * ((a.tiles_n + kPieceColumns - 1) / kPieceColumns);
-        grid = (pieces + 7) / 8 * 8 * kPieceRows * kPieceColumns;
+        const int32_t wide = piece_columns(a.tiles_n);
+        const int64_t pieces = (int64_t)((a.tiles_m + kPieceRows - 1) / kPieceRows) * ((a.tiles_n + wide - 1) / wide);
+        grid = (pieces + 7) / 8 * 8 * kPieceRows * wide;
         CHX_REQUIRE(grid < (int64_t(1) << 31), "linear plan: too many results");
     }
     kernel<<<(unsigned)grid, S::kThreads, S::kLds, s>>>(a);
