@@ -403,6 +403,7 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
 // is multiplied from registers, the next one's fragments come from LDS into others, so its place in the ring is free a unit early.
 // A row of x in a block is eight pieces of 16 bytes; piece c of row r lies at place c ^ (r & 7): the sixteen rows that a fragment is
 // read from then do not meet in one bank.
+
 // The tiles of experts that one XCD takes together: kPieceRows of rows times kPieceColumns, or of so many columns less that as few as may be are missing
 // from the last piece (work-groups without a tile, a quarter of all where three columns were counted as four: 2048 rows to 8 of 128 experts of 2048 x 768 164 us instead of
 // 188, 4096 rows to 8 of 64 of 2048 x 1280 217 instead of 269).
