@@ -176,10 +176,8 @@ def prepare(case, seed):
             s["logits"][1, s["tokens"][1]] = 1.0
             s["tokens"][2] = -1  # a place without a token
     s["case"] = dict(case)
-    if own:
-        s["ops"] = _ops()
-        if "w" in s:  # the layer's weights, laid out once when a program loads them
-            s["plan"] = s["ops"].LinearPlan(s["w"], b=s["b"], w_scale=s["scale"])
+    if own and "w" in s:  # the layer's weights, laid out once when a program loads them
+        s["plan"] = _ops().LinearPlan(s["w"], b=s["b"], w_scale=s["scale"])
     return s
 
 
@@ -233,8 +231,8 @@ def _experts(s):
 def _routing(s):
     c, logits = s["case"], s["logits"]
     if own:
-        return s["ops"].ExpertRouting(logits, c["top"], bias=s["bias"], score=c["score"], groups=c["groups"], top_groups=c["top_groups"],
-                                      group_best=c["group_best"], normalize=c["normalize"], scale=1.5)
+        return _ops().ExpertRouting(logits, c["top"], bias=s["bias"], score=c["score"], groups=c["groups"], top_groups=c["top_groups"],
+                                    group_best=c["group_best"], normalize=c["normalize"], scale=1.5)
     # (64 bits: the choice is between values that may differ in the last of 32)
     t, e, x = c["tokens"], c["experts"], logits.double()
     score = torch.softmax(x, dim=1) if c["score"] == "softmax" else 1 / (1 + torch.exp(-x))
@@ -257,7 +255,7 @@ def _routing(s):
 def _combine(s):
     c, x = s["case"], s["x"]
     if own:
-        return s["ops"].ExpertCombine(x, s["weights"], r=s["r"])
+        return _ops().ExpertCombine(x, s["weights"], r=s["r"])
     v = (x.reshape(c["tokens"], c["top"], -1).float() * s["weights"][:, :, None]).sum(1)
     return (v if s["r"] is None else v + s["r"].float()).to(x.dtype)
 
@@ -265,7 +263,7 @@ def _combine(s):
 def _logprobs(s):
     c, logits, tokens = s["case"], s["logits"], s["tokens"]
     if own:
-        return s["ops"].TokenLogProbs(logits, tokens, top=c["top"])
+        return _ops().TokenLogProbs(logits, tokens, top=c["top"])
     x = logits.float()
     d = x - x.max(dim=1, keepdim=True).values
     e = torch.exp(d)
