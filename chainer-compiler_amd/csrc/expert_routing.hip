@@ -119,9 +119,9 @@ __device__ void route(const RoutingArgs& a, int32_t t, double* keys, int32_t* ex
     const float base = most == -INFINITY ? 0.f : most;
     typedef typename std::conditional<kExact, uint64_t, uint32_t>::type Key;
     Key key[kPer];  // 0: not to be had (any more)
-    double score[kExact ? kPer : 1];
+    double sum = 0.0;  // of the softmax
     if constexpr (kExact) {
-        double sum = 0.0;
+        double score[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int e = lane + 64 * i;
@@ -183,18 +183,18 @@ __device__ void route(const RoutingArgs& a, int32_t t, double* keys, int32_t* ex
         for (int i = 0; i < kPer; ++i) key[i] = lane + 64 * i < a.E ? sortable(x[i]) : 0;
     }
     int32_t chosen = 0;
-    float of_chosen = 0.f;  // logit, or score
+    float of_chosen = -INFINITY;  // its logit
     for (int j = 0; j < a.k; ++j) {
         // this lane's best, the largest of all, and the lowest index among those that have it
         Key best = key[0];
         int32_t at = lane;
-        float value = kExact ? (float)score[0] : x[0];
+        float value = x[0];
 #pragma unroll
         for (int i = 1; i < kPer; ++i) {
             const bool better = key[i] > best;
             best = better ? key[i] : best;
             at = better ? lane + 64 * i : at;
-            value = better ? (kExact ? (float)score[kExact ? i : 0] : x[i]) : value;
+            value = better ? x[i] : value;
         }
         const uint32_t upper = kExact ? (uint32_t)((uint64_t)best >> 32) : (uint32_t)best;
         const uint32_t most_upper = wave_max(upper);
@@ -217,27 +217,35 @@ __device__ void route(const RoutingArgs& a, int32_t t, double* keys, int32_t* ex
         for (int i = 0; i < kPer; ++i)
             if (lane + 64 * i == which) key[i] = 0;
     }
-    float w = 0.f;
-    if constexpr (kExact) {
-        w = lane < a.k ? of_chosen : 0.f;
-    } else if (a.sigmoid) {
-        w = lane < a.k && of_chosen != -INFINITY ? 1.f / (1.f + expf(-of_chosen)) : 0.f;
-    } else {
-        w = lane < a.k ? expf(of_chosen - base) : 0.f;
-        if (!a.normalize) {
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) sum += expf(x[i] - base);
-            sum = wave_sum(sum);
-            w = sum > 0.f ? w / sum : 0.f;
+    if (kExact || a.sigmoid) {
+        // (Scores that only 64 bits hold still share a row among them, so the rounding to 32 comes last: with scores rounded first, rows whose logits all lay
+        // below -88 lost their experts.  A lane has one chosen expert, so this is one exponential and one division of 64 bits to a row.)
+        double w = 0.0;
+        if (lane < a.k && of_chosen != -INFINITY) {
+            w = a.sigmoid ? 1.0 / (1.0 + exp(-(double)of_chosen)) : exp((double)of_chosen - (double)base);
+            if (!a.sigmoid) w = w / sum;
         }
-    }
-    if (a.normalize) {
-        const float sum = wave_sum(w);
-        w = sum > 0.f ? w / sum : 0.f;
+        if (a.normalize) {
+            const double all = wave_sum(w);
+            w = all > 0.0 ? w / all : 0.0;
+        }
+        *weight = (float)(w * (double)a.scale);
+    } else {
+        float w = lane < a.k ? expf(of_chosen - base) : 0.f;
+        if (!a.normalize) {
+            float all = 0.f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) all += expf(x[i] - base);
+            all = wave_sum(all);
+            w = all > 0.f ? w / all : 0.f;
+        } else {
+            // (the largest logit is among the chosen: their sum is 1 or more, or 0 in a row without any)
+            const float all = wave_sum(w);
+            w = all > 0.f ? w / all : 0.f;
+        }
+        *weight = w * a.scale;
     }
     *expert = chosen;
-    *weight = w * a.scale;
 }
 
 // The places [first, first + count) of the routing into the order, ascending; one wavefront.  at: LDS, where each expert's next place goes.

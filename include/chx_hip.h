@@ -488,7 +488,8 @@ int chx_hip_linear_plan_run_experts(
  *   the E experts are `groups` groups of neighbours; a group's score is the sum of its `group_best` (1 or 2) best keys, and only
  *   the top_groups best groups' experts can be chosen
  *   the k = experts->shape[1] largest keys are chosen, largest first; of equal ones (groups likewise) the lower index first
- *   weight = s of the chosen (not the key), over the sum of the chosen if `normalize` (0 where that sum is 0), times `scale`
+ *   weight = s of the chosen (not the key), over the sum of the chosen if `normalize` (0 where that sum is 0 in 64 bits), times `scale`; of a softmax without bias and
+ *   groups in float32, else in 64 bits and rounded at the end
  * A NaN logit counts as -inf, +inf as the largest finite number; an expert with -inf has s = 0 (without bias and groups it is chosen only when the others run out).
  *   experts int32 [T, k];  weights float32 [T, k]
  *   order   int32 [T k]: the places t k + j, those of expert 0 first, of one expert in ascending order

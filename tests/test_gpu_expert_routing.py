@@ -119,6 +119,39 @@ def test_a_bias_that_is_not_finite(g):
     check(g, normal(7, (9, 16), FLOAT), 3, bias=bias, groups=4, top_groups=2, group_best=2)
 
 
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("E", [20, 70, 600])
+@pytest.mark.parametrize("score,low,choice", [("sigmoid", (-86.0, -104.0), None), ("sigmoid", (-100.0, -690.0), None), ("sigmoid", (-86.0, -104.0), "zeros"),
+                                              ("sigmoid", (-100.0, -690.0), "groups"), ("softmax", (-70.0, -110.0), "moved"), ("softmax", (-100.0, -690.0), "moved")])
+def test_weights_of_very_low_scores(g, score, low, choice, E, normalize):
+    """Scores that 64 bits hold and 32 do not: their shares, and what is left of them after a scale that brings them back.
+
+    The score, the sum of four of them and their quotient are off by less than 700 * 2^-52 (an exponent of up to 700, rounded to 64 bits) and a few roundings of 2^-53; the
+    result is rounded to float32 once, by 2^-24 of itself."""
+    T, k = 21, 4
+    first, last = low
+    logits = (first + (last - first) * torch.rand(T, E, generator=torch.Generator().manual_seed(31))).cuda()
+    bias, groups = None, 1
+    if choice == "moved":  # the experts that have the scores are switched off, the next best ones are chosen
+        logits[:, 2] = 0.5
+        logits[:, 5] = 0.0
+        bias = torch.zeros(E, device="cuda")
+        bias[2] = bias[5] = -math.inf
+    elif choice == "zeros":
+        bias = torch.zeros(E, device="cuda")
+    elif choice == "groups":
+        groups = 5
+    scale = 1.5 if normalize else 2.0 ** 100
+    got = g.ops.ExpertRouting(logits, k, bias=bias, score=score, groups=groups, top_groups=groups, normalize=normalize, scale=scale)
+    want = reference(logits, k, bias, score, groups, groups, 1, normalize, scale)
+    for i in (0, 2, 3):
+        assert torch.equal(got[i].cpu().long(), want[i])
+    y = got[1].double().cpu()
+    assert bool((want[1].sum(1) > 0).all()) and ((y - want[1]).abs() <= (2.0 ** -24 + 2.0 ** -40) * want[1] + 2.0 ** -150).all()
+    if normalize:
+        assert ((y.sum(1) - scale).abs() <= 4 * 2.0 ** -24 * scale).all()
+
+
 def test_strides_and_no_rows(g):
     space = normal(8, (80, 150), HALF)
     check(g, space[::2, 3:67], 4)
