@@ -81,7 +81,7 @@ __device__ __forceinline__ u32x4 chunk_of(const char* row, int64_t col, int32_t 
 }
 
 // gelu(v) = v Phi(v) = max(v, 0) - z Phi(-z), z = |v|.  For float16 results Phi(-z) = exp(-z^2 / 2) P(t), t = 1 / (1 + 0.4 z), with P fitted by least
-// squares to the relative error over 0 <= z <= 9: 2.6e-6, where rounding the result to float16 takes 4.9e-4.  Some 15 instructions; the
+// squares to the relative error over 0 <= z <= 9: 2.6e-6, with the rounding of the exponent up to 6e-6 at z = 9, where rounding the result to float16 takes 4.9e-4.  Some 15 instructions; the
 // library's erff takes three times as many.
 __device__ __forceinline__ float gelu_short(float v) {
     const float z = __builtin_fabsf(v);
@@ -97,9 +97,9 @@ __device__ __forceinline__ float gelu_short(float v) {
     return __builtin_fmaf(-fminf(z, 64.f), tail, fmaxf(v, 0.f));           // (infinite z: 0 of it)
 }
 
-template <LinearType kType, int kCount>
+// kShort: for a result that is rounded to float16, with hardware exponentials and reciprocals; else to float32's own accuracy.
+template <bool kShort, int kCount>
 __device__ __forceinline__ void activate(float (&v)[kCount], int32_t act) {
-    constexpr bool kFloat = Of<kType>::kFloat;
     switch (act) {
         case CHX_HIP_ACT_RELU:
 #pragma unroll
@@ -107,19 +107,19 @@ __device__ __forceinline__ void activate(float (&v)[kCount], int32_t act) {
             break;
         case CHX_HIP_ACT_GELU:
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) v[i] = kFloat ? 0.5f * v[i] * erfcf(-0.70710678f * v[i]) : gelu_short(v[i]);
+            for (int i = 0; i < kCount; ++i) v[i] = kShort ? gelu_short(v[i]) : 0.5f * v[i] * erfcf(-0.70710678f * v[i]);
             break;
         case CHX_HIP_ACT_GELU_TANH:
             // 0.5 v (1 + tanh u) = v / (1 + exp(-2 u))
 #pragma unroll
             for (int i = 0; i < kCount; ++i) {
                 const float u = 0.7978845608f * __builtin_fmaf(0.044715f * v[i] * v[i], v[i], v[i]);
-                v[i] = kFloat ? v[i] / (1.f + expf(-2.f * u)) : v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.8853901f * u));
+                v[i] = kShort ? v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.8853901f * u)) : v[i] / (1.f + expf(-2.f * u));
             }
             break;
         case CHX_HIP_ACT_SILU:
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) v[i] = kFloat ? v[i] / (1.f + expf(-v[i])) : v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950f * v[i]));
+            for (int i = 0; i < kCount; ++i) v[i] = kShort ? v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950f * v[i])) : v[i] / (1.f + expf(-v[i]));
             break;
         default: break;
     }
@@ -130,7 +130,8 @@ template <LinearType kType, int kCount>
 __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[kCount], int64_t row, int32_t n) {
     if (n >= a.N) return;
     const bool whole = n + kCount <= a.N;
-    activate<kType, kCount>(v, a.activation);
+    if (!Of<kType>::kFloat && a.y_half) activate<true, kCount>(v, a.activation);
+    else activate<false, kCount>(v, a.activation);
     if (a.r) {
         const char* p = a.r + row * a.r_row + (int64_t)n * a.r_col;
         if (whole && a.vector_r) {

@@ -467,7 +467,8 @@ void chx_hip_linear_plan_destroy(chx_hip_linear_plan* plan);
  *      one run of rows
  *   y  [.., N] likewise, float16 or float32 (float32 only for float32 x)
  *   r  NULL, or of y's shape and type; may be y itself
- * Sums and epilogue are float32, in an order that depends on the sizes alone; the result is rounded once.  y must not overlap x, itself,
+ * Sums and epilogue are float32, in an order that depends on the sizes alone; the result is rounded once.  (Activations of float16 results, which are rounded by up to 2^-11, are
+ * off by up to 2^-17 before that; those of float32 results, of whichever rows, by float32's own roundings.)  y must not overlap x, itself,
  * nor r unless it is r.  workspace: for many rows that are not whole 16-byte pieces, aligned to 16; y_rows: rows of y. */
 int chx_hip_linear_plan_workspace(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int64_t y_rows, size_t* bytes);
 int chx_hip_linear_plan_run(

@@ -93,6 +93,38 @@ def test_epilogue(g, kind, w_kind, act):
         check(plan.run(x, activation=act, r=r.half()), *formula(x, w, scale, b, act, r.half()), k)
 
 
+def activated(g, w_kind, values, act, r=None):
+    """act of each of the values as a float32 result of float16 rows: against the unit matrix the sums are the values themselves."""
+    n = 64
+    x = values.reshape(-1, n).cuda()
+    eye = torch.eye(n)
+    plan = g.ops.LinearPlan(eye.to(w_kind).cuda(), w_scale=torch.ones(n, device="cuda") if w_kind == torch.int8 else None)
+    return plan.run(x, activation=act, dtype=FLOAT, r=r).cpu().reshape(-1)
+
+
+@pytest.mark.parametrize("kind,w_kind", TYPES)
+@pytest.mark.parametrize("few", [True, False])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_float32_results_of_activations(g, kind, w_kind, few, act):
+    """Results of 32 bits, whatever the rows are: relative bounds, for every value from -11 to 11 (float16 ones: all there are; SiLU: from -80).
+
+    In units of 2^-24 of the result.  GELU, v erfc(-v / sqrt(2)) / 2: the argument is off by 1.5 units, which changes erfc by (v^2 + 1) times as much, erfc by 8, two
+    products by 2.  By tanh, v / (1 + exp(-2 u)): u of four roundings and three constants is off by 6 units, which changes the quotient by 2 |u| times as
+    much, exp by 4, a sum and a quotient by 3.  SiLU: exp 4, sum, quotient and its rounding 3.  Where exp(-2 u) is above 2^128 the quotient may be 0: it is |v| 2^-128 there, or less."""
+    v = torch.arange(0, 1 << 15, dtype=torch.int32).to(torch.int16).view(HALF)
+    v = v[(v <= (80 if act == "silu" else 11)) & (v >= 2.0 ** -10)]
+    v = torch.cat([-v, v[v <= 11]])
+    v = v[: len(v) // 64 * 64 if not few else 64 * 30]
+    if few:
+        v = torch.cat([v, torch.linspace(-11, 11, 64 * 2).half()])
+    y = activated(g, w_kind, v.to(kind), act).double()
+    x = v.double()
+    want = ACTS[act](x)
+    u = math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)
+    units = {"gelu": 1.5 * (x ** 2 + 1) + 10, "gelu_tanh": 12 * u.abs() + 7, "silu": 7.0 + 0 * x}[act]
+    assert ((y - want).abs() <= units * 2.0 ** -24 * want.abs() + x.abs() * 2.0 ** -127).all()
+
+
 @pytest.mark.parametrize("kind", [HALF, FLOAT])
 @pytest.mark.parametrize("m", [5, 200])
 def test_layouts(g, kind, m):
