@@ -6,6 +6,7 @@
 // rounded once.  w is the first operand of an instruction, so that a lane's results are neighbouring columns of one row of y.
 #pragma once
 
+#include <cfloat>
 #include <type_traits>
 
 #include "linear_plan.h"
@@ -97,9 +98,11 @@ __device__ __forceinline__ float gelu_short(float v) {
     return __builtin_fmaf(-fminf(z, 64.f), tail, fmaxf(v, 0.f));           // (infinite z: 0 of it)
 }
 
-// kShort: for a result that is rounded to float16, with hardware exponentials and reciprocals; else to float32's own accuracy.
+// kShort: for a result that is rounded to float16, with hardware exponentials and reciprocals; else to float32's own accuracy.  A sum of -inf gives the limit, 0: what is
+// multiplied with a factor that becomes 0 is kept finite (a NaN stays one in that factor).
 template <bool kShort, int kCount>
 __device__ __forceinline__ void activate(float (&v)[kCount], int32_t act) {
+    auto finite = [](float o) { return fmaxf(o, -FLT_MAX); };
     switch (act) {
         case CHX_HIP_ACT_RELU:
 #pragma unroll
@@ -107,19 +110,20 @@ __device__ __forceinline__ void activate(float (&v)[kCount], int32_t act) {
             break;
         case CHX_HIP_ACT_GELU:
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) v[i] = kShort ? gelu_short(v[i]) : 0.5f * v[i] * erfcf(-0.70710678f * v[i]);
+            for (int i = 0; i < kCount; ++i) v[i] = kShort ? gelu_short(v[i]) : 0.5f * finite(v[i]) * erfcf(-0.70710678f * v[i]);
             break;
         case CHX_HIP_ACT_GELU_TANH:
             // 0.5 v (1 + tanh u) = v / (1 + exp(-2 u))
 #pragma unroll
             for (int i = 0; i < kCount; ++i) {
                 const float u = 0.7978845608f * __builtin_fmaf(0.044715f * v[i] * v[i], v[i], v[i]);
-                v[i] = kShort ? v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.8853901f * u)) : v[i] / (1.f + expf(-2.f * u));
+                v[i] = kShort ? finite(v[i]) * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.8853901f * u)) : finite(v[i]) / (1.f + expf(-2.f * u));
             }
             break;
         case CHX_HIP_ACT_SILU:
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) v[i] = kShort ? v[i] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950f * v[i])) : v[i] / (1.f + expf(-v[i]));
+            for (int i = 0; i < kCount; ++i)
+                v[i] = kShort ? finite(v[i]) * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950f * v[i])) : finite(v[i]) / (1.f + expf(-v[i]));
             break;
         default: break;
     }

@@ -447,7 +447,7 @@ int chx_hip_softmax_f32(const chx_hip_tensor* x, int32_t axis, int32_t is_onnx_s
  * What lies in device memory (orders, offsets, tokens) is checked by the kernels: places outside their range are left out. */
 
 /* What an epilogue applies to a sum v.  GELU: v Phi(v), Phi the normal distribution; GELU_TANH: its approximation
- * 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))); SILU: v / (1 + exp(-v)). */
+ * 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))); SILU: v / (1 + exp(-v)).  All but NONE give 0 for -inf, and keep +inf and NaN. */
 enum { CHX_HIP_ACT_NONE = 0, CHX_HIP_ACT_RELU = 1, CHX_HIP_ACT_GELU = 2, CHX_HIP_ACT_GELU_TANH = 3, CHX_HIP_ACT_SILU = 4 };
 
 /* The weights of a layer, laid out once for its products:

@@ -125,6 +125,26 @@ def test_float32_results_of_activations(g, kind, w_kind, few, act):
     assert ((y - want).abs() <= units * 2.0 ** -24 * want.abs() + x.abs() * 2.0 ** -127).all()
 
 
+@pytest.mark.parametrize("kind,w_kind", TYPES)
+@pytest.mark.parametrize("rows", [2, 300])
+@pytest.mark.parametrize("act", sorted(ACTS))
+def test_activations_of_infinite_sums(g, kind, w_kind, rows, act):
+    """An infinite sum gives the activation's limit, in every type and in both kernels: itself, and 0 (without an activation itself) on the lower side; a NaN stays one."""
+    n = 64
+    x = torch.zeros(rows, n, dtype=kind)
+    x[:, 0], x[1:, 0] = math.inf, -math.inf
+    w = torch.zeros(n, n)
+    w[:, 0] = 1
+    b = torch.zeros(n, dtype=FLOAT)
+    b[7] = math.nan
+    plan = g.ops.LinearPlan(w.to(w_kind).cuda(), b=b.cuda(), w_scale=torch.ones(n, device="cuda") if w_kind == torch.int8 else None)
+    for dtype in {kind, FLOAT}:
+        y = plan.run(x.cuda(), activation=act, dtype=dtype).cpu()
+        assert bool(torch.isnan(y[:, 7]).all())
+        y[:, 7] = y[:, 6]
+        assert bool((y[0] == math.inf).all()) and bool((y[1:] == (0 if act else -math.inf)).all()), y[:2, :2]
+
+
 @pytest.mark.parametrize("kind", [HALF, FLOAT])
 @pytest.mark.parametrize("m", [5, 200])
 def test_layouts(g, kind, m):
