@@ -326,11 +326,12 @@ __global__ __launch_bounds__(64 * waves_of(kPer)) void routing_kernel(RoutingArg
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int e = threadIdx.x; e < a.E; e += 64 * waves_of(kPer)) counts[e] = 0;
     __syncthreads();
-    const int32_t begin = blockIdx.x * a.chunk, end = min(begin + a.chunk, a.T);
-    for (int32_t t = begin + wave; t < end; t += waves_of(kPer)) {
+    // (unsigned: with close to 2^31 rows, a chunk's end and the step behind it lie above)
+    const uint32_t begin = blockIdx.x * (uint32_t)a.chunk, end = min(begin + (uint32_t)a.chunk, (uint32_t)a.T);
+    for (uint32_t t = begin + wave; t < end; t += waves_of(kPer)) {
         int32_t e;
         float w;
-        route<kPer, kExact>(a, t, keys[wave], &e, &w);
+        route<kPer, kExact>(a, (int32_t)t, keys[wave], &e, &w);
         if (lane < a.k) {
             a.experts[(int64_t)t * a.k + lane] = e;
             a.weights[(int64_t)t * a.k + lane] = w;
@@ -373,8 +374,8 @@ __global__ __launch_bounds__(1024) void routing_order_kernel(RoutingArgs a) {
     if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[a.E] = total;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const int32_t begin = blockIdx.x * a.chunk, end = min(begin + a.chunk, a.T);
-    put_in_order(a.experts + (int64_t)begin * a.k, begin * a.k, (end - begin) * a.k, at, a.order, bits_of(a.E));
+    const uint32_t begin = blockIdx.x * (uint32_t)a.chunk, end = min(begin + (uint32_t)a.chunk, (uint32_t)a.T);
+    put_in_order(a.experts + (int64_t)begin * a.k, (int32_t)(begin * a.k), (int32_t)((end - begin) * a.k), at, a.order, bits_of(a.E));
 }
 
 template <int kPer>

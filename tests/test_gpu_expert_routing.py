@@ -179,6 +179,21 @@ def test_recorded_twice(g, T):
                 assert torch.equal(a, b)
 
 
+def test_almost_2_to_the_31_rows(g):
+    """The most rows there can be: the last chunk's end, and a wavefront's step behind it, are above 2^31.  (4 GB of logits, 26 GB of results.)"""
+    T = 2 ** 31 - 9
+    logits = torch.zeros(T, 1, dtype=HALF, device="cuda")
+    experts, weights, order, offsets = g.ops.ExpertRouting(logits, 1)
+    assert offsets.tolist() == [0, T]
+    step = 1 << 28
+    for first in range(0, T, step):
+        last = min(first + step, T)
+        assert not bool(experts[first:last].any()) and bool((weights[first:last] == 1).all())
+        assert torch.equal(order[first:last], torch.arange(first, last, dtype=torch.int32, device="cuda"))
+    del logits, experts, weights, order
+    torch.cuda.empty_cache()
+
+
 # ---- the weighted sum -----------------------------------------------------------------------------------
 
 def check_sum(g, x, weights, r=None, out=None):
