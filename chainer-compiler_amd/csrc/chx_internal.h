@@ -180,6 +180,16 @@ inline bool aligned(const void* p, size_t a) {
 }
 
 int launch_check(const char* kernel);
+// A launch has fewer than 2^32 threads.  Work of more groups of 256 goes in several: launch(first, count) for each.
+template <typename F>
+int in_launches(int64_t groups, const char* kernel, F launch) {
+    constexpr int64_t kMost = int64_t(1) << 23;
+    for (int64_t first = 0; first < groups; first += kMost) {
+        launch(first, (unsigned)(groups - first < kMost ? groups - first : kMost));
+        CHX_PROPAGATE(launch_check(kernel));
+    }
+    return CHX_HIP_OK;
+}
 
 // Stream-ordered scratch memory for one call.
 // device address of the scratch array of chx_hip_reduce_min_max_noalloc on the current device, looked up once (reduce_cast.hip)

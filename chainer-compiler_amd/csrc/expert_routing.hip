@@ -410,6 +410,7 @@ struct CombineArgs {
     char* y;
     int64_t x_row, x_col, r_row, r_col, y_row, y_col;  // bytes
     int64_t pieces, total;                              // of kWidth columns
+    int64_t first;                                      // work-group of this launch
     int32_t N, k;
 };
 
@@ -428,7 +429,7 @@ __device__ __forceinline__ void load_piece(const char* p, int64_t col, float* v)
 // Bound by bytes, each of x read once: a lane has 16 bytes of every row of a sum under way at a time (four rows; kWidth 1: one element, for arrays of other strides and alignments).
 template <typename T, int kWidth>
 __global__ __launch_bounds__(256) void expert_combine_kernel(CombineArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t at = (a.first + blockIdx.x) * 256 + threadIdx.x;
     if (at >= a.total) return;
     const int64_t t = at / a.pieces, n = (at - t * a.pieces) * kWidth;
     const char* x = a.x + t * a.k * a.x_row + n * a.x_col;
@@ -594,15 +595,15 @@ extern "C" int chx_hip_expert_combine(const chx_hip_tensor* x, const chx_hip_ten
     a.k = (int32_t)k;
     a.pieces = wide ? N / (16 / es) : N;
     a.total = T * a.pieces;
-    const int64_t blocks = (a.total + 255) / 256;
-    CHX_REQUIRE(blocks < (int64_t(1) << 31), "%s: too many results", op);
     const hipStream_t s = as_stream(stream);
-    if (es == 2) {
-        if (wide) expert_combine_kernel<_Float16, 8><<<(unsigned)blocks, 256, 0, s>>>(a);
-        else expert_combine_kernel<_Float16, 1><<<(unsigned)blocks, 256, 0, s>>>(a);
-    } else {
-        if (wide) expert_combine_kernel<float, 4><<<(unsigned)blocks, 256, 0, s>>>(a);
-        else expert_combine_kernel<float, 1><<<(unsigned)blocks, 256, 0, s>>>(a);
-    }
-    return launch_check("expert_combine_kernel");
+    return in_launches((a.total + 255) / 256, "expert_combine_kernel", [&](int64_t first, unsigned count) {
+        a.first = first;
+        if (es == 2) {
+            if (wide) expert_combine_kernel<_Float16, 8><<<count, 256, 0, s>>>(a);
+            else expert_combine_kernel<_Float16, 1><<<count, 256, 0, s>>>(a);
+        } else {
+            if (wide) expert_combine_kernel<float, 4><<<count, 256, 0, s>>>(a);
+            else expert_combine_kernel<float, 1><<<count, 256, 0, s>>>(a);
+        }
+    });
 }

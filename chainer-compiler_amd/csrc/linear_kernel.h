@@ -409,15 +409,6 @@ __global__ __launch_bounds__((64 * RowsShape<kType, kRowTiles, kFragments>::kWav
 // A row of x in a block is eight pieces of 16 bytes; piece c of row r lies at place c ^ (r & 7): the sixteen rows that a fragment is
 // read from then do not meet in one bank.
 
-// The tiles of experts that one XCD takes together: kPieceRows of rows times kPieceColumns, or of so many columns less that as few as may be are missing
-// from the last piece (work-groups without a tile, a quarter of all where three columns were counted as four: 2048 rows to 8 of 128 experts of 2048 x 768 164 us instead of
-// 188, 4096 rows to 8 of 64 of 2048 x 1280 217 instead of 269).
-constexpr int32_t kPieceRows = 2, kPieceColumns = 4;
-__host__ __device__ inline int32_t piece_columns(int32_t tiles_n) {
-    const int32_t across = (tiles_n + kPieceColumns - 1) / kPieceColumns;
-    return (tiles_n + across - 1) / across;
-}
-
 template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN>
 struct TileShape {
     static constexpr int kThreads = 64 * kWavesM * kWavesN, kRows = kWavesM * kRowFragments * 16, kGroups = kWavesN, kRing = 3;
@@ -651,14 +642,7 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
     auto kernel = linear_tile_kernel<kType, kRowFragments, kWavesM, kWavesN, kExperts>;
     if constexpr (S::kLds > 65536)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
-    int64_t grid = (int64_t)a.tiles_m * a.tiles_n;
-    if (kExperts) {  // (whole pieces, the same number for each XCD)
-        const int32_t wide = piece_columns(a.tiles_n);
-        const int64_t pieces = (int64_t)((a.tiles_m + kPieceRows - 1) / kPieceRows) * ((a.tiles_n + wide - 1) / wide);
-        grid = (pieces + 7) / 8 * 8 * kPieceRows * wide;
-        CHX_REQUIRE(grid < (int64_t(1) << 31), "linear plan: too many results");
-    }
-    kernel<<<(unsigned)grid, S::kThreads, S::kLds, s>>>(a);
+    kernel<<<(unsigned)(kExperts ? expert_grid(a.tiles_m, a.tiles_n) : (int64_t)a.tiles_m * a.tiles_n), S::kThreads, S::kLds, s>>>(a);
     return launch_check("linear_tile_kernel");
 }
 

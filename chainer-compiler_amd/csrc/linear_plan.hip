@@ -26,11 +26,12 @@ struct LayoutArgs {
     int32_t N, K, units, groups, type;
     int64_t w_group;
     int64_t kilobytes;  // of all
+    int64_t first;      // work-group of this launch
 };
 
 // One lane writes 16 bytes, a wavefront 1 KB: a fragment, or two of int8.  Runs once per layer; w is read through its strides.
 __global__ __launch_bounds__(256) void linear_layout_kernel(LayoutArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t at = (a.first + blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (at >= a.kilobytes) return;
     const int lane = threadIdx.x & 63, each = a.type == kHalfInt8 ? 2 : 4;
     const int part = (int)(at % each);
@@ -60,11 +61,11 @@ struct VectorArgs {
     int64_t s_e, s_n;  // bytes
     float* out;
     int32_t N, n_padded, half;
-    int64_t total;
+    int64_t total, first;
 };
 
 __global__ __launch_bounds__(256) void linear_vector_kernel(VectorArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t at = (a.first + blockIdx.x) * 256 + threadIdx.x;
     if (at >= a.total) return;
     const int64_t e = at / a.n_padded, n = at % a.n_padded;
     const char* p = a.v + e * a.s_e + n * a.s_n;
@@ -77,12 +78,13 @@ struct RowsArgs {
     int64_t x_row, x_col;  // bytes
     char* out;
     int64_t pitch, pieces;  // bytes of a row; 16-byte pieces of all
+    int64_t first;
     int32_t K;
 };
 
 template <typename T>
 __global__ __launch_bounds__(256) void linear_pieces_kernel(RowsArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t at = (a.first + blockIdx.x) * 256 + threadIdx.x;
     if (at >= a.pieces) return;
     constexpr int kCount = 16 / sizeof(T);
     const int64_t row = at / (a.pitch / 16), k0 = at % (a.pitch / 16) * kCount;
@@ -313,22 +315,25 @@ int launch(Call& call, void* workspace, size_t workspace_bytes, hipStream_t s) {
     const int32_t height = c.fragments > 0 ? 16 * c.row_tiles : c.tile == kTile256 ? 256 : c.tile == kTile128 ? 128 : 64;
     const int32_t width = c.fragments > 0 ? 16 * c.fragments : std::max(height, 128);
     // The most tiles of rows there can be: experts' tiles begin anew with each of them.
-    const int64_t tiles_m = a.order ? a.M / height + std::min(a.M, a.experts) : (a.M + height - 1) / height;
+    const int64_t tiles_m = a.order ? a.M / height + std::min(a.M, a.experts) : ((int64_t)a.M + height - 1) / height;
     // (those of few rows take all fragments of whole groups)
     const int64_t tiles_n = c.fragments > 0 ? (int64_t)a.n_padded / width : (a.N + width - 1) / width;
-    CHX_REQUIRE(tiles_m * tiles_n < (int64_t(1) << 31), "linear plan: too many results");
+    const int64_t work_groups = c.fragments == 0 && a.order ? expert_grid(tiles_m, tiles_n) : tiles_m * tiles_n;
+    const int64_t threads = c.fragments > 0 || c.tile == kTile256 ? 512 : 256;
+    CHX_REQUIRE(work_groups * threads < (int64_t(1) << 32), "linear plan: too many results: %lld work-groups of %lld threads, and a launch has fewer than 2^32 threads",
+                (long long)work_groups, (long long)threads);
     a.tiles_m = (int32_t)tiles_m;
     a.tiles_n = (int32_t)tiles_n;
     if (into_pieces(c, call.direct, call.x_rows, a.K, a.order != nullptr, kType)) {
-        RowsArgs r = {a.x, a.x_row, a.x_col, static_cast<char*>(workspace), pitch_of(a.K, kType), 0, a.K};
+        RowsArgs r = {a.x, a.x_row, a.x_col, static_cast<char*>(workspace), pitch_of(a.K, kType), 0, 0, a.K};
         CHX_REQUIRE(workspace != nullptr && aligned(workspace, 16) && (int64_t)workspace_bytes >= r.pitch * call.x_rows,
                     "linear plan: a workspace of %lld bytes, aligned to 16, is needed for rows like these", (long long)(r.pitch * call.x_rows));
         r.pieces = r.pitch / 16 * call.x_rows;
-        CHX_REQUIRE(r.pieces < (int64_t(1) << 38), "linear plan: too many rows");
-        const unsigned blocks = (unsigned)((r.pieces + 255) / 256);
-        if (kType == kFloatFloat) linear_pieces_kernel<uint32_t><<<blocks, 256, 0, s>>>(r);
-        else linear_pieces_kernel<uint16_t><<<blocks, 256, 0, s>>>(r);
-        CHX_PROPAGATE(launch_check("linear_pieces_kernel"));
+        CHX_PROPAGATE(in_launches((r.pieces + 255) / 256, "linear_pieces_kernel", [&](int64_t first, unsigned count) {
+            r.first = first;
+            if (kType == kFloatFloat) linear_pieces_kernel<uint32_t><<<count, 256, 0, s>>>(r);
+            else linear_pieces_kernel<uint16_t><<<count, 256, 0, s>>>(r);
+        }));
         a.x = r.out;
         a.x_row = r.pitch;
         a.x_col = kType == kFloatFloat ? 4 : 2;
@@ -395,23 +400,20 @@ extern "C" int chx_hip_linear_plan_create(
     p.w = static_cast<char*>(memory);
     char* next = p.w + E * p.w_expert;
     LayoutArgs l = {static_cast<const char*>(w->data), lead ? w->strides[0] : 0, w->strides[lead], w->strides[lead + 1], p.w, p.N, p.K, p.units,
-                    (int32_t)groups, (int32_t)p.type, p.w_group, E * groups * p.units * unit_bytes(p.type) / 1024};
-    int rc = CHX_HIP_OK;
-    const int64_t blocks = (l.kilobytes + 3) / 4;
-    if (blocks >= (int64_t(1) << 31)) {
-        set_error("linear plan: too many weights");
-        rc = CHX_HIP_EINVAL;
-    } else {
-        linear_layout_kernel<<<(unsigned)blocks, 256, 0, as_stream(stream)>>>(l);
-        rc = launch_check("linear_layout_kernel");
-    }
+                    (int32_t)groups, (int32_t)p.type, p.w_group, E * groups * p.units * unit_bytes(p.type) / 1024, 0};
+    int rc = in_launches((l.kilobytes + 3) / 4, "linear_layout_kernel", [&](int64_t first, unsigned count) {
+        l.first = first;
+        linear_layout_kernel<<<count, 256, 0, as_stream(stream)>>>(l);
+    });
     auto vector = [&](const chx_hip_tensor* t) {
         float* out_v = reinterpret_cast<float*>(next);
         next += vector_bytes;
         if (rc != CHX_HIP_OK) return out_v;
-        VectorArgs v = {static_cast<const char*>(t->data), lead ? t->strides[0] : 0, t->strides[lead], out_v, p.N, p.n_padded, t->dtype == CHX_HIP_FLOAT16, E * p.n_padded};
-        linear_vector_kernel<<<(unsigned)((v.total + 255) / 256), 256, 0, as_stream(stream)>>>(v);
-        rc = launch_check("linear_vector_kernel");
+        VectorArgs v = {static_cast<const char*>(t->data), lead ? t->strides[0] : 0, t->strides[lead], out_v, p.N, p.n_padded, t->dtype == CHX_HIP_FLOAT16, E * p.n_padded, 0};
+        rc = in_launches((v.total + 255) / 256, "linear_vector_kernel", [&](int64_t first, unsigned count) {
+            v.first = first;
+            linear_vector_kernel<<<count, 256, 0, as_stream(stream)>>>(v);
+        });
         return out_v;
     };
     if (w_scale) p.scale = vector(w_scale);

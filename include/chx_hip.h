@@ -469,7 +469,8 @@ void chx_hip_linear_plan_destroy(chx_hip_linear_plan* plan);
  *   r  NULL, or of y's shape and type; may be y itself
  * Sums and epilogue are float32, in an order that depends on the sizes alone; the result is rounded once.  (Activations of float16 results, which are rounded by up to 2^-11, are
  * off by up to 2^-17 before that; those of float32 results, of whichever rows, by float32's own roundings.)  y must not overlap x, itself,
- * nor r unless it is r.  workspace: for many rows that are not whole 16-byte pieces, aligned to 16; y_rows: rows of y. */
+ * nor r unless it is r (between the first and the last byte of each).  Fewer than 2^31 rows; results whose tiles are more than one launch has are refused (2^34 elements,
+ * N taken as whole 64s, are not).  workspace: for many rows that are not whole 16-byte pieces, aligned to 16; y_rows: rows of y. */
 int chx_hip_linear_plan_workspace(const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int64_t y_rows, size_t* bytes);
 int chx_hip_linear_plan_run(
         const chx_hip_linear_plan* plan, const chx_hip_tensor* x, int32_t activation, const chx_hip_tensor* r, chx_hip_tensor* y, void* workspace,

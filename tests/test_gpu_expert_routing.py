@@ -235,3 +235,15 @@ def test_sums_of_any_strides(g, dtype):
         y.fill_(7.0)
         assert bool((out == 7.0).all())
     assert g.ops.ExpertCombine(plain, weights, r=r, out=r) is r and torch.equal(r, want)
+
+
+def test_more_sums_than_one_launch_has(g):
+    """More than 2^31 results, an element to a lane: what lies behind the first launch's part."""
+    T, n = (1 << 19) + 3, 4099
+    x = torch.randint(-4, 5, (64, n), dtype=torch.int8, device="cuda").half().repeat(T // 64 + 1, 1)[:T]
+    weights = 2.0 * torch.ones(T, 1, device="cuda")
+    y = g.ops.ExpertCombine(x, weights)
+    for first in range(0, T, 1 << 16):
+        assert torch.equal(y[first: first + (1 << 16)], 2 * x[first: first + (1 << 16)])
+    del x, y
+    torch.cuda.empty_cache()

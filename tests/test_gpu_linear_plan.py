@@ -363,3 +363,25 @@ def test_a_feed_forward_layer_with_experts_and_its_answer(g):
         torch.cuda.synchronize()
         for a, c in zip(recorded, layer()):
             assert torch.equal(a, c)
+
+
+def test_more_work_than_one_launch_has(g):
+    """More than 2^31 threads' work in the launches that lay weights out and bring rows into whole pieces: what lies behind the first launch's part."""
+    experts, n, k = 70, 16384, 16384
+    w = normal(60, (n, k), HALF, k ** -0.5)
+    x = normal(61, (2, k), HALF)
+    plan = g.ops.LinearPlan(w.expand(experts, n, k))                                  # 38 GB laid out
+    order = torch.arange(experts, dtype=torch.int32, device="cuda")
+    offsets = torch.arange(experts + 1, dtype=torch.int32, device="cuda")
+    y = plan.run_experts(x[:1].expand(experts, k).contiguous(), order, offsets)
+    plan.close()
+    assert torch.equal(y, y[:1].expand(experts, n))
+    check(y[-1:], *formula(x[:1], w, None, None, "", None), k)
+    n, k, rows = 64, 16385, (1 << 20) + 5                                              # 34 GB of pieces
+    x, plan = normal(62, (1, k), HALF), g.ops.LinearPlan(normal(63, (n, k), HALF, k ** -0.5))
+    y = plan.run(x.expand(rows, k))
+    few = plan.run(x.expand(300, k))
+    check(few[:1], *formula(x, normal(63, (n, k), HALF, k ** -0.5), None, None, "", None), k)
+    assert torch.equal(y[:300], y[-300:]) and torch.equal(y[:1].expand(rows, n), y) and torch.allclose(y[:1].float(), few[:1].float(), atol=2e-2)
+    del w, x, y
+    torch.cuda.empty_cache()

@@ -210,5 +210,54 @@ def launches(host):
             assert size.value == 0
 
 
+@pytest.mark.parametrize("case", ["large"])
+def test_sizes_at_the_bounds(host_so, case):
+    host_hip.run_case(host_so, __file__, case)
+
+
+def large(host):
+    """Launches have fewer than 2^32 threads: more work than that goes in several, and products of more results are refused before anything runs."""
+    T, lib = host.tensor, host.lib
+    address = host.malloc(64)
+
+    def threads():
+        """Of each launch: name, threads."""
+        lines = host.launches()
+        return [(line, int(line.split("grid=")[1].split(",")[0]) * int(line.split("block=")[1].split()[0])) for line in lines]
+
+    def some(name, least):
+        found = threads()
+        assert len(found) > 1 and all(name in line and n < 2 ** 32 for line, n in found) and sum(n for _, n in found) >= least, found
+
+    # (descriptors of memory that nobody touches)
+    rows, n = (1 << 20) + 3, 4099
+    host.check(lib.chx_hip_expert_combine(ref(T("float16", (rows, n), base=address + (1 << 40))), ref(T("float32", (rows, 1), base=address + (1 << 45))), None, ref(T("float16", (rows, n), base=address)), None))
+    some("expert_combine_kernel", rows * n)
+    host.clear()
+    plan = make(host, T("float16", (64, 16385)))[1]
+    host.clear()
+    rows = 1 << 20
+    x, y, size = T("float16", (rows, 16385), [0, 1]), T("float16", (rows, 64), base=address + (1 << 40)), ctypes.c_size_t()
+    host.check(lib.chx_hip_linear_plan_workspace(plan, ref(x), ctypes.c_int64(rows), ctypes.byref(size)))
+    assert size.value == rows * 16448 * 2
+    host.check(lib.chx_hip_linear_plan_run(plan, ref(x), 0, None, ref(y), ctypes.c_void_p((address + (1 << 45)) & ~15), size, None))
+    found = threads()
+    assert "linear_tile_kernel" in found.pop()[0]
+    assert len(found) > 1 and all("linear_pieces_kernel" in line and n < 2 ** 32 for line, n in found) and sum(n for _, n in found) >= size.value // 16, found
+    # a result of 2^31 - 1 rows, whose tiles are more than a launch has
+    rows = (1 << 31) - 1
+    x, y = T("float16", (rows, 16385), [0, 1]), T("float16", (rows, 64), base=address + (1 << 40))
+    host.check(lib.chx_hip_linear_plan_workspace(plan, ref(x), ctypes.c_int64(rows), ctypes.byref(size)))
+    host.clear()
+    refused(host, lib.chx_hip_linear_plan_run(plan, ref(x), 0, None, ref(y), ctypes.c_void_p((address + (1 << 45)) & ~15), size, None), "fewer than 2^32 threads")
+    # the layout of many weights
+    memory = T("int8", (64, 64, 128))
+    host.check(lib.chx_hip_linear_plan_create(ref(T("int8", (16384, 16384, 128), [0, 128, 1], base=memory.data)), ref(T("float32", (16384, 16384), [0, 0], base=memory.data)), None, None, ctypes.byref(plan)))
+    found = threads()
+    assert len(found) > 1 and all(n < 2 ** 32 for _, n in found), found
+    layout = sum(n for line, n in found if "linear_layout_kernel" in line)
+    assert layout >= 16384 * 16384 * 128 // 16 and sum(n for line, n in found if "linear_vector_kernel" in line) >= 16384 * 16384
+
+
 if __name__ == "__main__":
     host_hip.main(globals())
