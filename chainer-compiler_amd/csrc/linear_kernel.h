@@ -646,32 +646,39 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
     return launch_check("linear_tile_kernel");
 }
 
-template <LinearType kType, int kRowTiles, int kFragments>
+// kForExperts: whether experts take this size too.
+template <LinearType kType, int kRowTiles, int kFragments, bool kForExperts>
 int rows_of(const LinearArgs& a, bool direct, hipStream_t s) {
-    if (a.order) return direct ? launch_rows<kType, kRowTiles, kFragments, true, true>(a, s) : launch_rows<kType, kRowTiles, kFragments, false, true>(a, s);
+    if (a.order) {
+        if constexpr (kForExperts) return direct ? launch_rows<kType, kRowTiles, kFragments, true, true>(a, s) : launch_rows<kType, kRowTiles, kFragments, false, true>(a, s);
+        CHX_FAIL(CHX_HIP_EUNSUPPORTED, "linear plan: no kernel for experts' %d tiles of rows and %d fragments", kRowTiles, kFragments);
+    }
     return direct ? launch_rows<kType, kRowTiles, kFragments, true, false>(a, s) : launch_rows<kType, kRowTiles, kFragments, false, false>(a, s);
 }
 
-template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN>
+template <LinearType kType, int kRowFragments, int kWavesM, int kWavesN, bool kForExperts>
 int tile_of(const LinearArgs& a, hipStream_t s) {
-    return a.order ? launch_tile<kType, kRowFragments, kWavesM, kWavesN, true>(a, s) : launch_tile<kType, kRowFragments, kWavesM, kWavesN, false>(a, s);
+    if (a.order) {
+        if constexpr (kForExperts) return launch_tile<kType, kRowFragments, kWavesM, kWavesN, true>(a, s);
+        CHX_FAIL(CHX_HIP_EUNSUPPORTED, "linear plan: no kernel for experts' tiles of %d rows", 16 * kRowFragments * kWavesM);
+    }
+    return launch_tile<kType, kRowFragments, kWavesM, kWavesN, false>(a, s);
 }
 
 }  // namespace
 
 template <LinearType kType>
 int LinearKernels<kType>::rows(const LinearArgs& a, int row_tiles, int fragments, bool direct, hipStream_t s) {
-    // (the grid is made for these numbers: any others are refused)
+    // (the grid is made for these numbers: any others are refused.  What a choice never gives is not built.)
     switch (row_tiles * 8 + fragments) {
-        case 8 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 1, 1>(a, direct, s); else break;  // (two fragments of int8 are one piece)
-        case 16 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 2, 1>(a, direct, s); else break;
-        case 32 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 4, 1>(a, direct, s); else break;
-        case 8 + 2: return rows_of<kType, 1, 2>(a, direct, s);
-        case 8 + 4: return rows_of<kType, 1, 4>(a, direct, s);
-        case 16 + 2: return rows_of<kType, 2, 2>(a, direct, s);
-        case 16 + 4: return rows_of<kType, 2, 4>(a, direct, s);
-        case 32 + 2: return rows_of<kType, 4, 2>(a, direct, s);
-        case 32 + 4: return rows_of<kType, 4, 4>(a, direct, s);
+        case 8 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 1, 1, true>(a, direct, s); else break;  // (two fragments of int8 are one piece)
+        case 16 + 1: if constexpr (kType != kHalfInt8) return rows_of<kType, 2, 1, true>(a, direct, s); else break;
+        case 8 + 2: return rows_of<kType, 1, 2, true>(a, direct, s);
+        case 8 + 4: return rows_of<kType, 1, 4, true>(a, direct, s);
+        case 16 + 2: return rows_of<kType, 2, 2, true>(a, direct, s);
+        case 16 + 4: return rows_of<kType, 2, 4, true>(a, direct, s);
+        case 32 + 2: if constexpr (kType == kFloatFloat) return rows_of<kType, 4, 2, false>(a, direct, s); else break;
+        case 32 + 4: return rows_of<kType, 4, 4, true>(a, direct, s);
         default: break;
     }
     CHX_FAIL(CHX_HIP_EUNSUPPORTED, "linear plan: no kernel for %d tiles of rows and %d fragments", row_tiles, fragments);
@@ -679,8 +686,8 @@ int LinearKernels<kType>::rows(const LinearArgs& a, int row_tiles, int fragments
 
 template <LinearType kType>
 int LinearKernels<kType>::tile(const LinearArgs& a, LinearTile t, hipStream_t s) {
-    if (t == kTile64) return tile_of<kType, 2, 2, 2>(a, s);
-    if constexpr (kType != kFloatFloat) return t == kTile256 ? tile_of<kType, 8, 2, 4>(a, s) : tile_of<kType, 4, 2, 2>(a, s);
+    if (t == kTile64) return tile_of<kType, 2, 2, 2, true>(a, s);
+    if constexpr (kType != kFloatFloat) return t == kTile256 ? tile_of<kType, 8, 2, 4, kType == kHalfHalf>(a, s) : tile_of<kType, 4, 2, 2, true>(a, s);
     CHX_FAIL(CHX_HIP_EUNSUPPORTED, "linear plan: no kernel for tiles of 128 rows of float32");
 }
 

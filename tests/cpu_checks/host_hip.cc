@@ -2,6 +2,7 @@
 // take the place of libamdhip64's.  Two devices, whose memory is host memory; streams, captures and graphs as far as the
 // library uses them; kernels are written to a log instead of run, all but the one that copies results to the host.
 //   hh_log / hh_clear         what happened since hh_clear, a line each
+//   hh_kernels                all kernels of the library, a line each
 //   hh_device_of(p)           the device whose memory p is, -1: none
 //   hh_prefer(text)           event pairs around launches of kernels with this in their name measure a tenth of the others
 //   hh_no_memory(n)           there is none for requests of exactly n bytes (0: for all)
@@ -125,6 +126,13 @@ hipError_t stop(hipStream_t s) {  // a call that a recording stream does not tak
 
 extern "C" {
 
+const char* hh_kernels() {
+    Lock lock(g_mutex);
+    static std::string& text = *new std::string;
+    text.clear();
+    for (const auto& k : g_kernels) text += k.second + "\n";
+    return text.c_str();
+}
 const char* hh_log() {
     static std::string copy;
     Lock lock(g_mutex);

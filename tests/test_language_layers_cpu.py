@@ -210,7 +210,7 @@ def launches(host):
             assert size.value == 0
 
 
-@pytest.mark.parametrize("case", ["large"])
+@pytest.mark.parametrize("case", ["large", "reached"])
 def test_sizes_at_the_bounds(host_so, case):
     host_hip.run_case(host_so, __file__, case)
 
@@ -257,6 +257,43 @@ def large(host):
     assert len(found) > 1 and all(n < 2 ** 32 for _, n in found), found
     layout = sum(n for line, n in found if "linear_layout_kernel" in line)
     assert layout >= 16384 * 16384 * 128 // 16 and sum(n for line, n in found if "linear_vector_kernel" in line) >= 16384 * 16384
+
+
+def reached(host):
+    """Every kernel of the products is what some call takes: sizes over the range of each type, with rows that can be copied in whole pieces and others, small and large weights."""
+    T, lib = host.tensor, host.lib
+    host.hh.hh_kernels.restype = ctypes.c_char_p
+    names = {k for k in host.hh.hh_kernels().decode().splitlines() if "linear_rows_kernel" in k or "linear_tile_kernel" in k}
+    memory, result = T("int8", (64,)).data, T("int8", (64,)).data + (1 << 45)  # (descriptors of memory that nobody touches)
+    taken = set()
+
+    def note():
+        taken.update(line.split(" grid=")[0] for line in host.launches() if line.split(" grid=")[0] in names)
+        host.clear()
+
+    for kind, w_kind in (("float16", "float16"), ("float16", "int8"), ("float32", "float32")):
+        for K, columns in ((128, (16, 600, 1100, 2100, 4200, 9000, 20000)), (8192, (600, 1100, 2100, 4200, 9000))):
+            for N in columns:
+                scale = T("float32", (N,), [0], base=memory) if w_kind == "int8" else None
+                plan = make(host, T(w_kind, (N, K), [0, 0], base=memory), scale)[1]
+                for M in (1, 8, 9, 32, 33, 64, 65, 100, 150, 200, 300, 500, 700, 1000, 2000, 5000):
+                    for gap in (0, 1):
+                        host.check(lib.chx_hip_linear_plan_run(plan, ref(T(kind, (M, K), [K + gap, 1], base=memory)), 0, None, ref(T(kind, (M, N), base=result)),
+                                                               ctypes.c_void_p(1 << 20), ctypes.c_size_t(1 << 40), None))
+                        note()
+                lib.chx_hip_linear_plan_destroy(plan)
+        for E in (1, 8, 64):
+            for K, N in ((128, 30), (128, 128), (128, 200), (128, 768), (128, 2000), (2048, 2048), (4096, 60), (4096, 128), (4096, 4096)):
+                scale = T("float32", (E, N), [0, 0], base=memory) if w_kind == "int8" else None
+                plan = make(host, T(w_kind, (E, N, K), [0, 0, 0], base=memory), scale)[1]
+                for each in (1, 4, 6, 8, 12, 13, 24, 25, 33, 64, 100, 300, 1000, 1 << 16):
+                    for pitch in (K, K + 1, 0):  # (0: one row again and again, however many)
+                        M = E * each
+                        host.check(lib.chx_hip_linear_plan_run_experts(plan, ref(T(kind, (M, K), [pitch, 1], base=memory)), ref(T("int32", (M,), base=memory)), ref(T("int32", (E + 1,), base=memory)), 0,
+                                                                       ref(T(kind, (M, N), base=result)), ctypes.c_void_p(1 << 20), ctypes.c_size_t(1 << 40), None))
+                        note()
+                lib.chx_hip_linear_plan_destroy(plan)
+    assert len(names) > 20 and names == taken, sorted(names - taken)
 
 
 if __name__ == "__main__":
