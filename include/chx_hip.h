@@ -451,7 +451,7 @@ int chx_hip_softmax_f32(const chx_hip_tensor* x, int32_t axis, int32_t is_onnx_s
 enum { CHX_HIP_ACT_NONE = 0, CHX_HIP_ACT_RELU = 1, CHX_HIP_ACT_GELU = 2, CHX_HIP_ACT_GELU_TANH = 3, CHX_HIP_ACT_SILU = 4 };
 
 /* The weights of a layer, laid out once for its products:
- *   w        [N, K], or [E, N, K] for a layer with E experts: float16, float32 or int8, any strides
+ *   w        [N, K], or [E, N, K] for a layer with E experts: float16, float32 or int8, any strides; E up to 65536, N up to 2^24, K below 2^22, 2^21 and 2^23
  *   w_scale  float32 [N] / [E, N] of int8 weights (a weight is w * w_scale), else NULL
  *   b        float16 or float32 [N] / [E, N], or NULL
  * create() copies all of them and waits for the stream (CHX_HIP_EUNSUPPORTED on one that is being captured).  A plan belongs to the device it was created on and may be used by

@@ -9,6 +9,8 @@ import math
 import pytest
 import torch
 
+import linear_sizes
+
 pytestmark = pytest.mark.gpu
 
 HALF, FLOAT = torch.float16, torch.float32
@@ -384,4 +386,65 @@ def test_more_work_than_one_launch_has(g):
     check(few[:1], *formula(x, normal(63, (n, k), HALF, k ** -0.5), None, None, "", None), k)
     assert torch.equal(y[:300], y[-300:]) and torch.equal(y[:1].expand(rows, n), y) and torch.allclose(y[:1].float(), few[:1].float(), atol=2e-2)
     del w, x, y
+    torch.cuda.empty_cache()
+
+
+def whole(seed, shape, dtype):
+    """Whole numbers: their products' sums are exact in float32, in any order."""
+    return torch.randint(-3, 4, shape, generator=torch.Generator().manual_seed(seed), dtype=torch.int8).to(dtype).cuda()
+
+
+KINDS = {linear_sizes.HALF: (HALF, HALF), linear_sizes.INT8: (HALF, torch.int8), linear_sizes.FLOAT: (FLOAT, FLOAT)}
+
+
+@pytest.mark.parametrize("which,kernel,m,blocks,n", linear_sizes.PLAIN)
+def test_long_products(g, which, kernel, m, blocks, n):
+    """Every kernel over enough of k that its rings and loops come round, number for number."""
+    kind, w_kind = KINDS[which]
+    k = blocks * linear_sizes.BLOCK[which]
+    x, w = whole(40, (m, k), kind), whole(41, (n, k), w_kind)
+    scale = torch.full((n,), 0.5, device="cuda") if w_kind == torch.int8 else None
+    y = g.ops.LinearPlan(w, w_scale=scale).run(x, dtype=FLOAT)
+    want = x.double() @ w.double().T
+    assert torch.equal(y.double(), want if scale is None else 0.5 * want)
+
+
+@pytest.mark.parametrize("which,kernel,experts,fan,m,blocks,n", linear_sizes.EXPERTS)
+def test_long_products_of_experts(g, which, kernel, experts, fan, m, blocks, n):
+    """Likewise, with experts of few and of many rows, so that tiles lack none, some or nearly all of theirs."""
+    kind, w_kind = KINDS[which]
+    k = blocks * linear_sizes.BLOCK[which]
+    chosen, order, offsets = routed(42, m, experts)
+    x, w = whole(43, (m // fan, k), kind), whole(44, (experts, n, k), w_kind)
+    scale = torch.full((experts, n), 0.5, device="cuda") if w_kind == torch.int8 else None
+    y = g.ops.LinearPlan(w, w_scale=scale).run_experts(x, order, offsets, dtype=FLOAT)
+    for e in range(experts):
+        p = (chosen == e).nonzero()[:, 0].cuda()
+        want = x[p // fan].double() @ w[e].double().T
+        assert torch.equal(y[p].double(), want if scale is None else 0.5 * want)
+
+
+@pytest.mark.parametrize("k", [2 ** 22 + 64, 2 ** 22 + 3])
+def test_rows_too_long_for_a_tile(g, k):
+    """Rows of 8 MB and more (weights of 8 bits alone have as many columns) are left to the kernel for few rows, whatever their number."""
+    rows, n = 20000, 64
+    x, w, scale = whole(45, (1, k), HALF), whole(46, (n, k), torch.int8), torch.full((n,), 0.5, device="cuda")
+    y = g.ops.LinearPlan(w, w_scale=scale).run(x.expand(rows, k), dtype=FLOAT)
+    assert torch.equal(y.double(), 0.5 * (x.double() @ w.double().T).expand(rows, n))
+
+
+@pytest.mark.parametrize("fan", [1, 2])
+def test_experts_rows_over_more_than_4_GiB(g, fan):
+    """Rows that 32 bits of an address do not reach: gathered from x of 4.3 GB, in a mixed order."""
+    k, n, experts = 16448, 48, 3
+    places = (2 ** 17 + 10) * fan
+    x = torch.randint(-2, 3, (places // fan, k), generator=torch.Generator(device="cuda").manual_seed(47), dtype=torch.int8, device="cuda").half()
+    assert x.numel() * 2 > 2 ** 32
+    w = whole(48, (experts, n, k), HALF)
+    chosen, order, offsets = routed(49, places, experts)
+    y = g.ops.LinearPlan(w).run_experts(x, order, offsets, dtype=FLOAT)
+    for e in range(experts):
+        for p in (chosen == e).nonzero()[:, 0].cuda().split(1 << 14):
+            assert torch.equal(y[p], x[p // fan].float() @ w[e].float().T)
+    del x, y
     torch.cuda.empty_cache()

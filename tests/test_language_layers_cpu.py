@@ -4,6 +4,7 @@ import ctypes
 import pytest
 
 import host_hip
+import linear_sizes
 
 
 @pytest.fixture(scope="module")
@@ -210,7 +211,7 @@ def launches(host):
             assert size.value == 0
 
 
-@pytest.mark.parametrize("case", ["large", "reached"])
+@pytest.mark.parametrize("case", ["large", "reached", "long_products"])
 def test_sizes_at_the_bounds(host_so, case):
     host_hip.run_case(host_so, __file__, case)
 
@@ -250,6 +251,14 @@ def large(host):
     host.check(lib.chx_hip_linear_plan_workspace(plan, ref(x), ctypes.c_int64(rows), ctypes.byref(size)))
     host.clear()
     refused(host, lib.chx_hip_linear_plan_run(plan, ref(x), 0, None, ref(y), ctypes.c_void_p((address + (1 << 45)) & ~15), size, None), "fewer than 2^32 threads")
+    for kind, columns in (("float16", 1 << 22), ("float32", 1 << 21), ("int8", 1 << 23)):
+        scale = T("float32", (1,)) if kind == "int8" else None
+        host.clear()
+        refused(host, make(host, T(kind, (1, columns), [0, 0]), scale)[0], "too long")
+        rc, longest = make(host, T(kind, (1, columns - 128), [0, 0]), scale)
+        host.check(rc)
+        lib.chx_hip_linear_plan_destroy(longest)
+    host.clear()
     # the layout of many weights
     memory = T("int8", (64, 64, 128))
     host.check(lib.chx_hip_linear_plan_create(ref(T("int8", (16384, 16384, 128), [0, 128, 1], base=memory.data)), ref(T("float32", (16384, 16384), [0, 0], base=memory.data)), None, None, ctypes.byref(plan)))
@@ -294,6 +303,34 @@ def reached(host):
                         note()
                 lib.chx_hip_linear_plan_destroy(plan)
     assert len(names) > 20 and names == taken, sorted(names - taken)
+
+
+def long_products(host):
+    """The sizes whose results test_gpu_linear_plan.py checks over the kernels' steady state take the kernels that they stand for."""
+    T, lib = host.tensor, host.lib
+    names = {linear_sizes.HALF: ("float16", "float16"), linear_sizes.INT8: ("float16", "int8"), linear_sizes.FLOAT: ("float32", "float32")}
+    fragments_of = {64: "2, 2, 2", 128: "4, 2, 2", 256: "8, 2, 4"}
+
+    def launched(which, kernel, experts, m, blocks, n, fan=1):
+        kind, w_kind = names[which]
+        K, lead = blocks * linear_sizes.BLOCK[which], (experts,) if experts else ()
+        plan = make(host, T(w_kind, lead + (n, K)), T("float32", lead + (n,)) if w_kind == "int8" else None)[1]
+        host.clear()
+        x, y = T(kind, (m // fan, K)), T("float32", (m, n))
+        if experts:
+            host.check(lib.chx_hip_linear_plan_run_experts(plan, ref(x), ref(T("int32", (m,))), ref(T("int32", (experts + 1,))), 0, ref(y), None, ctypes.c_size_t(0), None))
+        else:
+            host.check(lib.chx_hip_linear_plan_run(plan, ref(x), 0, None, ref(y), None, ctypes.c_size_t(0), None))
+        if kernel[0] == "rows":
+            want = "linear_rows_kernel<(chx::LinearType)%d, %d, %d, true, %s" % (which, kernel[1], kernel[2], "true" if experts else "false")
+        else:
+            want = "linear_tile_kernel<(chx::LinearType)%d, %s, %s" % (which, fragments_of[kernel[1]], "true" if experts else "false")
+        assert len(host.launches()) == 1 and want in host.launches()[0], (which, kernel, experts, m, blocks, n, host.launches())
+
+    for which, kernel, m, blocks, n in linear_sizes.PLAIN:
+        launched(which, kernel, 0, m, blocks, n)
+    for which, kernel, experts, fan, m, blocks, n in linear_sizes.EXPERTS:
+        launched(which, kernel, experts, m, blocks, n, fan)
 
 
 if __name__ == "__main__":
