@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TensorUtils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -571,8 +572,13 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor entropy = at::empty(rows, floats), top_logprobs = at::empty(best, floats), top_tokens = at::empty(best, floats.dtype(at::kLong));
         const at::Tensor logprobs = given ? at::empty(rows, floats) : at::Tensor();
         const int64_t V = logits.size(-1), R = entropy.numel();
-        // (views; the library takes a matrix and vectors)
-        if (logits.dim() != 2) logits = logits.view({R, V});
+        // (views; the library takes a matrix and vectors.  Tokens are few: they are copied where they are no run, logits are not.)
+        if (logits.dim() != 2) {
+            const int64_t matrix[] = {R, V};
+            const auto strides = at::detail::computeStride(logits.sizes(), logits.strides(), matrix);
+            if (!strides) fail(PyExc_ValueError, "the leading axes of the logits are not one run of rows");
+            logits = logits.as_strided(matrix, *strides);
+        }
         const at::Tensor flat_top = top_logprobs.view({R, top}), flat_best = top_tokens.view({R, top}), flat_entropy = entropy.view({R});
         size_t bytes = 0;
         checked([&] { return chx_hip_token_logprobs_workspace(R, V, top, &bytes); });
@@ -581,7 +587,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
         void* s = current_stream();
         void* memory = bytes ? space.data_ptr() : nullptr;
         if (given) {
-            const at::Tensor flat_tokens = tokens.view({R}), flat_logprobs = logprobs.view({R});
+            const at::Tensor flat_tokens = tokens.reshape({R}), flat_logprobs = logprobs.view({R});
             Operand kd(flat_tokens), pd(flat_logprobs);
             checked([&] { return chx_hip_token_logprobs(ld.ptr, kd.ptr, pd.ptr, ed.ptr, td.ptr, bd.ptr, memory, bytes, s); });
         } else {

@@ -375,8 +375,8 @@ def ExpertCombine(x, weights, r=None, out=None):
 
 
 def TokenLogProbs(logits, tokens=None, top=0):
-    """chx_hip_token_logprobs over the last axis of logits [.., V]: (log probabilities of `tokens` [..] or None, entropy [..], the
-    `top` best log probabilities [.., top], their tokens int64 [.., top])."""
+    """chx_hip_token_logprobs over the last axis of logits [.., V], whose leading axes are one run of rows: (log probabilities of
+    `tokens` [..], of any strides, or None, entropy [..], the `top` best log probabilities [.., top], their tokens int64 [.., top])."""
     return capi.native().token_logprobs(logits, tokens, top)
 
 

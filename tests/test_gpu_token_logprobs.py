@@ -124,6 +124,18 @@ def test_strides(g, dtype, V):
     assert g.ops.TokenLogProbs(plain[:0], tokens[:0], top=2)[2].shape == (0, 2)
 
 
+def test_tokens_and_logits_of_a_shifted_text(g):
+    """What a text's scores are asked with: the tokens one place further, which is a slice of several axes; logits whose leading axes are not one run of rows are refused."""
+    B, T, V = 3, 5, 900
+    logits, text = normal(7, (B, T, V), HALF, 2.0), torch.randint(0, V, (B, T + 1), generator=torch.Generator().manual_seed(8)).cuda()
+    got, want = g.ops.TokenLogProbs(logits, text[:, 1:], top=3), g.ops.TokenLogProbs(logits, text[:, 1:].contiguous(), top=3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    check(g, logits, text[:, 1:], 3)
+    check(g, logits[:, ::1, 5:], text[:, :T] % 800, 3)
+    with pytest.raises(ValueError, match="one run of rows"):
+        g.ops.TokenLogProbs(logits[:, :-1], text[:, 1:T])
+
+
 def test_recorded_and_on_two_streams(g):
     """Calls that split rows, recorded side by side, replayed with eager calls in between; and on two streams at once."""
     logits = normal(5, (3, 30000), HALF, 2.0), normal(6, (2, 50000), HALF, 2.0)
