@@ -110,6 +110,16 @@ long long integer(PyObject* o) {
     return v;
 }
 
+// One that fits the library's argument.
+int32_t integer32(PyObject* o, const char* name) {
+    const long long v = integer(o);
+    if (v != static_cast<int32_t>(v)) {
+        PyErr_Format(PyExc_ValueError, "%s is not a number of 32 bits", name);
+        throw PythonError();
+    }
+    return static_cast<int32_t>(v);
+}
+
 at::ScalarType scalar_type(PyObject* o) {
     if (!THPDtype_Check(o)) fail(PyExc_TypeError, "a torch dtype is expected");
     return reinterpret_cast<THPDtype*>(o)->scalar_type;
@@ -519,10 +529,10 @@ PyObject* expert_routing(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& logits = on_device(a[0], "logits");
         if (logits.dim() != 2) fail(PyExc_ValueError, "logits must be a matrix");
         const int64_t T = logits.size(0), E = logits.size(1), k = integer(a[1]);
-        if (k < 1) fail(PyExc_ValueError, "at least one expert is chosen");
+        if (k < 1 || k > E) fail(PyExc_ValueError, "at least one expert is chosen, and no more than there are");
         Operand ld(logits), bd(optional_on_device(a[2], "bias"));
-        const int32_t sigmoid = static_cast<int32_t>(integer(a[3])), groups = static_cast<int32_t>(integer(a[4])), top_groups = static_cast<int32_t>(integer(a[5]));
-        const int32_t group_best = static_cast<int32_t>(integer(a[6])), normalize = static_cast<int32_t>(integer(a[7]));
+        const int32_t sigmoid = integer32(a[3], "score"), groups = integer32(a[4], "groups"), top_groups = integer32(a[5], "top_groups");
+        const int32_t group_best = integer32(a[6], "group_best"), normalize = integer32(a[7], "normalize");
         const float scale = static_cast<float>(number(a[8]));
         size_t bytes = 0;
         checked([&] { return chx_hip_expert_routing_workspace(T, E, &bytes); });
@@ -568,10 +578,12 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
             tokens = on_device(a[1], "tokens");
             if (tokens.sizes() != at::IntArrayRef(rows)) fail(PyExc_ValueError, "a token for each row of the logits is expected");
         }
+        const int64_t V = logits.size(-1), R = c10::multiply_integers(rows);
+        size_t bytes = 0;
+        checked([&] { return chx_hip_token_logprobs_workspace(R, V, top, &bytes); });  // (which refuses sizes before results of them are allocated)
         const at::TensorOptions floats = logits.options().dtype(at::kFloat);
         const at::Tensor entropy = at::empty(rows, floats), top_logprobs = at::empty(best, floats), top_tokens = at::empty(best, floats.dtype(at::kLong));
         const at::Tensor logprobs = given ? at::empty(rows, floats) : at::Tensor();
-        const int64_t V = logits.size(-1), R = entropy.numel();
         // (views; the library takes a matrix and vectors.  Tokens are few: they are copied where they are no run, logits are not.)
         if (logits.dim() != 2) {
             const int64_t matrix[] = {R, V};
@@ -580,8 +592,6 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
             logits = logits.as_strided(matrix, *strides);
         }
         const at::Tensor flat_top = top_logprobs.view({R, top}), flat_best = top_tokens.view({R, top}), flat_entropy = entropy.view({R});
-        size_t bytes = 0;
-        checked([&] { return chx_hip_token_logprobs_workspace(R, V, top, &bytes); });
         const at::Tensor space = scratch(bytes, logits);
         Operand ld(logits), ed(flat_entropy), td(flat_top), bd(flat_best);
         void* s = current_stream();

@@ -161,6 +161,26 @@ def test_strides_and_no_rows(g):
     assert empty[0].shape == (0, 4) and empty[2].shape == (0,) and empty[3].cpu().tolist() == [0] * 151
 
 
+def test_numbers_that_are_refused(g):
+    """Of more than 32 bits, or more experts or alternatives than there are: before results of such sizes are allocated."""
+    logits = normal(18, (4096, 64), FLOAT)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    for names in ({"groups": 2 ** 32 + 1}, {"groups": 2, "top_groups": 2 ** 32 + 1}, {"group_best": 2 ** 32 + 1}):
+        with pytest.raises(ValueError):
+            g.ops.ExpertRouting(logits, 2, **names)
+    for k in (0, 65, 10 ** 6):
+        with pytest.raises(ValueError):
+            g.ops.ExpertRouting(logits, k)
+    for top in (65, 10 ** 6):
+        with pytest.raises(g.capi.ChxHipError):
+            g.ops.TokenLogProbs(logits, None, top=top)
+    with pytest.raises(ValueError):
+        g.ops.TokenLogProbs(logits, None, top=-1)
+    assert torch.cuda.max_memory_allocated() == before
+
+
 @pytest.mark.parametrize("T", [20, 900])
 def test_recorded_twice(g, T):
     """Two recorded calls side by side, replayed with eager calls in between."""
