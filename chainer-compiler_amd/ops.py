@@ -363,7 +363,8 @@ def ExpertRouting(logits, k, bias=None, score="softmax", groups=1, top_groups=No
     """chx_hip_expert_routing: (experts int32 [T, k], weights float32 [T, k], order int32 [T k], offsets int32 [E + 1]) for logits
     [T, E].  score: "softmax" or "sigmoid"; bias float32 [E] is added to the scores for the choice alone; the experts of
     the top_groups (by default all) best of `groups` groups can be chosen, a group's score being the sum of its group_best (1 or
-    2) best; the weights are divided by their sum if `normalize`, and multiplied by `scale`."""
+    2) best; the weights are divided by their sum if `normalize`, and multiplied by `scale`.  Of equal scores the lower index comes first;
+    without bias and groups it is the logits that are compared, also where the scores of two are equal in 64 bits."""
     return capi.native().expert_routing(logits, k, bias, ("softmax", "sigmoid").index(score), groups, groups if top_groups is None else top_groups,
                                         group_best, 1 if normalize else 0, scale)
 

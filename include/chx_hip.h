@@ -490,6 +490,8 @@ int chx_hip_linear_plan_run_experts(
  *   the E experts are `groups` groups of neighbours; a group's score is the sum of its `group_best` (1 or 2) best keys, and only
  *   the top_groups best groups' experts can be chosen
  *   the k = experts->shape[1] largest keys are chosen, largest first; of equal ones (groups likewise) the lower index first
+ *   (Without bias and groups it is the logits that are ranked, of which the scores are a monotonic function.  The one difference: logits that differ while their scores are equal in 64
+ *   bits, sigmoids of logits above 36 or softmaxes of logits 745 below the largest, are then told apart by the logit; with a bias, also one of zeros, or groups by the index.)
  *   weight = s of the chosen (not the key), over the sum of the chosen if `normalize` (0 where that sum is 0 in 64 bits), times `scale`; of a softmax without bias and
  *   groups in float32, else in 64 bits and rounded at the end
  * A NaN logit counts as -inf, +inf as the largest finite number; an expert with -inf has s = 0 (without bias and groups it is chosen only when the others run out).

@@ -152,6 +152,18 @@ def test_weights_of_very_low_scores(g, score, low, choice, E, normalize):
         assert ((y.sum(1) - scale).abs() <= 4 * 2.0 ** -24 * scale).all()
 
 
+def test_scores_that_are_equal_in_64_bits(g):
+    """Sigmoids of 40, 50 and 60 are all 1, softmaxes of -900 and -800 beside 1 both 0: without bias and groups their logits tell them apart, else their index does."""
+    zeros = torch.zeros(4, device="cuda")
+    x = torch.tensor([[40.0, 60.0, 50.0, 1.0]], device="cuda")
+    assert g.ops.ExpertRouting(x, 3, score="sigmoid")[0].cpu().tolist() == [[1, 2, 0]]
+    assert g.ops.ExpertRouting(x, 3, score="sigmoid", bias=zeros)[0].cpu().tolist() == [[0, 1, 2]]
+    assert g.ops.ExpertRouting(x, 3, score="sigmoid", groups=2, top_groups=2)[0].cpu().tolist() == [[0, 1, 2]]
+    x = torch.tensor([[0.0, -900.0, -800.0, 1.0]], device="cuda")
+    assert g.ops.ExpertRouting(x, 3)[0].cpu().tolist() == [[3, 0, 2]]
+    assert g.ops.ExpertRouting(x, 3, bias=zeros)[0].cpu().tolist() == [[3, 0, 1]]
+
+
 def test_strides_and_no_rows(g):
     space = normal(8, (80, 150), HALF)
     check(g, space[::2, 3:67], 4)
