@@ -8,7 +8,7 @@
 //
 // The arithmetic is what comes next: a float16 logit takes 8 issue slots of a lane (4 of them the exponential), which keep the vector
 // units busy for 60 us of 4096 rows of 65,536.  Their sums are therefore kept relative to a number M in units of log 2, the rounded m log2(e): y = x log2(e) - M is one fused
-// multiply-add that also converts x, exact to its own rounding, and M drops out at the end.  (float32 logits may be too large for that product: x - m first.)
+// multiply-add that also converts x, exact to its own rounding, and M drops out at the end (whole_row).  (float32 logits may be too large for that product: x - m first.)
 //
 // The alternatives are found in the same pass.  What is below a threshold cannot be among the `top` best: the top-th largest of the maxima that the
 // lanes found in their first 32 logits has top logits at or above it.  32 logits of a lane are compared by their maximum alone; what
@@ -74,10 +74,23 @@ __device__ __forceinline__ float maximum_of(float x) {
     return kHalf ? x * kLog2e : x;
 }
 
-// x - m as a natural logarithm.
+// A row's sums when they are whole: s and t relative to the largest logit itself, low: what m lacks of it.  M is the rounded m log2(e), so the largest logit's term is 2^low and not 1;
+// left in, a token that is certain had a log probability of up to 1e-7 instead of 0, above 0 as often as below.  The largest logit is the float16 number next to M / log2(e): M is off
+// by 2^-24 of itself, and such numbers are 2^-11 apart.
+struct Row {
+    float m, low, s, t;
+};
 template <bool kHalf>
-__device__ __forceinline__ float log_of(float x, float m) {
-    return kHalf ? log2_of<true>(x, m) * kLn2 : x - m;
+__device__ __forceinline__ Row whole_row(const Sums& z) {
+    if (!kHalf || z.s == 0.f) return {z.m, 0.f, z.s, z.t};
+    const float low = log2_of<true>((float)(_Float16)(z.m * kLn2), z.m), one = __builtin_amdgcn_exp2f(low);
+    return {z.m, low, z.s / one, (z.t - low * z.s) / one};  // (of that term alone exactly 1 and 0)
+}
+
+// x less the largest logit, as a natural logarithm.
+template <bool kHalf>
+__device__ __forceinline__ float log_of(float x, const Row& z) {
+    return kHalf ? (log2_of<true>(x, z.m) - z.low) * kLn2 : x - z.m;
 }
 
 // The sums relative to a larger maximum.
@@ -169,18 +182,19 @@ __device__ __forceinline__ Given given(const LogprobArgs& a, int64_t row) {
 
 // What is reported for a row: of its token and its entropy by one lane, of an alternative by whoever has it.
 template <bool kHalf>
-__device__ __forceinline__ void report_row(const LogprobArgs& a, int64_t row, const Sums& z, const Given& g) {
+__device__ __forceinline__ void report_row(const LogprobArgs& a, int64_t row, const Row& z, const Given& g) {
     // (no logit above -inf: no token has a probability)
     const bool none = z.s == 0.f;
     const float log_s = none ? 0.f : logf(z.s);
-    if (a.logprob) a.logprob[row] = g.in_place_of != 1.f ? g.in_place_of : none ? -INFINITY : log_of<kHalf>(g.logit, z.m) - log_s;
-    a.entropy[row] = none ? 0.f : log_s - kLn2 * z.t / z.s;
+    if (a.logprob) a.logprob[row] = g.in_place_of != 1.f ? g.in_place_of : none ? -INFINITY : log_of<kHalf>(g.logit, z) - log_s;
+    const float entropy = none ? 0.f : log_s - kLn2 * z.t / z.s;
+    a.entropy[row] = entropy < 0.f ? 0.f : entropy;  // (a NaN stays)
 }
 
 template <bool kHalf>
-__device__ __forceinline__ void report_best(const LogprobArgs& a, int64_t row, const Sums& z, int32_t rank, uint64_t entry) {
+__device__ __forceinline__ void report_best(const LogprobArgs& a, int64_t row, const Row& z, int32_t rank, uint64_t entry) {
     const bool none = z.s == 0.f;
-    a.top_logprob[row * a.top + rank] = none ? -INFINITY : log_of<kHalf>(of_sortable((uint32_t)(entry >> 32)), z.m) - logf(z.s);
+    a.top_logprob[row * a.top + rank] = none ? -INFINITY : log_of<kHalf>(of_sortable((uint32_t)(entry >> 32)), z) - logf(z.s);
     a.top_token[row * a.top + rank] = (int64_t)(uint32_t)~(uint32_t)entry;
 }
 
@@ -351,10 +365,11 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
         count = a.top;
     }
     if constexpr (kTeam == 1) {
-        if (lane == 0) report_row<kHalf>(a, row, z, g);
+        const Row whole = whole_row<kHalf>(z);
+        if (lane == 0) report_row<kHalf>(a, row, whole, g);
         const uint64_t mine = lane < count ? list[lane] : 0;
         const int32_t rank = before_in(list, count, mine);
-        if (lane < count && rank < a.top) report_best<kHalf>(a, row, z, rank, mine);
+        if (lane < count && rank < a.top) report_best<kHalf>(a, row, whole, rank, mine);
         return;
     }
     if (lane == 0) {
@@ -364,9 +379,10 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
     __syncthreads();
     z = lane < kTeam ? sums[lane] : Sums{kNoMaximum[kHalf], 0.f, 0.f};
     join_lanes<kHalf>(z);
-    const bool whole = a.parts == 1;
+    const bool one_part = a.parts == 1;
+    const Row whole = whole_row<kHalf>(z);
     if (threadIdx.x == 0) {
-        if (whole) report_row<kHalf>(a, row, z, g);
+        if (one_part) report_row<kHalf>(a, row, whole, g);
         else a.sums[blockIdx.x] = z;
     }
     if (a.top == 0) return;
@@ -375,10 +391,10 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
 #pragma unroll
     for (int w = 0; w < kTeam; ++w) rank += before_in(lists[w], counts[w], mine);
     if (lane < count && rank < a.top) {
-        if (whole) report_best<kHalf>(a, row, z, rank, mine);
+        if (one_part) report_best<kHalf>(a, row, whole, rank, mine);
         else a.lists[(int64_t)blockIdx.x * a.top + rank] = mine;
     }
-    if (!whole) {  // a part may have fewer logits than alternatives
+    if (!one_part) {  // a part may have fewer logits than alternatives
         int32_t all = 0;
 #pragma unroll
         for (int w = 0; w < kTeam; ++w) all += counts[w];
@@ -411,13 +427,14 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(LogprobArgs a)
         const uint64_t e = i == (int32_t)threadIdx.x ? first : from[i];
         if (e >= bound) list[atomicAdd(&count, 1)] = e;  // (in any order: they are ranked)
     }
-    join_lanes<kHalf>(z);
-    if (threadIdx.x == 0) report_row<kHalf>(a, row, z, g);
+    join_lanes<kHalf>(z);  // (each wavefront has all parts)
+    const Row whole = whole_row<kHalf>(z);
+    if (threadIdx.x == 0) report_row<kHalf>(a, row, whole, g);
     __syncthreads();
     for (int32_t i = threadIdx.x; i < count; i += 256) {
         const uint64_t mine = list[i];
         const int32_t rank = before_in(list, count, mine);
-        if (rank < a.top) report_best<kHalf>(a, row, z, rank, mine);
+        if (rank < a.top) report_best<kHalf>(a, row, whole, rank, mine);
     }
 }
 

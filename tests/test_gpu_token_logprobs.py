@@ -99,6 +99,26 @@ def test_masked_rows(g, dtype, V):
         check(g, logits, tokens, top)
 
 
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("R,V", [(2000, 1), (40, 60), (2100, 5000), (7, 9000), (6, 100003), (600, 9000)])
+def test_a_token_that_is_certain(g, dtype, R, V):
+    """The only token of a row has log probability 0 and the row entropy 0, whatever its logit is: no rounding is left of it.  Nor are log probabilities above 0 and entropies below."""
+    logits = torch.full((R, V), -math.inf, dtype=dtype, device="cuda")
+    tokens = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(9)).cuda()
+    values = normal(10, (R,), dtype, 6.0)
+    values[: R // 2] *= 4.0 ** torch.arange(R // 2, device="cuda").remainder(9).sub(2).to(dtype)
+    values = values.clamp(-60000, 60000)
+    logits[torch.arange(R, device="cuda"), tokens] = values
+    logp, entropy, best, which = g.ops.TokenLogProbs(logits, tokens, top=1)
+    assert torch.equal(which[:, 0], tokens)
+    assert bool((logp == 0).all()) and bool((entropy == 0).all()) and bool((best == 0).all())
+    if V > 1:
+        other = (tokens + 1 + torch.arange(R, device="cuda") % (V - 1)) % V
+        logits[torch.arange(R, device="cuda"), other] = values - (torch.arange(R, device="cuda") % 24).to(dtype)  # from as likely down to 4e-11
+        logp, entropy, best, _ = check(g, logits, tokens, 2)
+        assert bool((logp <= 0).all()) and bool((best <= 0).all()) and bool((entropy >= 0).all())
+
+
 def test_tokens_outside_the_vocabulary(g):
     logits = normal(3, (6, 500), HALF)
     for dtype in (torch.int32, torch.int64):
