@@ -129,7 +129,8 @@ __device__ __forceinline__ void activate(float (&v)[kCount], int32_t act) {
     }
 }
 
-// kCount neighbouring columns (a multiple of 4, from a multiple of 4 on) of one row of the result.
+// kCount neighbouring columns (a multiple of 4, from a multiple of 4 on) of one row of the result.  Rows that are not whole 8-byte pieces are stored an element at a time: 4096 x 4096 x
+// 16385 in float16 556 us, 16384 columns 422; 512 rows 92 and 78, one row 29 and 22.
 template <LinearType kType, int kCount>
 __device__ __forceinline__ void finish(const LinearArgs& a, float (&v)[kCount], int64_t row, int32_t n) {
     if (n >= a.N) return;
@@ -236,7 +237,7 @@ __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, u
 //
 // Bound by the bytes of w, each read once.  A work-group takes kFragments fragments' columns (16 each) and all k, its kWaves wavefronts every
 // kWaves-th block of two units: w goes from memory straight into registers, kDeep blocks ahead of the products, and the wavefronts' sums
-// are added in LDS, in one order.  x comes from the caches.  Up to 16 rows are loaded as fragments; of more, a block (128 bytes of every row) is copied
+// are added in LDS, in one order.  x comes from the caches.  A work-group of 16 rows loads them as fragments; one of more copies a block (128 bytes of every row)
 // into LDS of the wavefront's own, because lanes next to each other that load from different rows take a cache access each: 64 rows x 4096 x
 // 16384, 32 columns to a work-group, 36 us instead of 48 (with 64 columns it takes 27).  Rows that are not there repeat the last one; their results are dropped.
 template <LinearType kType, int kRowTiles, int kFragments>
