@@ -607,6 +607,88 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// cache_append(keys, values, k, v, tables, lengths, counts or None)
+PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 7);
+        Operand keys(on_device(a[0], "keys")), values(on_device(a[1], "values")), k(on_device(a[2], "k")), v(on_device(a[3], "v"));
+        Operand tables(on_device(a[4], "tables")), lengths(on_device(a[5], "lengths")), counts(optional_on_device(a[6], "counts"));
+        void* s = current_stream();
+        checked([&] { return chx_hip_cache_append(keys.ptr, values.ptr, k.ptr, v.ptr, tables.ptr, lengths.ptr, counts.ptr, s); });
+        Py_RETURN_NONE;
+    });
+}
+
+// tree_attention(q, keys, values, tables, lengths, parents or None, counts or None, scale, mass or None, out or None)
+PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 10);
+        const at::Tensor& q = on_device(a[0], "q");
+        Operand qd(q), keys(on_device(a[1], "keys")), values(on_device(a[2], "values")), tables(on_device(a[3], "tables")), lengths(on_device(a[4], "lengths"));
+        Operand parents(optional_on_device(a[5], "parents")), counts(optional_on_device(a[6], "counts")), mass(optional_on_device(a[8], "mass"));
+        const float scale = static_cast<float>(number(a[7]));
+        size_t bytes = 0;
+        checked([&] { return chx_hip_tree_attention_workspace(qd.ptr, keys.ptr, tables.ptr, mass.ptr != nullptr, &bytes); });
+        const at::Tensor y = result(a[9], q.sizes(), q.options()), space = scratch(bytes, q);
+        Operand yd(y);
+        void* s = current_stream();
+        checked([&] {
+            return chx_hip_tree_attention(qd.ptr, keys.ptr, values.ptr, tables.ptr, lengths.ptr, parents.ptr, counts.ptr, scale, mass.ptr, yd.ptr, bytes ? space.data_ptr() : nullptr, bytes, s);
+        });
+        return wrapped(a[9], y);
+    });
+}
+
+// cache_accept(keys, values, tables, lengths, accepted, mass or None) -> new lengths
+PyObject* cache_accept(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 6);
+        const at::Tensor& lengths = on_device(a[3], "lengths");
+        Operand keys(on_device(a[0], "keys")), values(on_device(a[1], "values")), tables(on_device(a[2], "tables")), ld(lengths), accepted(on_device(a[4], "accepted"));
+        Operand mass(optional_on_device(a[5], "mass"));
+        const at::Tensor made = at::empty(lengths.sizes(), lengths.options().dtype(at::kInt));
+        Operand md(made);
+        void* s = current_stream();
+        checked([&] { return chx_hip_cache_accept(keys.ptr, values.ptr, tables.ptr, ld.ptr, accepted.ptr, mass.ptr, md.ptr, s); });
+        return THPVariable_Wrap(made);
+    });
+}
+
+// cache_evict(keys, values, tables, lengths, mass, keep, recent) -> new lengths
+PyObject* cache_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 7);
+        const at::Tensor &pages = on_device(a[0], "keys"), &table = on_device(a[2], "tables"), &lengths = on_device(a[3], "lengths");
+        if (pages.dim() != 4 || table.dim() != 2) fail(PyExc_ValueError, "keys need four axes and tables two");
+        Operand keys(pages), values(on_device(a[1], "values")), tables(table), ld(lengths), mass(on_device(a[4], "mass"));
+        const int64_t keep = integer(a[5]), recent = integer(a[6]);
+        size_t bytes = 0;
+        checked([&] { return chx_hip_cache_evict_workspace(table.size(0), pages.size(2), table.size(1) * pages.size(1), keep, &bytes); });
+        const at::Tensor made = at::empty(lengths.sizes(), lengths.options().dtype(at::kInt)), space = scratch(bytes, pages);
+        Operand md(made);
+        void* s = current_stream();
+        checked([&] { return chx_hip_cache_evict(keys.ptr, values.ptr, tables.ptr, ld.ptr, mass.ptr, keep, recent, md.ptr, bytes ? space.data_ptr() : nullptr, bytes, s); });
+        return THPVariable_Wrap(made);
+    });
+}
+
+// cross_attention(q, keys, values, lengths or None, scale, out or None)
+PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        need(n, 6);
+        const at::Tensor& q = on_device(a[0], "q");
+        Operand qd(q), keys(on_device(a[1], "keys")), values(on_device(a[2], "values")), lengths(optional_on_device(a[3], "lengths"));
+        const float scale = static_cast<float>(number(a[4]));
+        size_t bytes = 0;
+        checked([&] { return chx_hip_cross_attention_workspace(qd.ptr, keys.ptr, &bytes); });
+        const at::Tensor y = result(a[5], q.sizes(), q.options()), space = scratch(bytes, q);
+        Operand yd(y);
+        void* s = current_stream();
+        checked([&] { return chx_hip_cross_attention(qd.ptr, keys.ptr, values.ptr, lengths.ptr, scale, yd.ptr, bytes ? space.data_ptr() : nullptr, bytes, s); });
+        return wrapped(a[5], y);
+    });
+}
+
 // ---- runs of the virtual machine (chxvm.py); its library is loaded by the caller, who hands the entry points over ----
 struct Machine {
     decltype(&chxvm_program_run_to_host) run;
@@ -730,6 +812,11 @@ PyMethodDef methods[] = {
         {"expert_routing", fast(expert_routing), METH_FASTCALL, nullptr},
         {"expert_combine", fast(expert_combine), METH_FASTCALL, nullptr},
         {"token_logprobs", fast(token_logprobs), METH_FASTCALL, nullptr},
+        {"cache_append", fast(cache_append), METH_FASTCALL, nullptr},
+        {"tree_attention", fast(tree_attention), METH_FASTCALL, nullptr},
+        {"cache_accept", fast(cache_accept), METH_FASTCALL, nullptr},
+        {"cache_evict", fast(cache_evict), METH_FASTCALL, nullptr},
+        {"cross_attention", fast(cross_attention), METH_FASTCALL, nullptr},
         {"vm_init", fast(vm_init), METH_FASTCALL, nullptr},
         {"vm_run", fast(vm_run), METH_FASTCALL, nullptr},
         {"vm_outputs", vm_outputs, METH_O, nullptr},

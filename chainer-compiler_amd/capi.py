@@ -41,6 +41,8 @@ EXPORTS = [
     "chx_hip_graph_launch", "chx_hip_graph_destroy", "chx_hip_gemm_f32", "chx_hip_linear_f32", "chx_hip_max_pool_f32", "chx_hip_average_pool_f32", "chx_hip_fixed_batch_norm_f32", "chx_hip_conv_f32", "chx_hip_softmax_f32",
     "chx_hip_linear_plan_create", "chx_hip_linear_plan_destroy", "chx_hip_linear_plan_workspace", "chx_hip_linear_plan_run", "chx_hip_linear_plan_run_experts",
     "chx_hip_expert_routing_workspace", "chx_hip_expert_routing", "chx_hip_expert_combine", "chx_hip_token_logprobs_workspace", "chx_hip_token_logprobs",
+    "chx_hip_cache_append", "chx_hip_tree_attention_workspace", "chx_hip_tree_attention", "chx_hip_cache_accept", "chx_hip_cache_evict_workspace", "chx_hip_cache_evict",
+    "chx_hip_cross_attention_workspace", "chx_hip_cross_attention",
 ]
 
 

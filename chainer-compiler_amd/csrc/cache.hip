@@ -1,0 +1,510 @@
+// A cache of keys and values in pages: rows appended, drafted rows that were accepted moved together, and eviction by accumulated weight.
+//
+// All of it is bound by the bytes that move (few rows: by the launches).  Work-groups own what they write: in a move within the cache, a work-group has all
+// rows of a sequence's head, of keys or values, and a slice of their elements, so that no row is read by one group after another has written it.
+#include <cstring>
+#include <initializer_list>
+
+#include "cache.h"
+
+namespace chx {
+
+int check_rows(const chx_hip_tensor* t, int ndim, int32_t dtype, const char* what, const char* name) {
+    CHX_PROPAGATE(check_tensor(t, name));
+    CHX_REQUIRE(t->dtype == CHX_HIP_FLOAT16 || t->dtype == CHX_HIP_FLOAT32, "%s: %s must be float16 or float32, not %s", what, name, dtype_name(t->dtype));
+    CHX_REQUIRE(dtype == 0 || t->dtype == dtype, "%s: %s must be %s, as the others are, not %s", what, name, dtype_name(dtype), dtype_name(t->dtype));
+    CHX_REQUIRE(t->ndim == ndim, "%s: %s needs %d axes, not %d", what, name, ndim, t->ndim);
+    const int64_t es = dtype_size(t->dtype);
+    bool whole = aligned(t->data, (size_t)es);
+    for (int i = 0; i < ndim; ++i) whole = whole && (t->shape[i] <= 1 || t->strides[i] % es == 0);
+    CHX_REQUIRE(whole, "%s: %s is not made of whole elements", what, name);
+    CHX_REQUIRE(t->shape[ndim - 1] <= 1 || t->strides[ndim - 1] == es, "%s: the last axis of %s has gaps", what, name);
+    return CHX_HIP_OK;
+}
+
+int check_numbers(const chx_hip_tensor* t, int ndim, int64_t n0, int64_t n1, const char* what, const char* name) {
+    CHX_PROPAGATE(check_tensor(t, name));
+    CHX_REQUIRE(t->dtype == CHX_HIP_INT32, "%s: %s must be int32, not %s", what, name, dtype_name(t->dtype));
+    CHX_REQUIRE(t->ndim == ndim && (n0 < 0 || t->shape[0] == n0) && (ndim < 2 || n1 < 0 || t->shape[1] == n1), "%s: %s has another shape than the others ask for", what, name);
+    CHX_REQUIRE(numel(*t) == 0 || (is_contiguous(*t) && aligned(t->data, 4)), "%s: %s must be contiguous", what, name);
+    return CHX_HIP_OK;
+}
+
+int check_cache(const chx_hip_tensor* keys, const chx_hip_tensor* values, const chx_hip_tensor* tables, const chx_hip_tensor* lengths, const char* what, CacheArgs* c) {
+    CHX_PROPAGATE(check_rows(keys, 4, 0, what, "keys"));
+    CHX_PROPAGATE(check_rows(values, 4, keys->dtype, what, "values"));
+    CHX_REQUIRE(same_shape(*keys, *values), "%s: keys and values must have one shape", what);
+    CHX_REQUIRE(keys->shape[1] >= 1 && keys->shape[2] >= 1 && keys->shape[3] >= 1 && keys->shape[3] <= 256, "%s: a page needs a place, a head and 1 to 256 elements", what);
+    CHX_REQUIRE(keys->shape[0] < (int64_t(1) << 31) && keys->shape[2] < (int64_t(1) << 16), "%s: 2^31 pages or 2^16 heads", what);
+    CHX_PROPAGATE(check_tensor(tables, "tables"));
+    CHX_REQUIRE(tables->dtype == CHX_HIP_INT32 && tables->ndim == 2, "%s: tables must be an int32 matrix", what);
+    CHX_REQUIRE(numel(*tables) == 0 || (aligned(tables->data, 4) && (tables->shape[1] == 1 || tables->strides[1] == 4) && tables->strides[0] % 4 == 0), "%s: a row of tables must be contiguous", what);
+    CHX_REQUIRE(tables->shape[0] < (int64_t(1) << 24), "%s: 2^24 sequences", what);
+    CHX_REQUIRE(keys->shape[1] < (int64_t(1) << 30) && tables->shape[1] < (int64_t(1) << 30) && tables->shape[1] * keys->shape[1] < (int64_t(1) << 30), "%s: a sequence of 2^30 places", what);
+    CHX_PROPAGATE(check_numbers(lengths, 1, tables->shape[0], 0, what, "lengths"));
+    memset(c, 0, sizeof(*c));
+    c->k = static_cast<char*>(keys->data);
+    c->v = static_cast<char*>(values->data);
+    c->k_page = stride_of(*keys, 0), c->k_row = stride_of(*keys, 1), c->k_head = stride_of(*keys, 2);
+    c->v_page = stride_of(*values, 0), c->v_row = stride_of(*values, 1), c->v_head = stride_of(*values, 2);
+    c->tables = static_cast<const int32_t*>(tables->data);
+    c->table_row = tables->strides[0] / 4;
+    c->lengths = static_cast<const int32_t*>(lengths->data);
+    c->B = (int32_t)tables->shape[0];
+    c->groups = (int32_t)keys->shape[2];
+    c->D = (int32_t)keys->shape[3];
+    c->pages = (int32_t)keys->shape[0];
+    c->page_rows = (int32_t)keys->shape[1];
+    c->places = (int32_t)(tables->shape[1] * keys->shape[1]);
+    return CHX_HIP_OK;
+}
+
+int check_mass(const chx_hip_tensor* mass, const CacheArgs& c, const char* what) {
+    CHX_PROPAGATE(check_tensor(mass, "mass"));
+    CHX_REQUIRE(mass->dtype == CHX_HIP_FLOAT32 && mass->ndim == 3, "%s: mass must be float32 with three axes", what);
+    CHX_REQUIRE(mass->shape[0] == c.B && mass->shape[1] == c.groups && mass->shape[2] >= c.places, "%s: mass must have a number for each sequence, head and place", what);
+    if (numel(*mass) == 0) return CHX_HIP_OK;
+    CHX_REQUIRE(aligned(mass->data, 4) && mass->strides[0] % 4 == 0 && mass->strides[1] % 4 == 0 && (mass->shape[2] == 1 || mass->strides[2] == 4), "%s: the last axis of mass has gaps", what);
+    CHX_REQUIRE(elements_apart(*mass), "%s: elements of mass overlap", what);
+    return CHX_HIP_OK;
+}
+
+int check_apart(const Named& written, const Named* others, int count, const char* what) {
+    if (written.t == nullptr || numel(*written.t) == 0) return CHX_HIP_OK;
+    for (int i = 0; i < count; ++i) {
+        if (others[i].t == nullptr || numel(*others[i].t) == 0) continue;
+        CHX_REQUIRE(!arrays_overlap(*written.t, *others[i].t), "%s: %s and %s overlap", what, written.name, others[i].name);
+    }
+    return CHX_HIP_OK;
+}
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Bytes of a row that are copied at once: what all distances, addresses and the row itself are multiples of.
+int unit_of(std::initializer_list<int64_t> bytes) {
+    int64_t all = 16;
+    for (int64_t b : bytes) all |= b;
+    return (int)(all & -all);
+}
+int64_t at_of(const void* p) {
+    return (int64_t)reinterpret_cast<intptr_t>(p);
+}
+
+__device__ __forceinline__ int32_t clamped(int32_t v, int32_t most) {
+    return max(0, min(v, most));
+}
+
+// ---- append -------------------------------------------------------------------------------------------
+
+struct AppendArgs {
+    CacheArgs c;
+    const char *k, *v;
+    int64_t k_batch, k_token, k_head, v_batch, v_token, v_head;
+    const int32_t* counts;
+    int32_t T, units;   // units of a row
+    int64_t pieces;     // B T groups units
+};
+
+// A lane moves one unit of a key and of its value.
+template <typename Unit>
+__global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a, int64_t first) {
+    const int64_t i = (first + blockIdx.x) * 256 + threadIdx.x;
+    if (i >= a.pieces) return;
+    const int64_t row = i / a.units;
+    const int32_t u = (int32_t)(i - row * a.units);
+    const int64_t bt = row / a.c.groups;
+    const int32_t h = (int32_t)(row - bt * a.c.groups), b = (int32_t)(bt / a.T), t = (int32_t)(bt - (int64_t)b * a.T);
+    if (a.counts && t >= a.counts[b]) return;
+    const int64_t p = (int64_t)a.c.lengths[b] + t;
+    if (p < 0 || p >= a.c.places) return;
+    const Place at = place_of(a.c, b, (int32_t)p);
+    if (at.page < 0) return;
+    const Unit k = reinterpret_cast<const Unit*>(a.k + b * a.k_batch + t * a.k_token + h * a.k_head)[u];
+    const Unit v = reinterpret_cast<const Unit*>(a.v + b * a.v_batch + t * a.v_token + h * a.v_head)[u];
+    reinterpret_cast<Unit*>(a.c.k + at.page * a.c.k_page + at.row * a.c.k_row + h * a.c.k_head)[u] = k;
+    reinterpret_cast<Unit*>(a.c.v + at.page * a.c.v_page + at.row * a.c.v_row + h * a.c.v_head)[u] = v;
+}
+
+// ---- moves within the cache ---------------------------------------------------------------------------
+
+constexpr int32_t kMostAccepted = 256;
+constexpr int kSlice = 128;  // bytes of a row that a work-group moves
+
+struct MoveArgs {
+    CacheArgs c;
+    float* mass;  // null: none
+    int64_t mass_batch, mass_head;
+    int32_t row_bytes, slices;
+    // accepted
+    const int32_t* accepted;
+    int32_t most;
+    int32_t* new_lengths;
+    // evicted
+    int32_t keep, recent;
+    int32_t* lists;  // [B][groups][1 + 2 most]: how many places move, where to, where from
+};
+
+// A slice of a head's row at a place; null: no place.
+struct Rows {
+    char* base;
+    int64_t page, row;
+};
+__device__ __forceinline__ char* row_at(const MoveArgs& a, const Rows& r, int32_t b, int64_t p) {
+    if (p < 0 || p >= a.c.places) return nullptr;
+    const Place at = place_of(a.c, b, (int32_t)p);
+    return at.page < 0 ? nullptr : r.base + at.page * r.page + at.row * r.row;
+}
+
+// Drafted rows that were accepted.  A work-group has at most 256 slices of 128 bytes: all are read before the first is written.  blockIdx: sequence, head, then keys' slices, values' slices, mass.
+template <typename Unit>
+__global__ __launch_bounds__(256) void cache_accept_kernel(MoveArgs a) {
+    __shared__ Unit rows[kMostAccepted * kSlice / sizeof(Unit)];
+    __shared__ int32_t from[kMostAccepted];
+    __shared__ int32_t count;
+    const int32_t each = 2 * a.slices + (a.mass ? 1 : 0), what = blockIdx.x % each, h = blockIdx.x / each % a.c.groups, b = blockIdx.x / each / a.c.groups;
+    const int32_t length = clamped(a.c.lengths[b], a.c.places), i = threadIdx.x;
+    if (i == 0) count = a.most;
+    __syncthreads();
+    if (i < a.most) {
+        from[i] = a.accepted[(int64_t)b * a.most + i];
+        if (from[i] < 0) atomicMin(&count, i);
+    }
+    __syncthreads();
+    const int32_t n = count;
+    if (what == 0 && h == 0 && i == 0) a.new_lengths[b] = min(length + n, a.c.places);
+    if (what == 2 * a.slices) {
+        float* mass = a.mass + b * a.mass_batch + h * a.mass_head;
+        const int64_t p = i < n ? (int64_t)length + from[i] : a.c.places;
+        const float v = p < a.c.places ? mass[p] : 0.f;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (p < a.c.places && length + i < a.c.places) mass[length + i] = v;
+        return;
+    }
+    const int32_t slice = what % a.slices * kSlice, bytes = min(kSlice, a.row_bytes - slice), units = bytes / (int32_t)sizeof(Unit);
+    const Rows r = what < a.slices ? Rows{a.c.k + h * a.c.k_head + slice, a.c.k_page, a.c.k_row} : Rows{a.c.v + h * a.c.v_head + slice, a.c.v_page, a.c.v_row};
+    for (int32_t j = i; j < n * units; j += 256) {
+        const char* at = row_at(a, r, b, (int64_t)length + from[j / units]);
+        if (at) rows[j] = reinterpret_cast<const Unit*>(at)[j % units];
+    }
+    __syncthreads();
+    for (int32_t j = i; j < n * units; j += 256) {
+        if (!row_at(a, r, b, (int64_t)length + from[j / units])) continue;
+        char* to = row_at(a, r, b, (int64_t)length + j / units);
+        if (to) reinterpret_cast<Unit*>(to)[j % units] = rows[j];
+    }
+}
+
+// ---- eviction -----------------------------------------------------------------------------------------
+
+// Larger numbers first, a NaN before all.
+__device__ __forceinline__ uint32_t sortable(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.f);  // (-0 is 0)
+    return v != v ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+
+// A head's places that stay: the threshold of the `best` largest of n weights by three histograms of 11, 11 and 10 bits, of equal ones the lower places; then the
+// list of moves, places that go in front of best and places that stay behind it, both in ascending order.
+__global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
+    constexpr int kWaves = 16, kBins = 2048;
+    __shared__ int32_t bins[kBins];
+    __shared__ int32_t of_waves[kWaves];
+    __shared__ uint32_t found_bin;
+    __shared__ int32_t found_above;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int32_t h = blockIdx.x % a.c.groups, b = blockIdx.x / a.c.groups;
+    const int32_t length = clamped(a.c.lengths[b], a.c.places);
+    int32_t* list = a.lists + (int64_t)blockIdx.x * (1 + 2 * a.most);
+    if (h == 0 && threadIdx.x == 0) a.new_lengths[b] = min(length, a.keep);
+    if (length <= a.keep) {
+        if (threadIdx.x == 0) list[0] = 0;
+        return;
+    }
+    const int32_t n = length - a.recent, best = a.keep - a.recent;
+    const float* mass = a.mass + b * a.mass_batch + h * a.mass_head;
+    uint32_t least = 0;      // upper bits of the threshold
+    int32_t wanted = best;   // how many with those bits
+    if (best > 0) {
+        for (int digit = 0; digit < 3; ++digit) {
+            const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+            const uint32_t above = digit == 0 ? 0 : ~0u << (shift + bits);
+            for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
+            __syncthreads();
+            for (int32_t i = threadIdx.x; i - lane < n; i += 1024) {
+                const uint32_t key = i < n ? sortable(mass[i]) : 0;
+                const bool counts = i < n && ((key ^ least) & above) == 0;
+                const uint32_t bin = (key >> shift) & ((1u << bits) - 1);
+                // (equal weights, as of places that nobody has looked at, would queue for one bin)
+                const uint64_t all = __builtin_amdgcn_ballot_w64(counts);
+                if (all == 0) continue;
+                const int leader = __builtin_ctzll(all);
+                const uint32_t its = __builtin_amdgcn_readlane(bin, leader);
+                if (__builtin_amdgcn_ballot_w64(counts && bin != its) == 0) {
+                    if (lane == leader) atomicAdd(&bins[its], __popcll(all));
+                } else if (counts) {
+                    atomicAdd(&bins[bin], 1);
+                }
+            }
+            __syncthreads();
+            // the bin in which the wanted one is, from above: a lane has two bins
+            const int32_t hi = bins[kBins - 1 - 2 * threadIdx.x], lo = bins[kBins - 2 - 2 * threadIdx.x];
+            int32_t upto = hi + lo;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int32_t o = __shfl_up(upto, d);
+                if (lane >= d) upto += o;
+            }
+            if (lane == 63) of_waves[wave] = upto;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) upto += of_waves[w];
+            const int32_t before = upto - hi - lo;
+            if (before < wanted && wanted <= before + hi) found_bin = kBins - 1 - 2 * threadIdx.x, found_above = before;
+            else if (before + hi < wanted && wanted <= upto) found_bin = kBins - 2 - 2 * threadIdx.x, found_above = before + hi;
+            __syncthreads();
+            least |= found_bin << shift;
+            wanted -= found_above;
+            __syncthreads();
+        }
+    }
+    // `wanted` of those that equal the threshold stay, the lower places first; each wavefront has a run of places
+    const int32_t run = (n + kWaves * 64 - 1) / (kWaves * 64) * 64, from = wave * run, to = min(from + run, n);
+    auto of_wave = [&](int32_t mine) {  // what the wavefronts before this one have
+        __syncthreads();
+        if (lane == 0) of_waves[wave] = mine;
+        __syncthreads();
+        int32_t before = 0;
+        for (int w = 0; w < wave; ++w) before += of_waves[w];
+        return before;
+    };
+    int32_t equal = 0;
+    for (int32_t i = from + lane; i - lane < to; i += 64) equal += __popcll(__builtin_amdgcn_ballot_w64(i < to && best > 0 && sortable(mass[i]) == least));
+    const int32_t equal_before = of_wave(equal);
+    int32_t holes = 0, movers = 0, holes_before = 0, movers_before = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        int32_t rank = equal_before;
+        holes = movers = 0;
+        for (int32_t i = from + lane; i - lane < to; i += 64) {
+            const uint32_t key = i < to ? sortable(mass[i]) : 0;
+            const uint64_t same = __builtin_amdgcn_ballot_w64(i < to && best > 0 && key == least), below = (1ull << lane) - 1;
+            const bool stays = best > 0 && (key > least || (key == least && rank + __popcll(same & below) < wanted));
+            rank += __popcll(same);
+            const uint64_t hole = __builtin_amdgcn_ballot_w64(i < to && i < best && !stays), mover = __builtin_amdgcn_ballot_w64(i < to && i >= best && stays);
+            if (pass == 1) {
+                if ((hole >> lane) & 1) list[1 + holes_before + holes + __popcll(hole & below)] = i;
+                if ((mover >> lane) & 1) list[1 + a.most + movers_before + movers + __popcll(mover & below)] = i;
+            }
+            holes += __popcll(hole);
+            movers += __popcll(mover);
+        }
+        if (pass == 0) {
+            holes_before = of_wave(holes);
+            movers_before = of_wave(movers);
+        }
+    }
+    if (threadIdx.x == 1023) list[0] = holes_before + holes;
+}
+
+// The moves of a head's list, then the latest places behind them, `recent` of them from length - recent to keep - recent: those may overlap themselves, so they go in
+// ascending pieces, each read before it is written.  blockIdx as for cache_accept_kernel.
+template <typename Unit>
+__global__ __launch_bounds__(1024) void cache_evict_kernel(MoveArgs a) {
+    constexpr int kAtOnce = 4;
+    const int32_t each = 2 * a.slices + 1, what = blockIdx.x % each, h = blockIdx.x / each % a.c.groups, b = blockIdx.x / each / a.c.groups;
+    const int32_t length = clamped(a.c.lengths[b], a.c.places);
+    if (length <= a.keep) return;
+    const int32_t* list = a.lists + (int64_t)(b * a.c.groups + h) * (1 + 2 * a.most);
+    const int32_t moves = list[0], latest = length - a.recent, to = a.keep - a.recent;
+    const int32_t *to_list = list + 1, *from_list = list + 1 + a.most;
+    if (what == 2 * a.slices) {
+        float* mass = a.mass + b * a.mass_batch + h * a.mass_head;
+        for (int32_t i = threadIdx.x; i < moves; i += 1024) mass[to_list[i]] = mass[from_list[i]];
+        for (int32_t i0 = 0; i0 < a.recent; i0 += 1024) {
+            const int32_t i = i0 + threadIdx.x;
+            const float v = i < a.recent ? mass[latest + i] : 0.f;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what is read here, or was above, may be written next)
+            __syncthreads();
+            if (i < a.recent) mass[to + i] = v;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        for (int32_t i = a.keep + threadIdx.x; i < length; i += 1024) mass[i] = 0.f;
+        return;
+    }
+    const int32_t slice = what % a.slices * kSlice, bytes = min(kSlice, a.row_bytes - slice), units = bytes / (int32_t)sizeof(Unit);
+    const Rows r = what < a.slices ? Rows{a.c.k + h * a.c.k_head + slice, a.c.k_page, a.c.k_row} : Rows{a.c.v + h * a.c.v_head + slice, a.c.v_page, a.c.v_row};
+    const int32_t rows = 1024 / units, mine = threadIdx.x / units, u = threadIdx.x % units;  // (units: at most 64)
+    for (int32_t i0 = 0; i0 < moves; i0 += rows * kAtOnce) {
+        Unit v[kAtOnce];
+        bool there[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int32_t i = i0 + j * rows + mine;
+            const char* at = mine < rows && i < moves ? row_at(a, r, b, from_list[i]) : nullptr;
+            there[j] = at != nullptr;
+            if (at) v[j] = reinterpret_cast<const Unit*>(at)[u];
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            char* at = there[j] ? row_at(a, r, b, to_list[i0 + j * rows + mine]) : nullptr;
+            if (at) reinterpret_cast<Unit*>(at)[u] = v[j];
+        }
+    }
+    for (int32_t i0 = 0; i0 < a.recent; i0 += rows * kAtOnce) {
+        Unit v[kAtOnce];
+        bool there[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int32_t i = i0 + j * rows + mine;
+            const char* at = mine < rows && i < a.recent ? row_at(a, r, b, latest + i) : nullptr;
+            there[j] = at != nullptr;
+            if (at) v[j] = reinterpret_cast<const Unit*>(at)[u];
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            char* at = there[j] ? row_at(a, r, b, to + i0 + j * rows + mine) : nullptr;
+            if (at) reinterpret_cast<Unit*>(at)[u] = v[j];
+        }
+    }
+}
+
+// Launches for units of 16, 8, 4 or 2 bytes.
+template <typename F>
+int by_unit(int unit, F f) {
+    switch (unit) {
+        case 16: return f(u32x4{});
+        case 8: return f(uint64_t{});
+        case 4: return f(uint32_t{});
+        default: return f(uint16_t{});
+    }
+}
+
+int unit_of_cache(const CacheArgs& c, int32_t row_bytes) {
+    return unit_of({at_of(c.k), at_of(c.v), c.k_page, c.k_row, c.k_head, c.v_page, c.v_row, c.v_head, row_bytes});
+}
+
+int check_moves(const chx_hip_tensor* keys, const chx_hip_tensor* values, const chx_hip_tensor* tables, const chx_hip_tensor* lengths, const chx_hip_tensor* more,
+                const chx_hip_tensor* mass, const chx_hip_tensor* new_lengths, const char* what, MoveArgs* a) {
+    memset(a, 0, sizeof(*a));
+    CHX_PROPAGATE(check_cache(keys, values, tables, lengths, what, &a->c));
+    CHX_REQUIRE(elements_apart(*keys) && elements_apart(*values), "%s: elements of keys or values overlap", what);
+    if (mass) {
+        CHX_PROPAGATE(check_mass(mass, a->c, what));
+        a->mass = static_cast<float*>(mass->data);
+        a->mass_batch = mass->strides[0] / 4;
+        a->mass_head = mass->strides[1] / 4;
+    }
+    CHX_PROPAGATE(check_numbers(new_lengths, 1, a->c.B, 0, what, "new_lengths"));
+    const Named all[] = {{values, "values"}, {tables, "tables"}, {lengths, "lengths"}, {more, "accepted"}, {mass, "mass"}, {new_lengths, "new_lengths"}};
+    CHX_PROPAGATE(check_apart({keys, "keys"}, all, 6, what));
+    CHX_PROPAGATE(check_apart({values, "values"}, all + 1, 5, what));
+    CHX_PROPAGATE(check_apart({mass, "mass"}, all + 1, 3, what));
+    CHX_PROPAGATE(check_apart({new_lengths, "new_lengths"}, all + 1, 4, what));
+    a->new_lengths = static_cast<int32_t*>(new_lengths->data);
+    a->row_bytes = a->c.D * dtype_size(keys->dtype);
+    a->slices = (a->row_bytes + kSlice - 1) / kSlice;
+    CHX_REQUIRE((int64_t)a->c.B * a->c.groups * (2 * a->slices + 1) < (int64_t(1) << 22), "%s: more sequences and heads than one launch has", what);
+    return CHX_HIP_OK;
+}
+
+int64_t evict_workspace(int64_t sequences, int64_t heads, int64_t places, int64_t keep) {
+    // (places that move are at most as many as stay, or as are left)
+    const int64_t most = keep < places - keep ? keep : places > keep ? places - keep : 0;
+    return 4 * sequences * heads * (1 + 2 * most);
+}
+
+}  // namespace
+}  // namespace chx
+
+using namespace chx;
+
+extern "C" int chx_hip_cache_append(
+        chx_hip_tensor* keys, chx_hip_tensor* values, const chx_hip_tensor* k, const chx_hip_tensor* v, const chx_hip_tensor* tables, const chx_hip_tensor* lengths,
+        const chx_hip_tensor* counts, void* stream) {
+    const char* what = "cache append";
+    AppendArgs a;
+    memset(&a, 0, sizeof(a));
+    CHX_PROPAGATE(check_cache(keys, values, tables, lengths, what, &a.c));
+    CHX_REQUIRE(elements_apart(*keys) && elements_apart(*values), "%s: elements of keys or values overlap", what);
+    CHX_PROPAGATE(check_rows(k, 4, keys->dtype, what, "k"));
+    CHX_PROPAGATE(check_rows(v, 4, keys->dtype, what, "v"));
+    CHX_REQUIRE(same_shape(*k, *v) && k->shape[0] == a.c.B && k->shape[2] == a.c.groups && k->shape[3] == a.c.D, "%s: k and v must be [sequences, tokens, heads, elements] as the cache has them", what);
+    CHX_REQUIRE(k->shape[1] < (int64_t(1) << 30), "%s: 2^30 tokens", what);
+    if (counts) {
+        CHX_PROPAGATE(check_numbers(counts, 1, a.c.B, 0, what, "counts"));
+        a.counts = static_cast<const int32_t*>(counts->data);
+    }
+    const Named all[] = {{values, "values"}, {k, "k"}, {v, "v"}, {tables, "tables"}, {lengths, "lengths"}, {counts, "counts"}};
+    CHX_PROPAGATE(check_apart({keys, "keys"}, all, 6, what));
+    CHX_PROPAGATE(check_apart({values, "values"}, all + 1, 5, what));
+    if (numel(*k) == 0 || numel(*keys) == 0 || a.c.places == 0) return CHX_HIP_OK;
+    a.k = static_cast<const char*>(k->data);
+    a.v = static_cast<const char*>(v->data);
+    a.k_batch = stride_of(*k, 0), a.k_token = stride_of(*k, 1), a.k_head = stride_of(*k, 2);
+    a.v_batch = stride_of(*v, 0), a.v_token = stride_of(*v, 1), a.v_head = stride_of(*v, 2);
+    a.T = (int32_t)k->shape[1];
+    const int32_t row_bytes = a.c.D * dtype_size(keys->dtype);
+    const int unit = unit_of({unit_of_cache(a.c, row_bytes), at_of(a.k), at_of(a.v), a.k_batch, a.k_token, a.k_head, a.v_batch, a.v_token, a.v_head});
+    a.units = row_bytes / unit;
+    a.pieces = (int64_t)a.c.B * a.T * a.c.groups * a.units;
+    return by_unit(unit, [&](auto u) {
+        return in_launches((a.pieces + 255) / 256, "cache_append_kernel",
+                           [&](int64_t first, unsigned count) { cache_append_kernel<decltype(u)><<<count, 256, 0, as_stream(stream)>>>(a, first); });
+    });
+}
+
+extern "C" int chx_hip_cache_accept(
+        chx_hip_tensor* keys, chx_hip_tensor* values, const chx_hip_tensor* tables, const chx_hip_tensor* lengths, const chx_hip_tensor* accepted, chx_hip_tensor* mass,
+        chx_hip_tensor* new_lengths, void* stream) {
+    const char* what = "cache accept";
+    MoveArgs a;
+    CHX_PROPAGATE(check_tensor(accepted, "accepted"));
+    CHX_PROPAGATE(check_moves(keys, values, tables, lengths, accepted, mass, new_lengths, what, &a));
+    CHX_PROPAGATE(check_numbers(accepted, 2, a.c.B, -1, what, "accepted"));
+    CHX_REQUIRE(accepted->shape[1] <= kMostAccepted, "%s: at most %d rows of a sequence, not %lld", what, kMostAccepted, (long long)accepted->shape[1]);
+    if (a.c.B == 0) return CHX_HIP_OK;
+    a.accepted = static_cast<const int32_t*>(accepted->data);
+    a.most = (int32_t)accepted->shape[1];
+    const unsigned grid = (unsigned)(a.c.B * a.c.groups * (2 * a.slices + (a.mass ? 1 : 0)));
+    return by_unit(unit_of_cache(a.c, a.row_bytes), [&](auto u) {
+        cache_accept_kernel<decltype(u)><<<grid, 256, 0, as_stream(stream)>>>(a);
+        return launch_check("cache_accept_kernel");
+    });
+}
+
+extern "C" int chx_hip_cache_evict_workspace(int64_t sequences, int64_t heads, int64_t places, int64_t keep, size_t* bytes) {
+    CHX_REQUIRE(bytes != nullptr, "cache evict: null output");
+    CHX_REQUIRE(sequences >= 0 && heads >= 0 && places >= 0 && sequences < (int64_t(1) << 24) && heads < (int64_t(1) << 16) && places < (int64_t(1) << 30), "cache evict: numbers of a cache out of range");
+    CHX_REQUIRE(keep >= 0, "cache evict: keep is negative");
+    *bytes = (size_t)evict_workspace(sequences, heads, places, keep);
+    return CHX_HIP_OK;
+}
+
+extern "C" int chx_hip_cache_evict(
+        chx_hip_tensor* keys, chx_hip_tensor* values, const chx_hip_tensor* tables, const chx_hip_tensor* lengths, chx_hip_tensor* mass, int64_t keep, int64_t recent,
+        chx_hip_tensor* new_lengths, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "cache evict";
+    MoveArgs a;
+    CHX_PROPAGATE(check_tensor(mass, "mass"));
+    CHX_PROPAGATE(check_moves(keys, values, tables, lengths, nullptr, mass, new_lengths, what, &a));
+    CHX_REQUIRE(recent >= 0 && recent <= keep, "%s: 0 to keep places can be recent, not %lld of %lld", what, (long long)recent, (long long)keep);
+    const int64_t needed = evict_workspace(a.c.B, a.c.groups, a.c.places, keep);
+    CHX_REQUIRE((int64_t)workspace_bytes >= needed && (needed == 0 || (workspace != nullptr && aligned(workspace, 4))), "%s: a workspace of %lld bytes, aligned to 4, is needed", what,
+                (long long)needed);
+    if (a.c.B == 0) return CHX_HIP_OK;
+    a.keep = (int32_t)(keep < a.c.places ? keep : a.c.places);  // (no sequence is longer)
+    a.recent = (int32_t)(recent < a.keep ? recent : a.keep);
+    a.most = (int32_t)((needed / 4 / ((int64_t)a.c.B * a.c.groups) - 1) / 2);
+    a.lists = static_cast<int32_t*>(workspace);
+    cache_choose_kernel<<<(unsigned)(a.c.B * a.c.groups), 1024, 0, as_stream(stream)>>>(a);
+    CHX_PROPAGATE(launch_check("cache_choose_kernel"));
+    if (a.keep >= a.c.places) return CHX_HIP_OK;
+    const unsigned grid = (unsigned)(a.c.B * a.c.groups * (2 * a.slices + 1));
+    return by_unit(unit_of_cache(a.c, a.row_bytes), [&](auto u) {
+        cache_evict_kernel<decltype(u)><<<grid, 1024, 0, as_stream(stream)>>>(a);
+        return launch_check("cache_evict_kernel");
+    });
+}

@@ -381,6 +381,42 @@ def TokenLogProbs(logits, tokens=None, top=0):
     return capi.native().token_logprobs(logits, tokens, top)
 
 
+def CacheAppend(keys, values, k, v, tables, lengths, counts=None):
+    """chx_hip_cache_append: row t of k[b] and v[b] ([B, T, G, D]) to place lengths[b] + t of sequence b, for t below counts[b] (int32 [B]; all by
+    default).  keys and values are pages [P, R, G, D], tables int32 [B, M] the pages of each sequence, lengths int32 [B]; those stay as they are."""
+    capi.native().cache_append(keys, values, k, v, tables, lengths, counts)
+
+
+def TreeAttention(q, keys, values, tables, lengths, parents=None, counts=None, scale=None, mass=None, out=None):
+    """chx_hip_tree_attention: the result [B, T, H, D] of T drafted tokens, whose own keys and values lie behind the cache's lengths[b] places (CacheAppend).
+    Each sees those places, itself and, with parents int32 [B, T] (the index of an earlier token, -1 for none), its ancestors, else all tokens before it: one
+    token, or a piece of a prompt.  Tokens from counts[b] on have results of 0.  scale: by default 1 / sqrt(D).  mass float32 [B, G, M R or more]: weights are added for the cache's places,
+    and set for the tokens' own."""
+    return capi.native().tree_attention(q, keys, values, tables, lengths, parents, counts, _scale_of(q, scale), mass, out)
+
+
+def CacheAccept(keys, values, tables, lengths, accepted, mass=None):
+    """chx_hip_cache_accept: of the drafted tokens behind lengths[b], those in accepted int32 [B, A] (up to a negative one) are moved together; keys, values
+    and mass are changed in place, the new lengths int32 [B] are returned."""
+    return capi.native().cache_accept(keys, values, tables, lengths, accepted, mass)
+
+
+def CacheEvict(keys, values, tables, lengths, mass, keep, recent):
+    """chx_hip_cache_evict: sequences of more than `keep` places are cut to that many, each head by itself: the last `recent`, in their order, behind the keep - recent others
+    with the most mass; keys, values and mass are changed in place, the new lengths int32 [B] are returned."""
+    return capi.native().cache_evict(keys, values, tables, lengths, mass, keep, recent)
+
+
+def CrossAttention(q, keys, values, lengths=None, scale=None, out=None):
+    """chx_hip_cross_attention: softmax(scale q . keys) values for q [B, T, H, D] over an encoder's states [B, S, G, D], H a multiple of G, of which sequence b has
+    lengths[b] (int32 [B]; all by default).  scale: by default 1 / sqrt(D)."""
+    return capi.native().cross_attention(q, keys, values, lengths, _scale_of(q, scale), out)
+
+
+def _scale_of(q, scale):
+    return scale if scale is not None else 1.0 / max(1, q.shape[-1] if q.dim() else 1) ** 0.5
+
+
 def _pool_out(in_dim, p0, p1, k, s, cover_all):
     if cover_all:
         return (in_dim + p0 + p1 - k + s - 1) // s + 1

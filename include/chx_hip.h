@@ -522,6 +522,59 @@ int chx_hip_token_logprobs(
         const chx_hip_tensor* logits, const chx_hip_tensor* tokens, chx_hip_tensor* logprobs, chx_hip_tensor* entropy, chx_hip_tensor* top_logprobs,
         chx_hip_tensor* top_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
+/* A cache of keys and values in pages.  Of what follows:
+ *   keys, values  [pages, R, G, D]: pages of R places, G heads of D elements (1 to 256), float16 or float32, of one type and shape; any strides, elements of the last axis
+ *                 next to each other
+ *   tables        int32 [B, M]: the pages of sequence b, in order; place p of it is row p % R of page tables[b, p / R].  Rows may lie apart, M R below 2^30.  A number that is no page's
+ *                 stands for places that are not there: nothing is written to them, and nobody sees them
+ *   lengths       int32 [B]: how many places of a sequence hold rows (numbers outside 0 to M R count as the nearer of them)
+ *   mass          float32 [B, G, M R or more]: what attention has weighted each place with so far
+ * A page may be in several tables (or twice in one) where it is only read.  Arrays that are written share no memory with any other and have their elements apart; int32 arrays other than
+ * tables are contiguous. */
+
+/* Rows behind what is there: place lengths[b] + t of sequence b takes k[b, t] and v[b, t], for t below counts[b] (int32 [B]; NULL: all).  k, v [B, T, G, D] of the cache's
+ * type, any strides.  lengths stay as they are. */
+int chx_hip_cache_append(
+        chx_hip_tensor* keys, chx_hip_tensor* values, const chx_hip_tensor* k, const chx_hip_tensor* v, const chx_hip_tensor* tables, const chx_hip_tensor* lengths,
+        const chx_hip_tensor* counts, void* stream);
+
+/* Attention of drafted tokens over a cache that holds their own rows behind its lengths[b] others (chx_hip_cache_append).  Token t of sequence b sees those others, itself and
+ *   parents == NULL   the tokens before it: one token being generated (T = 1), or a piece of a prompt
+ *   parents           int32 [B, T], T up to 256: its ancestors in a tree; parents[b, t] is a token before t, or anything else for one that follows the others
+ *     y[b, t, h] = sum_p w_p values[p, h / (H / G)],  w = softmax(scale q[b, t, h] . keys[p, h / (H / G)])  over the places p that it sees
+ *   q, y    [B, T, H, D], H a multiple of G, any strides; y overlaps nothing
+ *   counts  int32 [B]: how many tokens a sequence has (numbers outside 0 to T as the nearer); NULL: T.  The others' results are 0
+ *   scale   above 0
+ *   mass    NULL, or gets the weights of each place, over all tokens and the heads that share its own: added for places below lengths[b], set for the tokens' own
+ * Products are of the operands as they are, sums float32; float16 weights are rounded to float16 before they are multiplied with values (2^-11 of each, as much as the result's own
+ * rounding is).  A place whose weight rounds to 0 adds nothing, whatever it holds; a token that sees nothing, or has no score above -inf, has a result of 0.
+ * workspace: aligned to 16. */
+int chx_hip_tree_attention_workspace(const chx_hip_tensor* q, const chx_hip_tensor* keys, const chx_hip_tensor* tables, int32_t with_mass, size_t* bytes);
+int chx_hip_tree_attention(
+        const chx_hip_tensor* q, const chx_hip_tensor* keys, const chx_hip_tensor* values, const chx_hip_tensor* tables, const chx_hip_tensor* lengths, const chx_hip_tensor* parents,
+        const chx_hip_tensor* counts, float scale, chx_hip_tensor* mass, chx_hip_tensor* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The drafted tokens that were accepted, next to each other: place lengths[b] + j takes key, value and mass (or NULL) of place lengths[b] + accepted[b, j].  accepted int32 [B, A], A up to 256, in
+ * any order; a sequence's end at its first negative one.  new_lengths int32 [B]: lengths and how many were accepted.  All rows of a sequence are read before any is written. */
+int chx_hip_cache_accept(
+        chx_hip_tensor* keys, chx_hip_tensor* values, const chx_hip_tensor* tables, const chx_hip_tensor* lengths, const chx_hip_tensor* accepted, chx_hip_tensor* mass,
+        chx_hip_tensor* new_lengths, void* stream);
+
+/* Eviction: a sequence of more than `keep` places is cut to that many, each head by itself.  The last `recent` (0 to keep) places stay, and of the others the keep - recent with
+ * the most mass (of equal ones the lower place first, a NaN before all others).  Those of them that lie below keep - recent stay where they are; the rest, in ascending order, take the places
+ * below it that have become free, in ascending order; behind them come the recent ones in their order.  mass moves along and is 0 from keep on; keys and values there stay
+ * as they are.  new_lengths int32 [B].  (So the oldest places lose their order, which attention does not ask for, and the recent ones do not.)  workspace: aligned to 4; places: M R. */
+int chx_hip_cache_evict_workspace(int64_t sequences, int64_t heads, int64_t places, int64_t keep, size_t* bytes);
+int chx_hip_cache_evict(
+        chx_hip_tensor* keys, chx_hip_tensor* values, const chx_hip_tensor* tables, const chx_hip_tensor* lengths, chx_hip_tensor* mass, int64_t keep, int64_t recent,
+        chx_hip_tensor* new_lengths, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention to an encoder's states: as above, each of q's rows [B, T, H, D] over the first lengths[b] (int32 [B]; NULL: all) of S states, keys and values [B, S, G, D]. */
+int chx_hip_cross_attention_workspace(const chx_hip_tensor* q, const chx_hip_tensor* keys, size_t* bytes);
+int chx_hip_cross_attention(
+        const chx_hip_tensor* q, const chx_hip_tensor* keys, const chx_hip_tensor* values, const chx_hip_tensor* lengths, float scale, chx_hip_tensor* y, void* workspace,
+        size_t workspace_bytes, void* stream);
+
 /* ---- pooling on quantized tensors ------------------------------------------------------ */
 
 /* MaxPoolOp::RunImpl, runtime/ops/pooling.cc:47-61, as it occurs in a quantized
