@@ -61,11 +61,15 @@ __device__ __forceinline__ u32x4 chunk_of(const char* row, int32_t at, int32_t b
     return v;
 }
 
+// A number that all lanes of a wavefront have, where the compiler goes by memory or a division for it.
+__device__ __forceinline__ int32_t uniform(int32_t v) {
+    return __builtin_amdgcn_readfirstlane(v);
+}
 __device__ __forceinline__ int32_t length_of(const AttentionArgs& a, int32_t b) {
-    return a.lengths ? max(0, min(a.lengths[b], a.places)) : a.places;
+    return a.lengths ? max(0, min(uniform(a.lengths[b]), a.places)) : a.places;
 }
 __device__ __forceinline__ int32_t count_of(const AttentionArgs& a, int32_t b) {
-    return a.counts ? max(0, min(a.counts[b], a.T)) : a.T;
+    return a.counts ? max(0, min(uniform(a.counts[b]), a.T)) : a.T;
 }
 
 __device__ __forceinline__ Place place_in(const AttentionArgs& a, int32_t b, int32_t p) {
@@ -178,220 +182,277 @@ __device__ __forceinline__ void store(const AttentionArgs& a, char* row, int32_t
         if (element + j < a.D) to[j] = v[j];
 }
 
-template <bool kHalf, int kSize>
-struct Tile {
-    static constexpr int kWaves = 4, kRowsOfWave = 32, kRows = kWaves * kRowsOfWave;
-    static constexpr int kKeyBlocks = kHalf || kSize < 256 ? 2 : 1;  // of 32 places
-    static constexpr int kKeys = 32 * kKeyBlocks;
-    static constexpr int kBytes = kKeys * Head<kHalf, kSize>::kRow;  // of k or v
-    static constexpr int kLds = 2 * kBytes + (int)sizeof(Nodes);
-};
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+template <typename V>
+__device__ __forceinline__ __attribute__((address_space(3))) V* lds_pointer(uint32_t at) {
+    return (__attribute__((address_space(3))) V*)(uintptr_t)at;
+}
 
-// One work-group: 128 rows, four wavefronts with 32 each, and the places of one part.  k and v go through LDS.
-template <bool kHalf, int kSize>
-__global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
+// ---- a wavefront's work on a block of places: 32 rows, a lane's row is lane & 31 ---------------------------------
+
+// Scores of blocks of 32 places, whose keys lie in LDS from `keys` on; 32 rows to a lane's column.
+template <bool kHalf, int kSize, int kCount>
+__device__ __forceinline__ void find_scores(const char* keys, const u32x4 (&q)[Head<kHalf, kSize>::kSteps], f32x16 (&score)[kCount]) {
     using H = Head<kHalf, kSize>;
-    using W = Tile<kHalf, kSize>;
-    constexpr int kSteps = H::kSteps, kBlocks = H::kBlocks, kKeyBlocks = W::kKeyBlocks, kKeys = W::kKeys;
-    extern __shared__ __attribute__((aligned(128))) char attention_lds[];
-    char *k_lds = attention_lds, *v_lds = attention_lds + W::kBytes;
-    Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + 2 * W::kBytes);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int32_t part = blockIdx.x % a.parts, of_tile = blockIdx.x / a.parts, row_tile = of_tile % a.row_tiles;
-    const int32_t b = of_tile / a.row_tiles / a.groups, group = of_tile / a.row_tiles % a.groups;
-    const int32_t rows = a.T * a.fan, length = length_of(a, b), count = count_of(a, b);
-    const int32_t first_row = row_tile * W::kRows, r = first_row + wave * W::kRowsOfWave + (lane & 31);
-    const int32_t t = r < rows ? r / a.fan : a.T, head = group * a.fan + (r - t * a.fan);
-    // the places that any row of the work-group sees
-    const int32_t last_t = min((min(first_row + W::kRows, rows) - 1) / a.fan, count - 1), first_t = first_row / a.fan;
-    int32_t end = last_t < first_t ? 0 : a.kind == kCross ? length : a.kind == kChain ? length + last_t + 1 : length + count;
-    end = min(end, a.places);
-    const int32_t tiles = (end + kKeys - 1) / kKeys, each = (tiles + a.parts - 1) / a.parts;
-    const int32_t begin_tile = part * each, end_tile = min(begin_tile + each, tiles);
-    const bool any_drafted = a.kind == kTree && end_tile * kKeys > length && begin_tile < end_tile;
-    if (any_drafted) find_ancestors(nodes, a.parents + (int64_t)b * a.T, a.T);
-    const Sight sight = sight_of(a, t, length, count);
-    // places below this are seen by all rows of the wavefront
-    int32_t plain = sight.limit;
+    const int lane = threadIdx.x & 63, row = lane & 31;
+    // (chunk 2 s + half of row, its place turned: s comes in by one more exclusive or; 32 rows on, all is the same)
+    uint32_t at = lds_address(keys) + row * H::kRow + (((lane >> 5) ^ H::turned(row)) << 4);
+    asm volatile("" : "+v"(at));  // (the others are made from it where they are used)
 #pragma unroll
-    for (int d = 16; d; d /= 2) plain = min(plain, __shfl_xor(plain, d));
-    plain = __builtin_amdgcn_readfirstlane(plain);
-
-    const int32_t row_bytes = a.D * H::kElement;
-    u32x4 q[kSteps];
-    {
-        const char* at = a.q + b * a.q_batch + t * a.q_token + head * a.q_head;
+    for (int n = 0; n < kCount; ++n) score[n] = f32x16{};
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) q[s] = r < rows ? chunk_of<kHalf>(at, (2 * s + half) * 16, row_bytes, a.q_whole) : u32x4{0, 0, 0, 0};
+    for (int s = 0; s < H::kSteps; ++s) {
+#pragma unroll
+        for (int n = 0; n < kCount; ++n) score[n] = score_of<kHalf>(*lds_pointer<u32x4>((at ^ (s << 5)) + n * 32 * H::kRow), q[s], score[n]);
     }
+}
 
-    f32x16 acc[kBlocks];
-    float m, l;
-    uint32_t marks[3][kBlocks / 2];  // a bit for each result: whether inf, -inf, NaN of v have weight in it
-    // A result that is not finite has one of v that is not, or 0 times one: places of no weight add nothing, whatever they hold.  Then the sums are made
-    // again, first of what is inf, -inf and NaN, as ones, then of the rest.
-    for (int special = 0; special < 5; ++special) {
-        m = kNoMaximum;
-        l = 0.f;
+// Weights in the scores' place; the sums so far are brought to the new maximum.
+template <bool kHalf, int kBlocks, int kCount>
+__device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCount], f32x16 (&acc)[kBlocks], float& m, float& l) {
+    float most = score[0][0];
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n) acc[n] = f32x16{};
-        for (int32_t tile = begin_tile; tile < end_tile; ++tile) {
-            const int32_t p0 = tile * kKeys;
-            __syncthreads();
-            for (int i = threadIdx.x; i < kKeys * H::kChunks; i += 256) {
-                const int row = i / H::kChunks, at = (i % H::kChunks ^ H::turned(row)) * 16;
-                u32x4 kc = {0, 0, 0, 0}, vc = {0, 0, 0, 0};
-                if (p0 + row < end) {
-                    const Place p = place_in(a, b, p0 + row);
-                    if (p.page >= 0) {
-                        kc = chunk_of<kHalf>(a.k + p.page * a.k_page + p.row * a.k_row + group * a.k_head, at, row_bytes, a.k_whole);
-                        vc = chunk_of<kHalf>(a.v + p.page * a.v_page + p.row * a.v_row + group * a.v_head, at, row_bytes, a.k_whole);
-                    }
-                }
-                *reinterpret_cast<u32x4*>(k_lds + i * 16) = kc;
-                *reinterpret_cast<u32x4*>(v_lds + i * 16) = vc;
-            }
-            const int32_t mine = p0 + (lane & (kKeys - 1));
-            const uint64_t there = __builtin_amdgcn_ballot_w64(mine < end && place_in(a, b, mine).page >= 0);
-            __syncthreads();
-
-            f32x16 score[kKeyBlocks];
+    for (int n = 0; n < kCount; ++n)
 #pragma unroll
-            for (int n = 0; n < kKeyBlocks; ++n) {
-                score[n] = f32x16{};
-                const int row = n * 32 + (lane & 31);
-                const char* at = k_lds + row * H::kRow;
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, score[n][i]);
+    most = fmaxf(most, with_other_half(most)) * scale2;
+    if (__builtin_amdgcn_ballot_w64(most > m + kLag)) {
+        const float next = fmaxf(m, most), f = __builtin_amdgcn_exp2f(m - next);
+        l *= f;
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    const u32x4 kc = *reinterpret_cast<const u32x4*>(at + (((2 * s + half) ^ H::turned(row)) << 4));
-                    score[n] = score_of<kHalf>(kc, q[s], score[n]);
-                }
-            }
-            constexpr uint64_t kAll = kKeys == 64 ? ~0ull : (1ull << (kKeys & 63)) - 1;
-            if (p0 + kKeys > plain || (there & kAll) != kAll) {
+        for (int n = 0; n < kBlocks; ++n) acc[n] *= f;
+        m = next;
+    }
+    const float less = m - kRaise<kHalf>;
 #pragma unroll
-                for (int n = 0; n < kKeyBlocks; ++n) score[n] = hide(score[n], (seen_of(sight, nodes, p0 + 32 * n) & (uint32_t)(there >> (32 * n))) >> (4 * half));
-            }
-            float most = score[0][0];
+    for (int n = 0; n < kCount; ++n)
 #pragma unroll
-            for (int n = 0; n < kKeyBlocks; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) most = fmaxf(most, score[n][i]);
-            most = fmaxf(most, with_other_half(most)) * a.scale2;
-            if (__builtin_amdgcn_ballot_w64(most > m + kLag)) {
-                const float next = fmaxf(m, most), f = __builtin_amdgcn_exp2f(m - next);
-                l *= f;
-#pragma unroll
-                for (int n = 0; n < kBlocks; ++n) acc[n] *= f;
-                m = next;
-            }
-            const float less = m - kRaise<kHalf>;
-#pragma unroll
-            for (int n = 0; n < kKeyBlocks; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    score[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][i], a.scale2, -less));
-                    l += score[n][i];
-                }
-
-            auto second = [&](auto replaced) __attribute__((always_inline)) {
-                if constexpr (kHalf) {
-#pragma unroll
-                    for (int kb = 0; kb < 2 * kKeyBlocks; ++kb) {
-                        half8 w;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = (_Float16)score[kb >> 1][8 * (kb & 1) + j];
-#pragma unroll
-                        for (int n = 0; n < kBlocks; ++n) {
-                            union {
-                                short4v part[2];
-                                half8 whole;
-                            } vf;
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int row = kb * 16 + e * 8 + 4 * half + ((lane & 15) >> 2), c = 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                                const char* at = v_lds + row * H::kRow + ((c ^ H::turned(row)) << 4) + 8 * (lane & 1);
-                                vf.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)at);
-                            }
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) vf.whole[j] = (_Float16)replaced((float)vf.whole[j]);
-                            acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, w, acc[n], 0, 0, 0);
-                        }
-                    }
-                } else {
-                    constexpr int kWide = H::kWide;
-#pragma unroll
-                    for (int n = 0; n < kKeyBlocks; ++n)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int row = n * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-#pragma unroll
-                            for (int w = 0; w < kBlocks / kWide; ++w) {
-                                const int at = (kWide * (lane & 31) + 32 * kWide * w) * 4;
-                                const char* from = v_lds + row * H::kRow + (((at >> 4) ^ H::turned(row)) << 4) + (at & 15);
-                                float vf[kWide];
-                                __builtin_memcpy(vf, from, sizeof(vf));
-#pragma unroll
-                                for (int j = 0; j < kWide; ++j) acc[w * kWide + j] = __builtin_amdgcn_mfma_f32_32x32x2f32(replaced(vf[j]), score[n][i], acc[w * kWide + j], 0, 0, 0);
-                            }
-                        }
-                }
-            };
-            if (special == 0) second([](float v) { return v; });
-            else second([special](float v) { return special == 4 ? (v - v == 0.f ? v : 0.f) : special == 3 ? (v != v ? 1.f : 0.f) : v == (special == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f; });
+        for (int i = 0; i < 16; ++i) {
+            score[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][i], scale2, -less));
+            l += score[n][i];
         }
-        if (special == 0) {
-            float zero = 0.f;
+}
+
+// What is added up in place of v: itself, or (where results are made again) ones for what is inf, -inf and NaN, or what is finite.
+enum { kAll, kInfinities, kNegativeInfinities, kNans, kFinite };
+__device__ __forceinline__ float replaced(float v, int32_t special) {
+    return special == kFinite ? (v - v == 0.f ? v : 0.f) : special == kNans ? (v != v ? 1.f : 0.f) : v == (special == kInfinities ? INFINITY : -INFINITY) ? 1.f : 0.f;
+}
+
+// acc += v^T weights^T, v's rows in LDS from `values` on.
+template <bool kHalf, int kSize, bool kSpecial, int kCount>
+__device__ __forceinline__ void add_values(const char* values, const f32x16 (&weight)[kCount], int32_t special, f32x16 (&acc)[kSize / 32]) {
+    using H = Head<kHalf, kSize>;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    if constexpr (kHalf) {
+        // 16 lanes read 4 rows of 16 elements, which are transposed on the way: a lane gets 4 rows of one element.  Two such reads make a fragment; 16 rows on, all is the same, and
+        // 32 elements on one more exclusive or
+        uint32_t at[2];
 #pragma unroll
-            for (int n = 0; n < kBlocks; ++n)
+        for (int e = 0; e < 2; ++e) {
+            const int row = e * 8 + 4 * half + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            at[e] = lds_address(values) + row * H::kRow + ((c ^ H::turned(row)) << 4) + 8 * (lane & 1);
+            asm volatile("" : "+v"(at[e]));
+        }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(acc[n][i], 0.f, zero);
-            if (!__syncthreads_or(zero != 0.f)) break;
-        } else if (special < 4) {
+        for (int kb = 0; kb < 2 * kCount; ++kb) {
+            half8 w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = (_Float16)weight[kb >> 1][8 * (kb & 1) + j];
+#pragma unroll
+            for (int n = 0; n < H::kBlocks; ++n) {
+                union {
+                    short4v part[2];
+                    half8 whole;
+                } vf;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) vf.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_pointer<short4v>((at[e] ^ (n << 6)) + kb * 16 * H::kRow));
+                if constexpr (kSpecial) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) vf.whole[j] = (_Float16)replaced((float)vf.whole[j], special);
+                }
+                acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, w, acc[n], 0, 0, 0);
+            }
+        }
+    } else {
+        // a lane reads kWide elements of one row; row i of a block is turned by what 16 rows have in common
+        constexpr int kWide = H::kWide;
+        typedef float Wide __attribute__((ext_vector_type(kWide)));
+        uint32_t at = lds_address(values) + 4 * half * H::kRow + 4 * kWide * (lane & 31);
+        asm volatile("" : "+v"(at));
+        const uint32_t turn = half << 4;  // of row 4 half
+#pragma unroll
+        for (int n = 0; n < kCount; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = n * 32 + 8 * (i >> 2) + (i & 3);
+                const uint32_t turned = (H::turned(row) << 4) ^ turn;
+#pragma unroll
+                for (int w = 0; w < H::kBlocks / kWide; ++w) {
+                    const Wide vf = *lds_pointer<Wide>((at ^ turned) + row * H::kRow + 128 * kWide * w);
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j)
+                        acc[w * kWide + j] = __builtin_amdgcn_mfma_f32_32x32x2f32(kSpecial ? replaced(vf[j], special) : vf[j], weight[n][i], acc[w * kWide + j], 0, 0, 0);
+                }
+            }
+    }
+}
+
+// Whether a lane has a sum that is not finite.
+template <int kBlocks>
+__device__ __forceinline__ bool not_finite(const f32x16 (&acc)[kBlocks]) {
+    float zero = 0.f;
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(acc[n][i], 0.f, zero);
+    return zero != 0.f;
+}
+
+// The sums of a row, added up again where one of them is not finite: then v is not, or it is the product of 0 and something infinite, and places of no weight add nothing, whatever they hold.
+// `pass` goes over the places once, with what stands for v.  `any`: of all that make the passes together.
+template <int kBlocks, typename Pass, typename Any>
+__device__ __forceinline__ void add_up(f32x16 (&acc)[kBlocks], Pass pass, Any any) {
+    uint32_t marks[3][kBlocks / 2];  // a bit for each sum: whether it has an inf, -inf, NaN
+#pragma unroll 1
+    for (int32_t special = kAll; special <= kFinite; ++special) {
+        pass(special);
+        if (special == kAll) {
+            if (!any(not_finite(acc))) return;
+        } else if (special < kFinite) {
 #pragma unroll
             for (int n = 0; n < kBlocks; n += 2) {
                 uint32_t found = 0;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) found |= (uint32_t)(acc[n + i / 16][i & 15] > 0.f) << i;
-                marks[special - 1][n / 2] = found;
+#pragma unroll
+                for (int k = 0; k < 3; ++k) marks[k][n / 2] = special == k + 1 ? found : marks[k][n / 2];
             }
-        } else {
-#pragma unroll
-            for (int n = 0; n < kBlocks; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int bit = 16 * (n & 1) + i;
-                    if ((marks[0][n / 2] >> bit) & 1) acc[n][i] += INFINITY;
-                    if ((marks[1][n / 2] >> bit) & 1) acc[n][i] -= INFINITY;
-                    if ((marks[2][n / 2] >> bit) & 1) acc[n][i] = NAN;
-                }
         }
     }
-
-    l += with_other_half(l);
-    const int64_t group_rows = ((int64_t)b * a.groups + group) * rows;
-    if (a.parts > 1) {
-        const int64_t at = (int64_t)blockIdx.x * W::kRows + wave * W::kRowsOfWave + (lane & 31);
-        if (half == 0) *reinterpret_cast<f32x2*>(a.part_stats + 2 * at) = f32x2{m, l};
-        if (begin_tile >= end_tile || r >= rows) return;
-        float* to = a.part_sums + at * kSize;
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n)
+    for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int bit = 16 * (n & 1) + i;
+            float v = acc[n][i];
+            v += (marks[0][n / 2] >> bit) & 1 ? INFINITY : 0.f;
+            v -= (marks[1][n / 2] >> bit) & 1 ? INFINITY : 0.f;
+            acc[n][i] = (marks[2][n / 2] >> bit) & 1 ? NAN : v;
+        }
+}
+
+// ---- rows of k and v into LDS ---------------------------------------------------------------------------------------
+
+// Asynchronous copies of 16 bytes a lane into LDS, lane i's to lds + 16 i (the same for all lanes), counted like loads.
+__device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(uniform(lds)) : "memory", "m0");
+}
+__device__ __forceinline__ void copy_to_lds(const char* from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
+}
+
+__device__ const u32x4 kZeros[1] = {{0, 0, 0, 0}};  // what rows that are not there are read from
+
+// What a lane knows of kPlaces places from p0 on: of place p0 + lane % kPlaces, where it lies; of all, which are there.
+template <int kPlaces>
+struct Places {
+    Place at;
+    uint64_t there;
+    __device__ __forceinline__ void look_up(const AttentionArgs& a, int32_t b, int32_t p0, int32_t end) {
+        const int32_t p = p0 + (int)(threadIdx.x & (kPlaces - 1));
+        at = {-1, 0};
+        if (p < end) at = place_in(a, b, p);
+    }
+    __device__ __forceinline__ bool whole() const {
+        constexpr uint64_t kAllOfThem = kPlaces == 64 ? ~0ull : (1ull << (kPlaces & 63)) - 1;
+        return (there & kAllOfThem) == kAllOfThem;
+    }
+    // (waits for the tables)
+    __device__ __forceinline__ void settle() {
+        there = __builtin_amdgcn_ballot_w64(at.page >= 0);
+    }
+};
+
+// One of the arrays that is copied from.
+struct From {
+    const char* base;  // of the group's head
+    int64_t page, row;
+    uint32_t of_lane;  // how far the lane's row is from the first one of an instruction
+};
+template <typename H>
+__device__ __forceinline__ From from_of(const char* base, int64_t page, int64_t row) {
+    return {base, page, row, (uint32_t)((threadIdx.x & 63) / H::kChunks * row)};
+}
+
+// Whether the rows of every instruction's copies lie in one page, at distances that 32 bits hold, and fill the kernel's: then their address is one of the wavefront's and an offset.
+template <typename H>
+__device__ __forceinline__ bool in_runs(const AttentionArgs& a) {
+    constexpr int32_t kRows = 64 / H::kChunks;
+    return a.k_whole && (a.tables == nullptr || a.page_rows % kRows == 0) && a.D * H::kElement == H::kRow && a.k_row >= 0 && a.k_row < (1 << 24) && a.v_row >= 0 && a.v_row < (1 << 24);
+}
+
+// Copies first, first + 1, .. (kCount of them, 1024 bytes of LDS each) of a tile's rows.
+template <typename H, int kPlaces, int kCount>
+__device__ __forceinline__ void copy_rows(const AttentionArgs& a, const From& f, const Places<kPlaces>& places, bool runs, uint32_t lds, char* to, int32_t first) {
+    constexpr int kRows = 64 / H::kChunks;
+    const int lane = threadIdx.x & 63;
+    if (runs && places.whole()) {
+#pragma unroll
+        for (int j = 0; j < kCount; ++j) {
+            const int32_t i = first + j, row = i * kRows + lane / H::kChunks;
+            const int32_t page = __builtin_amdgcn_readlane(places.at.page, i * kRows), at = __builtin_amdgcn_readlane(places.at.row, i * kRows);
+            copy_to_lds(f.of_lane + (((lane % H::kChunks) ^ H::turned(row)) << 4), f.base + page * f.page + at * f.row, lds + i * 1024);
+        }
+        return;
+    }
+    const int32_t row_bytes = a.D * H::kElement;
+#pragma unroll 1
+    for (int j = 0; j < kCount; ++j) {
+        const int32_t i = first + j, row = i * kRows + lane / H::kChunks, c = ((lane % H::kChunks) ^ H::turned(row)) << 4;
+        const int32_t page = __shfl(places.at.page, row), at = __shfl(places.at.row, row);
+        const char* from = f.base + page * f.page + at * f.row;
+        if (a.k_whole) {
+            copy_to_lds(page >= 0 && c < row_bytes ? from + c : reinterpret_cast<const char*>(kZeros), lds + i * 1024);
+        } else {
+            u32x4 v = {0, 0, 0, 0};
+            if (page >= 0) v = chunk_of<H::kElement == 2>(from, c, row_bytes, false);
+            *reinterpret_cast<u32x4*>(to + i * 1024 + lane * 16) = v;
+        }
+    }
+}
+
+// ---- results ----------------------------------------------------------------------------------------------------------
+
+// A row's results, or what there is of them: 16 elements of it in blocks of 32 to a lane.
+template <bool kHalf, int kSize>
+__device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)[kSize / 32], float m, float l, int32_t b, int32_t group, int32_t r, int64_t part_row, bool any) {
+    using H = Head<kHalf, kSize>;
+    const int half = (threadIdx.x & 63) >> 5;
+    const int32_t rows = a.T * a.fan;
+    l += with_other_half(l);
+    if (a.parts > 1) {
+        if (half == 0) *reinterpret_cast<f32x2*>(a.part_stats + 2 * part_row) = f32x2{m, l};
+        if (!any || r >= rows) return;
+        float* to = a.part_sums + part_row * kSize;
+#pragma unroll
+        for (int n = 0; n < H::kBlocks; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) to[H::element(n, i, half)] = acc[n][i];
         return;
     }
     if (r >= rows) return;
-    if (a.sums != nullptr && half == 0) a.sums[group_rows + r] = sum_of<kHalf>(m, l);
+    if (a.sums != nullptr && half == 0) a.sums[((int64_t)b * a.groups + group) * rows + r] = sum_of<kHalf>(m, l);
     const float share = l == 0.f ? 0.f : 1.f / l;
+    const int32_t t = r / a.fan, head = group * a.fan + (r - t * a.fan);
     char* y = a.y + b * a.y_batch + t * a.y_token + head * a.y_head;
 #pragma unroll
-    for (int n = 0; n < kBlocks; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[n][i] *= share;
+    for (int n = 0; n < H::kBlocks; ++n) acc[n] *= share;
     if constexpr (kHalf) {
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n)
+        for (int n = 0; n < H::kBlocks; ++n)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const half4 v = {(_Float16)acc[n][i], (_Float16)acc[n][i + 1], (_Float16)acc[n][i + 2], (_Float16)acc[n][i + 3]};
@@ -400,7 +461,7 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
     } else {
         constexpr int kWide = H::kWide;
 #pragma unroll
-        for (int n = 0; n < kBlocks; n += kWide)
+        for (int n = 0; n < H::kBlocks; n += kWide)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float v __attribute__((ext_vector_type(kWide)));
@@ -409,6 +470,134 @@ __global__ __launch_bounds__(256) void attention_kernel(AttentionArgs a) {
                 store<kWide>(a, y, H::element(n, i, half), v);
             }
     }
+}
+
+// What a work-group works on.
+struct Job {
+    int32_t b, group, part, row_tile;
+    int32_t rows, length, count, end;  // end: of the places that any of its rows sees
+    int32_t begin_tile, end_tile;      // of its part
+};
+__device__ __forceinline__ Job job_of(const AttentionArgs& a, int32_t tile_rows, int32_t tile_places) {
+    Job j;
+    const int32_t of_tile = uniform(blockIdx.x / a.parts), of_group = uniform(of_tile / a.row_tiles);
+    j.part = blockIdx.x - of_tile * a.parts;
+    j.row_tile = of_tile - of_group * a.row_tiles;
+    j.b = uniform(of_group / a.groups);
+    j.group = of_group - j.b * a.groups;
+    j.rows = a.T * a.fan;
+    j.length = length_of(a, j.b);
+    j.count = count_of(a, j.b);
+    const int32_t first_t = j.row_tile * tile_rows / a.fan, last_t = min((min((j.row_tile + 1) * tile_rows, j.rows) - 1) / a.fan, j.count - 1);
+    j.end = last_t < first_t ? 0 : a.kind == kCross ? j.length : a.kind == kChain ? j.length + last_t + 1 : j.length + j.count;
+    j.end = min(j.end, a.places);
+    const int32_t tiles = (j.end + tile_places - 1) / tile_places, each = uniform((tiles + a.parts - 1) / a.parts);
+    j.begin_tile = j.part * each;
+    j.end_tile = min(j.begin_tile + each, tiles);
+    return j;
+}
+
+// A lane's row, and what the rows of its wavefront see.
+struct Row {
+    int32_t r, t, head;
+    Sight sight;
+    int32_t plain;  // places below this are seen by all of them
+};
+__device__ __forceinline__ Row row_of(const AttentionArgs& a, const Job& j, int32_t r) {
+    Row row;
+    row.r = r;
+    row.t = r < j.rows ? r / a.fan : a.T;
+    row.head = j.group * a.fan + (r - row.t * a.fan);
+    row.sight = sight_of(a, row.t, j.length, j.count);
+    int32_t plain = row.sight.limit;
+#pragma unroll
+    for (int d = 16; d; d /= 2) plain = min(plain, __shfl_xor(plain, d));
+    row.plain = __builtin_amdgcn_readfirstlane(plain);
+    return row;
+}
+template <bool kHalf, int kSize>
+__device__ __forceinline__ void load_row(const AttentionArgs& a, const Job& j, const Row& row, u32x4 (&q)[Head<kHalf, kSize>::kSteps]) {
+    using H = Head<kHalf, kSize>;
+    const int half = (threadIdx.x & 63) >> 5;
+    const char* at = a.q + j.b * a.q_batch + row.t * a.q_token + row.head * a.q_head;
+#pragma unroll
+    for (int s = 0; s < H::kSteps; ++s) q[s] = row.r < j.rows ? chunk_of<kHalf>(at, (2 * s + half) * 16, a.D * H::kElement, a.q_whole) : u32x4{0, 0, 0, 0};
+}
+
+// ---- many rows --------------------------------------------------------------------------------------------------------
+//
+// A work-group has 128 rows, its four wavefronts 32 each, and goes over the places of one part in tiles that it copies into LDS together: two of them, the next one on its way while this one
+// is worked on.
+template <bool kHalf, int kSize>
+struct Tile {
+    static constexpr int kWaves = 4, kRows = kWaves * 32;
+    static constexpr int kBlocksOf = Head<kHalf, kSize>::kRow <= 512 ? 2 : 1;  // of 32 places
+    static constexpr int kPlaces = 32 * kBlocksOf;
+    static constexpr int kBytes = kPlaces * Head<kHalf, kSize>::kRow;  // of k or v
+    static constexpr int kCopies = kBytes / 1024 / kWaves;
+    static constexpr int kBuffers = 4 * kBytes <= 128 * 1024 ? 2 : 1;
+    static constexpr int kLds = 2 * kBuffers * kBytes + (int)sizeof(Nodes);
+};
+
+template <bool kHalf, int kSize>
+__global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1)) void attention_rows_kernel(AttentionArgs a) {
+    using H = Head<kHalf, kSize>;
+    using W = Tile<kHalf, kSize>;
+    static_assert(W::kBuffers == 2, "one tile on its way");
+    extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
+    Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + 4 * W::kBytes);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
+    const Job job = job_of(a, W::kRows, W::kPlaces);
+    if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors(nodes, a.parents + (int64_t)job.b * a.T, a.T);
+    const Row row = row_of(a, job, job.row_tile * W::kRows + wave * 32 + (lane & 31));
+    u32x4 q[H::kSteps];
+    load_row<kHalf, kSize>(a, job, row, q);
+    const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row), v = from_of<H>(a.v + job.group * a.v_head, a.v_page, a.v_row);
+    const bool runs = in_runs<H>(a);
+    const uint32_t lds = lds_address(attention_lds);
+    f32x16 acc[H::kBlocks];
+    float m, l;
+
+    auto pass = [&](int32_t special) __attribute__((always_inline)) {
+        m = kNoMaximum;
+        l = 0.f;
+#pragma unroll
+        for (int n = 0; n < H::kBlocks; ++n) acc[n] = f32x16{};
+        if (job.begin_tile >= job.end_tile) return;
+        Places<W::kPlaces> next;
+        auto copy = [&](int32_t tile) __attribute__((always_inline)) {
+            const int32_t at = (tile & 1) * 2 * W::kBytes;
+            copy_rows<H, W::kPlaces, W::kCopies>(a, k, next, runs, lds + at, attention_lds + at, wave * W::kCopies);
+            copy_rows<H, W::kPlaces, W::kCopies>(a, v, next, runs, lds + at + W::kBytes, attention_lds + at + W::kBytes, wave * W::kCopies);
+        };
+        next.look_up(a, job.b, job.begin_tile * W::kPlaces, job.end);
+        next.settle();
+        copy(job.begin_tile);
+        for (int32_t tile = job.begin_tile; tile < job.end_tile; ++tile) {
+            const uint64_t there = next.there;
+            const bool whole = next.whole();
+            next.look_up(a, job.b, (tile + 1) * W::kPlaces, job.end);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            next.settle();
+            if (tile + 1 < job.end_tile) copy(tile + 1);
+            const char* keys = attention_lds + (tile & 1) * 2 * W::kBytes;
+            const int32_t p0 = tile * W::kPlaces;
+            f32x16 score[W::kBlocksOf];
+            find_scores<kHalf, kSize>(keys, q, score);
+            if (p0 + W::kPlaces > row.plain || !whole) {
+#pragma unroll
+                for (int n = 0; n < W::kBlocksOf; ++n) score[n] = hide(score[n], (seen_of(row.sight, nodes, p0 + 32 * n) & (uint32_t)(there >> (32 * n))) >> (4 * half));
+            }
+            find_weights<kHalf>(a.scale2, score, acc, m, l);
+            if (special == kAll) add_values<kHalf, kSize, false>(keys + W::kBytes, score, special, acc);
+            else add_values<kHalf, kSize, true>(keys + W::kBytes, score, special, acc);
+        }
+        __syncthreads();
+    };
+    add_up(acc, pass, [](bool mine) { return __syncthreads_or(mine) != 0; });
+    finish_row<kHalf, kSize>(a, acc, m, l, job.b, job.group, row.r, (int64_t)blockIdx.x * W::kRows + wave * 32 + (lane & 31), job.begin_tile < job.end_tile);
 }
 
 // A row's parts, by a wavefront: y = sum_i l_i 2^(m_i - m) (sums_i / l_i) over its sum of l_i 2^(m_i - m), in the order of the parts.
@@ -505,11 +694,11 @@ __global__ __launch_bounds__(256) void attention_mass_kernel(AttentionArgs a) {
 template <bool kHalf, int kSize>
 int attend_of(const AttentionArgs& a, hipStream_t s) {
     using W = Tile<kHalf, kSize>;
-    auto kernel = attention_kernel<kHalf, kSize>;
+    auto kernel = attention_rows_kernel<kHalf, kSize>;
     if constexpr (W::kLds > 65536)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, W::kLds));
     kernel<<<(unsigned)((int64_t)a.B * a.groups * a.row_tiles * a.parts), 256, W::kLds, s>>>(a);
-    return launch_check("attention_kernel");
+    return launch_check("attention_rows_kernel");
 }
 template <bool kHalf, int kSize>
 int join_of(const AttentionArgs& a, hipStream_t s) {
