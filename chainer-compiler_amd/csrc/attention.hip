@@ -8,10 +8,11 @@
 namespace chx {
 namespace {
 
-// How rows and places are shared out.  Parts: as many as give each compute unit two work-groups, of at least four tiles each.
+// How rows and places are shared out: the kernel for few rows up to 32, that for many from there on; parts as many as give each compute unit two work-groups, of at least 256 places each.
 void share_out(AttentionArgs* a) {
-    a->tile_rows = 128;
-    a->row_tiles = (int32_t)(((int64_t)a->T * a->fan + a->tile_rows - 1) / a->tile_rows);
+    const int64_t rows = (int64_t)a->T * a->fan;
+    a->tile_rows = rows <= 32 ? 32 : 128;
+    a->row_tiles = (int32_t)((rows + a->tile_rows - 1) / a->tile_rows);
     const int64_t groups = (int64_t)a->B * a->groups * a->row_tiles, most = (a->places + 255) / 256;
     int64_t parts = (512 + groups - 1) / (groups < 1 ? 1 : groups);
     parts = parts > most ? most : parts;

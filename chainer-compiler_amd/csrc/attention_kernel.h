@@ -81,30 +81,36 @@ struct Nodes {
     uint32_t sees[kMostNodes][kMostNodes / 32];
     int16_t up[kMostNodes];
 };
+template <int kThreads>
 __device__ __forceinline__ void find_ancestors(Nodes* nodes, const int32_t* parents, int32_t T) {
-    const int i = threadIdx.x;
+    constexpr int kOf = kMostNodes / kThreads;  // nodes of a lane
     const int words = (T + 31) / 32;
-    if (i < T) {
+    for (int i = threadIdx.x; i < T; i += kThreads) {
         const int32_t p = parents[i];
         nodes->up[i] = (int16_t)(p >= 0 && p < i ? p : -1);
         for (int w = 0; w < words; ++w) nodes->sees[i][w] = w == i / 32 ? 1u << (i & 31) : 0;
     }
     __syncthreads();
     for (int reach = 1; reach < T; reach *= 2) {
-        uint32_t more[kMostNodes / 32];
-        int32_t up = -1, next = -1;
-        if (i < T) up = nodes->up[i];
-        if (up >= 0) {
-            next = nodes->up[up];
+        uint32_t more[kOf][kMostNodes / 32];
+        int32_t up[kOf], next[kOf];
 #pragma unroll
-            for (int w = 0; w < kMostNodes / 32; ++w) more[w] = w < words ? nodes->sees[up][w] : 0;
+        for (int j = 0; j < kOf; ++j) {
+            const int i = j * kThreads + threadIdx.x;
+            up[j] = i < T ? nodes->up[i] : -1;
+            next[j] = up[j] >= 0 ? nodes->up[up[j]] : -1;
+#pragma unroll
+            for (int w = 0; w < kMostNodes / 32; ++w) more[j][w] = w < words && up[j] >= 0 ? nodes->sees[up[j]][w] : 0;
         }
         __syncthreads();
-        if (up >= 0) {
-            nodes->up[i] = (int16_t)next;
+#pragma unroll
+        for (int j = 0; j < kOf; ++j) {
+            const int i = j * kThreads + threadIdx.x;
+            if (up[j] < 0) continue;
+            nodes->up[i] = (int16_t)next[j];
 #pragma unroll
             for (int w = 0; w < kMostNodes / 32; ++w)
-                if (w < words) nodes->sees[i][w] |= more[w];
+                if (w < words) nodes->sees[i][w] |= more[j][w];
         }
         __syncthreads();
     }
@@ -361,17 +367,10 @@ template <int kPlaces>
 struct Places {
     Place at;
     uint64_t there;
-    __device__ __forceinline__ void look_up(const AttentionArgs& a, int32_t b, int32_t p0, int32_t end) {
+    __device__ __forceinline__ Places(const AttentionArgs& a, int32_t b, int32_t p0, int32_t end) {
         const int32_t p = p0 + (int)(threadIdx.x & (kPlaces - 1));
         at = {-1, 0};
         if (p < end) at = place_in(a, b, p);
-    }
-    __device__ __forceinline__ bool whole() const {
-        constexpr uint64_t kAllOfThem = kPlaces == 64 ? ~0ull : (1ull << (kPlaces & 63)) - 1;
-        return (there & kAllOfThem) == kAllOfThem;
-    }
-    // (waits for the tables)
-    __device__ __forceinline__ void settle() {
         there = __builtin_amdgcn_ballot_w64(at.page >= 0);
     }
 };
@@ -387,27 +386,19 @@ __device__ __forceinline__ From from_of(const char* base, int64_t page, int64_t 
     return {base, page, row, (uint32_t)((threadIdx.x & 63) / H::kChunks * row)};
 }
 
-// Whether the rows of every instruction's copies lie in one page, at distances that 32 bits hold, and fill the kernel's: then their address is one of the wavefront's and an offset.
+// Whether the rows of every instruction's copies (of four, where it has fewer) lie in one page, at distances that 32 bits hold, and fill the kernel's: then their address is one of the
+// wavefront's and an offset.
 template <typename H>
 __device__ __forceinline__ bool in_runs(const AttentionArgs& a) {
-    constexpr int32_t kRows = 64 / H::kChunks;
+    constexpr int32_t kRows = 64 / H::kChunks < 4 ? 4 : 64 / H::kChunks;
     return a.k_whole && (a.tables == nullptr || a.page_rows % kRows == 0) && a.D * H::kElement == H::kRow && a.k_row >= 0 && a.k_row < (1 << 24) && a.v_row >= 0 && a.v_row < (1 << 24);
 }
 
-// Copies first, first + 1, .. (kCount of them, 1024 bytes of LDS each) of a tile's rows.
+// The same for places anywhere: kCount copies from the first-th of the tile on.  What is not there is 0.
 template <typename H, int kPlaces, int kCount>
-__device__ __forceinline__ void copy_rows(const AttentionArgs& a, const From& f, const Places<kPlaces>& places, bool runs, uint32_t lds, char* to, int32_t first) {
+__device__ __forceinline__ void copy_rows(const AttentionArgs& a, const From& f, const Places<kPlaces>& places, uint32_t lds, char* to, int32_t first) {
     constexpr int kRows = 64 / H::kChunks;
     const int lane = threadIdx.x & 63;
-    if (runs && places.whole()) {
-#pragma unroll
-        for (int j = 0; j < kCount; ++j) {
-            const int32_t i = first + j, row = i * kRows + lane / H::kChunks;
-            const int32_t page = __builtin_amdgcn_readlane(places.at.page, i * kRows), at = __builtin_amdgcn_readlane(places.at.row, i * kRows);
-            copy_to_lds(f.of_lane + (((lane % H::kChunks) ^ H::turned(row)) << 4), f.base + page * f.page + at * f.row, lds + i * 1024);
-        }
-        return;
-    }
     const int32_t row_bytes = a.D * H::kElement;
 #pragma unroll 1
     for (int j = 0; j < kCount; ++j) {
@@ -421,6 +412,57 @@ __device__ __forceinline__ void copy_rows(const AttentionArgs& a, const From& f,
             if (page >= 0) v = chunk_of<H::kElement == 2>(from, c, row_bytes, false);
             *reinterpret_cast<u32x4*>(to + i * 1024 + lane * 16) = v;
         }
+    }
+}
+
+// Where a tile's places lie whose rows come in runs of kRun, all of them there: known to the wavefront, and asked for through the scalar cache, so that nobody waits for copies
+// that are on their way to have it.  (Tables do not change while a kernel runs.)  A wavefront keeps what it copies itself: kOwn places from own on.
+template <typename H, int kPlaces, int kOwn>
+struct Runs {
+    static constexpr int kRun = 64 / H::kChunks < 4 ? 4 : 64 / H::kChunks, kCount = kOwn / kRun;
+    int32_t page[kCount], row[kCount];
+    bool good;
+    __device__ __forceinline__ void look_up(const AttentionArgs& a, int32_t b, int32_t p0, int32_t own, int32_t end, bool runs) {
+        good = runs && p0 + kPlaces <= end;
+        if (!good) return;
+        if (a.tables == nullptr) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) page[i] = b, row[i] = p0 + own + i * kRun;
+            return;
+        }
+        const auto* table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.tables + b * a.table_row);
+        if constexpr (kOwn < kPlaces) good = all_there(a, table, p0, kPlaces);
+        int32_t at = uniform((int32_t)((uint32_t)(p0 + own) / (uint32_t)a.page_rows)), r = p0 + own - at * a.page_rows;
+        uint32_t outside = 0;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            page[i] = table[at];
+            row[i] = r;
+            r += kRun;
+            if (r >= a.page_rows) r = 0, ++at;
+        }
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) outside |= (uint32_t)page[i] >= (uint32_t)a.pages;
+        good = good && outside == 0;
+    }
+    static __device__ __forceinline__ bool all_there(const AttentionArgs& a, const __attribute__((address_space(4))) int32_t* table, int32_t p0, int32_t places) {
+        const int32_t first = uniform((int32_t)((uint32_t)p0 / (uint32_t)a.page_rows)), last = uniform((int32_t)((uint32_t)(p0 + places - 1) / (uint32_t)a.page_rows));
+        uint32_t outside = 0;
+        for (int32_t i = first; i <= last; ++i) outside |= (uint32_t)table[i] >= (uint32_t)a.pages;
+        return outside == 0;
+    }
+};
+
+// The copies of a wavefront's own places: kCount of them from the first-th of the tile on.
+template <typename H, int kCount, typename R>
+__device__ __forceinline__ void copy_runs(const From& f, const R& runs, uint32_t lds, int32_t first) {
+    constexpr int kRows = 64 / H::kChunks;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) {
+        const int32_t row = (first + j) * kRows + lane / H::kChunks;
+        copy_to_lds(f.of_lane + (((lane % H::kChunks) ^ H::turned(row)) << 4), f.base + runs.page[j * kRows / R::kRun] * f.page + (runs.row[j * kRows / R::kRun] + j * kRows % R::kRun) * f.row,
+                    lds + (first + j) * 1024);
     }
 }
 
@@ -548,7 +590,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + 4 * W::kBytes);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const Job job = job_of(a, W::kRows, W::kPlaces);
-    if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors(nodes, a.parents + (int64_t)job.b * a.T, a.T);
+    if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<256>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const Row row = row_of(a, job, job.row_tile * W::kRows + wave * 32 + (lane & 31));
     u32x4 q[H::kSteps];
     load_row<kHalf, kSize>(a, job, row, q);
@@ -564,29 +606,39 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
 #pragma unroll
         for (int n = 0; n < H::kBlocks; ++n) acc[n] = f32x16{};
         if (job.begin_tile >= job.end_tile) return;
-        Places<W::kPlaces> next;
+        Runs<H, W::kPlaces, W::kPlaces / W::kWaves> next;
+        uint64_t there = 0, there_next = 0;
         auto copy = [&](int32_t tile) __attribute__((always_inline)) {
             const int32_t at = (tile & 1) * 2 * W::kBytes;
-            copy_rows<H, W::kPlaces, W::kCopies>(a, k, next, runs, lds + at, attention_lds + at, wave * W::kCopies);
-            copy_rows<H, W::kPlaces, W::kCopies>(a, v, next, runs, lds + at + W::kBytes, attention_lds + at + W::kBytes, wave * W::kCopies);
+            if (next.good) {
+                copy_runs<H, W::kCopies>(k, next, lds + at, wave * W::kCopies);
+                copy_runs<H, W::kCopies>(v, next, lds + at + W::kBytes, wave * W::kCopies);
+                there_next = ~0ull;
+            } else {
+                const Places<W::kPlaces> places(a, job.b, tile * W::kPlaces, job.end);
+                copy_rows<H, W::kPlaces, W::kCopies>(a, k, places, lds + at, attention_lds + at, wave * W::kCopies);
+                copy_rows<H, W::kPlaces, W::kCopies>(a, v, places, lds + at + W::kBytes, attention_lds + at + W::kBytes, wave * W::kCopies);
+                there_next = W::kPlaces == 64 ? places.there : places.there | ~0ull << 32;
+            }
         };
-        next.look_up(a, job.b, job.begin_tile * W::kPlaces, job.end);
-        next.settle();
+        auto look_up = [&](int32_t tile) __attribute__((always_inline)) { next.look_up(a, job.b, tile * W::kPlaces, wave * (W::kPlaces / W::kWaves), job.end, runs); };
+        look_up(job.begin_tile);
         copy(job.begin_tile);
+        look_up(job.begin_tile + 1);
         for (int32_t tile = job.begin_tile; tile < job.end_tile; ++tile) {
-            const uint64_t there = next.there;
-            const bool whole = next.whole();
-            next.look_up(a, job.b, (tile + 1) * W::kPlaces, job.end);
+            there = there_next;
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            next.settle();
-            if (tile + 1 < job.end_tile) copy(tile + 1);
+            if (tile + 1 < job.end_tile) {
+                copy(tile + 1);
+                look_up(tile + 2);
+            }
             const char* keys = attention_lds + (tile & 1) * 2 * W::kBytes;
             const int32_t p0 = tile * W::kPlaces;
             f32x16 score[W::kBlocksOf];
             find_scores<kHalf, kSize>(keys, q, score);
-            if (p0 + W::kPlaces > row.plain || !whole) {
+            if (p0 + W::kPlaces > row.plain || there != ~0ull) {
 #pragma unroll
                 for (int n = 0; n < W::kBlocksOf; ++n) score[n] = hide(score[n], (seen_of(row.sight, nodes, p0 + 32 * n) & (uint32_t)(there >> (32 * n))) >> (4 * half));
             }
@@ -598,6 +650,143 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     };
     add_up(acc, pass, [](bool mine) { return __syncthreads_or(mine) != 0; });
     finish_row<kHalf, kSize>(a, acc, m, l, job.b, job.group, row.r, (int64_t)blockIdx.x * W::kRows + wave * 32 + (lane & 31), job.begin_tile < job.end_tile);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------
+//
+// A work-group has 32 rows, and its wavefronts share out the places of its part, 32 at a time, each with copies, maxima and sums of its own; those are joined at the end, in one order.  Bound by the
+// bytes of k and v: a wavefront has a block of one of them on its way while it works on the other's, without waiting for the rest.
+template <bool kHalf, int kSize>
+struct Few {
+    static constexpr int kBytes = 32 * Head<kHalf, kSize>::kRow;  // of a block of k or v
+    static constexpr int kWaves = kBytes <= 16 * 1024 ? 4 : 2;
+    static constexpr int kPlaces = 32 * kWaves;                    // of a round
+    static constexpr int kCopies = kBytes / 1024;
+    static constexpr int kJoin = kWaves * 32 * (kSize + 4) * 4;    // the wavefronts' sums, rows not in the same banks
+    static constexpr int kRing = kWaves * 2 * kBytes;
+    static constexpr int kWork = kRing > kJoin ? kRing : kJoin;
+    static constexpr int kLds = kWork + kWaves * 64 * 4 + (int)sizeof(Nodes);
+};
+
+template <bool kHalf, int kSize>
+__global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1)) void attention_places_kernel(AttentionArgs a) {
+    using H = Head<kHalf, kSize>;
+    using W = Few<kHalf, kSize>;
+    constexpr int kWaves = W::kWaves;
+    extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
+    float* stats = reinterpret_cast<float*>(attention_lds + W::kWork);  // [wave][m of 32 rows, l of 32 rows]
+    Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + W::kWork + kWaves * 64 * 4);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
+    const Job job = job_of(a, 32, W::kPlaces);
+    if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<64 * kWaves>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
+    const Row row = row_of(a, job, job.row_tile * 32 + (lane & 31));
+    u32x4 q[H::kSteps];
+    load_row<kHalf, kSize>(a, job, row, q);
+    const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row), v = from_of<H>(a.v + job.group * a.v_head, a.v_page, a.v_row);
+    const bool runs = in_runs<H>(a);
+    char *keys = attention_lds + wave * 2 * W::kBytes, *values = keys + W::kBytes;
+    const uint32_t keys_at = lds_address(keys), values_at = keys_at + W::kBytes;
+    // this wavefront's blocks of 32 places: every kWaves-th, as far as there are places
+    const int32_t first = job.begin_tile * kWaves + wave, last = min(job.end_tile * kWaves, (job.end + 31) / 32);
+    f32x16 acc[H::kBlocks];
+    float m, l;
+
+    auto pass = [&](int32_t special) __attribute__((always_inline)) {
+        m = kNoMaximum;
+        l = 0.f;
+#pragma unroll
+        for (int n = 0; n < H::kBlocks; ++n) acc[n] = f32x16{};
+        if (first >= last) return;
+        Runs<H, 32, 32> next;
+        uint64_t there = 0;
+        auto copy = [&](const From& f, int32_t block, uint32_t lds, char* to) __attribute__((always_inline)) {
+            if (next.good) {
+                copy_runs<H, W::kCopies>(f, next, lds, 0);
+                there = ~0ull;
+            } else {
+                const Places<32> places(a, job.b, block * 32, job.end);
+                copy_rows<H, 32, W::kCopies>(a, f, places, lds, to, 0);
+                there = places.there;
+            }
+        };
+        next.look_up(a, job.b, first * 32, 0, job.end, runs);
+        copy(k, first, keys_at, keys);
+        copy(v, first, values_at, values);
+#pragma unroll 1
+        for (int32_t block = first; block < last; block += kWaves) {
+            const bool more = block + kWaves < last;
+            const uint32_t seen_there = (uint32_t)there;
+            next.look_up(a, job.b, (block + kWaves) * 32, 0, job.end, runs && more);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies) : "memory");  // (v's copies came behind)
+            f32x16 score[1];
+            find_scores<kHalf, kSize>(keys, q, score);
+            const int32_t p0 = block * 32;
+            if (p0 + 32 > row.plain || seen_there != ~0u) score[0] = hide(score[0], (seen_of(row.sight, nodes, p0) & seen_there) >> (4 * half));
+            if (more) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                copy(k, block + kWaves, keys_at, keys);
+            }
+            find_weights<kHalf>(a.scale2, score, acc, m, l);
+            if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            if (special == kAll) add_values<kHalf, kSize, false>(values, score, special, acc);
+            else add_values<kHalf, kSize, true>(values, score, special, acc);
+            if (more) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                copy(v, block + kWaves, values_at, values);
+            }
+        }
+    };
+    add_up(acc, pass, [](bool mine) { return __builtin_amdgcn_ballot_w64(mine) != 0; });
+
+    // The wavefronts' sums, relative to the largest of their maxima; of those with an infinite one, what weighs nothing adds nothing.
+    l += with_other_half(l);
+    if (half == 0) {
+        stats[wave * 64 + lane] = m;
+        stats[wave * 64 + 32 + lane] = l;
+    }
+    __syncthreads();
+    float most = kNoMaximum, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, stats[w * 64 + (lane & 31)]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += stats[w * 64 + 32 + (lane & 31)] * __builtin_amdgcn_exp2f(stats[w * 64 + (lane & 31)] - most);
+    const float f = __builtin_amdgcn_exp2f(m - most);
+    constexpr int kPitch = kSize + 4;
+    float* sums = reinterpret_cast<float*>(attention_lds);
+#pragma unroll
+    for (int n = 0; n < H::kBlocks; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float part = f == 0.f || l == 0.f ? 0.f : acc[n][i] * f;
+            sums[(wave * 32 + (lane & 31)) * kPitch + H::element(n, i, half)] = part;
+        }
+    __syncthreads();
+    const int64_t part_row = (int64_t)blockIdx.x * 32;
+    if (a.parts > 1 && threadIdx.x < 32) *reinterpret_cast<f32x2*>(a.part_stats + 2 * (part_row + lane)) = f32x2{most, total};
+    if (a.parts > 1 && job.begin_tile >= job.end_tile) return;
+    if (a.parts == 1 && threadIdx.x < 32) {
+        if (a.sums != nullptr && row.r < job.rows) a.sums[((int64_t)job.b * a.groups + job.group) * job.rows + row.r] = sum_of<kHalf>(most, total);
+        stats[lane] = total == 0.f ? 0.f : 1.f / total;  // (of wave 0, which has read its own)
+    }
+    if (a.parts == 1) __syncthreads();
+    const int32_t rows = min(32, job.rows - job.row_tile * 32);
+#pragma unroll 2
+    for (int i = threadIdx.x; i < rows * (kSize / 4); i += 64 * kWaves) {
+        const int r = i / (kSize / 4), e = i % (kSize / 4) * 4;
+        f32x4 sum = *reinterpret_cast<const f32x4*>(sums + r * kPitch + e);
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += *reinterpret_cast<const f32x4*>(sums + (w * 32 + r) * kPitch + e);
+        if (a.parts > 1) {
+            *reinterpret_cast<f32x4*>(a.part_sums + (part_row + r) * kSize + e) = sum;
+            continue;
+        }
+        sum *= stats[r];
+        const int32_t all = job.row_tile * 32 + r, t = all / a.fan, head = job.group * a.fan + (all - t * a.fan);
+        char* y = a.y + job.b * a.y_batch + t * a.y_token + head * a.y_head;
+        if constexpr (kHalf) store<4>(a, y, e, half4{(_Float16)sum[0], (_Float16)sum[1], (_Float16)sum[2], (_Float16)sum[3]});
+        else store<4>(a, y, e, sum);
+    }
 }
 
 // A row's parts, by a wavefront: y = sum_i l_i 2^(m_i - m) (sums_i / l_i) over its sum of l_i 2^(m_i - m), in the order of the parts.
@@ -650,7 +839,7 @@ __global__ __launch_bounds__(256) void attention_mass_kernel(AttentionArgs a) {
     const int32_t b = of / a.groups, group = of % a.groups, rows = a.T * a.fan, length = length_of(a, b), count = count_of(a, b);
     const int32_t end = (int32_t)min((int64_t)length + count, (int64_t)a.places), block_end = min((block + 1) * 4 * kPlaces, end);
     if (block * 4 * kPlaces >= end) return;
-    if (a.kind == kTree && block_end > length) find_ancestors(&nodes, a.parents + (int64_t)b * a.T, a.T);
+    if (a.kind == kTree && block_end > length) find_ancestors<256>(&nodes, a.parents + (int64_t)b * a.T, a.T);
     const int32_t p0 = (block * 4 + wave) * kPlaces;
     if (p0 >= end) return;
     const int32_t row_bytes = a.D * H::kElement, mine = p0 + (lane & 31);
@@ -694,11 +883,14 @@ __global__ __launch_bounds__(256) void attention_mass_kernel(AttentionArgs a) {
 template <bool kHalf, int kSize>
 int attend_of(const AttentionArgs& a, hipStream_t s) {
     using W = Tile<kHalf, kSize>;
-    auto kernel = attention_rows_kernel<kHalf, kSize>;
-    if constexpr (W::kLds > 65536)  // (has to be asked for, on every device)
-        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, W::kLds));
-    kernel<<<(unsigned)((int64_t)a.B * a.groups * a.row_tiles * a.parts), 256, W::kLds, s>>>(a);
-    return launch_check("attention_rows_kernel");
+    using F = Few<kHalf, kSize>;
+    const bool few = a.tile_rows == 32;
+    auto kernel = few ? attention_places_kernel<kHalf, kSize> : attention_rows_kernel<kHalf, kSize>;
+    const int lds = few ? F::kLds : W::kLds;
+    if (lds > 65536)  // (has to be asked for, on every device)
+        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    kernel<<<(unsigned)((int64_t)a.B * a.groups * a.row_tiles * a.parts), few ? 64 * F::kWaves : 256, lds, s>>>(a);
+    return launch_check(few ? "attention_places_kernel" : "attention_rows_kernel");
 }
 template <bool kHalf, int kSize>
 int join_of(const AttentionArgs& a, hipStream_t s) {
