@@ -241,15 +241,22 @@ __device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCoun
         }
 }
 
-// What is added up in place of v: itself, or (where results are made again) ones for what is inf, -inf and NaN, or what is finite.
+// What is added up in place of v, all of it in LDS: itself, or (where results are made again) ones for what is inf, -inf and NaN, or what is finite.
 enum { kAll, kInfinities, kNegativeInfinities, kNans, kFinite };
-__device__ __forceinline__ float replaced(float v, int32_t special) {
-    return special == kFinite ? (v - v == 0.f ? v : 0.f) : special == kNans ? (v != v ? 1.f : 0.f) : v == (special == kInfinities ? INFINITY : -INFINITY) ? 1.f : 0.f;
+template <bool kHalf>
+__device__ __forceinline__ void replace_values(char* values, int32_t bytes, int32_t special, int32_t thread, int32_t threads) {
+    using E = std::conditional_t<kHalf, _Float16, float>;
+#pragma unroll 1
+    for (int32_t i = thread; i < bytes / (int32_t)sizeof(E); i += threads) {
+        const float v = (float)reinterpret_cast<const E*>(values)[i];
+        const bool finite = v - v == 0.f, marked = special == kNans ? v != v : v == (special == kInfinities ? INFINITY : -INFINITY);
+        reinterpret_cast<E*>(values)[i] = (E)(special == kFinite ? (finite ? v : 0.f) : marked ? 1.f : 0.f);
+    }
 }
 
 // acc += v^T weights^T, v's rows in LDS from `values` on.
-template <bool kHalf, int kSize, bool kSpecial, int kCount>
-__device__ __forceinline__ void add_values(const char* values, const f32x16 (&weight)[kCount], int32_t special, f32x16 (&acc)[kSize / 32]) {
+template <bool kHalf, int kSize, int kCount>
+__device__ __forceinline__ void add_values(const char* values, const f32x16 (&weight)[kCount], f32x16 (&acc)[kSize / 32]) {
     using H = Head<kHalf, kSize>;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     if constexpr (kHalf) {
@@ -275,10 +282,6 @@ __device__ __forceinline__ void add_values(const char* values, const f32x16 (&we
                 } vf;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) vf.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_pointer<short4v>((at[e] ^ (n << 6)) + kb * 16 * H::kRow));
-                if constexpr (kSpecial) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) vf.whole[j] = (_Float16)replaced((float)vf.whole[j], special);
-                }
                 acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, w, acc[n], 0, 0, 0);
             }
         }
@@ -299,8 +302,7 @@ __device__ __forceinline__ void add_values(const char* values, const f32x16 (&we
                 for (int w = 0; w < H::kBlocks / kWide; ++w) {
                     const Wide vf = *lds_pointer<Wide>((at ^ turned) + row * H::kRow + 128 * kWide * w);
 #pragma unroll
-                    for (int j = 0; j < kWide; ++j)
-                        acc[w * kWide + j] = __builtin_amdgcn_mfma_f32_32x32x2f32(kSpecial ? replaced(vf[j], special) : vf[j], weight[n][i], acc[w * kWide + j], 0, 0, 0);
+                    for (int j = 0; j < kWide; ++j) acc[w * kWide + j] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[j], weight[n][i], acc[w * kWide + j], 0, 0, 0);
                 }
             }
     }
@@ -557,13 +559,24 @@ __device__ __forceinline__ Row row_of(const AttentionArgs& a, const Job& j, int3
     row.plain = __builtin_amdgcn_readfirstlane(plain);
     return row;
 }
+// The rows of a wavefront; those that are not whole pieces go through `space` in LDS, of 32 rows.
 template <bool kHalf, int kSize>
-__device__ __forceinline__ void load_row(const AttentionArgs& a, const Job& j, const Row& row, u32x4 (&q)[Head<kHalf, kSize>::kSteps]) {
+__device__ __forceinline__ void load_rows(const AttentionArgs& a, const Job& j, const Row& row, char* space, u32x4 (&q)[Head<kHalf, kSize>::kSteps]) {
     using H = Head<kHalf, kSize>;
-    const int half = (threadIdx.x & 63) >> 5;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int32_t row_bytes = a.D * H::kElement;
     const char* at = a.q + j.b * a.q_batch + row.t * a.q_token + row.head * a.q_head;
+    if (a.q_whole) {
 #pragma unroll
-    for (int s = 0; s < H::kSteps; ++s) q[s] = row.r < j.rows ? chunk_of<kHalf>(at, (2 * s + half) * 16, a.D * H::kElement, a.q_whole) : u32x4{0, 0, 0, 0};
+        for (int s = 0; s < H::kSteps; ++s) q[s] = row.r < j.rows ? chunk_of<kHalf>(at, (2 * s + half) * 16, row_bytes, true) : u32x4{0, 0, 0, 0};
+        return;
+    }
+    u32x4* mine = reinterpret_cast<u32x4*>(space) + (lane & 31) * H::kChunks;
+#pragma unroll 1
+    for (int c = half; c < H::kChunks; c += 2) mine[c] = row.r < j.rows ? chunk_of<kHalf>(at, c * 16, row_bytes, false) : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < H::kSteps; ++s) q[s] = mine[2 * s + half];  // (what this lane has written itself)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // ---- many rows --------------------------------------------------------------------------------------------------------
@@ -593,7 +606,8 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<256>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const Row row = row_of(a, job, job.row_tile * W::kRows + wave * 32 + (lane & 31));
     u32x4 q[H::kSteps];
-    load_row<kHalf, kSize>(a, job, row, q);
+    load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 32 * H::kRow, q);
+    if (!a.q_whole) __syncthreads();  // (the tiles come where they lay)
     const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row), v = from_of<H>(a.v + job.group * a.v_head, a.v_page, a.v_row);
     const bool runs = in_runs<H>(a);
     const uint32_t lds = lds_address(attention_lds);
@@ -634,7 +648,11 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
                 copy(tile + 1);
                 look_up(tile + 2);
             }
-            const char* keys = attention_lds + (tile & 1) * 2 * W::kBytes;
+            char* keys = attention_lds + (tile & 1) * 2 * W::kBytes;
+            if (special != kAll) {
+                replace_values<kHalf>(keys + W::kBytes, W::kBytes, special, threadIdx.x, 256);
+                __syncthreads();
+            }
             const int32_t p0 = tile * W::kPlaces;
             f32x16 score[W::kBlocksOf];
             find_scores<kHalf, kSize>(keys, q, score);
@@ -643,8 +661,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
                 for (int n = 0; n < W::kBlocksOf; ++n) score[n] = hide(score[n], (seen_of(row.sight, nodes, p0 + 32 * n) & (uint32_t)(there >> (32 * n))) >> (4 * half));
             }
             find_weights<kHalf>(a.scale2, score, acc, m, l);
-            if (special == kAll) add_values<kHalf, kSize, false>(keys + W::kBytes, score, special, acc);
-            else add_values<kHalf, kSize, true>(keys + W::kBytes, score, special, acc);
+            add_values<kHalf, kSize>(keys + W::kBytes, score, acc);
         }
         __syncthreads();
     };
@@ -681,7 +698,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<64 * kWaves>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const Row row = row_of(a, job, job.row_tile * 32 + (lane & 31));
     u32x4 q[H::kSteps];
-    load_row<kHalf, kSize>(a, job, row, q);
+    load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 2 * W::kBytes, q);
     const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row), v = from_of<H>(a.v + job.group * a.v_head, a.v_page, a.v_row);
     const bool runs = in_runs<H>(a);
     char *keys = attention_lds + wave * 2 * W::kBytes, *values = keys + W::kBytes;
@@ -729,8 +746,8 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
             find_weights<kHalf>(a.scale2, score, acc, m, l);
             if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            if (special == kAll) add_values<kHalf, kSize, false>(values, score, special, acc);
-            else add_values<kHalf, kSize, true>(values, score, special, acc);
+            if (special != kAll) replace_values<kHalf>(values, W::kBytes, special, lane, 64);
+            add_values<kHalf, kSize>(values, score, acc);
             if (more) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 copy(v, block + kWaves, values_at, values);
@@ -828,56 +845,144 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     }
 }
 
-// The weights that each place is given, over a group's rows: a wavefront takes 32 places and all rows, of which the first pass has left m + log2(l).
+// The weights that each place is given, over a group's rows, of which the first pass has left m + log2(l).  The scores are made again, here as q k^T: a lane has one place, and
+// its weights add up without another lane's.  Rows lie in LDS, 128 at a time; a wavefront goes over blocks of 32 places with copies of its own.  Bound by the bytes of k.
 template <bool kHalf, int kSize>
-__global__ __launch_bounds__(256) void attention_mass_kernel(AttentionArgs a) {
+struct Mass {
+    static constexpr int kBytes = 32 * Head<kHalf, kSize>::kRow;  // of a block of k
+    static constexpr int kRows = kBytes <= 16 * 1024 ? 128 : 64;
+    static constexpr int kWaves = kBytes <= 16 * 1024 ? 4 : 2, kThreads = 64 * kWaves;
+    static constexpr int kBuffers = kBytes <= 8 * 1024 ? 2 : 1;
+    static constexpr int kCopies = kBytes / 1024;
+    static constexpr int kOfRows = kRows * Head<kHalf, kSize>::kRow;
+    static constexpr int kLds = kOfRows + kWaves * kBuffers * kBytes + kRows * 12 + (int)sizeof(Nodes);
+};
+
+template <bool kHalf, int kSize>
+__global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass_kernel(AttentionArgs a, int32_t runs_of_places) {
     using H = Head<kHalf, kSize>;
-    constexpr int kSteps = H::kSteps, kPlaces = 32;
-    __shared__ Nodes nodes;
+    using W = Mass<kHalf, kSize>;
+    extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
+    float* less = reinterpret_cast<float*>(attention_lds + W::kOfRows + W::kWaves * W::kBuffers * W::kBytes);  // of the rows: m + log2(l)
+    int32_t* limits = reinterpret_cast<int32_t*>(less + W::kRows);                                               // what they see, as in Sight
+    int32_t* sees = limits + W::kRows;
+    Nodes* nodes = reinterpret_cast<Nodes*>(sees + W::kRows);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int32_t blocks = (a.places + 4 * kPlaces - 1) / (4 * kPlaces), block = blockIdx.x % blocks, of = blockIdx.x / blocks;
-    const int32_t b = of / a.groups, group = of % a.groups, rows = a.T * a.fan, length = length_of(a, b), count = count_of(a, b);
-    const int32_t end = (int32_t)min((int64_t)length + count, (int64_t)a.places), block_end = min((block + 1) * 4 * kPlaces, end);
-    if (block * 4 * kPlaces >= end) return;
-    if (a.kind == kTree && block_end > length) find_ancestors<256>(&nodes, a.parents + (int64_t)b * a.T, a.T);
-    const int32_t p0 = (block * 4 + wave) * kPlaces;
-    if (p0 >= end) return;
-    const int32_t row_bytes = a.D * H::kElement, mine = p0 + (lane & 31);
-    Place at = {-1, 0};
-    if (mine < end) at = place_in(a, b, mine);
-    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(at.page >= 0);
-    u32x4 k[kSteps];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-        k[s] = at.page >= 0 ? chunk_of<kHalf>(a.k + at.page * a.k_page + at.row * a.k_row + group * a.k_head, (2 * s + half) * 16, row_bytes, a.k_whole) : u32x4{0, 0, 0, 0};
-    f32x16 total = {};
-    // (the rows of a chain that come before the first of these places do not see them)
-    const int32_t first_t = a.kind == kChain ? max(0, p0 - length) : 0;
-    for (int32_t r0 = first_t * a.fan / 32 * 32; r0 < count * a.fan; r0 += 32) {
-        const int32_t r = r0 + (lane & 31), t = r < rows ? r / a.fan : a.T, head = group * a.fan + (r - t * a.fan);
-        const Sight sight = sight_of(a, t, length, count);
-        const char* from = a.q + b * a.q_batch + t * a.q_token + head * a.q_head;
-        const float less = r < rows ? a.sums[(int64_t)of * rows + r] : INFINITY;
-        f32x16 score = {};
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const u32x4 q = r < rows ? chunk_of<kHalf>(from, (2 * s + half) * 16, row_bytes, a.q_whole) : u32x4{0, 0, 0, 0};
-            score = score_of<kHalf>(k[s], q, score);
+    Job job;
+    const int32_t of = uniform(blockIdx.x / runs_of_places), run = blockIdx.x - of * runs_of_places;
+    job.b = uniform(of / a.groups);
+    job.group = of - job.b * a.groups;
+    job.rows = a.T * a.fan;
+    job.length = length_of(a, job.b);
+    job.count = count_of(a, job.b);
+    job.end = min(job.length + job.count, a.places);
+    // a run of blocks of 32 places, of which the wavefronts have every kWaves-th
+    const int32_t blocks = (job.end + 31) / 32, each = uniform(((blocks + runs_of_places - 1) / runs_of_places + W::kWaves - 1) / W::kWaves * W::kWaves), last = min((run + 1) * each, blocks);
+    if (run * each >= last) return;
+    if (a.kind == kTree && last * 32 > job.length) find_ancestors<W::kThreads>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
+    const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row);
+    const bool runs = in_runs<H>(a);
+    char* keys = attention_lds + W::kOfRows + wave * W::kBuffers * W::kBytes;
+    const uint32_t keys_at = lds_address(keys);
+    const int32_t row_bytes = a.D * H::kElement, used = job.count * a.fan;
+    for (int32_t r0 = 0; r0 < used; r0 += W::kRows) {
+        __syncthreads();
+        for (int32_t i = threadIdx.x; i < W::kRows * H::kChunks; i += W::kThreads) {
+            const int32_t r = r0 + i / H::kChunks, c = i % H::kChunks, t = r / a.fan, head = job.group * a.fan + (r - t * a.fan);
+            u32x4 v = {0, 0, 0, 0};
+            if (r < used) v = chunk_of<kHalf>(a.q + job.b * a.q_batch + t * a.q_token + head * a.q_head, c * 16, row_bytes, a.q_whole);
+            reinterpret_cast<u32x4*>(attention_lds)[i / H::kChunks * H::kChunks + (c ^ H::turned(i / H::kChunks))] = v;
         }
-        score = hide(score, (seen_of(sight, &nodes, p0) & there) >> (4 * half));
+        static_assert(W::kRows <= W::kThreads, "a lane to a row");
+        if (threadIdx.x < W::kRows) {
+            const int32_t r = r0 + threadIdx.x, t = r / a.fan;
+            const Sight sight = sight_of(a, t, job.length, job.count);
+            less[threadIdx.x] = r < used ? a.sums[(int64_t)of * job.rows + r] : INFINITY;
+            limits[threadIdx.x] = sight.limit;
+            sees[threadIdx.x] = sight.node;
+        }
+        __syncthreads();
+        const int32_t row_blocks = (min(used - r0, W::kRows) + 31) / 32;
+        // (the rows of a chain do not see places behind the last of them)
+        const int32_t seen_end = a.kind == kChain ? min(job.end, job.length + (min(r0 + W::kRows, used) - 1) / a.fan + 1) : job.end;
+        Runs<H, 32, 32> next;
+        uint64_t there = 0, there_next = 0;
+        auto copy = [&](int32_t block, int buffer) __attribute__((always_inline)) {
+            if (next.good) {
+                copy_runs<H, W::kCopies>(k, next, keys_at + buffer * W::kBytes, 0);
+                there_next = ~0ull;
+            } else {
+                const Places<32> places(a, job.b, block * 32, job.end);
+                copy_rows<H, 32, W::kCopies>(a, k, places, keys_at + buffer * W::kBytes, keys + buffer * W::kBytes, 0);
+                there_next = places.there;
+            }
+        };
+        const int32_t first = run * each + wave;
+        if (first >= last) continue;
+        int buffer = 0;
+        next.look_up(a, job.b, first * 32, 0, job.end, runs);
+        copy(first, 0);
+#pragma unroll 1
+        for (int32_t block = first; block < last; block += W::kWaves) {
+            const bool more = block + W::kWaves < last;
+            const int32_t p0 = block * 32, p = p0 + (lane & 31);
+            there = there_next;
+            next.look_up(a, job.b, (block + W::kWaves) * 32, 0, job.end, runs && more);
+            float* to = a.mass + job.b * a.mass_batch + job.group * a.mass_head + p;
+            const bool mine = ((there >> lane) & 1) && half == 0;
+            const float before = mine && (p < job.length || r0 > 0) ? *to : 0.f;
+            if (W::kBuffers == 2 && more) {
+                copy(block + W::kWaves, buffer ^ 1);
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            }
+            u32x4 kf[H::kSteps];
+            {
+                uint32_t at = keys_at + buffer * W::kBytes + (lane & 31) * H::kRow + ((half ^ H::turned(lane & 31)) << 4);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) total[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(score[i], a.scale2, -less));
-    }
+                for (int s = 0; s < H::kSteps; ++s) kf[s] = *lds_pointer<u32x4>(at ^ (s << 5));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (W::kBuffers == 1 && more) copy(block + W::kWaves, 0);
+            float total = 0.f;
+            const bool plain = p0 + 32 <= job.length;
+#pragma unroll 1
+            for (int rb = 0; rb < (p0 < seen_end ? row_blocks : 0); ++rb) {
+                f32x16 score = {};
+                uint32_t at = lds_address(attention_lds) + (rb * 32 + (lane & 31)) * H::kRow + ((half ^ H::turned(lane & 31)) << 4);
+                asm volatile("" : "+v"(at));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+                for (int s = 0; s < H::kSteps; ++s) score = score_of<kHalf>(*lds_pointer<u32x4>(at ^ (s << 5)), kf[s], score);
+                const int row = rb * 32 + 4 * half;
+                // (a weight that is not seen is none, also of a row that has no number for its sum)
+                uint32_t seen = ~0u;
+                if (!plain || r0 + rb * 32 + 32 > used) {
+                    seen = 0;
 #pragma unroll
-        for (int d = 16; d; d /= 2) total[i] += __shfl_xor(total[i], d);
-        const int32_t p = p0 + 8 * (i >> 2) + 4 * half + (i & 3);
-        if ((lane & 31) == i && ((there >> (p - p0)) & 1)) {
-            float* to = a.mass + b * a.mass_batch + group * a.mass_head + p;
-            *to = (p < length ? *to : 0.f) + total[i];
+                    for (int i = 0; i < 16; ++i) {
+                        const int at_row = row + 8 * (i >> 2) + (i & 3), node = sees[at_row], other = p - job.length;
+                        const uint32_t word = nodes->sees[max(node, 0)][min(max(other, 0) >> 5, kMostNodes / 32 - 1)];
+                        const bool of_tree = (node >= 0) & (other >= 0) & (other < job.count) & ((word >> (other & 31)) & 1);
+                        seen |= (uint32_t)((p < limits[at_row]) | of_tree) << i;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const f32x4 l = *reinterpret_cast<const f32x4*>(less + row + 2 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i + j], a.scale2, -l[j]));
+                        total += (seen >> (i + j)) & 1 ? w : 0.f;
+                    }
+                }
+            }
+            total += with_other_half(total);
+            if (mine) *to = before + total;
+            buffer ^= W::kBuffers - 1;
         }
     }
+    // (places of a sequence without tokens stay as they are)
 }
 
 template <bool kHalf, int kSize>
@@ -899,7 +1004,15 @@ int join_of(const AttentionArgs& a, hipStream_t s) {
 }
 template <bool kHalf, int kSize>
 int mass_of(const AttentionArgs& a, hipStream_t s) {
-    attention_mass_kernel<kHalf, kSize><<<(unsigned)((int64_t)a.B * a.groups * ((a.places + 127) / 128)), 256, 0, s>>>(a);
+    using W = Mass<kHalf, kSize>;
+    // Runs of places: as many as give each compute unit two work-groups, of at least 128 places (a block to each wavefront).
+    const int64_t groups = (int64_t)a.B * a.groups, most = ((int64_t)a.places + 127) / 128;
+    int64_t runs = (512 + groups - 1) / groups;
+    runs = runs > most ? most : runs;
+    auto kernel = attention_mass_kernel<kHalf, kSize>;
+    if constexpr (W::kLds > 65536)  // (has to be asked for, on every device)
+        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, W::kLds));
+    kernel<<<(unsigned)(groups * runs), W::kThreads, W::kLds, s>>>(a, (int32_t)runs);
     return launch_check("attention_mass_kernel");
 }
 

@@ -205,9 +205,36 @@ __device__ __forceinline__ uint32_t sortable(float v) {
     return v != v ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
+// The weights as numbers to be compared: in LDS where a sequence's fit (kInLds: read once, eight loads of a lane under way), else from memory each time.
+constexpr int32_t kMostInLds = 36 * 1024;
+template <bool kInLds>
+struct Keys {
+    const float* mass;
+    uint32_t* keys;
+    __device__ __forceinline__ void load(int32_t n) {
+        if constexpr (kInLds) {
+            constexpr int kAtOnce = 8;
+            for (int32_t i0 = threadIdx.x; i0 < n; i0 += 1024 * kAtOnce) {
+                float v[kAtOnce];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) v[j] = i0 + j * 1024 < n ? mass[i0 + j * 1024] : 0.f;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j)
+                    if (i0 + j * 1024 < n) keys[i0 + j * 1024] = sortable(v[j]);
+            }
+            __syncthreads();
+        }
+    }
+    __device__ __forceinline__ uint32_t at(int32_t i) const {
+        return kInLds ? keys[i] : sortable(mass[i]);
+    }
+};
+
 // A head's places that stay: the threshold of the `best` largest of n weights by three histograms of 11, 11 and 10 bits, of equal ones the lower places; then the
 // list of moves, places that go in front of best and places that stay behind it, both in ascending order.
+template <bool kInLds>
 __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
+    extern __shared__ uint32_t choose_lds[];
     constexpr int kWaves = 16, kBins = 2048;
     __shared__ int32_t bins[kBins];
     __shared__ int32_t of_waves[kWaves];
@@ -223,7 +250,8 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
         return;
     }
     const int32_t n = length - a.recent, best = a.keep - a.recent;
-    const float* mass = a.mass + b * a.mass_batch + h * a.mass_head;
+    Keys<kInLds> keys = {a.mass + b * a.mass_batch + h * a.mass_head, choose_lds};
+    keys.load(n);
     uint32_t least = 0;      // upper bits of the threshold
     int32_t wanted = best;   // how many with those bits
     if (best > 0) {
@@ -233,7 +261,7 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
             for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
             __syncthreads();
             for (int32_t i = threadIdx.x; i - lane < n; i += 1024) {
-                const uint32_t key = i < n ? sortable(mass[i]) : 0;
+                const uint32_t key = i < n ? keys.at(i) : 0;
                 const bool counts = i < n && ((key ^ least) & above) == 0;
                 const uint32_t bin = (key >> shift) & ((1u << bits) - 1);
                 // (equal weights, as of places that nobody has looked at, would queue for one bin)
@@ -279,14 +307,14 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
         return before;
     };
     int32_t equal = 0;
-    for (int32_t i = from + lane; i - lane < to; i += 64) equal += __popcll(__builtin_amdgcn_ballot_w64(i < to && best > 0 && sortable(mass[i]) == least));
+    for (int32_t i = from + lane; i - lane < to; i += 64) equal += __popcll(__builtin_amdgcn_ballot_w64(i < to && best > 0 && keys.at(i) == least));
     const int32_t equal_before = of_wave(equal);
     int32_t holes = 0, movers = 0, holes_before = 0, movers_before = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int32_t rank = equal_before;
         holes = movers = 0;
         for (int32_t i = from + lane; i - lane < to; i += 64) {
-            const uint32_t key = i < to ? sortable(mass[i]) : 0;
+            const uint32_t key = i < to ? keys.at(i) : 0;
             const uint64_t same = __builtin_amdgcn_ballot_w64(i < to && best > 0 && key == least), below = (1ull << lane) - 1;
             const bool stays = best > 0 && (key > least || (key == least && rank + __popcll(same & below) < wanted));
             rank += __popcll(same);
@@ -499,7 +527,11 @@ extern "C" int chx_hip_cache_evict(
     a.recent = (int32_t)(recent < a.keep ? recent : a.keep);
     a.most = (int32_t)((needed / 4 / ((int64_t)a.c.B * a.c.groups) - 1) / 2);
     a.lists = static_cast<int32_t*>(workspace);
-    cache_choose_kernel<<<(unsigned)(a.c.B * a.c.groups), 1024, 0, as_stream(stream)>>>(a);
+    const bool in_lds = a.c.places <= kMostInLds;
+    auto choose = in_lds ? cache_choose_kernel<true> : cache_choose_kernel<false>;
+    if (in_lds && a.c.places > 12 * 1024)  // (has to be asked for, on every device)
+        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(choose), hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostInLds));
+    choose<<<(unsigned)(a.c.B * a.c.groups), 1024, in_lds ? 4 * a.c.places : 0, as_stream(stream)>>>(a);
     CHX_PROPAGATE(launch_check("cache_choose_kernel"));
     if (a.keep >= a.c.places) return CHX_HIP_OK;
     const unsigned grid = (unsigned)(a.c.B * a.c.groups * (2 * a.slices + 1));

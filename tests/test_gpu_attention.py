@@ -265,8 +265,16 @@ def test_what_is_not_finite_in_places_that_are_not_seen(g, dtype, T, value):
                 pool[page, row, 1] = value
             else:
                 pool[page, row, 0, 5] = value
-            got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths, parents=tree)
-            sees = line_of(None if tree is None else tree[0].tolist(), T)[:, bad]
+            mass = torch.zeros(1, 2, cache.tables.shape[1] * 16, device="cuda")
+            got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths, parents=tree, mass=mass)
+            line = line_of(None if tree is None else tree[0].tolist(), T)
+            sees = line[:, bad]
+            # (places that only rows without the bad one see have weights as ever; where v is bad, all have)
+            fine = torch.ones(90 + T, dtype=torch.bool)
+            if pool is cache.keys:
+                fine[:90] = False
+                fine[90:] = ~(line & sees[:, None]).any(0)
+            assert torch.isfinite(mass[0][:, : 90 + T][:, fine.cuda()]).all() and torch.isfinite(mass[0, 0]).all()
             assert torch.equal(got[0][~sees], clean[0][~sees])
             group = 1 if several else 0
             other = slice(0, 2) if group else slice(2, 4)
