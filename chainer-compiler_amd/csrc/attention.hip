@@ -8,13 +8,34 @@
 namespace chx {
 namespace {
 
-// How rows and places are shared out: the kernel for few rows up to 32, that for many from there on; parts as many as give each compute unit two work-groups, of at least 256 places each.
-void share_out(AttentionArgs* a) {
-    const int64_t rows = (int64_t)a->T * a->fan;
-    a->tile_rows = rows <= 32 ? 32 : 128;
+// How rows and places are shared out.
+//
+// Tiles of 128 rows read k and v once for all of them; those of 32 rows fill more compute units, and leave fewer rows empty.  us of the better number of parts, 32 rows / 128:
+//                                              float16: 64 elements   128          256          float32: 64       128          256
+//   3 x 197 rows of 12 heads, 577 places               13.0 / 19.7    18.9 / 26.3                25.5 / 34.2       42.4 / 54.1
+//   2 x 512 of 16, 512                                 13.3 / 14.3    20.2 / 23.8                30.4 / 40.1       63.6 / 62.5
+//   2 x 512 of 16, 1500                                25.1 / 34.6    38.6 / 40.1  93.0 / 71.5   68.5 / 74.5       154 / 135    502 / 251
+//   4 x 512 of 16, 1500                                41.3 / 36.1    68.8 / 57.9  188 / 115     126 / 123         311 / 238    999 / 453
+//   8 x 512 of 16, 1500                                68.2 / 45.1    139 / 82     373 / 224     251 / 209         616 / 471
+//   4 x 24 x 4 of 8, 8000                              27.4 / 28.0    57.5 / 45.9  112 / 98.5    84.5 / 84.9       171 / 176    504 / 328
+//   16 x 16 x 4 of 8, 4000 (half of 128 rows empty)    46.2 / 42.4    73.6 / 65.6  129 / 166     93.4 / 142        201 / 325    629 / 605
+// So: 128 from as many tiles on as there are compute units (half as many where a tile is much work), a tile of many places counted as several; in float32, whose products take the time, not
+// where half of the rows are empty.
+//
+// Parts: as many as give each compute unit two work-groups (float32, whose products take the time: little more than one), of at least 256 places each (float32: 128).  One token of 8 sequences, 2000 places, 8 heads of 128 elements: 1 part 38 us, 2 27, 4 20, 8 17, 12
+// 23; of one sequence of 32,768: 8 80, 24 40, 32 38, 64 40.
+void share_out(AttentionArgs* a, bool half) {
+    const int64_t rows = (int64_t)a->T * a->fan, sets = (int64_t)a->B * a->groups, tiles = (rows + 127) / 128;
+    const int size = attention_size(a->D);
+    bool few = rows <= 32;
+    if (!few && (half || size < 256)) {
+        const int64_t wide = sets * tiles * (a->places < 1024 ? 1 : a->places / 1024);
+        few = wide < (size == 64 || (half && size == 128) ? 256 : 128) || (!half && 2 * rows <= 128 * tiles);
+    }
+    a->tile_rows = few ? 32 : 128;
     a->row_tiles = (int32_t)((rows + a->tile_rows - 1) / a->tile_rows);
-    const int64_t groups = (int64_t)a->B * a->groups * a->row_tiles, most = (a->places + 255) / 256;
-    int64_t parts = (512 + groups - 1) / (groups < 1 ? 1 : groups);
+    const int64_t groups = sets * a->row_tiles, least = half ? 256 : 128, most = (a->places + least - 1) / least;
+    int64_t parts = (half ? 512 : 320) / (groups < 1 ? 1 : groups);
     parts = parts > most ? most : parts;
     a->parts = (int32_t)(parts < 1 ? 1 : parts > kMostParts ? kMostParts : parts);
 }
@@ -42,8 +63,8 @@ int check_queries(const chx_hip_tensor* q, int32_t dtype, int64_t B, const char*
     a->B = (int32_t)B;
     a->T = (int32_t)q->shape[1];
     a->fan = (int32_t)(q->shape[2] / a->groups);
-    share_out(a);
-    CHX_REQUIRE((int64_t)a->B * a->groups * a->row_tiles * a->parts < (int64_t(1) << 23), "%s: more tiles than one launch has", what);
+    share_out(a, q->dtype == CHX_HIP_FLOAT16);
+    CHX_REQUIRE(((int64_t)a->B * a->groups * a->parts + 7) * a->row_tiles < (int64_t(1) << 23), "%s: more tiles than one launch has", what);
     return CHX_HIP_OK;
 }
 

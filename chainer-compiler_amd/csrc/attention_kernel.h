@@ -521,14 +521,23 @@ struct Job {
     int32_t b, group, part, row_tile;
     int32_t rows, length, count, end;  // end: of the places that any of its rows sees
     int32_t begin_tile, end_tile;      // of its part
+    int64_t at;                        // where its part's sums go, in tiles
+    bool none;
 };
 __device__ __forceinline__ Job job_of(const AttentionArgs& a, int32_t tile_rows, int32_t tile_places) {
     Job j;
-    const int32_t of_tile = uniform(blockIdx.x / a.parts), of_group = uniform(of_tile / a.row_tiles);
-    j.part = blockIdx.x - of_tile * a.parts;
-    j.row_tile = of_tile - of_group * a.row_tiles;
-    j.b = uniform(of_group / a.groups);
-    j.group = of_group - j.b * a.groups;
+    // Work-groups go to the eight XCDs in turn.  Neighbours read neighbouring heads' rows of the same places; the tiles of rows that read the same part of k and v follow each other on one XCD,
+    // whose L2 they share.  (The grid is filled up to whole eights of parts.)
+    const uint32_t turn = blockIdx.x >> 3, of_turn = uniform(turn / a.row_tiles);
+    const int32_t set = of_turn * 8 + (blockIdx.x & 7), of_group = uniform((uint32_t)set / a.groups);
+    // (of a chain, the tiles with the most places first)
+    j.row_tile = a.row_tiles - 1 - (int32_t)(turn - of_turn * a.row_tiles);
+    j.group = set - of_group * a.groups;
+    j.b = uniform((uint32_t)of_group / a.parts);
+    j.part = of_group - j.b * a.parts;
+    j.at = (((int64_t)j.b * a.groups + j.group) * a.row_tiles + j.row_tile) * a.parts + j.part;
+    j.none = j.b >= a.B;
+    if (j.none) j.b = 0;
     j.rows = a.T * a.fan;
     j.length = length_of(a, j.b);
     j.count = count_of(a, j.b);
@@ -603,6 +612,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + 4 * W::kBytes);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const Job job = job_of(a, W::kRows, W::kPlaces);
+    if (job.none) return;
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<256>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const Row row = row_of(a, job, job.row_tile * W::kRows + wave * 32 + (lane & 31));
     u32x4 q[H::kSteps];
@@ -611,6 +621,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row), v = from_of<H>(a.v + job.group * a.v_head, a.v_page, a.v_row);
     const bool runs = in_runs<H>(a);
     const uint32_t lds = lds_address(attention_lds);
+    const bool idle = job.row_tile * W::kRows + wave * 32 >= job.rows;  // (copies, and meets the others)
     f32x16 acc[H::kBlocks];
     float m, l;
 
@@ -648,6 +659,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
                 copy(tile + 1);
                 look_up(tile + 2);
             }
+            if (special == kAll && idle) continue;
             char* keys = attention_lds + (tile & 1) * 2 * W::kBytes;
             if (special != kAll) {
                 replace_values<kHalf>(keys + W::kBytes, W::kBytes, special, threadIdx.x, 256);
@@ -666,7 +678,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
         __syncthreads();
     };
     add_up(acc, pass, [](bool mine) { return __syncthreads_or(mine) != 0; });
-    finish_row<kHalf, kSize>(a, acc, m, l, job.b, job.group, row.r, (int64_t)blockIdx.x * W::kRows + wave * 32 + (lane & 31), job.begin_tile < job.end_tile);
+    finish_row<kHalf, kSize>(a, acc, m, l, job.b, job.group, row.r, job.at * W::kRows + wave * 32 + (lane & 31), job.begin_tile < job.end_tile);
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
@@ -695,6 +707,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + W::kWork + kWaves * 64 * 4);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const Job job = job_of(a, 32, W::kPlaces);
+    if (job.none) return;
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<64 * kWaves>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const Row row = row_of(a, job, job.row_tile * 32 + (lane & 31));
     u32x4 q[H::kSteps];
@@ -779,7 +792,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
             sums[(wave * 32 + (lane & 31)) * kPitch + H::element(n, i, half)] = part;
         }
     __syncthreads();
-    const int64_t part_row = (int64_t)blockIdx.x * 32;
+    const int64_t part_row = job.at * 32;
     if (a.parts > 1 && threadIdx.x < 32) *reinterpret_cast<f32x2*>(a.part_stats + 2 * (part_row + lane)) = f32x2{most, total};
     if (a.parts > 1 && job.begin_tile >= job.end_tile) return;
     if (a.parts == 1 && threadIdx.x < 32) {
@@ -827,12 +840,21 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 #pragma unroll
     for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
     float sum[kOf] = {};
-    for (int p = 0; p < a.parts; ++p) {
-        const float w = __shfl(weight, p);
-        if (w == 0.f) continue;
-        const float* from = a.part_sums + (first + (int64_t)p * a.tile_rows) * kSize + lane * kOf;
+    typedef float Of __attribute__((ext_vector_type(kOf)));
+    // (eight parts' loads under way at once; a part without weight may hold anything)
+    const float* from = a.part_sums + first * kSize + lane * kOf;
+    const int64_t next = (int64_t)a.tile_rows * kSize;
+    constexpr int kAtOnce = 8;
+    for (int p = 0; p < a.parts; p += kAtOnce) {
+        Of v[kAtOnce];
 #pragma unroll
-        for (int j = 0; j < kOf; ++j) sum[j] = __builtin_fmaf(w, from[j], sum[j]);
+        for (int i = 0; i < kAtOnce; ++i) v[i] = *reinterpret_cast<const Of*>(from + min(p + i, a.parts - 1) * next);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const float w = p + i < a.parts ? __shfl(weight, (p + i) & 63) : 0.f;
+#pragma unroll
+            for (int j = 0; j < kOf; ++j) sum[j] = w == 0.f ? sum[j] : __builtin_fmaf(w, v[i][j], sum[j]);
+        }
     }
     if (a.sums != nullptr && lane == 0) a.sums[row] = sum_of<kHalf>(m, l);
     const float share = l == 0.f ? 0.f : 1.f / l;
@@ -994,7 +1016,7 @@ int attend_of(const AttentionArgs& a, hipStream_t s) {
     const int lds = few ? F::kLds : W::kLds;
     if (lds > 65536)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    kernel<<<(unsigned)((int64_t)a.B * a.groups * a.row_tiles * a.parts), few ? 64 * F::kWaves : 256, lds, s>>>(a);
+    kernel<<<(unsigned)(((int64_t)a.B * a.groups * a.parts + 7) / 8 * 8 * a.row_tiles), few ? 64 * F::kWaves : 256, lds, s>>>(a);
     return launch_check(few ? "attention_places_kernel" : "attention_rows_kernel");
 }
 template <bool kHalf, int kSize>
