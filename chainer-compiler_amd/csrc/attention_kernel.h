@@ -522,22 +522,19 @@ struct Job {
     int32_t rows, length, count, end;  // end: of the places that any of its rows sees
     int32_t begin_tile, end_tile;      // of its part
     int64_t at;                        // where its part's sums go, in tiles
-    bool none;
 };
 __device__ __forceinline__ Job job_of(const AttentionArgs& a, int32_t tile_rows, int32_t tile_places) {
     Job j;
     // Work-groups go to the eight XCDs in turn.  Neighbours read neighbouring heads' rows of the same places; the tiles of rows that read the same part of k and v follow each other on one XCD,
-    // whose L2 they share.  (The grid is filled up to whole eights of parts.)
-    const uint32_t turn = blockIdx.x >> 3, of_turn = uniform(turn / a.row_tiles);
-    const int32_t set = of_turn * 8 + (blockIdx.x & 7), of_group = uniform((uint32_t)set / a.groups);
+    // whose L2 they share; those of the last parts, fewer than eight, are dealt out evenly.
+    const uint32_t whole = a.B * a.groups * a.parts / 8 * 8 * a.row_tiles, turn = blockIdx.x < whole ? blockIdx.x >> 3 : blockIdx.x - whole, of_turn = uniform(turn / a.row_tiles);
+    const int32_t set = blockIdx.x < whole ? of_turn * 8 + (blockIdx.x & 7) : whole / a.row_tiles + of_turn, of_group = uniform((uint32_t)set / a.groups);
     // (of a chain, the tiles with the most places first)
     j.row_tile = a.row_tiles - 1 - (int32_t)(turn - of_turn * a.row_tiles);
     j.group = set - of_group * a.groups;
     j.b = uniform((uint32_t)of_group / a.parts);
     j.part = of_group - j.b * a.parts;
     j.at = (((int64_t)j.b * a.groups + j.group) * a.row_tiles + j.row_tile) * a.parts + j.part;
-    j.none = j.b >= a.B;
-    if (j.none) j.b = 0;
     j.rows = a.T * a.fan;
     j.length = length_of(a, j.b);
     j.count = count_of(a, j.b);
@@ -612,7 +609,6 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + 4 * W::kBytes);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const Job job = job_of(a, W::kRows, W::kPlaces);
-    if (job.none) return;
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<256>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const Row row = row_of(a, job, job.row_tile * W::kRows + wave * 32 + (lane & 31));
     u32x4 q[H::kSteps];
@@ -707,7 +703,6 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + W::kWork + kWaves * 64 * 4);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const Job job = job_of(a, 32, W::kPlaces);
-    if (job.none) return;
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<64 * kWaves>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const Row row = row_of(a, job, job.row_tile * 32 + (lane & 31));
     u32x4 q[H::kSteps];
@@ -1016,7 +1011,7 @@ int attend_of(const AttentionArgs& a, hipStream_t s) {
     const int lds = few ? F::kLds : W::kLds;
     if (lds > 65536)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    kernel<<<(unsigned)(((int64_t)a.B * a.groups * a.parts + 7) / 8 * 8 * a.row_tiles), few ? 64 * F::kWaves : 256, lds, s>>>(a);
+    kernel<<<(unsigned)((int64_t)a.B * a.groups * a.parts * a.row_tiles), few ? 64 * F::kWaves : 256, lds, s>>>(a);
     return launch_check(few ? "attention_places_kernel" : "attention_rows_kernel");
 }
 template <bool kHalf, int kSize>
