@@ -198,6 +198,19 @@ __device__ __forceinline__ __attribute__((address_space(3))) V* lds_pointer(uint
 
 // ---- a wavefront's work on a block of places: 32 rows, a lane's row is lane & 31 ---------------------------------
 
+// Steps of products whose operands come from LDS: load(i) asks for step i's, use(i) multiplies them, kAhead steps later.  The compiler alone puts each load right in front of its use and waits for it.
+template <int kSteps, int kAhead, typename Load, typename Use>
+__device__ __forceinline__ void in_steps(Load load, Use use) {
+#pragma unroll
+    for (int i = 0; i < kAhead && i < kSteps; ++i) load(i);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        if (i + kAhead < kSteps) load(i + kAhead);
+        __builtin_amdgcn_sched_barrier(6);  // (vector and scalar arithmetic may cross)
+        use(i);
+    }
+}
+
 // Scores of blocks of 32 places, whose keys lie in LDS from `keys` on; 32 rows to a lane's column.
 template <bool kHalf, int kSize, int kCount>
 __device__ __forceinline__ void find_scores(const char* keys, const u32x4 (&q)[Head<kHalf, kSize>::kSteps], f32x16 (&score)[kCount]) {
@@ -208,11 +221,17 @@ __device__ __forceinline__ void find_scores(const char* keys, const u32x4 (&q)[H
     asm volatile("" : "+v"(at));  // (the others are made from it where they are used)
 #pragma unroll
     for (int n = 0; n < kCount; ++n) score[n] = f32x16{};
+    constexpr int kAhead = kHalf ? 4 : 2;
+    u32x4 k[kAhead + 1][kCount];
+    in_steps<H::kSteps, kAhead>(
+            [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < H::kSteps; ++s) {
+                for (int n = 0; n < kCount; ++n) k[s % (kAhead + 1)][n] = *lds_pointer<u32x4>((at ^ (s << 5)) + n * 32 * H::kRow);
+            },
+            [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < kCount; ++n) score[n] = score_of<kHalf>(*lds_pointer<u32x4>((at ^ (s << 5)) + n * 32 * H::kRow), q[s], score[n]);
-    }
+                for (int n = 0; n < kCount; ++n) score[n] = score_of<kHalf>(k[s % (kAhead + 1)][n], q[s], score[n]);
+            });
 }
 
 // Weights in the scores' place; the sums so far are brought to the new maximum.
@@ -269,42 +288,44 @@ __device__ __forceinline__ void add_values(const char* values, const f32x16 (&we
             at[e] = lds_address(values) + row * H::kRow + ((c ^ H::turned(row)) << 4) + 8 * (lane & 1);
             asm volatile("" : "+v"(at[e]));
         }
+        half8 w[2 * kCount];
 #pragma unroll
-        for (int kb = 0; kb < 2 * kCount; ++kb) {
-            half8 w;
+        for (int kb = 0; kb < 2 * kCount; ++kb)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = (_Float16)weight[kb >> 1][8 * (kb & 1) + j];
+            for (int j = 0; j < 8; ++j) w[kb][j] = (_Float16)weight[kb >> 1][8 * (kb & 1) + j];
+        constexpr int kAhead = 6;
+        union {
+            short4v part[2];
+            half8 whole;
+        } v[kAhead + 1];
+        in_steps<2 * kCount * H::kBlocks, kAhead>(
+                [&](int i) __attribute__((always_inline)) {
+                    const int kb = i / H::kBlocks, n = i % H::kBlocks;
 #pragma unroll
-            for (int n = 0; n < H::kBlocks; ++n) {
-                union {
-                    short4v part[2];
-                    half8 whole;
-                } vf;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) vf.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_pointer<short4v>((at[e] ^ (n << 6)) + kb * 16 * H::kRow));
-                acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, w, acc[n], 0, 0, 0);
-            }
-        }
+                    for (int e = 0; e < 2; ++e) v[i % (kAhead + 1)].part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_pointer<short4v>((at[e] ^ (n << 6)) + kb * 16 * H::kRow));
+                },
+                [&](int i) __attribute__((always_inline)) {
+                    acc[i % H::kBlocks] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i % (kAhead + 1)].whole, w[i / H::kBlocks], acc[i % H::kBlocks], 0, 0, 0);
+                });
     } else {
         // a lane reads kWide elements of one row; row i of a block is turned by what 16 rows have in common
-        constexpr int kWide = H::kWide;
+        constexpr int kWide = H::kWide, kReads = H::kBlocks / kWide, kAhead = 3;
         typedef float Wide __attribute__((ext_vector_type(kWide)));
         uint32_t at = lds_address(values) + 4 * half * H::kRow + 4 * kWide * (lane & 31);
         asm volatile("" : "+v"(at));
         const uint32_t turn = half << 4;  // of row 4 half
+        Wide v[kAhead + 1];
+        in_steps<kCount * 16 * kReads, kAhead>(
+                [&](int i) __attribute__((always_inline)) {
+                    const int of = i / kReads, row = 8 * (of >> 2) + (of & 3);  // (16 to a block of 32)
+                    v[i % (kAhead + 1)] = *lds_pointer<Wide>((at ^ (H::turned(row) << 4) ^ turn) + row * H::kRow + 128 * kWide * (i % kReads));
+                },
+                [&](int i) __attribute__((always_inline)) {
+                    const int of = i / kReads, w = i % kReads;
 #pragma unroll
-        for (int n = 0; n < kCount; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int row = n * 32 + 8 * (i >> 2) + (i & 3);
-                const uint32_t turned = (H::turned(row) << 4) ^ turn;
-#pragma unroll
-                for (int w = 0; w < H::kBlocks / kWide; ++w) {
-                    const Wide vf = *lds_pointer<Wide>((at ^ turned) + row * H::kRow + 128 * kWide * w);
-#pragma unroll
-                    for (int j = 0; j < kWide; ++j) acc[w * kWide + j] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[j], weight[n][i], acc[w * kWide + j], 0, 0, 0);
-                }
-            }
+                    for (int j = 0; j < kWide; ++j)
+                        acc[w * kWide + j] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[i % (kAhead + 1)][j], weight[of / 16][of % 16], acc[w * kWide + j], 0, 0, 0);
+                });
     }
 }
 
