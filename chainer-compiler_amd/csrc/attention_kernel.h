@@ -145,9 +145,23 @@ template <bool kHalf>
 constexpr float kRaise = kHalf ? 6.f : 0.f;
 constexpr float kNoMaximum = -3e38f;
 
-// The largest of a lane and the one that has the row's other scores.
-__device__ __forceinline__ float with_other_half(float v) {
-    return __shfl_xor(v, 32);
+// A lane's value and that of the one with the row's other scores, in both.
+struct Halves {
+    float lower, upper;
+};
+__device__ __forceinline__ Halves both_halves(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    const auto both = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const uint32_t lower = both[0], upper = both[1];  // (numbers of their own: the compiler takes the first element's bits for those of any that is cast in place)
+    return {__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper)};
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+    const Halves h = both_halves(v);
+    return h.lower + h.upper;
+}
+__device__ __forceinline__ float largest_of_halves(float v) {
+    const Halves h = both_halves(v);
+    return fmaxf(h.lower, h.upper);
 }
 
 // The scores of 32 places and 32 rows, of one step's elements.
@@ -237,12 +251,14 @@ __device__ __forceinline__ void find_scores(const char* keys, const u32x4 (&q)[H
 // Weights in the scores' place; the sums so far are brought to the new maximum.
 template <bool kHalf, int kBlocks, int kCount>
 __device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCount], f32x16 (&acc)[kBlocks], float& m, float& l) {
-    float most = score[0][0];
+    float of[4] = {score[0][0], score[0][1], score[0][2], score[0][3]};  // (four chains, here and for the sum)
 #pragma unroll
     for (int n = 0; n < kCount; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) most = fmaxf(most, score[n][i]);
-    most = fmaxf(most, with_other_half(most)) * scale2;
+        for (int i = 0; i < 16; i += 4)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) of[j] = fmaxf(of[j], score[n][i + j]);
+    const float most = largest_of_halves(fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]))) * scale2;
     if (__builtin_amdgcn_ballot_w64(most > m + kLag)) {
         const float next = fmaxf(m, most), f = __builtin_amdgcn_exp2f(m - next);
         l *= f;
@@ -251,13 +267,15 @@ __device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCoun
         m = next;
     }
     const float less = m - kRaise<kHalf>;
+    float sum[4] = {};
 #pragma unroll
     for (int n = 0; n < kCount; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             score[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][i], scale2, -less));
-            l += score[n][i];
+            sum[i & 3] += score[n][i];
         }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // What is added up in place of v, all of it in LDS: itself, or (where results are made again) ones for what is inf, -inf and NaN, or what is finite.
@@ -403,10 +421,13 @@ struct From {
     const char* base;  // of the group's head
     int64_t page, row;
     uint32_t of_lane;  // how far the lane's row is from the first one of an instruction
+    bool near;         // every row is less than 4 GB behind base
 };
 template <typename H>
-__device__ __forceinline__ From from_of(const char* base, int64_t page, int64_t row) {
-    return {base, page, row, (uint32_t)((threadIdx.x & 63) / H::kChunks * row)};
+__device__ __forceinline__ From from_of(const AttentionArgs& a, const char* base, int64_t page, int64_t row, int32_t b) {
+    const uint32_t of_lane = (uint32_t)((threadIdx.x & 63) / H::kChunks * row);
+    if (a.tables == nullptr) return {base + b * page, 0, row, of_lane, row >= 0 && a.places * row < (int64_t(1) << 31)};
+    return {base, page, row, of_lane, page >= 0 && row >= 0 && page < (int64_t(1) << 31) && row < (int64_t(1) << 31) && (int64_t)a.pages * page + a.page_rows * row < (int64_t(1) << 32)};
 }
 
 // Whether the rows of every instruction's copies (of four, where it has fewer) lie in one page, at distances that 32 bits hold, and fill the kernel's: then their address is one of the
@@ -450,7 +471,7 @@ struct Runs {
         if (!good) return;
         if (a.tables == nullptr) {
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) page[i] = b, row[i] = p0 + own + i * kRun;
+            for (int i = 0; i < kCount; ++i) page[i] = 0, row[i] = p0 + own + i * kRun;
             return;
         }
         const auto* table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.tables + b * a.table_row);
@@ -481,12 +502,17 @@ template <typename H, int kCount, typename R>
 __device__ __forceinline__ void copy_runs(const From& f, const R& runs, uint32_t lds, int32_t first) {
     constexpr int kRows = 64 / H::kChunks;
     const int lane = threadIdx.x & 63;
+    auto all = [&](auto near) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < kCount; ++j) {
-        const int32_t row = (first + j) * kRows + lane / H::kChunks;
-        copy_to_lds(f.of_lane + (((lane % H::kChunks) ^ H::turned(row)) << 4), f.base + runs.page[j * kRows / R::kRun] * f.page + (runs.row[j * kRows / R::kRun] + j * kRows % R::kRun) * f.row,
-                    lds + (first + j) * 1024);
-    }
+        for (int j = 0; j < kCount; ++j) {
+            const int32_t row = (first + j) * kRows + lane / H::kChunks, page = runs.page[j * kRows / R::kRun], at = runs.row[j * kRows / R::kRun] + j * kRows % R::kRun;
+            const uint32_t of_lane = f.of_lane + (((lane % H::kChunks) ^ H::turned(row)) << 4);
+            if constexpr (decltype(near)::value) copy_to_lds(of_lane + ((uint32_t)page * (uint32_t)f.page + (uint32_t)at * (uint32_t)f.row), f.base, lds + (first + j) * 1024);
+            else copy_to_lds(of_lane, f.base + page * f.page + at * f.row, lds + (first + j) * 1024);
+        }
+    };
+    if (f.near) all(std::true_type());
+    else all(std::false_type());
 }
 
 // ---- results ----------------------------------------------------------------------------------------------------------
@@ -497,7 +523,7 @@ __device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)
     using H = Head<kHalf, kSize>;
     const int half = (threadIdx.x & 63) >> 5;
     const int32_t rows = a.T * a.fan;
-    l += with_other_half(l);
+    l = sum_of_halves(l);
     if (a.parts > 1) {
         if (half == 0) *reinterpret_cast<f32x2*>(a.part_stats + 2 * part_row) = f32x2{m, l};
         if (!any || r >= rows) return;
@@ -635,7 +661,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     u32x4 q[H::kSteps];
     load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 32 * H::kRow, q);
     if (!a.q_whole) __syncthreads();  // (the tiles come where they lay)
-    const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row), v = from_of<H>(a.v + job.group * a.v_head, a.v_page, a.v_row);
+    const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b), v = from_of<H>(a, a.v + job.group * a.v_head, a.v_page, a.v_row, job.b);
     const bool runs = in_runs<H>(a);
     const uint32_t lds = lds_address(attention_lds);
     const bool idle = job.row_tile * W::kRows + wave * 32 >= job.rows;  // (copies, and meets the others)
@@ -728,7 +754,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     const Row row = row_of(a, job, job.row_tile * 32 + (lane & 31));
     u32x4 q[H::kSteps];
     load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 2 * W::kBytes, q);
-    const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row), v = from_of<H>(a.v + job.group * a.v_head, a.v_page, a.v_row);
+    const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b), v = from_of<H>(a, a.v + job.group * a.v_head, a.v_page, a.v_row, job.b);
     const bool runs = in_runs<H>(a);
     char *keys = attention_lds + wave * 2 * W::kBytes, *values = keys + W::kBytes;
     const uint32_t keys_at = lds_address(keys), values_at = keys_at + W::kBytes;
@@ -786,7 +812,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     add_up(acc, pass, [](bool mine) { return __builtin_amdgcn_ballot_w64(mine) != 0; });
 
     // The wavefronts' sums, relative to the largest of their maxima; of those with an infinite one, what weighs nothing adds nothing.
-    l += with_other_half(l);
+    l = sum_of_halves(l);
     if (half == 0) {
         stats[wave * 64 + lane] = m;
         stats[wave * 64 + 32 + lane] = l;
@@ -918,7 +944,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     const int32_t blocks = (job.end + 31) / 32, each = uniform(((blocks + runs_of_places - 1) / runs_of_places + W::kWaves - 1) / W::kWaves * W::kWaves), last = min((run + 1) * each, blocks);
     if (run * each >= last) return;
     if (a.kind == kTree && last * 32 > job.length) find_ancestors<W::kThreads>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
-    const From k = from_of<H>(a.k + job.group * a.k_head, a.k_page, a.k_row);
+    const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b);
     const bool runs = in_runs<H>(a);
     char* keys = attention_lds + W::kOfRows + wave * W::kBuffers * W::kBytes;
     const uint32_t keys_at = lds_address(keys);
@@ -1015,7 +1041,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
                     }
                 }
             }
-            total += with_other_half(total);
+            total = sum_of_halves(total);
             if (mine) *to = before + total;
             buffer ^= W::kBuffers - 1;
         }
