@@ -248,10 +248,10 @@ __device__ __forceinline__ void find_scores(const char* keys, const u32x4 (&q)[H
             });
 }
 
-// Weights in the scores' place; the sums so far are brought to the new maximum.
+// The rows' maxima with these scores; the sums so far are brought to them.
 template <bool kHalf, int kBlocks, int kCount>
-__device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCount], f32x16 (&acc)[kBlocks], float& m, float& l) {
-    float of[4] = {score[0][0], score[0][1], score[0][2], score[0][3]};  // (four chains, here and for the sum)
+__device__ __forceinline__ void find_maxima(float scale2, const f32x16 (&score)[kCount], f32x16 (&acc)[kBlocks], float& m, float& l) {
+    float of[4] = {score[0][0], score[0][1], score[0][2], score[0][3]};  // (four chains, below for the sum too)
 #pragma unroll
     for (int n = 0; n < kCount; ++n)
 #pragma unroll
@@ -266,6 +266,11 @@ __device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCoun
         for (int n = 0; n < kBlocks; ++n) acc[n] *= f;
         m = next;
     }
+}
+
+// Weights in the scores' place.
+template <bool kHalf, int kCount>
+__device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCount], float m, float& l) {
     const float less = m - kRaise<kHalf>;
     float sum[4] = {};
 #pragma unroll
@@ -399,6 +404,10 @@ __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, u
 }
 __device__ __forceinline__ void copy_to_lds(const char* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
+}
+
+__device__ __forceinline__ void copy_number_to_lds(const float* from, uint32_t lds) {  // 4 bytes a lane, lane i's to lds + 4 i
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
 }
 
 __device__ const u32x4 kZeros[1] = {{0, 0, 0, 0}};  // what rows that are not there are read from
@@ -622,14 +631,16 @@ __device__ __forceinline__ void load_rows(const AttentionArgs& a, const Job& j, 
     if (a.q_whole) {
 #pragma unroll
         for (int s = 0; s < H::kSteps; ++s) q[s] = row.r < j.rows ? chunk_of<kHalf>(at, (2 * s + half) * 16, row_bytes, true) : u32x4{0, 0, 0, 0};
-        return;
-    }
-    u32x4* mine = reinterpret_cast<u32x4*>(space) + (lane & 31) * H::kChunks;
+    } else {
+        u32x4* mine = reinterpret_cast<u32x4*>(space) + (lane & 31) * H::kChunks;
 #pragma unroll 1
-    for (int c = half; c < H::kChunks; c += 2) mine[c] = row.r < j.rows ? chunk_of<kHalf>(at, c * 16, row_bytes, false) : u32x4{0, 0, 0, 0};
+        for (int c = half; c < H::kChunks; c += 2) mine[c] = row.r < j.rows ? chunk_of<kHalf>(at, c * 16, row_bytes, false) : u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int s = 0; s < H::kSteps; ++s) q[s] = mine[2 * s + half];  // (what this lane has written itself)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int s = 0; s < H::kSteps; ++s) q[s] = mine[2 * s + half];  // (what this lane has written itself)
+    }
+    // They are waited for here: a first use inside a loop would wait for everything that is under way, in every round of it.
+#pragma unroll
+    for (int s = 0; s < H::kSteps; ++s) asm volatile("" : "+v"(q[s]));
 }
 
 // ---- many rows --------------------------------------------------------------------------------------------------------
@@ -710,13 +721,18 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
             }
             const int32_t p0 = tile * W::kPlaces;
             f32x16 score[W::kBlocksOf];
+            __builtin_amdgcn_s_setprio(1);  // (before the wavefront of the other work-group, whose softmax then goes on under these products: 571 us of 2048 x 4096 rows without, 555 with)
             find_scores<kHalf, kSize>(keys, q, score);
+            __builtin_amdgcn_s_setprio(0);
             if (p0 + W::kPlaces > row.plain || there != ~0ull) {
 #pragma unroll
                 for (int n = 0; n < W::kBlocksOf; ++n) score[n] = hide(score[n], (seen_of(row.sight, nodes, p0 + 32 * n) & (uint32_t)(there >> (32 * n))) >> (4 * half));
             }
-            find_weights<kHalf>(a.scale2, score, acc, m, l);
+            find_maxima<kHalf>(a.scale2, score, acc, m, l);
+            find_weights<kHalf>(a.scale2, score, m, l);
+            __builtin_amdgcn_s_setprio(1);
             add_values<kHalf, kSize>(keys + W::kBytes, score, acc);
+            __builtin_amdgcn_s_setprio(0);
         }
         __syncthreads();
     };
@@ -798,7 +814,8 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 copy(k, block + kWaves, keys_at, keys);
             }
-            find_weights<kHalf>(a.scale2, score, acc, m, l);
+            find_maxima<kHalf>(a.scale2, score, acc, m, l);
+            find_weights<kHalf>(a.scale2, score, m, l);
             if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             if (special != kAll) replace_values<kHalf>(values, W::kBytes, special, lane, 64);
@@ -919,7 +936,7 @@ struct Mass {
     static constexpr int kBuffers = kBytes <= 8 * 1024 ? 2 : 1;
     static constexpr int kCopies = kBytes / 1024;
     static constexpr int kOfRows = kRows * Head<kHalf, kSize>::kRow;
-    static constexpr int kLds = kOfRows + kWaves * kBuffers * kBytes + kRows * 12 + (int)sizeof(Nodes);
+    static constexpr int kLds = kOfRows + kWaves * kBuffers * (kBytes + 256) + kRows * 12 + (int)sizeof(Nodes);
 };
 
 template <bool kHalf, int kSize>
@@ -927,7 +944,8 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     using H = Head<kHalf, kSize>;
     using W = Mass<kHalf, kSize>;
     extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
-    float* less = reinterpret_cast<float*>(attention_lds + W::kOfRows + W::kWaves * W::kBuffers * W::kBytes);  // of the rows: m + log2(l)
+    float* before = reinterpret_cast<float*>(attention_lds + W::kOfRows + W::kWaves * W::kBuffers * W::kBytes);  // what the places have already: [wave][buffer][64]
+    float* less = before + W::kWaves * W::kBuffers * 64;  // of the rows: m + log2(l)
     int32_t* limits = reinterpret_cast<int32_t*>(less + W::kRows);                                               // what they see, as in Sight
     int32_t* sees = limits + W::kRows;
     Nodes* nodes = reinterpret_cast<Nodes*>(sees + W::kRows);
@@ -947,7 +965,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b);
     const bool runs = in_runs<H>(a);
     char* keys = attention_lds + W::kOfRows + wave * W::kBuffers * W::kBytes;
-    const uint32_t keys_at = lds_address(keys);
+    const uint32_t keys_at = lds_address(keys), before_at = lds_address(before) + wave * W::kBuffers * 256;
     const int32_t row_bytes = a.D * H::kElement, used = job.count * a.fan;
     for (int32_t r0 = 0; r0 < used; r0 += W::kRows) {
         __syncthreads();
@@ -971,6 +989,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
         const int32_t seen_end = a.kind == kChain ? min(job.end, job.length + (min(r0 + W::kRows, used) - 1) / a.fan + 1) : job.end;
         Runs<H, 32, 32> next;
         uint64_t there = 0, there_next = 0;
+        float* mass = a.mass + job.b * a.mass_batch + job.group * a.mass_head;
         auto copy = [&](int32_t block, int buffer) __attribute__((always_inline)) {
             if (next.good) {
                 copy_runs<H, W::kCopies>(k, next, keys_at + buffer * W::kBytes, 0);
@@ -980,6 +999,9 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
                 copy_rows<H, 32, W::kCopies>(a, k, places, keys_at + buffer * W::kBytes, keys + buffer * W::kBytes, 0);
                 there_next = places.there;
             }
+            // (tokens' own places are set by the first of the rows)
+            const int32_t p = block * 32 + (lane & 31);
+            copy_number_to_lds(p < job.length || (r0 > 0 && p < job.end) ? mass + p : reinterpret_cast<const float*>(kZeros), before_at + buffer * 256);
         };
         const int32_t first = run * each + wave;
         if (first >= last) continue;
@@ -992,15 +1014,14 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
             const int32_t p0 = block * 32, p = p0 + (lane & 31);
             there = there_next;
             next.look_up(a, job.b, (block + W::kWaves) * 32, 0, job.end, runs && more);
-            float* to = a.mass + job.b * a.mass_batch + job.group * a.mass_head + p;
             const bool mine = ((there >> lane) & 1) && half == 0;
-            const float before = mine && (p < job.length || r0 > 0) ? *to : 0.f;
             if (W::kBuffers == 2 && more) {
                 copy(block + W::kWaves, buffer ^ 1);
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies) : "memory");
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies + 1) : "memory");
             } else {
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             }
+            const float so_far = before[(wave * W::kBuffers + buffer) * 64 + lane];
             u32x4 kf[H::kSteps];
             {
                 uint32_t at = keys_at + buffer * W::kBytes + (lane & 31) * H::kRow + ((half ^ H::turned(lane & 31)) << 4);
@@ -1042,7 +1063,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
                 }
             }
             total = sum_of_halves(total);
-            if (mine) *to = before + total;
+            if (mine) mass[p] = so_far + total;
             buffer ^= W::kBuffers - 1;
         }
     }
