@@ -10,6 +10,7 @@
 
 #include <cfloat>
 #include <cmath>
+#include <cstddef>
 #include <type_traits>
 
 #include "attention.h"
@@ -65,11 +66,15 @@ __device__ __forceinline__ u32x4 chunk_of(const char* row, int32_t at, int32_t b
 __device__ __forceinline__ int32_t uniform(int32_t v) {
     return __builtin_amdgcn_readfirstlane(v);
 }
+// (Of a work-group's sequence: the same for all its lanes, and through the scalar cache.)
+__device__ __forceinline__ int32_t number_at(const int32_t* p, int64_t i) {
+    return uniform(((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[i]);
+}
 __device__ __forceinline__ int32_t length_of(const AttentionArgs& a, int32_t b) {
-    return a.lengths ? max(0, min(uniform(a.lengths[b]), a.places)) : a.places;
+    return a.lengths ? max(0, min(number_at(a.lengths, b), a.places)) : a.places;
 }
 __device__ __forceinline__ int32_t count_of(const AttentionArgs& a, int32_t b) {
-    return a.counts ? max(0, min(uniform(a.counts[b]), a.T)) : a.T;
+    return a.counts ? max(0, min(number_at(a.counts, b), a.T)) : a.T;
 }
 
 __device__ __forceinline__ Place place_in(const AttentionArgs& a, int32_t b, int32_t p) {
@@ -78,9 +83,12 @@ __device__ __forceinline__ Place place_in(const AttentionArgs& a, int32_t b, int
 
 // Which nodes each node of a tree sees: words of 32 bits, of all nodes, in LDS.  Every step doubles the ancestors that a node knows of.
 struct Nodes {
-    uint32_t sees[kMostNodes][kMostNodes / 32];
     int16_t up[kMostNodes];
+    uint32_t sees[kMostNodes][kMostNodes / 32];  // (of T nodes: a launch has memory for no more)
 };
+inline int nodes_bytes(const AttentionArgs& a) {
+    return a.kind == kTree ? (int)offsetof(Nodes, sees) + a.T * (kMostNodes / 8) : 0;
+}
 template <int kThreads>
 __device__ __forceinline__ void find_ancestors(Nodes* nodes, const int32_t* parents, int32_t T) {
     constexpr int kOf = kMostNodes / kThreads;  // nodes of a lane
@@ -655,7 +663,7 @@ struct Tile {
     static constexpr int kBytes = kPlaces * Head<kHalf, kSize>::kRow;  // of k or v
     static constexpr int kCopies = kBytes / 1024 / kWaves;
     static constexpr int kBuffers = 4 * kBytes <= 128 * 1024 ? 2 : 1;
-    static constexpr int kLds = 2 * kBuffers * kBytes + (int)sizeof(Nodes);
+    static constexpr int kLds = 2 * kBuffers * kBytes;  // (and nodes)
 };
 
 template <bool kHalf, int kSize>
@@ -753,7 +761,7 @@ struct Few {
     static constexpr int kJoin = kWaves * 32 * (kSize + 4) * 4;    // the wavefronts' sums, rows not in the same banks
     static constexpr int kRing = kWaves * 2 * kBytes;
     static constexpr int kWork = kRing > kJoin ? kRing : kJoin;
-    static constexpr int kLds = kWork + kWaves * 64 * 4 + (int)sizeof(Nodes);
+    static constexpr int kLds = kWork + kWaves * 64 * 4;  // (and nodes)
 };
 
 template <bool kHalf, int kSize>
@@ -933,10 +941,9 @@ struct Mass {
     static constexpr int kBytes = 32 * Head<kHalf, kSize>::kRow;  // of a block of k
     static constexpr int kRows = kBytes <= 16 * 1024 ? 128 : 64;
     static constexpr int kWaves = kBytes <= 16 * 1024 ? 4 : 2, kThreads = 64 * kWaves;
-    static constexpr int kBuffers = kBytes <= 8 * 1024 ? 2 : 1;
     static constexpr int kCopies = kBytes / 1024;
     static constexpr int kOfRows = kRows * Head<kHalf, kSize>::kRow;
-    static constexpr int kLds = kOfRows + kWaves * kBuffers * (kBytes + 256) + kRows * 12 + (int)sizeof(Nodes);
+    static constexpr int kLds = kOfRows + kWaves * (kBytes + 256) + kRows * 12;  // (and nodes)
 };
 
 template <bool kHalf, int kSize>
@@ -944,8 +951,8 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     using H = Head<kHalf, kSize>;
     using W = Mass<kHalf, kSize>;
     extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
-    float* before = reinterpret_cast<float*>(attention_lds + W::kOfRows + W::kWaves * W::kBuffers * W::kBytes);  // what the places have already: [wave][buffer][64]
-    float* less = before + W::kWaves * W::kBuffers * 64;  // of the rows: m + log2(l)
+    float* before = reinterpret_cast<float*>(attention_lds + W::kOfRows + W::kWaves * W::kBytes);  // what the places have already: [wave][64]
+    float* less = before + W::kWaves * 64;  // of the rows: m + log2(l)
     int32_t* limits = reinterpret_cast<int32_t*>(less + W::kRows);                                               // what they see, as in Sight
     int32_t* sees = limits + W::kRows;
     Nodes* nodes = reinterpret_cast<Nodes*>(sees + W::kRows);
@@ -964,8 +971,8 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     if (a.kind == kTree && last * 32 > job.length) find_ancestors<W::kThreads>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
     const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b);
     const bool runs = in_runs<H>(a);
-    char* keys = attention_lds + W::kOfRows + wave * W::kBuffers * W::kBytes;
-    const uint32_t keys_at = lds_address(keys), before_at = lds_address(before) + wave * W::kBuffers * 256;
+    char* keys = attention_lds + W::kOfRows + wave * W::kBytes;
+    const uint32_t keys_at = lds_address(keys), before_at = lds_address(before) + wave * 256;
     const int32_t row_bytes = a.D * H::kElement, used = job.count * a.fan;
     for (int32_t r0 = 0; r0 < used; r0 += W::kRows) {
         __syncthreads();
@@ -990,24 +997,23 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
         Runs<H, 32, 32> next;
         uint64_t there = 0, there_next = 0;
         float* mass = a.mass + job.b * a.mass_batch + job.group * a.mass_head;
-        auto copy = [&](int32_t block, int buffer) __attribute__((always_inline)) {
+        auto copy = [&](int32_t block) __attribute__((always_inline)) {
             if (next.good) {
-                copy_runs<H, W::kCopies>(k, next, keys_at + buffer * W::kBytes, 0);
+                copy_runs<H, W::kCopies>(k, next, keys_at, 0);
                 there_next = ~0ull;
             } else {
                 const Places<32> places(a, job.b, block * 32, job.end);
-                copy_rows<H, 32, W::kCopies>(a, k, places, keys_at + buffer * W::kBytes, keys + buffer * W::kBytes, 0);
+                copy_rows<H, 32, W::kCopies>(a, k, places, keys_at, keys, 0);
                 there_next = places.there;
             }
             // (tokens' own places are set by the first of the rows)
             const int32_t p = block * 32 + (lane & 31);
-            copy_number_to_lds(p < job.length || (r0 > 0 && p < job.end) ? mass + p : reinterpret_cast<const float*>(kZeros), before_at + buffer * 256);
+            copy_number_to_lds(p < job.length || (r0 > 0 && p < job.end) ? mass + p : reinterpret_cast<const float*>(kZeros), before_at);
         };
         const int32_t first = run * each + wave;
         if (first >= last) continue;
-        int buffer = 0;
         next.look_up(a, job.b, first * 32, 0, job.end, runs);
-        copy(first, 0);
+        copy(first);
 #pragma unroll 1
         for (int32_t block = first; block < last; block += W::kWaves) {
             const bool more = block + W::kWaves < last;
@@ -1015,21 +1021,17 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
             there = there_next;
             next.look_up(a, job.b, (block + W::kWaves) * 32, 0, job.end, runs && more);
             const bool mine = ((there >> lane) & 1) && half == 0;
-            if (W::kBuffers == 2 && more) {
-                copy(block + W::kWaves, buffer ^ 1);
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies + 1) : "memory");
-            } else {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            }
-            const float so_far = before[(wave * W::kBuffers + buffer) * 64 + lane];
+            // the block goes into registers, and the next one's copies into its place are on their way while it is worked on
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            const float so_far = before[wave * 64 + lane];
             u32x4 kf[H::kSteps];
             {
-                uint32_t at = keys_at + buffer * W::kBytes + (lane & 31) * H::kRow + ((half ^ H::turned(lane & 31)) << 4);
+                uint32_t at = keys_at + (lane & 31) * H::kRow + ((half ^ H::turned(lane & 31)) << 4);
 #pragma unroll
                 for (int s = 0; s < H::kSteps; ++s) kf[s] = *lds_pointer<u32x4>(at ^ (s << 5));
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (W::kBuffers == 1 && more) copy(block + W::kWaves, 0);
+            if (more) copy(block + W::kWaves);
             float total = 0.f;
             const bool plain = p0 + 32 <= job.length;
 #pragma unroll 1
@@ -1037,19 +1039,24 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
                 f32x16 score = {};
                 uint32_t at = lds_address(attention_lds) + (rb * 32 + (lane & 31)) * H::kRow + ((half ^ H::turned(lane & 31)) << 4);
                 asm volatile("" : "+v"(at));
-#pragma unroll
-                for (int s = 0; s < H::kSteps; ++s) score = score_of<kHalf>(*lds_pointer<u32x4>(at ^ (s << 5)), kf[s], score);
+                constexpr int kAhead = kHalf ? 4 : 2;
+                u32x4 q[kAhead + 1];
+                in_steps<H::kSteps, kAhead>([&](int s) __attribute__((always_inline)) { q[s % (kAhead + 1)] = *lds_pointer<u32x4>(at ^ (s << 5)); },
+                                            [&](int s) __attribute__((always_inline)) { score = score_of<kHalf>(q[s % (kAhead + 1)], kf[s], score); });
                 const int row = rb * 32 + 4 * half;
                 // (a weight that is not seen is none, also of a row that has no number for its sum)
                 uint32_t seen = ~0u;
                 if (!plain || r0 + rb * 32 + 32 > used) {
                     seen = 0;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int at_row = row + 8 * (i >> 2) + (i & 3), node = sees[at_row], other = p - job.length;
-                        const uint32_t word = nodes->sees[max(node, 0)][min(max(other, 0) >> 5, kMostNodes / 32 - 1)];
-                        const bool of_tree = (node >= 0) & (other >= 0) & (other < job.count) & ((word >> (other & 31)) & 1);
-                        seen |= (uint32_t)((p < limits[at_row]) | of_tree) << i;
+                    for (int i = 0; i < 16; ++i) seen |= (uint32_t)(p < limits[row + 8 * (i >> 2) + (i & 3)]) << i;
+                    const int32_t other = p - job.length;  // the node that lies there
+                    if (a.kind == kTree && other >= 0 && other < job.count) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int32_t node = sees[row + 8 * (i >> 2) + (i & 3)];
+                            seen |= (node >= 0 ? (nodes->sees[node][other >> 5] >> (other & 31)) & 1 : 0) << i;
+                        }
                     }
                 }
 #pragma unroll
@@ -1064,7 +1071,6 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
             }
             total = sum_of_halves(total);
             if (mine) mass[p] = so_far + total;
-            buffer ^= W::kBuffers - 1;
         }
     }
     // (places of a sequence without tokens stay as they are)
@@ -1076,7 +1082,7 @@ int attend_of(const AttentionArgs& a, hipStream_t s) {
     using F = Few<kHalf, kSize>;
     const bool few = a.tile_rows == 32;
     auto kernel = few ? attention_places_kernel<kHalf, kSize> : attention_rows_kernel<kHalf, kSize>;
-    const int lds = few ? F::kLds : W::kLds;
+    const int lds = (few ? F::kLds : W::kLds) + nodes_bytes(a);
     if (lds > 65536)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     kernel<<<(unsigned)((int64_t)a.B * a.groups * a.parts * a.row_tiles), few ? 64 * F::kWaves : 256, lds, s>>>(a);
@@ -1095,9 +1101,10 @@ int mass_of(const AttentionArgs& a, hipStream_t s) {
     int64_t runs = (512 + groups - 1) / groups;
     runs = runs > most ? most : runs;
     auto kernel = attention_mass_kernel<kHalf, kSize>;
-    if constexpr (W::kLds > 65536)  // (has to be asked for, on every device)
-        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, W::kLds));
-    kernel<<<(unsigned)(groups * runs), W::kThreads, W::kLds, s>>>(a, (int32_t)runs);
+    const int lds = W::kLds + nodes_bytes(a);
+    if (lds > 65536)  // (has to be asked for, on every device)
+        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    kernel<<<(unsigned)(groups * runs), W::kThreads, lds, s>>>(a, (int32_t)runs);
     return launch_check("attention_mass_kernel");
 }
 
