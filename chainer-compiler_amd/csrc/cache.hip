@@ -158,41 +158,57 @@ __device__ __forceinline__ char* row_at(const MoveArgs& a, const Rows& r, int32_
 }
 
 // Drafted rows that were accepted.  A work-group has at most 256 slices of 128 bytes: all are read before the first is written.  blockIdx: sequence, head, then keys' slices, values' slices, mass.
+// Bound by the loads that wait for each other (accepted, tables, rows): where a row comes from and goes to is found once, by a lane for each.
 template <typename Unit>
 __global__ __launch_bounds__(256) void cache_accept_kernel(MoveArgs a) {
     __shared__ Unit rows[kMostAccepted * kSlice / sizeof(Unit)];
-    __shared__ int32_t from[kMostAccepted];
+    __shared__ const char* from_at[kMostAccepted];
+    __shared__ char* to_at[kMostAccepted];
     __shared__ int32_t count;
     const int32_t each = 2 * a.slices + (a.mass ? 1 : 0), what = blockIdx.x % each, h = blockIdx.x / each % a.c.groups, b = blockIdx.x / each / a.c.groups;
     const int32_t length = clamped(a.c.lengths[b], a.c.places), i = threadIdx.x;
     if (i == 0) count = a.most;
+    const int32_t slice = what % a.slices * kSlice;
+    const Rows r = what < a.slices ? Rows{a.c.k + h * a.c.k_head + slice, a.c.k_page, a.c.k_row} : Rows{a.c.v + h * a.c.v_head + slice, a.c.v_page, a.c.v_row};
     __syncthreads();
+    int32_t from = -1;
     if (i < a.most) {
-        from[i] = a.accepted[(int64_t)b * a.most + i];
-        if (from[i] < 0) atomicMin(&count, i);
+        from = a.accepted[(int64_t)b * a.most + i];
+        if (from < 0) atomicMin(&count, i);
+        const char* at = row_at(a, r, b, (int64_t)length + from);
+        char* to = row_at(a, r, b, (int64_t)length + i);
+        from_at[i] = to ? at : nullptr;
+        to_at[i] = at ? to : nullptr;
     }
     __syncthreads();
     const int32_t n = count;
     if (what == 0 && h == 0 && i == 0) a.new_lengths[b] = min(length + n, a.c.places);
     if (what == 2 * a.slices) {
         float* mass = a.mass + b * a.mass_batch + h * a.mass_head;
-        const int64_t p = i < n ? (int64_t)length + from[i] : a.c.places;
+        const int64_t p = i < n ? (int64_t)length + from : a.c.places;
         const float v = p < a.c.places ? mass[p] : 0.f;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (p < a.c.places && length + i < a.c.places) mass[length + i] = v;
         return;
     }
-    const int32_t slice = what % a.slices * kSlice, bytes = min(kSlice, a.row_bytes - slice), units = bytes / (int32_t)sizeof(Unit);
-    const Rows r = what < a.slices ? Rows{a.c.k + h * a.c.k_head + slice, a.c.k_page, a.c.k_row} : Rows{a.c.v + h * a.c.v_head + slice, a.c.v_page, a.c.v_row};
-    for (int32_t j = i; j < n * units; j += 256) {
-        const char* at = row_at(a, r, b, (int64_t)length + from[j / units]);
-        if (at) rows[j] = reinterpret_cast<const Unit*>(at)[j % units];
+    const int32_t bytes = min(kSlice, a.row_bytes - slice), units = bytes / (int32_t)sizeof(Unit);
+    constexpr int kAtOnce = 4;
+    for (int32_t j0 = i; j0 < n * units; j0 += 256 * kAtOnce) {
+        Unit v[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int32_t j = j0 + k * 256;
+            const char* at = j < n * units ? from_at[j / units] : nullptr;
+            if (at) v[k] = reinterpret_cast<const Unit*>(at)[j % units];
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+            if (j0 + k * 256 < n * units) rows[j0 + k * 256] = v[k];  // (also what is not there: it goes nowhere)
     }
     __syncthreads();
     for (int32_t j = i; j < n * units; j += 256) {
-        if (!row_at(a, r, b, (int64_t)length + from[j / units])) continue;
-        char* to = row_at(a, r, b, (int64_t)length + j / units);
+        char* to = to_at[j / units];
         if (to) reinterpret_cast<Unit*>(to)[j % units] = rows[j];
     }
 }
@@ -205,41 +221,58 @@ __device__ __forceinline__ uint32_t sortable(float v) {
     return v != v ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
-// The weights as numbers to be compared: in LDS where a sequence's fit (kInLds: read once, eight loads of a lane under way), else from memory each time.
+// The weights as numbers to be compared, four at a time: in LDS where a sequence's fit (kInLds: read once, eight loads of a lane under way), else from memory each time.  Behind the last
+// are zeros, which are less than any weight's.
 constexpr int32_t kMostInLds = 36 * 1024;
 template <bool kInLds>
 struct Keys {
     const float* mass;
-    uint32_t* keys;
-    __device__ __forceinline__ void load(int32_t n) {
+    u32x4* keys;
+    int32_t n;
+    __device__ __forceinline__ void load() {
         if constexpr (kInLds) {
             constexpr int kAtOnce = 8;
-            for (int32_t i0 = threadIdx.x; i0 < n; i0 += 1024 * kAtOnce) {
+            uint32_t* to = reinterpret_cast<uint32_t*>(keys);
+            const int32_t all = (n + 3) / 4 * 4;
+            for (int32_t i0 = threadIdx.x; i0 < all; i0 += 1024 * kAtOnce) {
                 float v[kAtOnce];
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) v[j] = i0 + j * 1024 < n ? mass[i0 + j * 1024] : 0.f;
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j)
-                    if (i0 + j * 1024 < n) keys[i0 + j * 1024] = sortable(v[j]);
+                    if (i0 + j * 1024 < all) to[i0 + j * 1024] = i0 + j * 1024 < n ? sortable(v[j]) : 0;
             }
             __syncthreads();
         }
     }
-    __device__ __forceinline__ uint32_t at(int32_t i) const {
-        return kInLds ? keys[i] : sortable(mass[i]);
+    __device__ __forceinline__ u32x4 at(int32_t quad) const {
+        if constexpr (kInLds) return keys[quad];
+        u32x4 k;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = 4 * quad + j < n ? sortable(mass[4 * quad + j]) : 0;
+        return k;
     }
 };
 
+// The sum of what the wavefronts before this one have, of 16.
+__device__ __forceinline__ int32_t before_wave(const int32_t* of_waves, int wave) {
+    const int lane = threadIdx.x & 63;
+    int32_t v = lane < wave ? of_waves[lane & 15] : 0;
+#pragma unroll
+    for (int d = 8; d; d /= 2) v += __shfl_xor(v, d);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
 // A head's places that stay: the threshold of the `best` largest of n weights by three histograms of 11, 11 and 10 bits, of equal ones the lower places; then the
-// list of moves, places that go in front of best and places that stay behind it, both in ascending order.
+// list of moves, places that go in front of best and places that stay behind it, both in ascending order.  One work-group to a head; bound by its instructions where sequences are long (32,768 places: six passes
+// over LDS), by its barriers where they are short.
 template <bool kInLds>
 __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
-    extern __shared__ uint32_t choose_lds[];
+    extern __shared__ u32x4 choose_lds[];
     constexpr int kWaves = 16, kBins = 2048;
     __shared__ int32_t bins[kBins];
-    __shared__ int32_t of_waves[kWaves];
-    __shared__ uint32_t found_bin;
-    __shared__ int32_t found_above;
+    __shared__ int32_t of_waves[3][kWaves];
+    __shared__ int32_t found[3];  // bin, how many are above it, how many are in it
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t h = blockIdx.x % a.c.groups, b = blockIdx.x / a.c.groups;
     const int32_t length = clamped(a.c.lengths[b], a.c.places);
@@ -249,95 +282,145 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
         if (threadIdx.x == 0) list[0] = 0;
         return;
     }
-    const int32_t n = length - a.recent, best = a.keep - a.recent;
-    Keys<kInLds> keys = {a.mass + b * a.mass_batch + h * a.mass_head, choose_lds};
-    keys.load(n);
+    const int32_t n = length - a.recent, best = a.keep - a.recent, quads = (n + 3) / 4;
+    if (best == 0) {  // (nothing of them stays, and nothing moves)
+        if (threadIdx.x == 0) list[0] = 0;
+        return;
+    }
+    Keys<kInLds> keys = {a.mass + b * a.mass_batch + h * a.mass_head, choose_lds, n};
+    for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
+    keys.load();
+    __syncthreads();
     uint32_t least = 0;      // upper bits of the threshold
     int32_t wanted = best;   // how many with those bits
-    if (best > 0) {
-        for (int digit = 0; digit < 3; ++digit) {
-            const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-            const uint32_t above = digit == 0 ? 0 : ~0u << (shift + bits);
-            for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
-            __syncthreads();
-            for (int32_t i = threadIdx.x; i - lane < n; i += 1024) {
-                const uint32_t key = i < n ? keys.at(i) : 0;
-                const bool counts = i < n && ((key ^ least) & above) == 0;
-                const uint32_t bin = (key >> shift) & ((1u << bits) - 1);
-                // (equal weights, as of places that nobody has looked at, would queue for one bin)
+    bool tie = false;        // whether some that equal the threshold go
+    for (int digit = 0; digit < 3; ++digit) {
+        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+        const uint32_t above = digit == 0 ? 0 : ~0u << (shift + bits);
+        for (int32_t i = threadIdx.x; i - lane < quads; i += 1024) {
+            const u32x4 key = i < quads ? keys.at(i) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool counts = i < quads && ((key[j] ^ least) & above) == 0;
                 const uint64_t all = __builtin_amdgcn_ballot_w64(counts);
                 if (all == 0) continue;
-                const int leader = __builtin_ctzll(all);
-                const uint32_t its = __builtin_amdgcn_readlane(bin, leader);
-                if (__builtin_amdgcn_ballot_w64(counts && bin != its) == 0) {
-                    if (lane == leader) atomicAdd(&bins[its], __popcll(all));
+                // (equal weights, as of places that nobody has looked at, would queue for one bin)
+                const uint32_t bin = (key[j] >> shift) & ((1u << bits) - 1), its = __builtin_amdgcn_readlane(bin, __builtin_ctzll(all));
+                if (__builtin_amdgcn_ballot_w64(counts && bin == its) == all) {
+                    if (lane == 0) atomicAdd(&bins[its], __popcll(all));
                 } else if (counts) {
                     atomicAdd(&bins[bin], 1);
                 }
             }
-            __syncthreads();
-            // the bin in which the wanted one is, from above: a lane has two bins
-            const int32_t hi = bins[kBins - 1 - 2 * threadIdx.x], lo = bins[kBins - 2 - 2 * threadIdx.x];
-            int32_t upto = hi + lo;
+        }
+        __syncthreads();
+        // the bin in which the wanted one is, from above: a lane has two bins, which it clears for the next digit
+        const int at = kBins - 2 - 2 * threadIdx.x;
+        const int32_t hi = bins[at + 1], lo = bins[at];
+        bins[at + 1] = bins[at] = 0;
+        int32_t upto = hi + lo;
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const int32_t o = __shfl_up(upto, d);
-                if (lane >= d) upto += o;
-            }
-            if (lane == 63) of_waves[wave] = upto;
-            __syncthreads();
-            for (int w = 0; w < wave; ++w) upto += of_waves[w];
-            const int32_t before = upto - hi - lo;
-            if (before < wanted && wanted <= before + hi) found_bin = kBins - 1 - 2 * threadIdx.x, found_above = before;
-            else if (before + hi < wanted && wanted <= upto) found_bin = kBins - 2 - 2 * threadIdx.x, found_above = before + hi;
-            __syncthreads();
-            least |= found_bin << shift;
-            wanted -= found_above;
-            __syncthreads();
+        for (int d = 1; d < 64; d *= 2) {
+            const int32_t o = __shfl_up(upto, d);
+            if (lane >= d) upto += o;
         }
+        if (lane == 63) of_waves[0][wave] = upto;
+        __syncthreads();
+        upto += before_wave(of_waves[0], wave);
+        const int32_t before = upto - hi - lo;
+        if (before < wanted && wanted <= before + hi) found[0] = at + 1, found[1] = before, found[2] = hi;
+        else if (before + hi < wanted && wanted <= upto) found[0] = at, found[1] = before + hi, found[2] = lo;
+        __syncthreads();
+        least |= (uint32_t)found[0] << shift;
+        wanted -= found[1];
+        tie = found[2] != wanted;
     }
-    // `wanted` of those that equal the threshold stay, the lower places first; each wavefront has a run of places
-    const int32_t run = (n + kWaves * 64 - 1) / (kWaves * 64) * 64, from = wave * run, to = min(from + run, n);
-    auto of_wave = [&](int32_t mine) {  // what the wavefronts before this one have
-        __syncthreads();
-        if (lane == 0) of_waves[wave] = mine;
-        __syncthreads();
-        int32_t before = 0;
-        for (int w = 0; w < wave; ++w) before += of_waves[w];
-        return before;
-    };
+    // `wanted` of those that equal the threshold stay, the lower places first; each wavefront has a run of places, a lane four next to each other
+    const uint64_t below = (1ull << lane) - 1;
+    const int32_t run = (quads + kWaves * 64 - 1) / (kWaves * 64) * 64, from = wave * run, to = min(from + run, quads);
     int32_t equal = 0;
-    for (int32_t i = from + lane; i - lane < to; i += 64) equal += __popcll(__builtin_amdgcn_ballot_w64(i < to && best > 0 && keys.at(i) == least));
-    const int32_t equal_before = of_wave(equal);
-    int32_t holes = 0, movers = 0, holes_before = 0, movers_before = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        int32_t rank = equal_before;
-        holes = movers = 0;
+    if (tie) {
         for (int32_t i = from + lane; i - lane < to; i += 64) {
-            const uint32_t key = i < to ? keys.at(i) : 0;
-            const uint64_t same = __builtin_amdgcn_ballot_w64(i < to && best > 0 && key == least), below = (1ull << lane) - 1;
-            const bool stays = best > 0 && (key > least || (key == least && rank + __popcll(same & below) < wanted));
-            rank += __popcll(same);
-            const uint64_t hole = __builtin_amdgcn_ballot_w64(i < to && i < best && !stays), mover = __builtin_amdgcn_ballot_w64(i < to && i >= best && stays);
-            if (pass == 1) {
-                if ((hole >> lane) & 1) list[1 + holes_before + holes + __popcll(hole & below)] = i;
-                if ((mover >> lane) & 1) list[1 + a.most + movers_before + movers + __popcll(mover & below)] = i;
-            }
-            holes += __popcll(hole);
-            movers += __popcll(mover);
+            const u32x4 key = i < to ? keys.at(i) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) equal += __popcll(__builtin_amdgcn_ballot_w64(key[j] == least));
         }
-        if (pass == 0) {
-            holes_before = of_wave(holes);
-            movers_before = of_wave(movers);
+        if (lane == 0) of_waves[0][wave] = equal;
+        __syncthreads();
+        equal = before_wave(of_waves[0], wave);
+    }
+    // which of a lane's four stay, which of those that do not are free places, which of those that do go there
+    int32_t rank = equal;
+    struct Four {
+        uint32_t holes, movers;
+    };
+    auto four_at = [&](int32_t i) __attribute__((always_inline)) {
+        const u32x4 key = i < to ? keys.at(i) : u32x4{0, 0, 0, 0};
+        uint32_t stays = 0;
+        if (tie) {
+            uint64_t same[4];
+            int32_t mine = rank;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                same[j] = __builtin_amdgcn_ballot_w64(key[j] == least);
+                mine += __popcll(same[j] & below);
+                rank += __popcll(same[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                stays |= (uint32_t)(key[j] > least || (key[j] == least && mine < wanted)) << j;
+                mine += key[j] == least;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) stays |= (uint32_t)(key[j] >= least) << j;
+        }
+        // (places behind the last do not stay, and are not below best)
+        const int32_t first = best - 4 * i;  // of the four, this many are below best
+        const uint32_t in_front = first >= 4 ? 15u : first > 0 ? (1u << first) - 1 : 0;
+        return Four{i < to ? ~stays & in_front : 0, stays & ~in_front & 15u};
+    };
+    int32_t holes = 0, movers = 0;
+    for (int32_t i = from + lane; i - lane < to; i += 64) {
+        const Four f = four_at(i);
+        holes += __popc(f.holes);
+        movers += __popc(f.movers);
+    }
+#pragma unroll
+    for (int d = 32; d; d /= 2) {
+        holes += __shfl_xor(holes, d);
+        movers += __shfl_xor(movers, d);
+    }
+    if (lane == 0) of_waves[1][wave] = holes, of_waves[2][wave] = movers;
+    __syncthreads();
+    holes = before_wave(of_waves[1], wave);
+    movers = before_wave(of_waves[2], wave);
+    rank = equal;
+    for (int32_t i = from + lane; i - lane < to; i += 64) {
+        const Four f = four_at(i);
+        if (__builtin_amdgcn_ballot_w64((f.holes | f.movers) != 0) == 0) continue;
+        int32_t hole_at = holes, mover_at = movers;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t of_holes = __builtin_amdgcn_ballot_w64((f.holes >> j) & 1), of_movers = __builtin_amdgcn_ballot_w64((f.movers >> j) & 1);
+            hole_at += __popcll(of_holes & below);
+            mover_at += __popcll(of_movers & below);
+            holes += __popcll(of_holes);
+            movers += __popcll(of_movers);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if ((f.holes >> j) & 1) list[1 + hole_at++] = 4 * i + j;
+            if ((f.movers >> j) & 1) list[1 + a.most + mover_at++] = 4 * i + j;
         }
     }
-    if (threadIdx.x == 1023) list[0] = holes_before + holes;
+    if (threadIdx.x == 1023) list[0] = holes;  // (with those before the last wavefront)
 }
 
 // The moves of a head's list, then the latest places behind them, `recent` of them from length - recent to keep - recent: those may overlap themselves, so they go in
 // ascending pieces, each read before it is written.  blockIdx as for cache_accept_kernel.
-template <typename Unit>
-__global__ __launch_bounds__(1024) void cache_evict_kernel(MoveArgs a) {
+template <typename Unit, int kThreads>
+__global__ __launch_bounds__(kThreads) void cache_evict_kernel(MoveArgs a) {
     constexpr int kAtOnce = 4;
     const int32_t each = 2 * a.slices + 1, what = blockIdx.x % each, h = blockIdx.x / each % a.c.groups, b = blockIdx.x / each / a.c.groups;
     const int32_t length = clamped(a.c.lengths[b], a.c.places);
@@ -347,8 +430,8 @@ __global__ __launch_bounds__(1024) void cache_evict_kernel(MoveArgs a) {
     const int32_t *to_list = list + 1, *from_list = list + 1 + a.most;
     if (what == 2 * a.slices) {
         float* mass = a.mass + b * a.mass_batch + h * a.mass_head;
-        for (int32_t i = threadIdx.x; i < moves; i += 1024) mass[to_list[i]] = mass[from_list[i]];
-        for (int32_t i0 = 0; i0 < a.recent; i0 += 1024) {
+        for (int32_t i = threadIdx.x; i < moves; i += kThreads) mass[to_list[i]] = mass[from_list[i]];
+        for (int32_t i0 = 0; i0 < a.recent; i0 += kThreads) {
             const int32_t i = i0 + threadIdx.x;
             const float v = i < a.recent ? mass[latest + i] : 0.f;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what is read here, or was above, may be written next)
@@ -357,45 +440,64 @@ __global__ __launch_bounds__(1024) void cache_evict_kernel(MoveArgs a) {
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        for (int32_t i = a.keep + threadIdx.x; i < length; i += 1024) mass[i] = 0.f;
+        for (int32_t i = a.keep + threadIdx.x; i < length; i += kThreads) mass[i] = 0.f;
         return;
     }
     const int32_t slice = what % a.slices * kSlice, bytes = min(kSlice, a.row_bytes - slice), units = bytes / (int32_t)sizeof(Unit);
     const Rows r = what < a.slices ? Rows{a.c.k + h * a.c.k_head + slice, a.c.k_page, a.c.k_row} : Rows{a.c.v + h * a.c.v_head + slice, a.c.v_page, a.c.v_row};
-    const int32_t rows = 1024 / units, mine = threadIdx.x / units, u = threadIdx.x % units;  // (units: at most 64)
-    for (int32_t i0 = 0; i0 < moves; i0 += rows * kAtOnce) {
+    const int32_t rows = kThreads / units, mine = threadIdx.x / units, u = threadIdx.x % units;  // (units: at most 64)
+    struct Piece {
         Unit v[kAtOnce];
-        bool there[kAtOnce];
+        char* to[kAtOnce];
+    };
+    // the i-th and following ones of `count` rows: read, with where they go, which is asked for at the same time
+    auto read = [&](Piece& piece, int32_t i0, int32_t count, auto from, auto to) __attribute__((always_inline)) {
+        const char* at[kAtOnce];
+        int32_t from_place[kAtOnce], to_place[kAtOnce];
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
             const int32_t i = i0 + j * rows + mine;
-            const char* at = mine < rows && i < moves ? row_at(a, r, b, from_list[i]) : nullptr;
-            there[j] = at != nullptr;
-            if (at) v[j] = reinterpret_cast<const Unit*>(at)[u];
+            const bool there = mine < rows && i < count;
+            from_place[j] = there ? from(i) : -1;
+            to_place[j] = there ? to(i) : -1;
         }
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-            char* at = there[j] ? row_at(a, r, b, to_list[i0 + j * rows + mine]) : nullptr;
-            if (at) reinterpret_cast<Unit*>(at)[u] = v[j];
+            at[j] = row_at(a, r, b, from_place[j]);
+            piece.to[j] = row_at(a, r, b, to_place[j]);
         }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            if (at[j] == nullptr) piece.to[j] = nullptr;
+            else piece.v[j] = reinterpret_cast<const Unit*>(at[j])[u];
+        }
+    };
+    auto write = [&](const Piece& piece) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+            if (piece.to[j]) reinterpret_cast<Unit*>(piece.to[j])[u] = piece.v[j];
+    };
+    auto read_moved = [&](Piece& piece, int32_t i0) __attribute__((always_inline)) { read(piece, i0, moves, [&](int32_t i) { return from_list[i]; }, [&](int32_t i) { return to_list[i]; }); };
+    auto read_latest = [&](Piece& piece, int32_t i0) __attribute__((always_inline)) { read(piece, i0, a.recent, [&](int32_t i) { return latest + i; }, [&](int32_t i) { return to + i; }); };
+    // The rows of the list, whose places are apart from those they come from; its last piece with the first of the latest rows, which may go where rows of the list came from.
+    const int32_t step = rows * kAtOnce;
+    Piece moved, late;
+    int32_t i0 = 0;
+    for (; i0 + step < moves; i0 += step) {
+        read_moved(moved, i0);
+        write(moved);
     }
-    for (int32_t i0 = 0; i0 < a.recent; i0 += rows * kAtOnce) {
-        Unit v[kAtOnce];
-        bool there[kAtOnce];
-#pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) {
-            const int32_t i = i0 + j * rows + mine;
-            const char* at = mine < rows && i < a.recent ? row_at(a, r, b, latest + i) : nullptr;
-            there[j] = at != nullptr;
-            if (at) v[j] = reinterpret_cast<const Unit*>(at)[u];
-        }
+    read_moved(moved, i0);
+    read_latest(late, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    write(moved);
+    write(late);
+    for (i0 = step; i0 < a.recent; i0 += step) {
+        read_latest(late, i0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) {
-            char* at = there[j] ? row_at(a, r, b, to + i0 + j * rows + mine) : nullptr;
-            if (at) reinterpret_cast<Unit*>(at)[u] = v[j];
-        }
+        write(late);
     }
 }
 
@@ -529,14 +631,16 @@ extern "C" int chx_hip_cache_evict(
     a.lists = static_cast<int32_t*>(workspace);
     const bool in_lds = a.c.places <= kMostInLds;
     auto choose = in_lds ? cache_choose_kernel<true> : cache_choose_kernel<false>;
-    if (in_lds && a.c.places > 12 * 1024)  // (has to be asked for, on every device)
+    if (in_lds && a.c.places > 12 * 1024 - 256)  // (has to be asked for, on every device)
         CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(choose), hipFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostInLds));
-    choose<<<(unsigned)(a.c.B * a.c.groups), 1024, in_lds ? 4 * a.c.places : 0, as_stream(stream)>>>(a);
+    choose<<<(unsigned)(a.c.B * a.c.groups), 1024, in_lds ? (4 * a.c.places + 15) / 16 * 16 : 0, as_stream(stream)>>>(a);
     CHX_PROPAGATE(launch_check("cache_choose_kernel"));
     if (a.keep >= a.c.places) return CHX_HIP_OK;
     const unsigned grid = (unsigned)(a.c.B * a.c.groups * (2 * a.slices + 1));
     return by_unit(unit_of_cache(a.c, a.row_bytes), [&](auto u) {
-        cache_evict_kernel<decltype(u)><<<grid, 1024, 0, as_stream(stream)>>>(a);
+        // (smaller work-groups where there are more than two of the larger ones to a compute unit)
+        if (grid > 512) cache_evict_kernel<decltype(u), 512><<<grid, 512, 0, as_stream(stream)>>>(a);
+        else cache_evict_kernel<decltype(u), 1024><<<grid, 1024, 0, as_stream(stream)>>>(a);
         return launch_check("cache_evict_kernel");
     });
 }
