@@ -40,6 +40,28 @@ struct Head {
     static __device__ __forceinline__ int turned(int row) {
         return kChunks == 8 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
     }
+    // Calls f(element of the head, kVector results of a lane next to each other from it on) for all of them.
+    static constexpr int kVector = kHalf ? 4 : kWide;
+    typedef float Vector __attribute__((ext_vector_type(kVector)));
+    template <typename F>
+    static __device__ __forceinline__ void in_vectors(const f32x16 (&acc)[kBlocks], int half, F f) {
+        if constexpr (kHalf) {
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) f(element(n, i, half), Vector{acc[n][i], acc[n][i + 1], acc[n][i + 2], acc[n][i + 3]});
+        } else {
+#pragma unroll
+            for (int n = 0; n < kBlocks; n += kWide)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    Vector v;
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j) v[j] = acc[n + j][i];
+                    f(element(n, i, half), v);
+                }
+        }
+    }
     // Element of the head that result (block, i) of a lane is; i = 0..15.
     static __device__ __forceinline__ int element(int block, int i, int half) {
         const int r = 8 * (i >> 2) + 4 * half + (i & 3);
@@ -545,10 +567,7 @@ __device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)
         if (half == 0) *reinterpret_cast<f32x2*>(a.part_stats + 2 * part_row) = f32x2{m, l};
         if (!any || r >= rows) return;
         float* to = a.part_sums + part_row * kSize;
-#pragma unroll
-        for (int n = 0; n < H::kBlocks; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) to[H::element(n, i, half)] = acc[n][i];
+        H::in_vectors(acc, half, [&](int element, typename H::Vector v) __attribute__((always_inline)) { *reinterpret_cast<typename H::Vector*>(to + element) = v; });
         return;
     }
     if (r >= rows) return;
@@ -558,26 +577,10 @@ __device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)
     char* y = a.y + b * a.y_batch + t * a.y_token + head * a.y_head;
 #pragma unroll
     for (int n = 0; n < H::kBlocks; ++n) acc[n] *= share;
-    if constexpr (kHalf) {
-#pragma unroll
-        for (int n = 0; n < H::kBlocks; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const half4 v = {(_Float16)acc[n][i], (_Float16)acc[n][i + 1], (_Float16)acc[n][i + 2], (_Float16)acc[n][i + 3]};
-                store<4>(a, y, H::element(n, i, half), v);
-            }
-    } else {
-        constexpr int kWide = H::kWide;
-#pragma unroll
-        for (int n = 0; n < H::kBlocks; n += kWide)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float v __attribute__((ext_vector_type(kWide)));
-#pragma unroll
-                for (int j = 0; j < kWide; ++j) v[j] = acc[n + j][i];
-                store<kWide>(a, y, H::element(n, i, half), v);
-            }
-    }
+    H::in_vectors(acc, half, [&](int element, typename H::Vector v) __attribute__((always_inline)) {
+        if constexpr (kHalf) store<4>(a, y, element, half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]});
+        else store<H::kVector>(a, y, element, v);
+    });
 }
 
 // What a work-group works on.
@@ -854,10 +857,8 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
 #pragma unroll
     for (int n = 0; n < H::kBlocks; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float part = f == 0.f || l == 0.f ? 0.f : acc[n][i] * f;
-            sums[(wave * 32 + (lane & 31)) * kPitch + H::element(n, i, half)] = part;
-        }
+        for (int i = 0; i < 16; ++i) acc[n][i] = f == 0.f || l == 0.f ? 0.f : acc[n][i] * f;
+    H::in_vectors(acc, half, [&](int element, typename H::Vector v) __attribute__((always_inline)) { *reinterpret_cast<typename H::Vector*>(sums + (wave * 32 + (lane & 31)) * kPitch + element) = v; });
     __syncthreads();
     const int64_t part_row = job.at * 32;
     if (a.parts > 1 && threadIdx.x < 32) *reinterpret_cast<f32x2*>(a.part_stats + 2 * (part_row + lane)) = f32x2{most, total};
