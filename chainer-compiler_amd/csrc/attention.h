@@ -25,6 +25,7 @@ struct AttentionArgs {
     int32_t kind;
     int32_t B, T, groups, fan, D;
     int32_t pages, page_rows;
+    Divisor by_fan, by_groups, by_page, by_row_tiles, by_parts;
     int32_t places;  // of a sequence, at most: of its table, or states
     float scale2;    // scale * log2(e): exponentials are powers of 2
     bool q_whole, k_whole, y_whole;  // whole 16-byte pieces at addresses that are multiples of 16 (y: 8)

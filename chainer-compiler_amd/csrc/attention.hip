@@ -64,6 +64,11 @@ int check_queries(const chx_hip_tensor* q, int32_t dtype, int64_t B, const char*
     a->T = (int32_t)q->shape[1];
     a->fan = (int32_t)(q->shape[2] / a->groups);
     share_out(a, q->dtype == CHX_HIP_FLOAT16);
+    a->by_fan = divisor_of(a->fan);
+    a->by_groups = divisor_of(a->groups);
+    a->by_page = divisor_of(a->page_rows);
+    a->by_row_tiles = divisor_of(a->row_tiles);
+    a->by_parts = divisor_of(a->parts);
     CHX_REQUIRE((int64_t)a->B * a->groups * a->parts * a->row_tiles < (int64_t(1) << 23), "%s: more tiles than one launch has", what);
     return CHX_HIP_OK;
 }

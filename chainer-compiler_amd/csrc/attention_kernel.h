@@ -515,7 +515,7 @@ struct Runs {
         }
         const auto* table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.tables + b * a.table_row);
         if constexpr (kOwn < kPlaces) good = all_there(a, table, p0, kPlaces);
-        int32_t at = uniform((int32_t)((uint32_t)(p0 + own) / (uint32_t)a.page_rows)), r = p0 + own - at * a.page_rows;
+        int32_t at = over(p0 + own, a.by_page), r = p0 + own - at * a.page_rows;
         uint32_t outside = 0;
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
@@ -529,7 +529,7 @@ struct Runs {
         good = good && outside == 0;
     }
     static __device__ __forceinline__ bool all_there(const AttentionArgs& a, const __attribute__((address_space(4))) int32_t* table, int32_t p0, int32_t places) {
-        const int32_t first = uniform((int32_t)((uint32_t)p0 / (uint32_t)a.page_rows)), last = uniform((int32_t)((uint32_t)(p0 + places - 1) / (uint32_t)a.page_rows));
+        const int32_t first = over(p0, a.by_page), last = over(p0 + places - 1, a.by_page);
         uint32_t outside = 0;
         for (int32_t i = first; i <= last; ++i) outside |= (uint32_t)table[i] >= (uint32_t)a.pages;
         return outside == 0;
@@ -573,7 +573,7 @@ __device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)
     if (r >= rows) return;
     if (a.sums != nullptr && half == 0) a.sums[((int64_t)b * a.groups + group) * rows + r] = sum_of<kHalf>(m, l);
     const float share = l == 0.f ? 0.f : 1.f / l;
-    const int32_t t = r / a.fan, head = group * a.fan + (r - t * a.fan);
+    const int32_t t = over(r, a.by_fan), head = group * a.fan + (r - t * a.fan);
     char* y = a.y + b * a.y_batch + t * a.y_token + head * a.y_head;
 #pragma unroll
     for (int n = 0; n < H::kBlocks; ++n) acc[n] *= share;
@@ -594,21 +594,22 @@ __device__ __forceinline__ Job job_of(const AttentionArgs& a, int32_t tile_rows,
     Job j;
     // Work-groups go to the eight XCDs in turn.  Neighbours read neighbouring heads' rows of the same places; the tiles of rows that read the same part of k and v follow each other on one XCD,
     // whose L2 they share; those of the last parts, fewer than eight, are dealt out evenly.
-    const uint32_t whole = a.B * a.groups * a.parts / 8 * 8 * a.row_tiles, turn = blockIdx.x < whole ? blockIdx.x >> 3 : blockIdx.x - whole, of_turn = uniform(turn / a.row_tiles);
-    const int32_t set = blockIdx.x < whole ? of_turn * 8 + (blockIdx.x & 7) : whole / a.row_tiles + of_turn, of_group = uniform((uint32_t)set / a.groups);
+    const int32_t whole_sets = a.B * a.groups * a.parts / 8 * 8;
+    const uint32_t whole = whole_sets * a.row_tiles, turn = blockIdx.x < whole ? blockIdx.x >> 3 : blockIdx.x - whole, of_turn = over(turn, a.by_row_tiles);
+    const int32_t set = blockIdx.x < whole ? of_turn * 8 + (blockIdx.x & 7) : whole_sets + of_turn, of_group = over(set, a.by_groups);
     // (of a chain, the tiles with the most places first)
     j.row_tile = a.row_tiles - 1 - (int32_t)(turn - of_turn * a.row_tiles);
     j.group = set - of_group * a.groups;
-    j.b = uniform((uint32_t)of_group / a.parts);
+    j.b = over(of_group, a.by_parts);
     j.part = of_group - j.b * a.parts;
     j.at = (((int64_t)j.b * a.groups + j.group) * a.row_tiles + j.row_tile) * a.parts + j.part;
     j.rows = a.T * a.fan;
     j.length = length_of(a, j.b);
     j.count = count_of(a, j.b);
-    const int32_t first_t = j.row_tile * tile_rows / a.fan, last_t = min((min((j.row_tile + 1) * tile_rows, j.rows) - 1) / a.fan, j.count - 1);
+    const int32_t first_t = over(j.row_tile * tile_rows, a.by_fan), last_t = min(over(min((j.row_tile + 1) * tile_rows, j.rows) - 1, a.by_fan), j.count - 1);
     j.end = last_t < first_t ? 0 : a.kind == kCross ? j.length : a.kind == kChain ? j.length + last_t + 1 : j.length + j.count;
     j.end = min(j.end, a.places);
-    const int32_t tiles = (j.end + tile_places - 1) / tile_places, each = uniform((tiles + a.parts - 1) / a.parts);
+    const int32_t tiles = (j.end + tile_places - 1) / tile_places, each = over(tiles + a.parts - 1, a.by_parts);
     j.begin_tile = j.part * each;
     j.end_tile = min(j.begin_tile + each, tiles);
     return j;
@@ -620,16 +621,16 @@ struct Row {
     Sight sight;
     int32_t plain;  // places below this are seen by all of them
 };
-__device__ __forceinline__ Row row_of(const AttentionArgs& a, const Job& j, int32_t r) {
+__device__ __forceinline__ Row row_of(const AttentionArgs& a, const Job& j, int32_t first) {  // first: of the wavefront's 32
     Row row;
-    row.r = r;
-    row.t = r < j.rows ? r / a.fan : a.T;
+    row.r = first + (int)(threadIdx.x & 31);
+    // (rows behind the last do what the last one does; their results go nowhere)
+    const int32_t r = min(row.r, j.rows - 1);
+    row.t = over(r, a.by_fan);
     row.head = j.group * a.fan + (r - row.t * a.fan);
     row.sight = sight_of(a, row.t, j.length, j.count);
-    int32_t plain = row.sight.limit;
-#pragma unroll
-    for (int d = 16; d; d /= 2) plain = min(plain, __shfl_xor(plain, d));
-    row.plain = __builtin_amdgcn_readfirstlane(plain);
+    const int32_t first_t = over(min(first, j.rows - 1), a.by_fan), last_t = over(min(first + 31, j.rows - 1), a.by_fan);
+    row.plain = last_t >= j.count ? 0 : a.kind == kChain ? j.length + first_t + 1 : j.length;
     return row;
 }
 // The rows of a wavefront; those that are not whole pieces go through `space` in LDS, of 32 rows.
@@ -641,17 +642,20 @@ __device__ __forceinline__ void load_rows(const AttentionArgs& a, const Job& j, 
     const char* at = a.q + j.b * a.q_batch + row.t * a.q_token + row.head * a.q_head;
     if (a.q_whole) {
 #pragma unroll
-        for (int s = 0; s < H::kSteps; ++s) q[s] = row.r < j.rows ? chunk_of<kHalf>(at, (2 * s + half) * 16, row_bytes, true) : u32x4{0, 0, 0, 0};
+        for (int s = 0; s < H::kSteps; ++s) q[s] = chunk_of<kHalf>(at, (2 * s + half) * 16, row_bytes, true);
     } else {
         u32x4* mine = reinterpret_cast<u32x4*>(space) + (lane & 31) * H::kChunks;
 #pragma unroll 1
-        for (int c = half; c < H::kChunks; c += 2) mine[c] = row.r < j.rows ? chunk_of<kHalf>(at, c * 16, row_bytes, false) : u32x4{0, 0, 0, 0};
+        for (int c = half; c < H::kChunks; c += 2) mine[c] = chunk_of<kHalf>(at, c * 16, row_bytes, false);
 #pragma unroll
         for (int s = 0; s < H::kSteps; ++s) q[s] = mine[2 * s + half];  // (what this lane has written itself)
     }
-    // They are waited for here: a first use inside a loop would wait for everything that is under way, in every round of it.
+}
+// They are waited for here, behind the first copies: a first use inside a loop would wait for everything that is under way, in every round of it.
+template <int kSteps>
+__device__ __forceinline__ void wait_for(u32x4 (&q)[kSteps]) {
 #pragma unroll
-    for (int s = 0; s < H::kSteps; ++s) asm volatile("" : "+v"(q[s]));
+    for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[s]));
 }
 
 // ---- many rows --------------------------------------------------------------------------------------------------------
@@ -679,7 +683,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const Job job = job_of(a, W::kRows, W::kPlaces);
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<256>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
-    const Row row = row_of(a, job, job.row_tile * W::kRows + wave * 32 + (lane & 31));
+    const Row row = row_of(a, job, job.row_tile * W::kRows + wave * 32);
     u32x4 q[H::kSteps];
     load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 32 * H::kRow, q);
     if (!a.q_whole) __syncthreads();  // (the tiles come where they lay)
@@ -714,6 +718,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
         auto look_up = [&](int32_t tile) __attribute__((always_inline)) { next.look_up(a, job.b, tile * W::kPlaces, wave * (W::kPlaces / W::kWaves), job.end, runs); };
         look_up(job.begin_tile);
         copy(job.begin_tile);
+        wait_for(q);
         look_up(job.begin_tile + 1);
         for (int32_t tile = job.begin_tile; tile < job.end_tile; ++tile) {
             there = there_next;
@@ -778,7 +783,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const Job job = job_of(a, 32, W::kPlaces);
     if (a.kind == kTree && job.begin_tile < job.end_tile && job.end_tile * W::kPlaces > job.length) find_ancestors<64 * kWaves>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
-    const Row row = row_of(a, job, job.row_tile * 32 + (lane & 31));
+    const Row row = row_of(a, job, job.row_tile * 32);
     u32x4 q[H::kSteps];
     load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 2 * W::kBytes, q);
     const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b), v = from_of<H>(a, a.v + job.group * a.v_head, a.v_page, a.v_row, job.b);
@@ -811,6 +816,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
         next.look_up(a, job.b, first * 32, 0, job.end, runs);
         copy(k, first, keys_at, keys);
         copy(v, first, values_at, values);
+        wait_for(q);
 #pragma unroll 1
         for (int32_t block = first; block < last; block += kWaves) {
             const bool more = block + kWaves < last;
@@ -880,7 +886,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
             continue;
         }
         sum *= stats[r];
-        const int32_t all = job.row_tile * 32 + r, t = all / a.fan, head = job.group * a.fan + (all - t * a.fan);
+        const int32_t all = job.row_tile * 32 + r, t = over(all, a.by_fan), head = job.group * a.fan + (all - t * a.fan);
         char* y = a.y + job.b * a.y_batch + t * a.y_token + head * a.y_head;
         if constexpr (kHalf) store<4>(a, y, e, half4{(_Float16)sum[0], (_Float16)sum[1], (_Float16)sum[2], (_Float16)sum[3]});
         else store<4>(a, y, e, sum);
@@ -895,7 +901,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     const int32_t rows = a.T * a.fan;
     const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= (int64_t)a.B * a.groups * rows) return;
-    const int32_t of = (int32_t)(row / rows), r = (int32_t)(row % rows), t = r / a.fan, head = of % a.groups * a.fan + (r - t * a.fan);
+    const int32_t of = (int32_t)(row / rows), r = (int32_t)(row % rows), t = over(r, a.by_fan), b = over(of, a.by_groups), head = (of - b * a.groups) * a.fan + (r - t * a.fan);
     const int32_t tile = r / a.tile_rows;
     const int64_t first = (((int64_t)of * a.row_tiles + tile) * a.parts) * a.tile_rows + (r - tile * a.tile_rows);
     f32x2 stat = {kNoMaximum, 0.f};
@@ -926,7 +932,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     }
     if (a.sums != nullptr && lane == 0) a.sums[row] = sum_of<kHalf>(m, l);
     const float share = l == 0.f ? 0.f : 1.f / l;
-    char* y = a.y + of / a.groups * a.y_batch + t * a.y_token + head * a.y_head;
+    char* y = a.y + b * a.y_batch + t * a.y_token + head * a.y_head;
 #pragma unroll
     for (int j = 0; j < kOf; ++j) {
         if (lane * kOf + j >= a.D) break;
@@ -960,7 +966,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     Job job;
     const int32_t of = uniform(blockIdx.x / runs_of_places), run = blockIdx.x - of * runs_of_places;
-    job.b = uniform(of / a.groups);
+    job.b = over(of, a.by_groups);
     job.group = of - job.b * a.groups;
     job.rows = a.T * a.fan;
     job.length = length_of(a, job.b);
@@ -978,14 +984,14 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     for (int32_t r0 = 0; r0 < used; r0 += W::kRows) {
         __syncthreads();
         for (int32_t i = threadIdx.x; i < W::kRows * H::kChunks; i += W::kThreads) {
-            const int32_t r = r0 + i / H::kChunks, c = i % H::kChunks, t = r / a.fan, head = job.group * a.fan + (r - t * a.fan);
+            const int32_t r = r0 + i / H::kChunks, c = i % H::kChunks, t = over(r, a.by_fan), head = job.group * a.fan + (r - t * a.fan);
             u32x4 v = {0, 0, 0, 0};
             if (r < used) v = chunk_of<kHalf>(a.q + job.b * a.q_batch + t * a.q_token + head * a.q_head, c * 16, row_bytes, a.q_whole);
             reinterpret_cast<u32x4*>(attention_lds)[i / H::kChunks * H::kChunks + (c ^ H::turned(i / H::kChunks))] = v;
         }
         static_assert(W::kRows <= W::kThreads, "a lane to a row");
         if (threadIdx.x < W::kRows) {
-            const int32_t r = r0 + threadIdx.x, t = r / a.fan;
+            const int32_t r = r0 + threadIdx.x, t = over(r, a.by_fan);
             const Sight sight = sight_of(a, t, job.length, job.count);
             less[threadIdx.x] = r < used ? a.sums[(int64_t)of * job.rows + r] : INFINITY;
             limits[threadIdx.x] = sight.limit;
@@ -994,7 +1000,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
         __syncthreads();
         const int32_t row_blocks = (min(used - r0, W::kRows) + 31) / 32;
         // (the rows of a chain do not see places behind the last of them)
-        const int32_t seen_end = a.kind == kChain ? min(job.end, job.length + (min(r0 + W::kRows, used) - 1) / a.fan + 1) : job.end;
+        const int32_t seen_end = a.kind == kChain ? min(job.end, job.length + over(min(r0 + W::kRows, used) - 1, a.by_fan) + 1) : job.end;
         Runs<H, 32, 32> next;
         uint64_t there = 0, there_next = 0;
         float* mass = a.mass + job.b * a.mass_batch + job.group * a.mass_head;

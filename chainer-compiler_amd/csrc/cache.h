@@ -5,6 +5,22 @@
 
 namespace chx {
 
+// Division of numbers below 2^31 by one that the host knows: n / d = (floor(n mul / 2^32) + n) >> shift with 2^(shift - 1) < d <= 2^shift and mul = floor(2^32 (2^shift - d) / d) + 1.  (A few
+// instructions, also scalar ones; a division by a number of 32 bits is some 20 to 40 of the vector units'.)
+struct Divisor {
+    uint32_t mul;
+    int32_t shift;
+};
+inline Divisor divisor_of(int32_t d) {
+    Divisor r = {1, 0};
+    while ((int64_t(1) << r.shift) < d) ++r.shift;
+    if (d > 0) r.mul = (uint32_t)((((uint64_t(1) << r.shift) - (uint64_t)d) << 32) / (uint64_t)d + 1);
+    return r;
+}
+__device__ __forceinline__ int32_t over(int32_t n, Divisor d) {
+    return (int32_t)((__umulhi((uint32_t)n, d.mul) + (uint32_t)n) >> d.shift);
+}
+
 struct CacheArgs {
     char *k, *v;
     int64_t k_page, k_row, k_head, v_page, v_row, v_head;  // bytes
@@ -12,6 +28,7 @@ struct CacheArgs {
     int64_t table_row;  // elements
     const int32_t* lengths;
     int32_t B, groups, D, pages, page_rows;
+    Divisor by_page;  // rows of a page
     int32_t places;  // of a sequence: of its table
 };
 
@@ -45,7 +62,7 @@ struct Place {
 };
 template <typename Args>
 __device__ __forceinline__ Place place_of(const Args& a, int32_t b, int32_t p) {
-    const int32_t i = (int32_t)((uint32_t)p / (uint32_t)a.page_rows), page = a.tables[b * a.table_row + i];
+    const int32_t i = over(p, a.by_page), page = a.tables[b * a.table_row + i];
     return {page < a.pages ? page : -1, p - i * a.page_rows};
 }
 

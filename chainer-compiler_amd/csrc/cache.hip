@@ -55,6 +55,7 @@ int check_cache(const chx_hip_tensor* keys, const chx_hip_tensor* values, const 
     c->D = (int32_t)keys->shape[3];
     c->pages = (int32_t)keys->shape[0];
     c->page_rows = (int32_t)keys->shape[1];
+    c->by_page = divisor_of(c->page_rows);
     c->places = (int32_t)(tables->shape[1] * keys->shape[1]);
     return CHX_HIP_OK;
 }
