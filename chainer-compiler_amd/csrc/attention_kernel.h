@@ -27,6 +27,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at any address of an element
 
 template <bool kHalf, int kSize>
 struct Head {
@@ -69,17 +70,33 @@ struct Head {
     }
 };
 
-// 16 bytes of a row of `bytes` bytes from byte `at` on, zeros behind its end.
+__device__ const u32x4 kZeros[1] = {{0, 0, 0, 0}};  // what is not there is read from here
+
+// 16 bytes of a row of `bytes` bytes from byte `at` on (a multiple of 16), zeros behind its end and of a row that is not there.  The last ones of a row that is not whole pieces are its last 16, moved
+// down.  (Addresses and values are chosen, here and below, where a branch that lanes take by themselves would do: where registers are short, the compiler puts moves of live ones before the point at which the
+// others come back, and those lose what they held.)
 template <bool kHalf>
-__device__ __forceinline__ u32x4 chunk_of(const char* row, int32_t at, int32_t bytes, bool whole) {
+__device__ __forceinline__ u32x4 chunk_of(const char* row, int32_t at, int32_t bytes, bool whole, bool there = true) {
+    const char* none = reinterpret_cast<const char*>(kZeros);
+    const bool any = there & (at < bytes);
+    if (whole) return *reinterpret_cast<const u32x4*>(any ? row + at : none);
+    if (bytes >= 16) {
+        const u32x4 v = *reinterpret_cast<const u32x4_any*>(any ? row + min(at, bytes - 16) : none);
+        const int32_t more = max(at + 16 - bytes, 0), bits = 8 * (more & 7);  // bytes of these that the row does not have
+        uint64_t lower = (uint64_t)v[1] << 32 | v[0], upper = (uint64_t)v[3] << 32 | v[2];
+        lower = more & 8 ? upper : lower;
+        upper = more & 8 ? 0 : upper;
+        lower = lower >> bits | (upper << 1) << (63 - bits);
+        upper >>= bits;
+        return u32x4{(uint32_t)lower, (uint32_t)(lower >> 32), (uint32_t)upper, (uint32_t)(upper >> 32)};
+    }
     u32x4 v = {0, 0, 0, 0};
-    if (whole) return at < bytes ? *reinterpret_cast<const u32x4*>(row + at) : v;
 #pragma unroll
     for (int j = 0; j < (kHalf ? 8 : 4); ++j) {
-        const int32_t b = at + j * (kHalf ? 2 : 4);
-        if (b >= bytes) break;
-        if constexpr (kHalf) v[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + b) << (16 * (j & 1));
-        else v[j] = *reinterpret_cast<const uint32_t*>(row + b);
+        const int32_t b = j * (kHalf ? 2 : 4);
+        const char* from = (any & (b < bytes)) ? row + b : none;  // (at is 0, or there is none of it)
+        if constexpr (kHalf) v[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(from) << (16 * (j & 1));
+        else v[j] = *reinterpret_cast<const uint32_t*>(from);
     }
     return v;
 }
@@ -113,7 +130,7 @@ inline int nodes_bytes(const AttentionArgs& a) {
 }
 template <int kThreads>
 __device__ __forceinline__ void find_ancestors(Nodes* nodes, const int32_t* parents, int32_t T) {
-    constexpr int kOf = kMostNodes / kThreads;  // nodes of a lane
+    constexpr int kOf = kThreads < kMostNodes ? kMostNodes / kThreads : 1;  // nodes of a lane
     const int words = (T + 31) / 32;
     for (int i = threadIdx.x; i < T; i += kThreads) {
         const int32_t p = parents[i];
@@ -150,20 +167,22 @@ __device__ __forceinline__ void find_ancestors(Nodes* nodes, const int32_t* pare
 struct Sight {
     int32_t limit, length, count;
     int32_t node;  // -1: none
+    bool trees;    // whether any row has one
 };
 __device__ __forceinline__ Sight sight_of(const AttentionArgs& a, int32_t t, int32_t length, int32_t count) {
-    if (t >= count) return {0, length, count, -1};
-    return {a.kind == kChain ? length + t + 1 : length, length, count, a.kind == kTree ? t : -1};
+    const int32_t limit = a.kind == kChain ? length + t + 1 : length;
+    return {t < count ? limit : 0, length, count, a.kind == kTree && t < count ? t : -1, a.kind == kTree};
 }
 // Which of the places p0 to p0 + 31 a row sees, a bit each.  (A node's words have only nodes before it and itself, all below count.)
 __device__ __forceinline__ uint32_t seen_of(const Sight& s, const Nodes* nodes, int32_t p0) {
     const int32_t below = s.limit - p0;
     uint32_t seen = below >= 32 ? ~0u : below > 0 ? (1u << below) - 1 : 0;
     const int32_t i = p0 - s.length;  // the node that lies at p0
-    if (s.node >= 0 && i > -32 && i < s.count) {
-        const uint32_t* words = nodes->sees[s.node];
-        const uint64_t two = i < 0 ? (uint64_t)words[0] << 32 : words[i >> 5] | (uint64_t)words[min((i >> 5) + 1, kMostNodes / 32 - 1)] << 32;
-        seen |= (uint32_t)(two >> (i & 31));
+    if (s.trees && i > -32 && i < s.count) {
+        const uint32_t* words = nodes->sees[max(s.node, 0)];
+        const uint64_t lower = i < 0 ? 0 : words[max(i >> 5, 0)], upper = words[min((i >> 5) + 1, kMostNodes / 32 - 1)];
+        const uint32_t seen_nodes = (uint32_t)((lower | upper << 32) >> (i & 31));
+        seen |= s.node >= 0 ? seen_nodes : 0;
     }
     return seen;
 }
@@ -428,29 +447,31 @@ __device__ __forceinline__ void add_up(f32x16 (&acc)[kBlocks], Pass pass, Any an
 
 // ---- rows of k and v into LDS ---------------------------------------------------------------------------------------
 
-// Asynchronous copies of 16 bytes a lane into LDS, lane i's to lds + 16 i (the same for all lanes), counted like loads.
+// Asynchronous copies of 16 bytes a lane into LDS, lane i's to lds + 16 i (the same for all lanes), counted like loads.  (Where the base's scalar registers come from a vector instruction, as a
+// v_readlane, five cycles have to pass before a memory instruction reads them, and the compiler does not see that this is one.)
 __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(uniform(lds)) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(uniform(lds)) : "memory", "m0");
+}
+// (Of some lanes only; all of them are there.)
+__device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds, uint64_t lanes) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b64 exec, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" : : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0");
 }
 __device__ __forceinline__ void copy_to_lds(const char* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
 }
-
 __device__ __forceinline__ void copy_number_to_lds(const float* from, uint32_t lds) {  // 4 bytes a lane, lane i's to lds + 4 i
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
 }
 
-__device__ const u32x4 kZeros[1] = {{0, 0, 0, 0}};  // what rows that are not there are read from
-
-// What a lane knows of kPlaces places from p0 on: of place p0 + lane % kPlaces, where it lies; of all, which are there.
+// What a lane knows of kPlaces places from p0 on, some of them before end: of place p0 + lane % kPlaces, where it lies; of all, which are there.
 template <int kPlaces>
 struct Places {
     Place at;
     uint64_t there;
     __device__ __forceinline__ Places(const AttentionArgs& a, int32_t b, int32_t p0, int32_t end) {
         const int32_t p = p0 + (int)(threadIdx.x & (kPlaces - 1));
-        at = {-1, 0};
-        if (p < end) at = place_in(a, b, p);
+        at = place_in(a, b, min(p, end - 1));
+        at.page = p < end ? at.page : -1;
         there = __builtin_amdgcn_ballot_w64(at.page >= 0);
     }
 };
@@ -461,39 +482,50 @@ struct From {
     int64_t page, row;
     uint32_t of_lane;  // how far the lane's row is from the first one of an instruction
     bool near;         // every row is less than 4 GB behind base
+    uint32_t bytes;    // of a row
 };
 template <typename H>
 __device__ __forceinline__ From from_of(const AttentionArgs& a, const char* base, int64_t page, int64_t row, int32_t b) {
     const uint32_t of_lane = (uint32_t)((threadIdx.x & 63) / H::kChunks * row);
-    if (a.tables == nullptr) return {base + b * page, 0, row, of_lane, row >= 0 && a.places * row < (int64_t(1) << 31)};
-    return {base, page, row, of_lane, page >= 0 && row >= 0 && page < (int64_t(1) << 31) && row < (int64_t(1) << 31) && (int64_t)a.pages * page + a.page_rows * row < (int64_t(1) << 32)};
+    if (a.tables == nullptr) return {base + b * page, 0, row, of_lane, row >= 0 && a.places * row < (int64_t(1) << 31), (uint32_t)(a.D * H::kElement)};
+    return {base, page, row, of_lane, page >= 0 && row >= 0 && page < (int64_t(1) << 31) && row < (int64_t(1) << 31) && (int64_t)a.pages * page + a.page_rows * row < (int64_t(1) << 32), (uint32_t)(a.D * H::kElement)};
 }
 
-// Whether the rows of every instruction's copies (of four, where it has fewer) lie in one page, at distances that 32 bits hold, and fill the kernel's: then their address is one of the
-// wavefront's and an offset.
+// Whether the rows of every instruction's copies (of four, where it has fewer) lie in one page, at distances that 32 bits hold: then their address is one of the wavefront's and an offset.
 template <typename H>
 __device__ __forceinline__ bool in_runs(const AttentionArgs& a) {
     constexpr int32_t kRows = 64 / H::kChunks < 4 ? 4 : 64 / H::kChunks;
-    return a.k_whole && (a.tables == nullptr || a.page_rows % kRows == 0) && a.D * H::kElement == H::kRow && a.k_row >= 0 && a.k_row < (1 << 24) && a.v_row >= 0 && a.v_row < (1 << 24);
+    return a.k_whole && (a.tables == nullptr || a.page_rows % kRows == 0) && a.k_row >= 0 && a.k_row < (1 << 24) && a.v_row >= 0 && a.v_row < (1 << 24);
 }
 
-// The same for places anywhere: kCount copies from the first-th of the tile on.  What is not there is 0.
+// kCount copies from the first-th of the tile on, for places anywhere.  What is not there, and what a row has less than the kernel's, is 0.
 template <typename H, int kPlaces, int kCount>
 __device__ __forceinline__ void copy_rows(const AttentionArgs& a, const From& f, const Places<kPlaces>& places, uint32_t lds, char* to, int32_t first) {
-    constexpr int kRows = 64 / H::kChunks;
+    constexpr int kRows = 64 / H::kChunks, kAtOnce = 2;
+    static_assert(kCount % kAtOnce == 0 || kCount < kAtOnce, "whole rounds");
     const int lane = threadIdx.x & 63;
     const int32_t row_bytes = a.D * H::kElement;
 #pragma unroll 1
-    for (int j = 0; j < kCount; ++j) {
-        const int32_t i = first + j, row = i * kRows + lane / H::kChunks, c = ((lane % H::kChunks) ^ H::turned(row)) << 4;
-        const int32_t page = __shfl(places.at.page, row), at = __shfl(places.at.row, row);
-        const char* from = f.base + page * f.page + at * f.row;
+    for (int j0 = 0; j0 < kCount; j0 += kAtOnce) {
+        const char* from[kAtOnce];
+        int32_t c[kAtOnce];
+        bool there[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce && j < kCount; ++j) {
+            const int32_t row = (first + j0 + j) * kRows + lane / H::kChunks, page = __shfl(places.at.page, row), at = __shfl(places.at.row, row);
+            c[j] = ((lane % H::kChunks) ^ H::turned(row)) << 4;
+            there[j] = page >= 0;
+            from[j] = f.base + page * f.page + at * f.row;
+        }
         if (a.k_whole) {
-            copy_to_lds(page >= 0 && c < row_bytes ? from + c : reinterpret_cast<const char*>(kZeros), lds + i * 1024);
+#pragma unroll
+            for (int j = 0; j < kAtOnce && j < kCount; ++j) copy_to_lds((there[j] & (c[j] < row_bytes)) ? from[j] + c[j] : reinterpret_cast<const char*>(kZeros), lds + (first + j0 + j) * 1024);
         } else {
-            u32x4 v = {0, 0, 0, 0};
-            if (page >= 0) v = chunk_of<H::kElement == 2>(from, c, row_bytes, false);
-            *reinterpret_cast<u32x4*>(to + i * 1024 + lane * 16) = v;
+            u32x4 v[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce && j < kCount; ++j) v[j] = chunk_of<H::kElement == 2>(from[j], c[j], row_bytes, false, there[j]);
+#pragma unroll
+            for (int j = 0; j < kAtOnce && j < kCount; ++j) *reinterpret_cast<u32x4*>(to + (first + j0 + j) * 1024 + lane * 16) = v[j];
         }
     }
 }
@@ -541,17 +573,26 @@ template <typename H, int kCount, typename R>
 __device__ __forceinline__ void copy_runs(const From& f, const R& runs, uint32_t lds, int32_t first) {
     constexpr int kRows = 64 / H::kChunks;
     const int lane = threadIdx.x & 63;
-    auto all = [&](auto near) __attribute__((always_inline)) {
+    auto all = [&](auto simple) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kCount; ++j) {
             const int32_t row = (first + j) * kRows + lane / H::kChunks, page = runs.page[j * kRows / R::kRun], at = runs.row[j * kRows / R::kRun] + j * kRows % R::kRun;
-            const uint32_t of_lane = f.of_lane + (((lane % H::kChunks) ^ H::turned(row)) << 4);
-            if constexpr (decltype(near)::value) copy_to_lds(of_lane + ((uint32_t)page * (uint32_t)f.page + (uint32_t)at * (uint32_t)f.row), f.base, lds + (first + j) * 1024);
-            else copy_to_lds(of_lane, f.base + page * f.page + at * f.row, lds + (first + j) * 1024);
+            const uint32_t c = ((lane % H::kChunks) ^ H::turned(row)) << 4;
+            // (rows that are shorter than the kernel's leave the rest as it is, which is 0)
+            if constexpr (decltype(simple)::value) copy_to_lds(f.of_lane + c + ((uint32_t)page * (uint32_t)f.page + (uint32_t)at * (uint32_t)f.row), f.base, lds + (first + j) * 1024);
+            else copy_to_lds(f.of_lane + c, f.base + page * f.page + at * f.row, lds + (first + j) * 1024, __builtin_amdgcn_ballot_w64(c < f.bytes));
         }
     };
-    if (f.near) all(std::true_type());
+    if (f.near && f.bytes == H::kRow) all(std::true_type());
     else all(std::false_type());
+}
+
+// Zeros where rows that are shorter than the kernel's do not come.
+template <typename H>
+__device__ __forceinline__ void clear_rest(const AttentionArgs& a, char* lds, int32_t bytes, int32_t thread, int32_t threads) {
+    if (a.D * H::kElement == H::kRow) return;
+    for (int32_t i = thread; i < bytes / 16; i += threads) reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // ---- results ----------------------------------------------------------------------------------------------------------
@@ -687,6 +728,10 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     u32x4 q[H::kSteps];
     load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 32 * H::kRow, q);
     if (!a.q_whole) __syncthreads();  // (the tiles come where they lay)
+    if (a.D * H::kElement != H::kRow) {
+        clear_rest<H>(a, attention_lds, 2 * W::kBuffers * W::kBytes, threadIdx.x, 256);
+        __syncthreads();
+    }
     const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b), v = from_of<H>(a, a.v + job.group * a.v_head, a.v_page, a.v_row, job.b);
     const bool runs = in_runs<H>(a);
     const uint32_t lds = lds_address(attention_lds);
@@ -786,6 +831,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     const Row row = row_of(a, job, job.row_tile * 32);
     u32x4 q[H::kSteps];
     load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 2 * W::kBytes, q);
+    clear_rest<H>(a, attention_lds + wave * 2 * W::kBytes, 2 * W::kBytes, lane, 64);
     const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b), v = from_of<H>(a, a.v + job.group * a.v_head, a.v_page, a.v_row, job.b);
     const bool runs = in_runs<H>(a);
     char *keys = attention_lds + wave * 2 * W::kBytes, *values = keys + W::kBytes;
@@ -979,15 +1025,15 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b);
     const bool runs = in_runs<H>(a);
     char* keys = attention_lds + W::kOfRows + wave * W::kBytes;
+    clear_rest<H>(a, keys, W::kBytes, lane, 64);
     const uint32_t keys_at = lds_address(keys), before_at = lds_address(before) + wave * 256;
     const int32_t row_bytes = a.D * H::kElement, used = job.count * a.fan;
     for (int32_t r0 = 0; r0 < used; r0 += W::kRows) {
         __syncthreads();
         for (int32_t i = threadIdx.x; i < W::kRows * H::kChunks; i += W::kThreads) {
             const int32_t r = r0 + i / H::kChunks, c = i % H::kChunks, t = over(r, a.by_fan), head = job.group * a.fan + (r - t * a.fan);
-            u32x4 v = {0, 0, 0, 0};
-            if (r < used) v = chunk_of<kHalf>(a.q + job.b * a.q_batch + t * a.q_token + head * a.q_head, c * 16, row_bytes, a.q_whole);
-            reinterpret_cast<u32x4*>(attention_lds)[i / H::kChunks * H::kChunks + (c ^ H::turned(i / H::kChunks))] = v;
+            reinterpret_cast<u32x4*>(attention_lds)[i / H::kChunks * H::kChunks + (c ^ H::turned(i / H::kChunks))] =
+                chunk_of<kHalf>(a.q + job.b * a.q_batch + t * a.q_token + head * a.q_head, c * 16, row_bytes, a.q_whole, r < used);
         }
         static_assert(W::kRows <= W::kThreads, "a lane to a row");
         if (threadIdx.x < W::kRows) {
@@ -1057,12 +1103,13 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
                     seen = 0;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) seen |= (uint32_t)(p < limits[row + 8 * (i >> 2) + (i & 3)]) << i;
-                    const int32_t other = p - job.length;  // the node that lies there
-                    if (a.kind == kTree && other >= 0 && other < job.count) {
+                    if (a.kind == kTree && p0 + 32 > job.length) {
+                        const int32_t other = max(0, min(p - job.length, job.count - 1));  // the node that lies there
+                        const uint32_t is = (p >= job.length) & (p < job.end);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int32_t node = sees[row + 8 * (i >> 2) + (i & 3)];
-                            seen |= (node >= 0 ? (nodes->sees[node][other >> 5] >> (other & 31)) & 1 : 0) << i;
+                            seen |= (((nodes->sees[max(node, 0)][other >> 5] >> (other & 31)) & is & (uint32_t)(node >= 0)) << i);
                         }
                     }
                 }
@@ -1081,6 +1128,80 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
         }
     }
     // (places of a sequence without tokens stay as they are)
+}
+
+// The same where places are few and rows many: a work-group has 32 places, whose keys stay in registers, and its wavefronts share out the rows, 32 at a time; their sums are added in one order.
+template <bool kHalf, int kSize>
+struct MassRows {
+    static constexpr int kWaves = Head<kHalf, kSize>::kRow <= 512 ? 8 : 4, kThreads = 64 * kWaves;  // (the keys of 1024 bytes want all registers)
+    static constexpr int kLds = kWaves * 32 * 4;                                                   // (and nodes)
+};
+
+template <bool kHalf, int kSize>
+__global__ __launch_bounds__((MassRows<kHalf, kSize>::kThreads)) void attention_mass_rows_kernel(AttentionArgs a) {
+    using H = Head<kHalf, kSize>;
+    using W = MassRows<kHalf, kSize>;
+    constexpr int kWaves = W::kWaves;
+    extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
+    float* sums = reinterpret_cast<float*>(attention_lds);  // [wave][32]
+    Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + W::kLds);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    Job job;
+    const int32_t blocks = (a.places + 31) / 32, of = uniform((uint32_t)blockIdx.x / (uint32_t)blocks), p0 = (blockIdx.x - of * blocks) * 32, p = p0 + (lane & 31);
+    job.b = over(of, a.by_groups);
+    job.group = of - job.b * a.groups;
+    job.rows = a.T * a.fan;
+    job.length = length_of(a, job.b);
+    job.count = count_of(a, job.b);
+    job.end = min(job.length + job.count, a.places);
+    if (p0 >= job.end || job.count == 0) return;
+    if (a.kind == kTree && p0 + 32 > job.length) find_ancestors<W::kThreads>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
+    Place at = place_in(a, job.b, min(p, job.end - 1));
+    at.page = p < job.end ? at.page : -1;
+    const int32_t row_bytes = a.D * H::kElement, used = job.count * a.fan;
+    u32x4 k[H::kSteps];
+#pragma unroll
+    for (int s = 0; s < H::kSteps; ++s)
+        k[s] = chunk_of<kHalf>(a.k + at.page * a.k_page + at.row * a.k_row + job.group * a.k_head, (2 * s + half) * 16, row_bytes, a.k_whole, at.page >= 0);
+    float total = 0.f;
+    // (the rows of a chain that come before the first of these places do not see them)
+    const int32_t first = (a.kind == kChain ? max(0, p0 - job.length) : 0) * a.fan / 32 * 32;
+    for (int32_t r0 = first + wave * 32; r0 < used; r0 += kWaves * 32) {
+        const int32_t r = min(r0 + (lane & 31), used - 1), t = over(r, a.by_fan), head = job.group * a.fan + (r - t * a.fan);
+        const char* from = a.q + job.b * a.q_batch + t * a.q_token + head * a.q_head;
+        const float mine = a.sums[(int64_t)of * job.rows + r];
+        f32x16 score = {};
+        constexpr int kAhead = 8;  // (of 256 elements of float32 the keys alone take half of the registers)
+        u32x4 q[kAhead + 1];
+        in_steps<H::kSteps, kAhead>([&](int s) __attribute__((always_inline)) { q[s % (kAhead + 1)] = chunk_of<kHalf>(from, (2 * s + half) * 16, row_bytes, a.q_whole); },
+                                    [&](int s) __attribute__((always_inline)) { score = score_of<kHalf>(q[s % (kAhead + 1)], k[s], score); });
+        const bool plain = p0 + 32 <= job.length && r0 + 32 <= used, trees = a.kind == kTree && p0 + 32 > job.length;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int at_row = 8 * (i >> 2) + 4 * half + (i & 3);
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i], a.scale2, -__shfl(mine, at_row)));
+            uint32_t seen = 1;
+            if (!plain) {
+                const int32_t token = __shfl(t, at_row);
+                seen = p < (a.kind == kChain ? job.length + token + 1 : job.length);
+                if (trees) {
+                    const int32_t other = max(0, min(p - job.length, job.count - 1));  // the node that lies there
+                    seen |= (nodes->sees[token][other >> 5] >> (other & 31)) & (uint32_t)(p >= job.length);
+                }
+                seen &= (uint32_t)(r0 + at_row < used) & (uint32_t)(p < job.end);
+            }
+            total += seen ? w : 0.f;
+        }
+    }
+    total = sum_of_halves(total);
+    if (half == 0) sums[wave * 32 + lane] = total;
+    __syncthreads();
+    if (threadIdx.x >= 32 || at.page < 0) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += sums[w * 32 + lane];
+    float* to = a.mass + job.b * a.mass_batch + job.group * a.mass_head + p;
+    *to = (p < job.length ? *to : 0.f) + sum;
 }
 
 template <bool kHalf, int kSize>
@@ -1104,7 +1225,13 @@ template <bool kHalf, int kSize>
 int mass_of(const AttentionArgs& a, hipStream_t s) {
     using W = Mass<kHalf, kSize>;
     // Runs of places: as many as give each compute unit two work-groups, of at least 128 places (a block to each wavefront).
-    const int64_t groups = (int64_t)a.B * a.groups, most = ((int64_t)a.places + 127) / 128;
+    const int64_t groups = (int64_t)a.B * a.groups, most = ((int64_t)a.places + 127) / 128, blocks = ((int64_t)a.places + 31) / 32;
+    // us of attention with mass, by places / by rows: 2 x 883 tokens x 4 rows of 4 heads over 1 place 243 / 90, 2048 x 4 of 8 over 1 467 / 223, 512 x 4 of 8 over 2000 156 / 116, but 2 x 256 x 4 of 8 over 4000
+    // (544 work-groups by places) 150 / 163.
+    if (groups * most < 256 && (int64_t)a.T * a.fan > 128) {
+        attention_mass_rows_kernel<kHalf, kSize><<<(unsigned)(groups * blocks), MassRows<kHalf, kSize>::kThreads, MassRows<kHalf, kSize>::kLds + nodes_bytes(a), s>>>(a);
+        return launch_check("attention_mass_rows_kernel");
+    }
     int64_t runs = (512 + groups - 1) / groups;
     runs = runs > most ? most : runs;
     auto kernel = attention_mass_kernel<kHalf, kSize>;
