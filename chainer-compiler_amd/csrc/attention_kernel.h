@@ -447,19 +447,28 @@ __device__ __forceinline__ void add_up(f32x16 (&acc)[kBlocks], Pass pass, Any an
 
 // ---- rows of k and v into LDS ---------------------------------------------------------------------------------------
 
-// Asynchronous copies of 16 bytes a lane into LDS, lane i's to lds + 16 i (the same for all lanes), counted like loads.  (Where the base's scalar registers come from a vector instruction, as a
-// v_readlane, five cycles have to pass before a memory instruction reads them, and the compiler does not see that this is one.)
+// Asynchronous copies of 16 bytes a lane into LDS, lane i's to lds + 16 i (the same for all lanes), counted like loads.  (The base goes through a scalar instruction: where the compiler has it from a vector
+// one, as a v_readlane, five cycles would have to pass before a memory instruction reads it, and it does not see that this is one.  Waiting them out in each copy: 599 us of 2048 x 4096 rows, so 594.)
 __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(uniform(lds)) : "memory", "m0");
+    const char* from;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0" : "=&s"(from) : "v"(offset), "s"(base), "s"(uniform(lds)) : "memory", "m0");
 }
 // (Of some lanes only; all of them are there.)
 __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds, uint64_t lanes) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b64 exec, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" : : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0");
+    const char* from;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dwordx4 %1, %0\n\ts_mov_b64 exec, -1"
+                 : "=&s"(from) : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0");
 }
 __device__ __forceinline__ void copy_to_lds(const char* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
 }
-__device__ __forceinline__ void copy_number_to_lds(const float* from, uint32_t lds) {  // 4 bytes a lane, lane i's to lds + 4 i
+// (4 bytes a lane, lane i's to lds + 4 i.)
+__device__ __forceinline__ void copy_number_to_lds(uint32_t offset, const char* base, uint32_t lds, uint64_t lanes) {
+    const char* from;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dword %1, %0\n\ts_mov_b64 exec, -1"
+                 : "=&s"(from) : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0");
+}
+__device__ __forceinline__ void copy_number_to_lds(const float* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
 }
 
@@ -483,19 +492,20 @@ struct From {
     uint32_t of_lane;  // how far the lane's row is from the first one of an instruction
     bool near;         // every row is less than 4 GB behind base
     uint32_t bytes;    // of a row
+    bool whole;        // rows and their distances are whole pieces of 16 bytes
 };
 template <typename H>
 __device__ __forceinline__ From from_of(const AttentionArgs& a, const char* base, int64_t page, int64_t row, int32_t b) {
     const uint32_t of_lane = (uint32_t)((threadIdx.x & 63) / H::kChunks * row);
-    if (a.tables == nullptr) return {base + b * page, 0, row, of_lane, row >= 0 && a.places * row < (int64_t(1) << 31), (uint32_t)(a.D * H::kElement)};
-    return {base, page, row, of_lane, page >= 0 && row >= 0 && page < (int64_t(1) << 31) && row < (int64_t(1) << 31) && (int64_t)a.pages * page + a.page_rows * row < (int64_t(1) << 32), (uint32_t)(a.D * H::kElement)};
+    if (a.tables == nullptr) return {base + b * page, 0, row, of_lane, row >= 0 && a.places * row < (int64_t(1) << 31), (uint32_t)(a.D * H::kElement), a.k_whole};
+    return {base, page, row, of_lane, page >= 0 && row >= 0 && page < (int64_t(1) << 31) && row < (int64_t(1) << 31) && (int64_t)a.pages * page + a.page_rows * row < (int64_t(1) << 32), (uint32_t)(a.D * H::kElement), a.k_whole};
 }
 
 // Whether the rows of every instruction's copies (of four, where it has fewer) lie in one page, at distances that 32 bits hold: then their address is one of the wavefront's and an offset.
 template <typename H>
 __device__ __forceinline__ bool in_runs(const AttentionArgs& a) {
     constexpr int32_t kRows = 64 / H::kChunks < 4 ? 4 : 64 / H::kChunks;
-    return a.k_whole && (a.tables == nullptr || a.page_rows % kRows == 0) && a.k_row >= 0 && a.k_row < (1 << 24) && a.v_row >= 0 && a.v_row < (1 << 24);
+    return (a.k_whole || H::kElement == 4) && (a.tables == nullptr || a.page_rows % kRows == 0) && a.k_row >= 0 && a.k_row < (1 << 24) && a.v_row >= 0 && a.v_row < (1 << 24);
 }
 
 // kCount copies from the first-th of the tile on, for places anywhere.  What is not there, and what a row has less than the kernel's, is 0.
@@ -583,8 +593,19 @@ __device__ __forceinline__ void copy_runs(const From& f, const R& runs, uint32_t
             else copy_to_lds(f.of_lane + c, f.base + page * f.page + at * f.row, lds + (first + j) * 1024, __builtin_amdgcn_ballot_w64(c < f.bytes));
         }
     };
-    if (f.near && f.bytes == H::kRow) all(std::true_type());
-    else all(std::false_type());
+    if (f.near && f.whole && f.bytes == H::kRow) all(std::true_type());
+    else if (H::kElement == 2 || f.whole) all(std::false_type());
+    else {
+        // Rows of float32 that are not whole pieces, by their elements: the same bytes in four times the copies.
+        int32_t place = lane;
+        asm volatile("" : "+v"(place));  // (the addresses are made where they are used, and not kept in registers)
+#pragma unroll
+        for (int j = 0; j < 4 * kCount; ++j) {
+            const int32_t row = first * kRows + j * 256 / H::kRow;
+            const uint32_t c = ((place >> 2 | (j * 16 & (H::kChunks - 1))) ^ H::turned(row)) << 4 | (place & 3) << 2;
+            copy_number_to_lds(c, f.base + runs.page[j * 256 / H::kRow / R::kRun] * f.page + (runs.row[j * 256 / H::kRow / R::kRun] + j * 256 / H::kRow % R::kRun) * f.row, lds + first * 1024 + j * 256, __builtin_amdgcn_ballot_w64(c < f.bytes));
+        }
+    }
 }
 
 // Zeros where rows that are shorter than the kernel's do not come.
@@ -1204,16 +1225,21 @@ __global__ __launch_bounds__((MassRows<kHalf, kSize>::kThreads)) void attention_
     *to = (p < job.length ? *to : 0.f) + sum;
 }
 
+// More than 64 KB has to be asked for, on every device: always for the largest tree, so that threads that call at once ask for the same.
+inline int ask_for_lds(const void* kernel, int lds) {
+    if (lds + (int)sizeof(Nodes) > 65536) CHX_HIP_CALL(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds + (int)sizeof(Nodes)));
+    return CHX_HIP_OK;
+}
+
 template <bool kHalf, int kSize>
 int attend_of(const AttentionArgs& a, hipStream_t s) {
     using W = Tile<kHalf, kSize>;
     using F = Few<kHalf, kSize>;
     const bool few = a.tile_rows == 32;
     auto kernel = few ? attention_places_kernel<kHalf, kSize> : attention_rows_kernel<kHalf, kSize>;
-    const int lds = (few ? F::kLds : W::kLds) + nodes_bytes(a);
-    if (lds > 65536)  // (has to be asked for, on every device)
-        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    kernel<<<(unsigned)((int64_t)a.B * a.groups * a.parts * a.row_tiles), few ? 64 * F::kWaves : 256, lds, s>>>(a);
+    const int lds = few ? F::kLds : W::kLds;
+    CHX_PROPAGATE(ask_for_lds(reinterpret_cast<const void*>(kernel), lds));
+    kernel<<<(unsigned)((int64_t)a.B * a.groups * a.parts * a.row_tiles), few ? 64 * F::kWaves : 256, lds + nodes_bytes(a), s>>>(a);
     return launch_check(few ? "attention_places_kernel" : "attention_rows_kernel");
 }
 template <bool kHalf, int kSize>
@@ -1235,10 +1261,8 @@ int mass_of(const AttentionArgs& a, hipStream_t s) {
     int64_t runs = (512 + groups - 1) / groups;
     runs = runs > most ? most : runs;
     auto kernel = attention_mass_kernel<kHalf, kSize>;
-    const int lds = W::kLds + nodes_bytes(a);
-    if (lds > 65536)  // (has to be asked for, on every device)
-        CHX_HIP_CALL(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    kernel<<<(unsigned)(groups * runs), W::kThreads, lds, s>>>(a, (int32_t)runs);
+    CHX_PROPAGATE(ask_for_lds(reinterpret_cast<const void*>(kernel), W::kLds));
+    kernel<<<(unsigned)(groups * runs), W::kThreads, W::kLds + nodes_bytes(a), s>>>(a, (int32_t)runs);
     return launch_check("attention_mass_kernel");
 }
 
