@@ -87,7 +87,7 @@ int run(AttentionArgs& a, const chx_hip_tensor* q, const chx_hip_tensor* keys, c
         chx_hip_tensor* y, void* workspace, size_t workspace_bytes, hipStream_t s, const char* what) {
     CHX_PROPAGATE(check_rows(y, 4, q->dtype, what, "y"));
     CHX_REQUIRE(same_shape(*q, *y), "%s: y must have q's shape", what);
-    CHX_REQUIRE(elements_apart(*y), "%s: elements of y overlap", what);
+    CHX_REQUIRE(numel(*y) == 0 || elements_apart(*y), "%s: elements of y overlap", what);
     CHX_PROPAGATE(check_apart({y, "y"}, read, reads, what));
     a.scale2 = scale * 1.44269504f;
     CHX_REQUIRE(scale > 0.f && a.scale2 > 0.f && std::isfinite(a.scale2), "%s: the scale must be a positive number", what);

@@ -118,9 +118,9 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a, int64_t
     const int64_t bt = row / a.c.groups;
     const int32_t h = (int32_t)(row - bt * a.c.groups), b = (int32_t)(bt / a.T), t = (int32_t)(bt - (int64_t)b * a.T);
     if (a.counts && t >= a.counts[b]) return;
-    const int64_t p = (int64_t)a.c.lengths[b] + t;
-    if (p < 0 || p >= a.c.places) return;
-    const Place at = place_of(a.c, b, (int32_t)p);
+    const int32_t p = clamped(a.c.lengths[b], a.c.places) + t;  // (both below 2^30)
+    if (p >= a.c.places) return;
+    const Place at = place_of(a.c, b, p);
     if (at.page < 0) return;
     const Unit k = reinterpret_cast<const Unit*>(a.k + b * a.k_batch + t * a.k_token + h * a.k_head)[u];
     const Unit v = reinterpret_cast<const Unit*>(a.v + b * a.v_batch + t * a.v_token + h * a.v_head)[u];
@@ -521,7 +521,7 @@ int check_moves(const chx_hip_tensor* keys, const chx_hip_tensor* values, const 
                 const chx_hip_tensor* mass, const chx_hip_tensor* new_lengths, const char* what, MoveArgs* a) {
     memset(a, 0, sizeof(*a));
     CHX_PROPAGATE(check_cache(keys, values, tables, lengths, what, &a->c));
-    CHX_REQUIRE(elements_apart(*keys) && elements_apart(*values), "%s: elements of keys or values overlap", what);
+    CHX_REQUIRE(numel(*keys) == 0 || (elements_apart(*keys) && elements_apart(*values)), "%s: elements of keys or values overlap", what);
     if (mass) {
         CHX_PROPAGATE(check_mass(mass, a->c, what));
         a->mass = static_cast<float*>(mass->data);
@@ -559,7 +559,7 @@ extern "C" int chx_hip_cache_append(
     AppendArgs a;
     memset(&a, 0, sizeof(a));
     CHX_PROPAGATE(check_cache(keys, values, tables, lengths, what, &a.c));
-    CHX_REQUIRE(elements_apart(*keys) && elements_apart(*values), "%s: elements of keys or values overlap", what);
+    CHX_REQUIRE(numel(*keys) == 0 || (elements_apart(*keys) && elements_apart(*values)), "%s: elements of keys or values overlap", what);
     CHX_PROPAGATE(check_rows(k, 4, keys->dtype, what, "k"));
     CHX_PROPAGATE(check_rows(v, 4, keys->dtype, what, "v"));
     CHX_REQUIRE(same_shape(*k, *v) && k->shape[0] == a.c.B && k->shape[2] == a.c.groups && k->shape[3] == a.c.D, "%s: k and v must be [sequences, tokens, heads, elements] as the cache has them", what);
@@ -610,6 +610,7 @@ extern "C" int chx_hip_cache_evict_workspace(int64_t sequences, int64_t heads, i
     CHX_REQUIRE(bytes != nullptr, "cache evict: null output");
     CHX_REQUIRE(sequences >= 0 && heads >= 0 && places >= 0 && sequences < (int64_t(1) << 24) && heads < (int64_t(1) << 16) && places < (int64_t(1) << 30), "cache evict: numbers of a cache out of range");
     CHX_REQUIRE(keep >= 0, "cache evict: keep is negative");
+    CHX_REQUIRE(sequences * heads < (int64_t(1) << 22), "cache evict: more sequences and heads than one launch has");
     *bytes = (size_t)evict_workspace(sequences, heads, places, keep);
     return CHX_HIP_OK;
 }
