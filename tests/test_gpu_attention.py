@@ -393,6 +393,84 @@ def test_a_pool_of_more_than_4_gib(g):
     close(got[0], want, room)
 
 
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("D,R,gap", [(80, 16, 8), (96, 8, 0), (192, 20, 16), (75, 16, 0), (75, 20, 3), (201, 64, 0), (40, 16, 8), (33, 8, 1), (3, 16, 0), (128, 1, 8)])
+@pytest.mark.parametrize("B,H,G,T,lengths", [(2, 4, 2, 3, [700, 333]), (1, 4, 1, 2, [4000]), (4, 16, 8, 300, [0, 200, 333, 64])])
+def test_rows_that_do_not_fill_a_tile(g, dtype, D, R, gap, B, H, G, T, lengths):
+    """What lies behind a row, here NaN, is no part of it, in whole tiles as in those that a sequence ends in; and results are the same each time."""
+    cache = Cache(80, dtype, B, G, D, R, lengths, T, gap=gap)
+    q = normal(81, (B, T, H, D), dtype, 2.0)
+    mass = torch.zeros(B, G, cache.tables.shape[1] * R, device="cuda")
+    got = check_tree(g, cache, q, None if T > 256 else tree_of(82, B, T), mass=mass)
+    for _ in range(3):
+        again = torch.zeros_like(mass)
+        assert torch.equal(got, g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths, parents=None if T > 256 else tree_of(82, B, T), mass=again))
+        assert torch.equal(mass, again)
+
+
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("D", [64, 75, 128, 256])
+@pytest.mark.parametrize("tree", [False, True])
+def test_mass_of_many_rows(g, dtype, D, tree):
+    """By rows where places are few, by places, in several rounds of rows, where they are many; sequences with fewer tokens than the batch."""
+    for B, G, H, T, lengths, counts in ((4, 1, 2, 200, [0, 300, 31, 95], [200, 77, 0, 129]), (4, 8, 16, 90, [1100, 0, 1500, 700], [90, 90, 33, 0])):
+        cache = Cache(83, dtype, B, G, D, 16, lengths, T)
+        mass = torch.rand((B, G, cache.tables.shape[1] * 16), generator=torch.Generator().manual_seed(84)).cuda()
+        check_tree(g, cache, normal(85, (B, T, H, D), dtype, 2.0), tree_of(86, B, T) if tree else None, numbers(counts), mass=mass)
+
+
+def test_places_that_are_not_seen_weigh_nothing(g):
+    """A key that no row sees, of another branch's node or of a page that is none, gets no mass, and a NaN there none."""
+    cache = Cache(87, HALF, 1, 1, 64, 16, [40], 150)
+    parents = torch.full((1, 150), -1, dtype=torch.int32, device="cuda")
+    cache.tables[0, 1] = cache.keys.shape[0]
+    mass = torch.full((1, 1, cache.tables.shape[1] * 16), 3.0, device="cuda")
+    q = normal(88, (1, 150, 2, 64), HALF)
+    got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths, parents=parents, mass=mass)
+    assert torch.isfinite(got).all() and torch.isfinite(mass).all()
+    assert (mass[0, 0, 16:32] == 3).all() and (mass[0, 0, 190:] == 3).all()
+    total = (mass[0, 0, :190].sum() - 3.0 * 40).item()  # each of 300 rows weighs 1, off by 2^-11 of a weight
+    assert abs(total - 300.0) < 300 * 2.0 ** -10
+
+
+def test_threads(g):
+    """Calls of different kernels from threads at once, each on a stream of its own."""
+    import threading
+    calls, want, got = [], [], {}
+    for i, (dtype, D, T, n) in enumerate(((HALF, 128, 1, 900), (FLOAT, 256, 2, 300), (HALF, 64, 256, 100), (FLOAT, 64, 40, 500))):
+        cache = Cache(90 + i, dtype, 1, 2, D, 16, [n], T)
+        calls.append((normal(95 + i, (1, T, 4, D), dtype), cache.keys, cache.values, cache.tables, cache.lengths, tree_of(99 + i, 1, T)))
+        want.append(g.ops.TreeAttention(*calls[-1]))
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i] = [g.ops.TreeAttention(*calls[i]) for _ in range(20)]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(one, want[i]) for i in range(4) for one in got[i])
+
+
+@pytest.mark.parametrize("dtype,D,P", [(HALF, 96, 12000), (FLOAT, 75, 7200)])
+def test_short_rows_in_a_pool_of_more_than_4_gib(g, dtype, D, P):
+    keys, values = (torch.zeros(P, 256, 8, D, dtype=dtype, device="cuda") for _ in range(2))
+    tables = numbers([[P - 1, 0, P - 500]])
+    k, v = normal(63, (1, 600, 8, D), dtype), normal(64, (1, 600, 8, D), dtype)
+    g.ops.CacheAppend(keys, values, k, v, tables, numbers([0]))
+    q = normal(65, (1, 1, 16, D), dtype, 2.0)
+    mass = torch.zeros(1, 8, 768, device="cuda")
+    got = g.ops.TreeAttention(q, keys, values, tables, numbers([599]), mass=mass)
+    want, room, weights, weights_room = attend(q[0].cpu(), k[0].cpu(), v[0].cpu(), torch.ones(1, 600, dtype=torch.bool), D ** -0.5)
+    close(got[0], want, room)
+    close(mass[0, :, :600], weights, weights_room + 2.0 ** -24 * weights)
+
+
 # ---- an encoder's states ----------------------------------------------------------------------------
 
 def check_cross(g, q, k, v, lengths=None, scale=None, out=None):

@@ -60,7 +60,7 @@ LAYOUTS = [(HALF, 16, 2, 128, "prgd", 0), (HALF, 1, 3, 80, "prgd", 0), (FLOAT, 2
 @pytest.mark.parametrize("dtype,R,G,D,layout,gap", LAYOUTS)
 @pytest.mark.parametrize("T", [1, 37])
 def test_append(g, dtype, R, G, D, layout, gap, T):
-    """Counts of none, some and too many; places before, over and behind the table's end; pages that are none.  All else stays as it is."""
+    """Counts of none, some and too many; lengths below 0 (as 0), over and behind the table's end; pages that are none.  All else stays as it is."""
     B, M = 6, -(-60 // R)
     p = Pages(1, dtype, B, M, R, G, D, layout, gap)
     p.tables[1, 0], p.tables[1, M - 1] = -1, p.keys.shape[0]
@@ -71,7 +71,7 @@ def test_append(g, dtype, R, G, D, layout, gap, T):
         want = p.copy()
         for b in range(B):
             for t in range(T if counts is None else min(T, int(counts[b]))):
-                at = p.at(b, int(lengths[b]) + t)
+                at = p.at(b, max(0, min(int(lengths[b]), p.places)) + t)
                 if at:
                     want[0][at], want[1][at] = k[b, t].cpu(), v[b, t].cpu()
         assert g.ops.CacheAppend(p.keys, p.values, k, v, p.tables, lengths, counts=counts) is None
