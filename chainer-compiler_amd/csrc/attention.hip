@@ -22,8 +22,25 @@ namespace {
 // So: 128 from as many tiles on as there are compute units (half as many where a tile is much work), a tile of many places counted as several; in float32, whose products take the time, not
 // where half of the rows are empty.
 //
-// Parts: as many as give each compute unit two work-groups (float32, whose products take the time: little more than one), of at least 256 places each (float32: 128).  One token of 8 sequences, 2000 places, 8 heads of 128 elements: 1 part 38 us, 2 27, 4 20, 8 17, 12
-// 23; of one sequence of 32,768: 8 80, 24 40, 32 38, 64 40.
+// Parts: as many as fill the compute units once, two work-groups to each (one where rows are longer than 256 bytes and the tiles take more than half of LDS), of at least 256 places each (float32: 128);
+// where they would have 4096 or more, several times as many, up to four, so that the units are even where sequences are not (where they are, 4 x 32768 places of 8 heads cost 118 us in 16, 125 in 32).  us of one token by parts, 8 heads of k and v:
+//                                              1     2     4     8     12    16    24    32    64
+//   float16, 128 elements,  8 of 2000          38    27    20    17    23
+//                           1 of 32768               (8: 80)                     40    38    40
+//            256 elements,  8 of 4000          89    58    43    47    52    60
+//                           2 of 30000         569   303   170   108   97    94    107   102   117
+//   float32, 64 elements,   8 of 4000          103   61    37    31    38    36    42    43
+//            128 elements,  8 of 4000          171   98    60    63    67    71    81    88
+//                           2 of 20000         786   405   214   116   89    72    85    73    89
+//            192 elements, 5 of 60215, 4 heads       7189  3620  1830  1239  1172  1034  925   809
+// One part, and no launch that joins them, where parts would be short: float16 below 1024 places, and below 2048 where whole sequences nearly fill the units.  us of 1 part / 2 / 4, 64 elements:
+//                                              577 places      1500            4000
+//   float16, 96 work-groups                    13 / 16 / 16    19 / 17 / 16
+//            192                               12 / 14 / 14    19 / 18 / 18    41 / 33 / 29
+//            252                               12 / 19 / 19    18 / 22 / 26    33 / 30 / 32
+//   float32, 96                                23 / 19 / 19    44 / 31 / 26
+//            192                               25 / 23 / 29    45 / 37 / 39    108 / 76 / 69
+//            252                               25 / 31 / 39    43 / 46 / 51    93 / 87 / 92
 void share_out(AttentionArgs* a, bool half) {
     const int64_t rows = (int64_t)a->T * a->fan, sets = (int64_t)a->B * a->groups, tiles = (rows + 127) / 128;
     const int size = attention_size(a->D);
@@ -35,8 +52,10 @@ void share_out(AttentionArgs* a, bool half) {
     a->tile_rows = few ? 32 : 128;
     a->row_tiles = (int32_t)((rows + a->tile_rows - 1) / a->tile_rows);
     const int64_t groups = sets * a->row_tiles, least = half ? 256 : 128, most = (a->places + least - 1) / least;
-    int64_t parts = (half ? 512 : 320) / (groups < 1 ? 1 : groups);
+    int64_t parts = (size * (half ? 2 : 4) <= 256 ? 512 : 256) / (groups < 1 ? 1 : groups);
+    if (parts > 0) parts *= a->places / parts / 2048 < 1 ? 1 : a->places / parts / 2048 > 4 ? 4 : a->places / parts / 2048;
     parts = parts > most ? most : parts;
+    if (a->places < (groups > 224 ? 2048 : half ? 1024 : 0)) parts = 1;
     a->parts = (int32_t)(parts < 1 ? 1 : parts > kMostParts ? kMostParts : parts);
 }
 
