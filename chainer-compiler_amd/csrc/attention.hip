@@ -209,7 +209,7 @@ extern "C" int chx_hip_tree_attention(
     if (mass) {
         CHX_PROPAGATE(check_mass(mass, c, what));
         CHX_PROPAGATE(check_apart({mass, "mass"}, read, 7, what));
-        CHX_REQUIRE((int64_t)a.B * a.groups * ((a.places + 127) / 128) < (int64_t(1) << 23), "%s: more places than one launch has", what);
+        CHX_REQUIRE((int64_t)a.B * a.groups * ((a.places + 31) / 32) < (int64_t(1) << 24), "%s: more places than one launch has", what);
         a.mass = static_cast<float*>(mass->data);
         a.mass_batch = mass->strides[0] / 4;
         a.mass_head = mass->strides[1] / 4;

@@ -1151,24 +1151,34 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
     // (places of a sequence without tokens stay as they are)
 }
 
-// The same where places are few and rows many: a work-group has 32 places, whose keys stay in registers, and its wavefronts share out the rows, 32 at a time; their sums are added in one order.
-template <bool kHalf, int kSize>
+// The same of many rows: a work-group has the keys of a few blocks of places in LDS, and its wavefronts go over the rows, every fourth 32 of them, with scores as in the first pass: a lane has one row, whose
+// m + log2(l) is one number, and adds up the places' weights over its rows in registers; lanes and wavefronts are added at the end, in one order.  Bound by the exponentials, one to a score.
+template <bool kHalf, int kSize, int kBlocks>
 struct MassRows {
-    static constexpr int kWaves = Head<kHalf, kSize>::kRow <= 512 ? 8 : 4, kThreads = 64 * kWaves;  // (the keys of 1024 bytes want all registers)
-    static constexpr int kLds = kWaves * 32 * 4;                                                   // (and nodes)
+    static constexpr int kWaves = 4, kPlaces = 32 * kBlocks;
+    static constexpr int kBytes = kPlaces * Head<kHalf, kSize>::kRow;
+    static constexpr int kLookUp = kPlaces < 64 ? kPlaces : 64;   // places that a wavefront looks up at once, where they do not come in runs
+    static constexpr int kSums = kWaves * kPlaces * 4;
+    static constexpr int kLds = kBytes + kSums;  // (and nodes)
 };
-
+// Blocks of a work-group: rows of q are read once for all of them.
 template <bool kHalf, int kSize>
-__global__ __launch_bounds__((MassRows<kHalf, kSize>::kThreads)) void attention_mass_rows_kernel(AttentionArgs a) {
+constexpr int kMassBlocks = Head<kHalf, kSize>::kRow <= 256 ? 4 : Head<kHalf, kSize>::kRow <= 512 ? 2 : 1;
+
+template <bool kHalf, int kSize, int kBlocks>
+__global__ __launch_bounds__(256, (Head<kHalf, kSize>::kRow <= 512 ? 2 : 1)) void attention_mass_rows_kernel(AttentionArgs a, int32_t tiles) {
     using H = Head<kHalf, kSize>;
-    using W = MassRows<kHalf, kSize>;
-    constexpr int kWaves = W::kWaves;
+    using W = MassRows<kHalf, kSize, kBlocks>;
+    constexpr int kOfWave = W::kPlaces / W::kWaves, kParts = W::kPlaces / W::kLookUp;
     extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
-    float* sums = reinterpret_cast<float*>(attention_lds);  // [wave][32]
-    Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + W::kLds);
+    float* sums = reinterpret_cast<float*>(attention_lds + W::kBytes);  // [wave][place]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + W::kLds);
+    // (all tiles of a head of k on one XCD, whose L2 then has its rows of q)
+    const int32_t whole_sets = a.B * a.groups / 8 * 8;
+    const uint32_t whole = (uint32_t)whole_sets * (uint32_t)tiles, turn = blockIdx.x < whole ? blockIdx.x >> 3 : blockIdx.x - whole, of_turn = uniform(turn / (uint32_t)tiles);
+    const int32_t of = blockIdx.x < whole ? of_turn * 8 + (blockIdx.x & 7) : whole_sets + of_turn, p0 = (int32_t)(turn - of_turn * tiles) * W::kPlaces;
     Job job;
-    const int32_t blocks = (a.places + 31) / 32, of = uniform((uint32_t)blockIdx.x / (uint32_t)blocks), p0 = (blockIdx.x - of * blocks) * 32, p = p0 + (lane & 31);
     job.b = over(of, a.by_groups);
     job.group = of - job.b * a.groups;
     job.rows = a.T * a.fan;
@@ -1176,51 +1186,129 @@ __global__ __launch_bounds__((MassRows<kHalf, kSize>::kThreads)) void attention_
     job.count = count_of(a, job.b);
     job.end = min(job.length + job.count, a.places);
     if (p0 >= job.end || job.count == 0) return;
-    if (a.kind == kTree && p0 + 32 > job.length) find_ancestors<W::kThreads>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
-    Place at = place_in(a, job.b, min(p, job.end - 1));
-    at.page = p < job.end ? at.page : -1;
-    const int32_t row_bytes = a.D * H::kElement, used = job.count * a.fan;
-    u32x4 k[H::kSteps];
+    if (a.kind == kTree && p0 + W::kPlaces > job.length) find_ancestors<256>(nodes, a.parents + (int64_t)job.b * a.T, a.T);
+    if (a.D * H::kElement != H::kRow) {
+        clear_rest<H>(a, attention_lds, W::kBytes, threadIdx.x, 256);
+        __syncthreads();
+    }
+    const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b);
+    const uint32_t lds = lds_address(attention_lds);
+    uint64_t there[kParts];
+    Runs<H, W::kPlaces, kOfWave> keys;
+    keys.look_up(a, job.b, p0, wave * kOfWave, job.end, in_runs<H>(a));
+    if (keys.good) {
+        constexpr int kCopies = W::kBytes / 1024 / W::kWaves;
+        copy_runs<H, kCopies>(k, keys, lds, wave * kCopies);
 #pragma unroll
-    for (int s = 0; s < H::kSteps; ++s)
-        k[s] = chunk_of<kHalf>(a.k + at.page * a.k_page + at.row * a.k_row + job.group * a.k_head, (2 * s + half) * 16, row_bytes, a.k_whole, at.page >= 0);
-    float total = 0.f;
-    // (the rows of a chain that come before the first of these places do not see them)
-    const int32_t first = (a.kind == kChain ? max(0, p0 - job.length) : 0) * a.fan / 32 * 32;
-    for (int32_t r0 = first + wave * 32; r0 < used; r0 += kWaves * 32) {
-        const int32_t r = min(r0 + (lane & 31), used - 1), t = over(r, a.by_fan), head = job.group * a.fan + (r - t * a.fan);
-        const char* from = a.q + job.b * a.q_batch + t * a.q_token + head * a.q_head;
-        const float mine = a.sums[(int64_t)of * job.rows + r];
-        f32x16 score = {};
-        constexpr int kAhead = 8;  // (of 256 elements of float32 the keys alone take half of the registers)
-        u32x4 q[kAhead + 1];
-        in_steps<H::kSteps, kAhead>([&](int s) __attribute__((always_inline)) { q[s % (kAhead + 1)] = chunk_of<kHalf>(from, (2 * s + half) * 16, row_bytes, a.q_whole); },
-                                    [&](int s) __attribute__((always_inline)) { score = score_of<kHalf>(q[s % (kAhead + 1)], k[s], score); });
-        const bool plain = p0 + 32 <= job.length && r0 + 32 <= used, trees = a.kind == kTree && p0 + 32 > job.length;
+        for (int i = 0; i < kParts; ++i) there[i] = ~0ull;
+    } else {
+        constexpr int kCopies = W::kLookUp * H::kRow / 1024 / W::kWaves;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int at_row = 8 * (i >> 2) + 4 * half + (i & 3);
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i], a.scale2, -__shfl(mine, at_row)));
-            uint32_t seen = 1;
-            if (!plain) {
-                const int32_t token = __shfl(t, at_row);
-                seen = p < (a.kind == kChain ? job.length + token + 1 : job.length);
-                if (trees) {
-                    const int32_t other = max(0, min(p - job.length, job.count - 1));  // the node that lies there
-                    seen |= (nodes->sees[token][other >> 5] >> (other & 31)) & (uint32_t)(p >= job.length);
-                }
-                seen &= (uint32_t)(r0 + at_row < used) & (uint32_t)(p < job.end);
-            }
-            total += seen ? w : 0.f;
+        for (int i = 0; i < kParts; ++i) {
+            const int32_t at = i * W::kLookUp * H::kRow;
+            const Places<W::kLookUp> places(a, job.b, p0 + i * W::kLookUp, job.end);
+            copy_rows<H, W::kLookUp, kCopies>(a, k, places, lds + at, attention_lds + at, wave * kCopies);
+            there[i] = places.there;
         }
     }
-    total = sum_of_halves(total);
-    if (half == 0) sums[wave * 32 + lane] = total;
+    const int32_t used = job.count * a.fan, row_bytes = a.D * H::kElement;
+    // (the rows of a chain that come before the first of these places do not see them)
+    int32_t first = (a.kind == kChain ? max(0, p0 - job.length) : 0) * a.fan / 32 * 32 + wave * 32;
+    f32x16 total[kBlocks];
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) total[n] = f32x16{};
+    struct Rows {
+        float less;  // m + log2(l)
+        u32x4 q[H::kSteps];
+    };
+    auto load = [&](Rows& r, int32_t at) __attribute__((always_inline)) {
+        const Row row = row_of(a, job, at);
+        r.less = a.sums[(int64_t)of * job.rows + min(row.r, job.rows - 1)];
+        const char* from = a.q + job.b * a.q_batch + row.t * a.q_token + row.head * a.q_head;
+        if (a.q_whole) {
+#pragma unroll
+            for (int s = 0; s < H::kSteps; ++s) r.q[s] = chunk_of<kHalf>(from, (2 * s + half) * 16, row_bytes, true);
+        } else {
+#pragma unroll
+            for (int s = 0; s < H::kSteps; ++s) r.q[s] = chunk_of<kHalf>(from, (2 * s + half) * 16, row_bytes, false);
+        }
+    };
+    auto add = [&](const Rows& r, int32_t at) __attribute__((always_inline)) {
+        constexpr int kAtOnce = kBlocks < 2 ? 1 : 2;
+        const Row row = row_of(a, job, at);
+#pragma unroll
+        for (int n0 = 0; n0 < kBlocks; n0 += kAtOnce) {
+            f32x16 score[kAtOnce];
+            find_scores<kHalf, kSize>(attention_lds + n0 * 32 * H::kRow, r.q, score);
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n) {
+                const int32_t p = p0 + 32 * (n0 + n);
+                const uint32_t here = (uint32_t)(there[(n0 + n) / 2 % kParts] >> (32 * ((n0 + n) & 1)));
+                uint32_t seen = ~0u;
+                if (p + 32 > row.plain || at + 32 > used || here != ~0u) {
+                    seen = (seen_of(row.sight, nodes, p) & here) >> (4 * half);
+                    seen = row.r < used ? seen : 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {  // (a weight that is not seen is none, also of a row that has no number for its sum)
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][i], a.scale2, -r.less));
+                        total[n0 + n][i] += (seen >> (8 * (i >> 2) + (i & 3))) & 1 ? w : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) total[n0 + n][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][i], a.scale2, -r.less));
+                }
+            }
+        }
+    };
+    Rows now;
+    load(now, min(first, used - 1));
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x >= 32 || at.page < 0) return;
+    if constexpr (H::kRow <= 256) {
+        // the next rows on their way while these are worked on
+#pragma unroll 1
+        while (first < used) {
+            Rows next;
+            load(next, min(first + W::kWaves * 32, used - 1));
+            add(now, first);
+            first += W::kWaves * 32;
+            if (first >= used) break;
+            load(now, min(first + W::kWaves * 32, used - 1));
+            add(next, first);
+            first += W::kWaves * 32;
+        }
+    } else {
+#pragma unroll 1
+        for (; first < used; first += W::kWaves * 32) {
+            add(now, first);
+            load(now, min(first + W::kWaves * 32, used - 1));  // (longer ones have no registers for two)
+        }
+    }
+    // Lanes of a half have the same places: eight of their sixteen go to the lane 16 on and come from it, four to the one 8 on, and so on, until each has one.
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = total[n][i];
+#pragma unroll
+        for (int w = 8; w; w /= 2) {
+            const bool upper = lane & (2 * w);
+#pragma unroll
+            for (int i = 0; i < w; ++i) {
+                const float mine = upper ? v[i + w] : v[i], other = upper ? v[i] : v[i + w];
+                v[i] = mine + __shfl_xor(other, 2 * w);
+            }
+        }
+        v[0] += __shfl_xor(v[0], 1);
+        const int i = (lane >> 1) & 15;
+        if ((lane & 1) == 0) sums[wave * W::kPlaces + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3)] = v[0];
+    }
+    __syncthreads();
+    const int32_t p = p0 + (int)threadIdx.x;
+    if (threadIdx.x >= W::kPlaces || p >= job.end || place_in(a, job.b, p).page < 0) return;
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += sums[w * 32 + lane];
+    for (int w = 0; w < W::kWaves; ++w) sum += sums[w * W::kPlaces + threadIdx.x];
     float* to = a.mass + job.b * a.mass_batch + job.group * a.mass_head + p;
     *to = (p < job.length ? *to : 0.f) + sum;
 }
@@ -1247,17 +1335,29 @@ int join_of(const AttentionArgs& a, hipStream_t s) {
     attention_join_kernel<kHalf, kSize><<<(unsigned)(((int64_t)a.B * a.groups * a.T * a.fan + 3) / 4), 256, 0, s>>>(a);
     return launch_check("attention_join_kernel");
 }
+template <bool kHalf, int kSize, int kBlocks>
+int mass_rows_of(const AttentionArgs& a, int64_t groups, int64_t tiles, hipStream_t s) {
+    using W = MassRows<kHalf, kSize, kBlocks>;
+    auto kernel = attention_mass_rows_kernel<kHalf, kSize, kBlocks>;
+    CHX_PROPAGATE(ask_for_lds(reinterpret_cast<const void*>(kernel), W::kLds));
+    kernel<<<(unsigned)(groups * tiles), 256, W::kLds + nodes_bytes(a), s>>>(a, (int32_t)tiles);
+    return launch_check("attention_mass_rows_kernel");
+}
 template <bool kHalf, int kSize>
 int mass_of(const AttentionArgs& a, hipStream_t s) {
     using W = Mass<kHalf, kSize>;
-    // Runs of places: as many as give each compute unit two work-groups, of at least 128 places (a block to each wavefront).
     const int64_t groups = (int64_t)a.B * a.groups, most = ((int64_t)a.places + 127) / 128, blocks = ((int64_t)a.places + 31) / 32;
-    // us of attention with mass, by places / by rows: 2 x 883 tokens x 4 rows of 4 heads over 1 place 243 / 90, 2048 x 4 of 8 over 1 467 / 223, 512 x 4 of 8 over 2000 156 / 116, but 2 x 256 x 4 of 8 over 4000
-    // (544 work-groups by places) 150 / 163.
-    if (groups * most < 256 && (int64_t)a.T * a.fan > 128) {
-        attention_mass_rows_kernel<kHalf, kSize><<<(unsigned)(groups * blocks), MassRows<kHalf, kSize>::kThreads, MassRows<kHalf, kSize>::kLds + nodes_bytes(a), s>>>(a);
-        return launch_check("attention_mass_rows_kernel");
+    // By rows where there are many.  us by places / by rows, 128 elements of float16, 8 heads: 2 x 2048 tokens x 4 rows over 4000 places 608 / 178, 2 x 256 x 4 over 4000 79 / 33, 16 x 64 x 4 over 300
+    // 27 / 20, but 40 x 8 over 30000 (whose keys take the time) 55 / 69.
+    const int64_t rows = (int64_t)a.T * a.fan;
+    if (rows > 384 || (rows > 128 && a.places < 8192)) {
+        // Blocks by themselves where there are few work-groups of several.  us of several / one: float16, 160 work-groups of several 33 / 51, 56 of them 40 / 34; float32, 192 of them 47 / 37.
+        constexpr int kBlocks = kMassBlocks<kHalf, kSize>;
+        const int64_t wide = groups * ((blocks + kBlocks - 1) / kBlocks);
+        if (kBlocks > 1 && wide < (kHalf ? 128 : 256)) return mass_rows_of<kHalf, kSize, 1>(a, groups, blocks, s);
+        return mass_rows_of<kHalf, kSize, kBlocks>(a, groups, (blocks + kBlocks - 1) / kBlocks, s);
     }
+    // By places, in runs of them: as many as give each compute unit two work-groups, of at least 128 places (a block to each wavefront).
     int64_t runs = (512 + groups - 1) / groups;
     runs = runs > most ? most : runs;
     auto kernel = attention_mass_kernel<kHalf, kSize>;

@@ -232,7 +232,8 @@ def launches(host):
     assert names(T=24, M=500, R=64, H=16, mass=True) == ["places", "join", "mass"]
     assert names(B=8, T=2048, M=64, R=64, H=16) == ["rows"]
     assert names(B=1, T=600, M=4, R=64, H=16, mass=True)[-1] == "mass_rows"
-    assert names(B=8, T=600, M=300, R=64, H=16, mass=True)[-1] == "mass"
+    assert names(B=8, T=600, M=300, R=64, H=16, mass=True)[-1] == "mass_rows"
+    assert names(B=8, T=40, M=300, R=64, H=16, mass=True)[-1] == "mass"
     # workspaces: parts' results and statistics, and the rows' sums
     size, c = ctypes.c_size_t(), Calls(host, T=1, M=500, R=64, address=1 << 46)
     n = c.names
@@ -288,7 +289,7 @@ def reached(host):
     taken = set()
     for dtype in ("float16", "float32"):
         for D in (1, 2, 4, 64, 75, 128, 200, 256):
-            for B, T, R, M in ((1, 1, 16, 4), (2, 1, 64, 500), (8, 600, 64, 4), (8, 2048, 64, 300), (64, 24, 1024, 40)):
+            for B, T, R, M in ((1, 1, 16, 4), (2, 1, 64, 500), (8, 600, 64, 4), (1, 600, 64, 4), (8, 2048, 64, 300), (64, 24, 1024, 40)):
                 c = Calls(host, dtype, B=B, T=T, H=16, G=4, D=D, R=R, M=M, address=1 << 46)
                 for op, with_ in ((c.append, {}), (c.tree, {}), (c.tree, {"mass": c.full_mass}), (c.accept, {"mass": c.full_mass}), (c.evict, {"keep": R * M // 2})):
                     host.clear()
