@@ -1118,10 +1118,21 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
                 in_steps<H::kSteps, kAhead>([&](int s) __attribute__((always_inline)) { q[s % (kAhead + 1)] = *lds_pointer<u32x4>(at ^ (s << 5)); },
                                             [&](int s) __attribute__((always_inline)) { score = score_of<kHalf>(q[s % (kAhead + 1)], kf[s], score); });
                 const int row = rb * 32 + 4 * half;
-                // (a weight that is not seen is none, also of a row that has no number for its sum)
-                uint32_t seen = ~0u;
-                if (!plain || r0 + rb * 32 + 32 > used) {
-                    seen = 0;
+                auto add = [&](uint32_t seen, auto some) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x4 l = *reinterpret_cast<const f32x4*>(less + row + 2 * i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i + j], a.scale2, -l[j]));
+                            total += !decltype(some)::value || ((seen >> (i + j)) & 1) ? w : 0.f;
+                        }
+                    }
+                };
+                if (plain && r0 + rb * 32 + 32 <= used) {
+                    add(~0u, std::false_type());
+                } else {  // (a weight that is not seen is none, also of a row that has no number for its sum)
+                    uint32_t seen = 0;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) seen |= (uint32_t)(p < limits[row + 8 * (i >> 2) + (i & 3)]) << i;
                     if (a.kind == kTree && p0 + 32 > job.length) {
@@ -1133,15 +1144,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
                             seen |= (((nodes->sees[max(node, 0)][other >> 5] >> (other & 31)) & is & (uint32_t)(node >= 0)) << i);
                         }
                     }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const f32x4 l = *reinterpret_cast<const f32x4*>(less + row + 2 * i);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i + j], a.scale2, -l[j]));
-                        total += (seen >> (i + j)) & 1 ? w : 0.f;
-                    }
+                    add(seen, std::true_type());
                 }
             }
             total = sum_of_halves(total);
