@@ -803,7 +803,9 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
             }
             const int32_t p0 = tile * W::kPlaces;
             f32x16 score[W::kBlocksOf];
-            __builtin_amdgcn_s_setprio(1);  // (before the wavefront of the other work-group, whose softmax then goes on under these products: 571 us of 2048 x 4096 rows without, 555 with)
+            // (its products go before the softmax of the other work-group's wavefront, which goes on under them, and its first product before the other's second.  2048 x 4096 rows without such an
+            // order, with the softmax last, and with both: 571, 555 and 556 us; 2 x 2048 tokens over 4000 places, as a chain, with the softmax last and with both: 328 and 315)
+            __builtin_amdgcn_s_setprio(2);
             find_scores<kHalf, kSize>(keys, q, score);
             __builtin_amdgcn_s_setprio(0);
             if (p0 + W::kPlaces > row.plain || there != ~0ull) {
