@@ -162,7 +162,7 @@ def test_sizes(g, dtype, tree, B, H, G, D, R, T, lengths):
 
 
 @pytest.mark.parametrize("dtype", [HALF, FLOAT])
-@pytest.mark.parametrize("H,G,D,T,length", [(8, 1, 128, 1, 9000), (2, 1, 64, 3, 20011), (2, 2, 256, 1, 5000), (4, 1, 96, 40, 6001)])
+@pytest.mark.parametrize("H,G,D,T,length", [(8, 1, 128, 1, 9000), (2, 1, 64, 3, 20011), (2, 2, 256, 1, 5000), (4, 1, 96, 40, 6001), (4, 1, 64, 80, 8300), (2, 2, 256, 90, 700)])
 def test_long_caches_in_parts(g, dtype, H, G, D, T, length):
     cache = Cache(5, dtype, 2, G, D, 64, [length, length // 9], T)
     check_tree(g, cache, normal(6, (2, T, H, D), dtype, 2.0), tree_of(7, 2, T), mass=torch.zeros(2, G, cache.tables.shape[1] * 64, device="cuda"))
