@@ -181,9 +181,9 @@ def test_evict(g, dtype, R, G, D, layout, gap, keep, recent):
     p.same(want)
 
 
-@pytest.mark.parametrize("n,keep,recent", [(5000, 4990, 1000), (5000, 700, 300), (3000, 2999, 2500), (9001, 4000, 0)])
+@pytest.mark.parametrize("n,keep,recent", [(5000, 4990, 1000), (5000, 700, 300), (3000, 2999, 2500), (9001, 4000, 0), (20000, 19000, 64), (40001, 500, 100), (40001, 39000, 1)])
 def test_evict_long(g, n, keep, recent):
-    """More places than a work-group has lanes, recent ones that overlap themselves over many pieces."""
+    """More places than a work-group has lanes, than LDS has room for; recent ones that overlap themselves over many pieces."""
     p = Pages(9, HALF, 2, -(-n // 16), 16, 2, 64)
     p.mass[1, 1] = (p.mass[1, 1] * 50).floor()
     before = [x[p.tables[:].long()].flatten(1, 2)[:, :n].cpu() for x in (p.keys, p.values)]
