@@ -72,6 +72,12 @@ struct Head {
 
 __device__ const u32x4 kZeros[1] = {{0, 0, 0, 0}};  // what is not there is read from here
 
+// What lies in memory at an address that has been chosen: said to be global memory's, which the compiler no longer sees then (it would ask whether it is LDS's, and wait for both).
+template <typename T>
+__device__ __forceinline__ T load_global(const char* p) {
+    return *(const __attribute__((address_space(1))) T*)(uintptr_t)p;
+}
+
 // 16 bytes of a row of `bytes` bytes from byte `at` on (a multiple of 16), zeros behind its end and of a row that is not there.  The last ones of a row that is not whole pieces are its last 16, moved
 // down.  (Addresses and values are chosen, here and below, where a branch that lanes take by themselves would do: where registers are short, the compiler puts moves of live ones before the point at which the
 // others come back, and those lose what they held.)
@@ -79,9 +85,9 @@ template <bool kHalf>
 __device__ __forceinline__ u32x4 chunk_of(const char* row, int32_t at, int32_t bytes, bool whole, bool there = true) {
     const char* none = reinterpret_cast<const char*>(kZeros);
     const bool any = there & (at < bytes);
-    if (whole) return *reinterpret_cast<const u32x4*>(any ? row + at : none);
+    if (whole) return load_global<u32x4>(any ? row + at : none);
     if (bytes >= 16) {
-        const u32x4 v = *reinterpret_cast<const u32x4_any*>(any ? row + min(at, bytes - 16) : none);
+        const u32x4 v = load_global<u32x4_any>(any ? row + min(at, bytes - 16) : none);
         const int32_t more = max(at + 16 - bytes, 0), bits = 8 * (more & 7);  // bytes of these that the row does not have
         uint64_t lower = (uint64_t)v[1] << 32 | v[0], upper = (uint64_t)v[3] << 32 | v[2];
         lower = more & 8 ? upper : lower;
@@ -95,8 +101,8 @@ __device__ __forceinline__ u32x4 chunk_of(const char* row, int32_t at, int32_t b
     for (int j = 0; j < (kHalf ? 8 : 4); ++j) {
         const int32_t b = j * (kHalf ? 2 : 4);
         const char* from = (any & (b < bytes)) ? row + b : none;  // (at is 0, or there is none of it)
-        if constexpr (kHalf) v[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(from) << (16 * (j & 1));
-        else v[j] = *reinterpret_cast<const uint32_t*>(from);
+        if constexpr (kHalf) v[j / 2] |= (uint32_t)load_global<uint16_t>(from) << (16 * (j & 1));
+        else v[j] = load_global<uint32_t>(from);
     }
     return v;
 }
@@ -1165,7 +1171,7 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
 
 // The same of many rows: a work-group has the keys of a few blocks of places in LDS, and its wavefronts go over the rows, every fourth 32 of them, with scores as in the first pass: a lane has one row, whose
 // m + log2(l) is one number, and adds up the places' weights over its rows in registers; lanes and wavefronts are added at the end, in one order.  Bound by the exponentials, one to a score: 2 x 2048 tokens over up to 4000 places, 32 heads over 8 of 128 elements, float16,
-// 181 us (by places, whose lanes read each row's number from LDS, 608).
+// 185 us (by places, whose lanes read each row's number from LDS, 608).
 template <bool kHalf, int kSize, int kBlocks>
 struct MassRows {
     static constexpr int kWaves = 4, kPlaces = 32 * kBlocks;
@@ -1252,7 +1258,9 @@ __global__ __launch_bounds__(256, (Head<kHalf, kSize>::kRow <= 512 ? 2 : 1)) voi
 #pragma unroll
         for (int n0 = 0; n0 < kBlocks; n0 += kAtOnce) {
             f32x16 score[kAtOnce];
+            __builtin_amdgcn_s_setprio(1);
             find_scores<kHalf, kSize>(attention_lds + n0 * 32 * H::kRow, r.q, score);
+            __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int n = 0; n < kAtOnce; ++n) {
                 const int32_t p = p0 + 32 * (n0 + n);
@@ -1277,25 +1285,10 @@ __global__ __launch_bounds__(256, (Head<kHalf, kSize>::kRow <= 512 ? 2 : 1)) voi
     load(now, min(first, used - 1));
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
-    if constexpr (H::kRow <= 256) {
-        // the next rows on their way while these are worked on
 #pragma unroll 1
-        while (first < used) {
-            Rows next;
-            load(next, min(first + W::kWaves * 32, used - 1));
-            add(now, first);
-            first += W::kWaves * 32;
-            if (first >= used) break;
-            load(now, min(first + W::kWaves * 32, used - 1));
-            add(next, first);
-            first += W::kWaves * 32;
-        }
-    } else {
-#pragma unroll 1
-        for (; first < used; first += W::kWaves * 32) {
-            add(now, first);
-            load(now, min(first + W::kWaves * 32, used - 1));  // (longer ones have no registers for two)
-        }
+    for (; first < used; first += W::kWaves * 32) {
+        add(now, first);
+        load(now, min(first + W::kWaves * 32, used - 1));  // (a second set of registers, for the next rows under these, gained nothing)
     }
     // Lanes of a half have the same places: eight of their sixteen go to the lane 16 on and come from it, four to the one 8 on, and so on, until each has one.
 #pragma unroll
@@ -1360,8 +1353,8 @@ template <bool kHalf, int kSize>
 int mass_of(const AttentionArgs& a, hipStream_t s) {
     using W = Mass<kHalf, kSize>;
     const int64_t groups = (int64_t)a.B * a.groups, most = ((int64_t)a.places + 127) / 128, blocks = ((int64_t)a.places + 31) / 32;
-    // By rows where there are many.  us by places / by rows, 128 elements of float16, 8 heads: 2 x 2048 tokens x 4 rows over 4000 places 608 / 178, 2 x 256 x 4 over 4000 79 / 33, 16 x 64 x 4 over 300
-    // 27 / 20, but 40 x 8 over 30000 (whose keys take the time) 55 / 69.
+    // By rows where there are many.  us by places / by rows, 128 elements of float16, 8 heads: 2 x 2048 tokens x 4 rows over 4000 places 608 / 185, 2 x 256 x 4 over 4000 79 / 29, 16 x 64 x 4 over 300
+    // 27 / 18, but 40 x 8 over 30000 (whose keys take the time) 55 / 69.
     const int64_t rows = (int64_t)a.T * a.fan;
     if (rows > 384 || (rows > 128 && a.places < 8192)) {
         // Blocks by themselves where there are few work-groups of several.  us of several / one: float16, 160 work-groups of several 33 / 51, 56 of them 40 / 34; float32, 192 of them 47 / 37.
@@ -1395,3 +1388,4 @@ int AttentionKernels<kHalf>::mass(const AttentionArgs& a, int size, hipStream_t 
 }
 
 }  // namespace chx
+
