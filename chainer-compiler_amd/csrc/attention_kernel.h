@@ -459,11 +459,12 @@ __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, u
     const char* from;
     asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0" : "=&s"(from) : "v"(offset), "s"(base), "s"(uniform(lds)) : "memory", "m0");
 }
-// (Of some lanes only; all of them are there.)
+// (Of some lanes only.)
 __device__ __forceinline__ void copy_to_lds(uint32_t offset, const char* base, uint32_t lds, uint64_t lanes) {
     const char* from;
-    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dwordx4 %1, %0\n\ts_mov_b64 exec, -1"
-                 : "=&s"(from) : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0");
+    uint64_t all;
+    asm volatile("s_mov_b32 m0, %4\n\ts_mov_b64 %0, %3\n\ts_and_saveexec_b64 %1, %5\n\tglobal_load_lds_dwordx4 %2, %0\n\ts_mov_b64 exec, %1"
+                 : "=&s"(from), "=&s"(all) : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void copy_to_lds(const char* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
@@ -471,8 +472,9 @@ __device__ __forceinline__ void copy_to_lds(const char* from, uint32_t lds) {
 // (4 bytes a lane, lane i's to lds + 4 i.)
 __device__ __forceinline__ void copy_number_to_lds(uint32_t offset, const char* base, uint32_t lds, uint64_t lanes) {
     const char* from;
-    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dword %1, %0\n\ts_mov_b64 exec, -1"
-                 : "=&s"(from) : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0");
+    uint64_t all;
+    asm volatile("s_mov_b32 m0, %4\n\ts_mov_b64 %0, %3\n\ts_and_saveexec_b64 %1, %5\n\tglobal_load_lds_dword %2, %0\n\ts_mov_b64 exec, %1"
+                 : "=&s"(from), "=&s"(all) : "v"(offset), "s"(base), "s"(uniform(lds)), "s"(lanes) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void copy_number_to_lds(const float* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(uniform(lds)) : "memory", "m0");
