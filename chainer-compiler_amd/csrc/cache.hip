@@ -231,20 +231,23 @@ struct Keys {
     const float* mass;
     u32x4* keys;
     int32_t n;
-    __device__ __forceinline__ void load() {
-        if constexpr (kInLds) {
-            constexpr int kAtOnce = 8;
-            uint32_t* to = reinterpret_cast<uint32_t*>(keys);
-            const int32_t all = (n + 3) / 4 * 4;
-            for (int32_t i0 = threadIdx.x; i0 < all; i0 += 1024 * kAtOnce) {
-                float v[kAtOnce];
+    // Calls f(key, whether it is one) for all of them, of all lanes of a wavefront at once.
+    template <typename F>
+    __device__ __forceinline__ void load(F f) {
+        constexpr int kAtOnce = 8;
+        uint32_t* to = reinterpret_cast<uint32_t*>(keys);
+        const int32_t all = (n + 3) / 4 * 4, lane = threadIdx.x & 63;
+        for (int32_t i0 = threadIdx.x; i0 - lane < all; i0 += 1024 * kAtOnce) {
+            float v[kAtOnce];
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) v[j] = i0 + j * 1024 < n ? mass[i0 + j * 1024] : 0.f;
+            for (int j = 0; j < kAtOnce; ++j) v[j] = i0 + j * 1024 < n ? mass[i0 + j * 1024] : 0.f;
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j)
-                    if (i0 + j * 1024 < all) to[i0 + j * 1024] = i0 + j * 1024 < n ? sortable(v[j]) : 0;
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int32_t i = i0 + j * 1024;
+                const uint32_t key = i < n ? sortable(v[j]) : 0;
+                if (i < all) to[i] = key;
+                f(key, i < n);
             }
-            __syncthreads();
         }
     }
     __device__ __forceinline__ u32x4 at(int32_t quad) const {
@@ -266,8 +269,8 @@ __device__ __forceinline__ int32_t before_wave(const int32_t* of_waves, int wave
 }
 
 // A head's places that stay: the threshold of the `best` largest of n weights by three histograms of 11, 11 and 10 bits, of equal ones the lower places; then the
-// list of moves, places that go in front of best and places that stay behind it, both in ascending order.  One work-group to a head; bound by its instructions where sequences are long (32,768 places: six passes
-// over LDS), by its barriers where they are short.  128 heads of 2080 places, 2048 to stay: 9.6 us; 32 of 32768, 8192 to stay: 24.
+// list of moves, places that go in front of best and places that stay behind it, both in ascending order.  One work-group to a head; bound by its instructions where sequences are long (32,768 places: four passes
+// over LDS, and one that fills it), by its barriers where they are short.  128 heads of 2080 places, 2048 to stay: 9.5 us; 32 of 32768, 8192 to stay: 22.
 template <bool kInLds>
 __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
     extern __shared__ u32x4 choose_lds[];
@@ -291,29 +294,29 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
     }
     Keys<kInLds> keys = {a.mass + b * a.mass_batch + h * a.mass_head, choose_lds, n};
     for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
-    keys.load();
     __syncthreads();
+    auto count = [&](uint32_t bin, bool counts) __attribute__((always_inline)) {
+        const uint64_t all = __builtin_amdgcn_ballot_w64(counts);
+        if (all == 0) return;
+        // (equal weights, as of places that nobody has looked at, would queue for one bin)
+        const uint32_t its = __builtin_amdgcn_readlane(bin, __builtin_ctzll(all));
+        if (__builtin_amdgcn_ballot_w64(counts && bin == its) == all) {
+            if (lane == 0) atomicAdd(&bins[its], __popcll(all));
+        } else if (counts) {
+            atomicAdd(&bins[bin], 1);
+        }
+    };
+    if constexpr (kInLds) keys.load([&](uint32_t key, bool counts) __attribute__((always_inline)) { count(key >> 21, counts); });  // (with the first histogram)
     uint32_t least = 0;      // upper bits of the threshold
     int32_t wanted = best;   // how many with those bits
     bool tie = false;        // whether some that equal the threshold go
     for (int digit = 0; digit < 3; ++digit) {
         const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
         const uint32_t above = digit == 0 ? 0 : ~0u << (shift + bits);
-        for (int32_t i = threadIdx.x; i - lane < quads; i += 1024) {
+        for (int32_t i = threadIdx.x; i - lane < quads && !(kInLds && digit == 0); i += 1024) {
             const u32x4 key = i < quads ? keys.at(i) : u32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool counts = i < quads && ((key[j] ^ least) & above) == 0;
-                const uint64_t all = __builtin_amdgcn_ballot_w64(counts);
-                if (all == 0) continue;
-                // (equal weights, as of places that nobody has looked at, would queue for one bin)
-                const uint32_t bin = (key[j] >> shift) & ((1u << bits) - 1), its = __builtin_amdgcn_readlane(bin, __builtin_ctzll(all));
-                if (__builtin_amdgcn_ballot_w64(counts && bin == its) == all) {
-                    if (lane == 0) atomicAdd(&bins[its], __popcll(all));
-                } else if (counts) {
-                    atomicAdd(&bins[bin], 1);
-                }
-            }
+            for (int j = 0; j < 4; ++j) count((key[j] >> shift) & ((1u << bits) - 1), 4 * i + j < n && ((key[j] ^ least) & above) == 0);
         }
         __syncthreads();
         // the bin in which the wanted one is, from above: a lane has two bins, which it clears for the next digit
@@ -385,6 +388,7 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
     int32_t holes = 0, movers = 0;
     for (int32_t i = from + lane; i - lane < to; i += 64) {
         const Four f = four_at(i);
+        if (kInLds && i < to) keys.keys[i][0] = f.holes << 4 | f.movers;  // (the lane's own, and no longer a key)
         holes += __popc(f.holes);
         movers += __popc(f.movers);
     }
@@ -399,7 +403,13 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
     movers = before_wave(of_waves[2], wave);
     rank = equal;
     for (int32_t i = from + lane; i - lane < to; i += 64) {
-        const Four f = four_at(i);
+        Four f;
+        if constexpr (kInLds) {
+            const uint32_t both = i < to ? keys.keys[i][0] : 0;
+            f = {both >> 4, both & 15};
+        } else {
+            f = four_at(i);
+        }
         if (__builtin_amdgcn_ballot_w64((f.holes | f.movers) != 0) == 0) continue;
         int32_t hole_at = holes, mover_at = movers;
 #pragma unroll
