@@ -510,6 +510,23 @@ def test_cross_strides(g, dtype):
     check_cross(g, together[:, :T, 0, :1], one.expand(B, S, 1, D), one.expand(B, S, 1, D))
 
 
+def test_states_of_more_than_2_gib(g):
+    """One sequence whose rows are further apart than 31 bits hold."""
+    S = 1_100_000
+    gen = torch.Generator(device="cuda").manual_seed(82)
+    k, v = (torch.zeros(1, S, 8, 128, dtype=HALF, device="cuda")[:, :, 7:] for _ in range(2))
+    for x in (k, v):
+        x.copy_(torch.randn(x.shape, generator=gen, device="cuda").half())
+    q = normal(83, (1, 2, 1, 128), HALF, 2.0)
+    got = g.ops.CrossAttention(q, k, v)
+    s = (q[0, :, 0].double() @ k[0, :, 0].double().T) * 128 ** -0.5
+    w, values = torch.softmax(s, 1), v[0, :, 0].double()
+    size = (q[0, :, 0].double().abs() @ k[0, :, 0].double().abs().T).amax(1, keepdim=True) * 128 ** -0.5
+    want = w @ values
+    room = (w @ values.abs()) * (2 * (2.0 ** -23 * 136 * size + 2.0 ** -22) + 2.0 ** -11 + 2.0 ** -24 * (S + 64)) + want.abs() * 2.0 ** -11 + w.amax(1, keepdim=True) * values.abs().sum(0) * 2.0 ** -31 + 2.0 ** -25
+    close(got[0, :, 0], want.cpu(), room.cpu())
+
+
 def test_nothing_to_attend_to(g):
     q = normal(78, (2, 3, 4, 64), HALF)
     none = torch.empty(2, 0, 4, 64, dtype=HALF, device="cuda")
