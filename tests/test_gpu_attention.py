@@ -378,6 +378,24 @@ def test_recorded_and_on_two_streams(g, dtype):
     assert all(torch.equal(one, want[i]) for i in range(2) for one in got[i])
 
 
+@pytest.mark.parametrize("dtype,D,T", [(HALF, 128, 200), (HALF, 256, 3), (FLOAT, 256, 2), (FLOAT, 128, 150)])
+def test_recorded_before_any_other_call(g, dtype, D, T):
+    """What a kernel needs, as more LDS than every one has, is asked for in a recording too; heads beside, so that many rows and few are met."""
+    cache = Cache(36, dtype, 2, 2, D, 16, [70, 400], T)
+    q, mass = normal(37, (2, T, 8, D), dtype, 2.0), torch.zeros(2, 2, cache.tables.shape[1] * 16, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths, mass=mass)
+    for _ in range(3):
+        mass.zero_()
+        q.copy_(q.flip(1))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept, again = mass.clone(), torch.zeros_like(mass)
+        assert torch.equal(got, check_tree(g, cache, q, mass=again)) and torch.equal(kept, again)
+
+
 def test_a_pool_of_more_than_4_gib(g):
     """Pages far apart: offsets that 32 bits do not hold."""
     P, R, G, D = 9000, 256, 8, 128  # 4.7 GB of keys
@@ -431,6 +449,25 @@ def test_places_that_are_not_seen_weigh_nothing(g):
     assert (mass[0, 0, 16:32] == 3).all() and (mass[0, 0, 190:] == 3).all()
     total = (mass[0, 0, :190].sum() - 3.0 * 40).item()  # each of 300 rows weighs 1, off by 2^-11 of a weight
     assert abs(total - 300.0) < 300 * 2.0 ** -10
+
+
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("T", [1, 7, 60, 200])
+def test_padding_holds_anything(g, dtype, T):
+    """Queries of tokens that a sequence does not have, and keys and values in its drafted places behind them, NaN: nobody else sees them."""
+    counts = [0, T // 2, T]
+    cache = Cache(92, dtype, 3, 2, 64, 16, [50, 333, 0], T)
+    q = normal(93, (3, T, 8, 64), dtype, 2.0)
+    for b, count in enumerate(counts):
+        q[b, count:] = math.nan
+        n = len(cache.rows[b][0]) - T
+        for p in range(n + count, n + T):
+            at = (int(cache.tables[b, p // 16]), p % 16)
+            cache.keys[at], cache.values[at] = math.nan, math.inf
+        for rows in cache.rows[b]:
+            rows[n + count:] = 0.0
+    for tree in (None, tree_of(94, 3, T)):
+        check_tree(g, cache, q, tree, numbers(counts), mass=torch.ones(3, 2, cache.tables.shape[1] * 16, device="cuda"))
 
 
 def test_threads(g):
