@@ -993,7 +993,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 #pragma unroll
     for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
     const float weight = stat[1] != 0.f ? __builtin_amdgcn_exp2f(stat[0] - m) : 0.f;
-    float l = weight == 0.f ? 0.f : stat[1] * weight;
+    // (A part whose sum is no number has a score that is none, which its maximum does not show: the row has no result, whatever that part would weigh.)
+    float l = weight == 0.f && stat[1] == stat[1] ? 0.f : stat[1] * weight;
 #pragma unroll
     for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
     float sum[kOf] = {};

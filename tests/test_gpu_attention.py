@@ -508,6 +508,34 @@ def test_short_rows_in_a_pool_of_more_than_4_gib(g, dtype, D, P):
     close(mass[0, :, :600], weights, weights_room + 2.0 ** -24 * weights)
 
 
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("length,M,far", [(1024, 128, False), (20, 2, False), (3000, 200, True), (40, 3, True)])
+def test_scores_that_are_no_number_wherever_they_lie(g, dtype, length, M, far):
+    """A token with a score that is NaN has NaN, whether its place shares a part of the cache with others (few places), is alone in one (the token's own, the first of its part), or lies in one
+    whose other scores weigh nothing."""
+    cache = Cache(100, dtype, 1, 8, 64, 16, [length], 1)
+    more = torch.full((1, M - cache.tables.shape[1]), int(cache.tables[0, 0]), dtype=torch.int32, device="cuda")
+    cache.tables = torch.cat([cache.tables, more], 1)
+    q = normal(101, (1, 1, 32, 64), dtype)
+    if far:  # one score that is 2^9 above all others, in the first part
+        q[..., 0] = 8.0
+        for p in range(length + 1):
+            cache.keys[int(cache.tables[0, p // 16]), p % 16, :, 0] = 64.0 if p == 3 else 0.0
+        for rows in cache.rows:
+            rows[0][:, :, 0] = 0.0
+            rows[0][3, :, 0] = 64.0
+    mass = torch.zeros(1, 8, M * 16, device="cuda")
+    clean = check_tree(g, cache, q, scale=1.0, mass=mass)
+    cache.keys[int(cache.tables[0, length // 16]), length % 16, 2:4, 7] = math.nan
+    mass.zero_()
+    got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths, scale=1.0, mass=mass)
+    touched = torch.zeros(32, dtype=torch.bool)
+    touched[8:16] = True
+    assert torch.isnan(got[0, 0, touched]).all() and torch.isnan(mass[0, 2:4, : length + 1]).all()
+    assert torch.equal(got[0, 0, ~touched], clean[0, 0, ~touched]) and torch.isfinite(mass[0, [0, 1, 4, 5, 6, 7]]).all()
+    assert (mass[0, :, length + 1:] == 0).all()
+
+
 # ---- an encoder's states ----------------------------------------------------------------------------
 
 def check_cross(g, q, k, v, lengths=None, scale=None, out=None):
