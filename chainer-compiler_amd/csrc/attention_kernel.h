@@ -243,6 +243,13 @@ __device__ __forceinline__ float sum_of(float m, float l) {
     return l == 0.f ? INFINITY : m - kRaise<kHalf> + log2f(l);
 }
 
+// Rounding to float16 of a weighted mean.  What is finite stays so: the weights were rounded to float16 before the products and their sum was not, so that a mean of 65504 and the like may come out up to
+// 2^-11 of it higher, which is infinity from 2^-12 on.
+__device__ __forceinline__ _Float16 to_half(float v) {
+    const float within = __builtin_amdgcn_fmed3f(v, -65504.f, 65504.f);
+    return (_Float16)(fabsf(v) <= FLT_MAX ? within : v);
+}
+
 // Elements of a result next to each other.
 template <int kCount, typename V>
 __device__ __forceinline__ void store(const AttentionArgs& a, char* row, int32_t element, V v) {
@@ -648,7 +655,7 @@ __device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)
 #pragma unroll
     for (int n = 0; n < H::kBlocks; ++n) acc[n] *= share;
     H::in_vectors(acc, half, [&](int element, typename H::Vector v) __attribute__((always_inline)) {
-        if constexpr (kHalf) store<4>(a, y, element, half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]});
+        if constexpr (kHalf) store<4>(a, y, element, half4{to_half(v[0]), to_half(v[1]), to_half(v[2]), to_half(v[3])});
         else store<H::kVector>(a, y, element, v);
     });
 }
@@ -971,7 +978,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
         sum *= stats[r];
         const int32_t all = job.row_tile * 32 + r, t = over(all, a.by_fan), head = job.group * a.fan + (all - t * a.fan);
         char* y = a.y + job.b * a.y_batch + t * a.y_token + head * a.y_head;
-        if constexpr (kHalf) store<4>(a, y, e, half4{(_Float16)sum[0], (_Float16)sum[1], (_Float16)sum[2], (_Float16)sum[3]});
+        if constexpr (kHalf) store<4>(a, y, e, half4{to_half(sum[0]), to_half(sum[1]), to_half(sum[2]), to_half(sum[3])});
         else store<4>(a, y, e, sum);
     }
 }
@@ -1020,7 +1027,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 #pragma unroll
     for (int j = 0; j < kOf; ++j) {
         if (lane * kOf + j >= a.D) break;
-        if constexpr (kHalf) reinterpret_cast<_Float16*>(y)[lane * kOf + j] = (_Float16)(sum[j] * share);
+        if constexpr (kHalf) reinterpret_cast<_Float16*>(y)[lane * kOf + j] = to_half(sum[j] * share);
         else reinterpret_cast<float*>(y)[lane * kOf + j] = sum[j] * share;
     }
 }

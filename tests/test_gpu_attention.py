@@ -536,6 +536,30 @@ def test_scores_that_are_no_number_wherever_they_lie(g, dtype, length, M, far):
     assert (mass[0, :, length + 1:] == 0).all()
 
 
+@pytest.mark.parametrize("T", [1, 300])
+def test_float16_values_next_to_the_largest(g, T):
+    """A mean of values that all are float16's largest is that one.  Weights are rounded before they are multiplied, the sum that divides is not: here nearly all of it is one weight between 2^13 and 2^14,
+    whose rounding is up to 2^-11 of it, and half of that is enough for a result that rounds to infinity."""
+    cache = Cache(115, HALF, 1, 1, 64, 16, [200], T)
+    cache.keys.fill_(0.0)
+    cache.keys[..., 0] = -60.0
+    at = [(int(cache.tables[0, p // 16]), p % 16) for p in (0, 128)]
+    cache.keys[at[0]][0, 0], cache.keys[at[1]][0, 0] = 0.0, 1.0
+    cache.values[..., :32], cache.values[..., 32:] = 65504.0, -65504.0
+    k, v = cache.rows[0]
+    k.zero_()
+    k[..., 0] = -60.0
+    k[0, 0, 0], k[128, 0, 0] = 0.0, 1.0
+    v[..., :32], v[..., 32:] = 65504.0, -65504.0
+    q = torch.zeros(1, T, 64, 64, dtype=HALF, device="cuda")
+    q[..., 0] = 4.859375 + torch.arange(64, device="cuda") / 256
+    check_tree(g, cache, q, scale=1.0)
+    cache.values[at[0]][0, 3] = math.inf
+    got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths, scale=1.0)
+    others = torch.arange(64) != 3
+    assert (got[..., 3] == math.inf).all() and torch.isfinite(got[..., others]).all()
+
+
 # ---- an encoder's states ----------------------------------------------------------------------------
 
 def check_cross(g, q, k, v, lengths=None, scale=None, out=None):
