@@ -31,7 +31,7 @@ struct AttentionArgs {
     bool q_whole, k_whole, y_whole;  // whole 16-byte pieces at addresses that are multiples of 16 (y: 8)
     // Rows r = t * fan + g of a group's heads are next to each other; a work-group takes a tile of them and one part of the places.
     int32_t row_tiles, tile_rows, parts;
-    float* part_sums;  // [B][groups][row_tiles][parts][tile_rows][size of the kernel], not yet divided
+    float* part_sums;  // [B][groups][row_tiles][parts][tile_rows][size of the kernel]: a part's own mean
     float* part_stats;  // [..][parts][tile_rows][2]: m, l: the weights' sum is l 2^m
     float* sums;  // [B][groups][T fan]: m + log2(l), where `mass` is asked for
     float* mass;

@@ -345,16 +345,23 @@ __device__ __forceinline__ void find_weights(float scale2, f32x16 (&score)[kCoun
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// What is added up in place of v, all of it in LDS: itself, or (where results are made again) ones for what is inf, -inf and NaN, or what is finite.
+// How often what is finite is halved where results are made again, in float32: weights are up to 2^kLag, there are fewer than 2^(32 - clz) places, and the sums of all of them are then below float32's
+// largest number whatever the values are.  (float16's values and weights are below 2^16 and 2^14, and 2^30 places of those no problem.)
+template <bool kHalf>
+__device__ __forceinline__ int halvings(const AttentionArgs& a) {
+    return kHalf ? 0 : (int)kLag + 32 - __builtin_clz(a.places | 1);
+}
+
+// What is added up in place of v, all of it in LDS: itself, or (where results are made again) ones for what is inf, -inf and NaN, or what is finite, times `less`.
 enum { kAll, kInfinities, kNegativeInfinities, kNans, kFinite };
 template <bool kHalf>
-__device__ __forceinline__ void replace_values(char* values, int32_t bytes, int32_t special, int32_t thread, int32_t threads) {
+__device__ __forceinline__ void replace_values(char* values, int32_t bytes, int32_t special, float less, int32_t thread, int32_t threads) {
     using E = std::conditional_t<kHalf, _Float16, float>;
 #pragma unroll 1
     for (int32_t i = thread; i < bytes / (int32_t)sizeof(E); i += threads) {
         const float v = (float)reinterpret_cast<const E*>(values)[i];
         const bool finite = v - v == 0.f, marked = special == kNans ? v != v : v == (special == kInfinities ? INFINITY : -INFINITY);
-        reinterpret_cast<E*>(values)[i] = (E)(special == kFinite ? (finite ? v : 0.f) : marked ? 1.f : 0.f);
+        reinterpret_cast<E*>(values)[i] = (E)(special == kFinite ? (finite ? v * less : 0.f) : marked ? 1.f : 0.f);
     }
 }
 
@@ -425,16 +432,17 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&acc)[kBlocks]) {
     return zero != 0.f;
 }
 
-// The sums of a row, added up again where one of them is not finite: then v is not, or it is the product of 0 and something infinite, and places of no weight add nothing, whatever they hold.
-// `pass` goes over the places once, with what stands for v.  `any`: of all that make the passes together.
+// The sums of a row, added up again where one of them is not finite: then v is not, or it is the product of 0 and something infinite, and places of no weight add nothing, whatever they hold; or the
+// sum is more than float32 holds, which the mean is not.  `pass` goes over the places once, with what stands for v.  `any`: of all that make the passes together.  Returns what the sums are to be
+// multiplied by (after the division by the weights' sum): 1, or a power of 2 where they were made of smaller values.
 template <int kBlocks, typename Pass, typename Any>
-__device__ __forceinline__ void add_up(f32x16 (&acc)[kBlocks], Pass pass, Any any) {
+__device__ __forceinline__ float add_up(f32x16 (&acc)[kBlocks], int halved, Pass pass, Any any) {
     uint32_t marks[3][kBlocks / 2];  // a bit for each sum: whether it has an inf, -inf, NaN
 #pragma unroll 1
     for (int32_t special = kAll; special <= kFinite; ++special) {
         pass(special);
         if (special == kAll) {
-            if (!any(not_finite(acc))) return;
+            if (!any(not_finite(acc))) return 1.f;
         } else if (special < kFinite) {
 #pragma unroll
             for (int n = 0; n < kBlocks; n += 2) {
@@ -456,6 +464,7 @@ __device__ __forceinline__ void add_up(f32x16 (&acc)[kBlocks], Pass pass, Any an
             v -= (marks[1][n / 2] >> bit) & 1 ? INFINITY : 0.f;
             acc[n][i] = (marks[2][n / 2] >> bit) & 1 ? NAN : v;
         }
+    return ldexpf(1.f, halved);
 }
 
 // ---- rows of k and v into LDS ---------------------------------------------------------------------------------------
@@ -633,13 +642,16 @@ __device__ __forceinline__ void clear_rest(const AttentionArgs& a, char* lds, in
 
 // ---- results ----------------------------------------------------------------------------------------------------------
 
-// A row's results, or what there is of them: 16 elements of it in blocks of 32 to a lane.
+// A row's results, or its mean over one part: 16 elements of it in blocks of 32 to a lane.
 template <bool kHalf, int kSize>
-__device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)[kSize / 32], float m, float l, int32_t b, int32_t group, int32_t r, int64_t part_row, bool any) {
+__device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)[kSize / 32], float more, float m, float l, int32_t b, int32_t group, int32_t r, int64_t part_row, bool any) {
     using H = Head<kHalf, kSize>;
     const int half = (threadIdx.x & 63) >> 5;
     const int32_t rows = a.T * a.fan;
     l = sum_of_halves(l);
+    const float share = l == 0.f ? 0.f : more / l;
+#pragma unroll
+    for (int n = 0; n < H::kBlocks; ++n) acc[n] *= share;
     if (a.parts > 1) {
         if (half == 0) *reinterpret_cast<f32x2*>(a.part_stats + 2 * part_row) = f32x2{m, l};
         if (!any || r >= rows) return;
@@ -649,11 +661,8 @@ __device__ __forceinline__ void finish_row(const AttentionArgs& a, f32x16 (&acc)
     }
     if (r >= rows) return;
     if (a.sums != nullptr && half == 0) a.sums[((int64_t)b * a.groups + group) * rows + r] = sum_of<kHalf>(m, l);
-    const float share = l == 0.f ? 0.f : 1.f / l;
     const int32_t t = over(r, a.by_fan), head = group * a.fan + (r - t * a.fan);
     char* y = a.y + b * a.y_batch + t * a.y_token + head * a.y_head;
-#pragma unroll
-    for (int n = 0; n < H::kBlocks; ++n) acc[n] *= share;
     H::in_vectors(acc, half, [&](int element, typename H::Vector v) __attribute__((always_inline)) {
         if constexpr (kHalf) store<4>(a, y, element, half4{to_half(v[0]), to_half(v[1]), to_half(v[2]), to_half(v[3])});
         else store<H::kVector>(a, y, element, v);
@@ -817,7 +826,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
             if (special == kAll && idle) continue;
             char* keys = attention_lds + (tile & 1) * 2 * W::kBytes;
             if (special != kAll) {
-                replace_values<kHalf>(keys + W::kBytes, W::kBytes, special, threadIdx.x, 256);
+                replace_values<kHalf>(keys + W::kBytes, W::kBytes, special, ldexpf(1.f, -halvings<kHalf>(a)), threadIdx.x, 256);
                 __syncthreads();
             }
             const int32_t p0 = tile * W::kPlaces;
@@ -839,8 +848,8 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
         }
         __syncthreads();
     };
-    add_up(acc, pass, [](bool mine) { return __syncthreads_or(mine) != 0; });
-    finish_row<kHalf, kSize>(a, acc, m, l, job.b, job.group, row.r, job.at * W::kRows + wave * 32 + (lane & 31), job.begin_tile < job.end_tile);
+    const float more = add_up(acc, halvings<kHalf>(a), pass, [](bool mine) { return __syncthreads_or(mine) != 0; });
+    finish_row<kHalf, kSize>(a, acc, more, m, l, job.b, job.group, row.r, job.at * W::kRows + wave * 32 + (lane & 31), job.begin_tile < job.end_tile);
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------
@@ -925,7 +934,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
             find_weights<kHalf>(a.scale2, score, m, l);
             if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(W::kCopies) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            if (special != kAll) replace_values<kHalf>(values, W::kBytes, special, lane, 64);
+            if (special != kAll) replace_values<kHalf>(values, W::kBytes, special, ldexpf(1.f, -halvings<kHalf>(a)), lane, 64);
             add_values<kHalf, kSize>(values, score, acc);
             if (more) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -933,9 +942,9 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
             }
         }
     };
-    add_up(acc, pass, [](bool mine) { return __builtin_amdgcn_ballot_w64(mine) != 0; });
+    const float more = add_up(acc, halvings<kHalf>(a), pass, [](bool mine) { return __builtin_amdgcn_ballot_w64(mine) != 0; });
 
-    // The wavefronts' sums, relative to the largest of their maxima; of those with an infinite one, what weighs nothing adds nothing.
+    // The wavefronts' sums, relative to the largest of their maxima and divided by the sum of all weights; of those with an infinite one, what weighs nothing adds nothing.
     l = sum_of_halves(l);
     if (half == 0) {
         stats[wave * 64 + lane] = m;
@@ -947,23 +956,19 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     for (int w = 0; w < kWaves; ++w) most = fmaxf(most, stats[w * 64 + (lane & 31)]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) total += stats[w * 64 + 32 + (lane & 31)] * __builtin_amdgcn_exp2f(stats[w * 64 + (lane & 31)] - most);
-    const float f = __builtin_amdgcn_exp2f(m - most);
+    const float f = __builtin_amdgcn_exp2f(m - most), share = total == 0.f ? 0.f : more / total;
     constexpr int kPitch = kSize + 4;
     float* sums = reinterpret_cast<float*>(attention_lds);
 #pragma unroll
     for (int n = 0; n < H::kBlocks; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[n][i] = f == 0.f || l == 0.f ? 0.f : acc[n][i] * f;
+        for (int i = 0; i < 16; ++i) acc[n][i] = f == 0.f || l == 0.f ? 0.f : acc[n][i] * f * share;
     H::in_vectors(acc, half, [&](int element, typename H::Vector v) __attribute__((always_inline)) { *reinterpret_cast<typename H::Vector*>(sums + (wave * 32 + (lane & 31)) * kPitch + element) = v; });
     __syncthreads();
     const int64_t part_row = job.at * 32;
     if (a.parts > 1 && threadIdx.x < 32) *reinterpret_cast<f32x2*>(a.part_stats + 2 * (part_row + lane)) = f32x2{most, total};
     if (a.parts > 1 && job.begin_tile >= job.end_tile) return;
-    if (a.parts == 1 && threadIdx.x < 32) {
-        if (a.sums != nullptr && row.r < job.rows) a.sums[((int64_t)job.b * a.groups + job.group) * job.rows + row.r] = sum_of<kHalf>(most, total);
-        stats[lane] = total == 0.f ? 0.f : 1.f / total;  // (of wave 0, which has read its own)
-    }
-    if (a.parts == 1) __syncthreads();
+    if (a.parts == 1 && a.sums != nullptr && threadIdx.x < 32 && row.r < job.rows) a.sums[((int64_t)job.b * a.groups + job.group) * job.rows + row.r] = sum_of<kHalf>(most, total);
     const int32_t rows = min(32, job.rows - job.row_tile * 32);
 #pragma unroll 2
     for (int i = threadIdx.x; i < rows * (kSize / 4); i += 64 * kWaves) {
@@ -975,7 +980,6 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
             *reinterpret_cast<f32x4*>(a.part_sums + (part_row + r) * kSize + e) = sum;
             continue;
         }
-        sum *= stats[r];
         const int32_t all = job.row_tile * 32 + r, t = over(all, a.by_fan), head = job.group * a.fan + (all - t * a.fan);
         char* y = a.y + job.b * a.y_batch + t * a.y_token + head * a.y_head;
         if constexpr (kHalf) store<4>(a, y, e, half4{to_half(sum[0]), to_half(sum[1]), to_half(sum[2]), to_half(sum[3])});
@@ -983,7 +987,7 @@ __global__ __launch_bounds__((64 * Few<kHalf, kSize>::kWaves), (Few<kHalf, kSize
     }
 }
 
-// A row's parts, by a wavefront (8 parts of 256 rows 4 us, 16 of those of 4 x 24 tokens and 32 heads 7.4): y = sum_i l_i 2^(m_i - m) (sums_i / l_i) over its sum of l_i 2^(m_i - m), in the order of the parts.
+// A row's parts, by a wavefront (8 parts of 256 rows 4 us, 16 of those of 4 x 24 tokens and 32 heads 7.4): y = sum_i w_i y_i with w_i = l_i 2^(m_i - m) over the sum of those and y_i the part's own mean, in the order of the parts.
 template <bool kHalf, int kSize>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     constexpr int kOf = kSize / 64;  // elements of a lane, next to each other
@@ -1004,6 +1008,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     float l = weight == 0.f && stat[1] == stat[1] ? 0.f : stat[1] * weight;
 #pragma unroll
     for (int d = 32; d; d /= 2) l += __shfl_xor(l, d);
+    const float part = weight == 0.f || l == 0.f ? 0.f : stat[1] * weight / l;
     float sum[kOf] = {};
     typedef float Of __attribute__((ext_vector_type(kOf)));
     // (eight parts' loads under way at once; a part without weight may hold anything)
@@ -1016,19 +1021,18 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
         for (int i = 0; i < kAtOnce; ++i) v[i] = *reinterpret_cast<const Of*>(from + min(p + i, a.parts - 1) * next);
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
-            const float w = p + i < a.parts ? __shfl(weight, (p + i) & 63) : 0.f;
+            const float w = p + i < a.parts ? __shfl(part, (p + i) & 63) : 0.f;
 #pragma unroll
             for (int j = 0; j < kOf; ++j) sum[j] = w == 0.f ? sum[j] : __builtin_fmaf(w, v[i][j], sum[j]);
         }
     }
     if (a.sums != nullptr && lane == 0) a.sums[row] = sum_of<kHalf>(m, l);
-    const float share = l == 0.f ? 0.f : 1.f / l;
     char* y = a.y + b * a.y_batch + t * a.y_token + head * a.y_head;
 #pragma unroll
     for (int j = 0; j < kOf; ++j) {
         if (lane * kOf + j >= a.D) break;
-        if constexpr (kHalf) reinterpret_cast<_Float16*>(y)[lane * kOf + j] = to_half(sum[j] * share);
-        else reinterpret_cast<float*>(y)[lane * kOf + j] = sum[j] * share;
+        if constexpr (kHalf) reinterpret_cast<_Float16*>(y)[lane * kOf + j] = to_half(sum[j]);
+        else reinterpret_cast<float*>(y)[lane * kOf + j] = sum[j];
     }
 }
 

@@ -547,7 +547,9 @@ int chx_hip_cache_append(
  *   scale   above 0
  *   mass    NULL, or gets the weights of each place, over all tokens and the heads that share its own: added for places below lengths[b], set for the tokens' own
  * Products are of the operands as they are, sums float32; float16 weights are rounded to float16 before they are multiplied with values (2^-11 of each, as much as the result's own
- * rounding is).  A place whose weight rounds to 0 adds nothing, whatever it holds; a token that sees nothing, or has no score above -inf, has a result of 0.
+ * rounding is).  A place whose weight rounds to 0 adds nothing, whatever it holds; a token that sees nothing, or has no score above -inf, has a result of 0; one with a score that is NaN or inf has NaN.
+ * (Scores go as powers of 2: from 2e38 on, of either sign, they count as infinite.)  Values may be as large as their type holds: a sum of weights and float32 values that float32 does not hold, which
+ * the mean is not, is made again of values halved up to 8 + log2(2 M R) times, where those that fall below 2^-126 lose bits, next to such sums.
  * workspace: aligned to 16. */
 int chx_hip_tree_attention_workspace(const chx_hip_tensor* q, const chx_hip_tensor* keys, const chx_hip_tensor* tables, int32_t with_mass, size_t* bytes);
 int chx_hip_tree_attention(

@@ -536,6 +536,33 @@ def test_scores_that_are_no_number_wherever_they_lie(g, dtype, length, M, far):
     assert (mass[0, :, length + 1:] == 0).all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 200])
+@pytest.mark.parametrize("T,length", [(1, 300), (40, 5000), (300, 77), (1, 20000)])
+def test_float32_values_next_to_the_largest(g, D, T, length):
+    """Means of values up to 3e38 of either sign are what they are: sums before the division would be above float32's largest.  In the same calls small values in other elements, and an infinite one."""
+    cache = Cache(110, FLOAT, 1, 2, D, 16, [length], T)
+    gen = torch.Generator().manual_seed(111)
+    big = (torch.rand(length + T, 2, D, generator=gen) * 2 - 1) * 3e38
+    big[:, 0, : D // 2] = big[:, 0, : D // 2].abs() * 0.5 + 1.5e38  # (all of one sign: the mean is as large)
+    big[:, 1, 5:9] = torch.randn(length + T, 4, generator=gen)
+    place = torch.arange(length + T, device="cuda")
+    cache.values[cache.tables[0].long()[place // 16], place % 16] = big.cuda()
+    cache.rows[0] = (cache.rows[0][0], big)
+    q = normal(112, (1, T, 4, D), FLOAT, 0.5)
+    q[0, T // 2] = 0.0  # (all places weigh the same)
+    mass = torch.zeros(1, 2, cache.tables.shape[1] * 16, device="cuda")
+    clean = check_tree(g, cache, q, mass=mass)
+    at = (int(cache.tables[0, 0]), 4)
+    cache.values[at][1, 3], cache.values[at][1, 6] = math.inf, -math.inf
+    got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths)
+    assert (got[0, :, 2:, 3] == math.inf).all() and (got[0, :, 2:, 6] == -math.inf).all()
+    others = torch.ones(4, D, dtype=torch.bool)
+    others[2:, 3] = others[2:, 6] = False
+    assert torch.isfinite(got[0][:, others]).all()
+    # (made once with the sums as they are and once smaller: two roundings apart at most, in products of sums and weights)
+    assert torch.allclose(got[0][:, others].double(), clean[0][:, others].double(), rtol=2.0 ** -20, atol=2.0 ** -100)
+
+
 @pytest.mark.parametrize("T", [1, 300])
 def test_float16_values_next_to_the_largest(g, T):
     """A mean of values that all are float16's largest is that one.  Weights are rounded before they are multiplied, the sum that divides is not: here nearly all of it is one weight between 2^13 and 2^14,
