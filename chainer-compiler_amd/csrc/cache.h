@@ -49,7 +49,8 @@ int check_numbers(const chx_hip_tensor* t, int ndim, int64_t n0, int64_t n1, con
 // float32 [B, heads, places or more] with elements next to each other along the last axis.
 int check_mass(const chx_hip_tensor* mass, const CacheArgs& c, const char* what);
 
-// Refuses a result or an updated array that meets another array (a null one, or one without elements, meets none).
+// Refuses a result or an updated array that meets another array (a null one, or one without elements, meets none): one whose first to last byte meet its own, unless both have the same shape and
+// strides and lie between each other's rows.
 struct Named {
     const chx_hip_tensor* t;
     const char* name;

@@ -524,7 +524,7 @@ int chx_hip_token_logprobs(
 
 /* A cache of keys and values in pages.  Of what follows:
  *   keys, values  [pages, R, G, D]: pages of R places, G heads of D elements (1 to 256), float16 or float32, of one type and shape; any strides, elements of the last axis
- *                 next to each other
+ *                 next to each other; both may be of one allocation, as [pages, 2, R, G, D]
  *   tables        int32 [B, M]: the pages of sequence b, in order; place p of it is row p % R of page tables[b, p / R].  Rows may lie apart, M R below 2^30.  A number that is no page's
  *                 stands for places that are not there: nothing is written to them, and nobody sees them
  *   lengths       int32 [B]: how many places of a sequence hold rows (numbers outside 0 to M R count as the nearer of them)

@@ -11,7 +11,7 @@ def host_so(tmp_path_factory):
     return host_hip.build(tmp_path_factory.mktemp("host_hip"))
 
 
-@pytest.mark.parametrize("case", ["caches", "append", "tree", "cross", "accept", "evict", "empty", "launches", "large", "reached"])
+@pytest.mark.parametrize("case", ["caches", "append", "tree", "cross", "accept", "evict", "empty", "launches", "large", "reached", "interleaved"])
 def test_case(host_so, case):
     host_hip.run_case(host_so, __file__, case)
 
@@ -296,6 +296,46 @@ def reached(host):
                     host.check(op(**with_))
                     taken.update(line.split(" grid=")[0] for line in host.launches())
     assert len(names) > 30 and names <= taken, sorted(names - taken)
+
+
+def interleaved(host):
+    """Keys and values of one allocation: taken where no byte is of both, refused where one is, whatever the order of the axes and the gaps between them."""
+    import itertools
+    import random
+    T, rng = host.tensor, random.Random(1)
+    found = {True: 0, False: 0}
+    for _ in range(600):
+        shape = [rng.choice([1, 2, 3]) for _ in range(3)] + [rng.choice([1, 2, 8])]
+        order, strides, inside = rng.sample(range(3), 3) + [3], [0] * 4, 1
+        for axis in reversed(order):
+            strides[axis] = inside if axis == 3 else inside + rng.choice([0, 0, 1, 5, inside, 3 * inside])
+            inside = strides[axis] * shape[axis]
+        offset = rng.choice([0, rng.randrange(2 * inside + 2), rng.choice(strides) // 2, shape[3]])
+        calls = Calls(host, P=shape[0], R=shape[1], G=shape[2], D=shape[3])
+        keys = T("float16", shape, strides, base=1 << 50)
+        values = shifted(keys, rng.choice([2, 2, 2, 1]) * offset * rng.choice([1, -1]))
+        used = [{t.data + sum(i * s for i, s in zip(index, t.strides)) + byte for index in itertools.product(*map(range, shape)) for byte in (0, 1)} for t in (keys, values)]
+        meet = bool(used[0] & used[1])
+        host.clear()
+        if values.data % 2:
+            refused(host, calls.append(keys=keys, values=values), "whole elements")
+            continue
+        found[meet] += 1
+        for op in (calls.append, calls.accept, calls.evict):
+            host.clear()
+            if meet:
+                refused(host, op(keys=keys, values=values), "keys and values overlap")
+            else:
+                host.check(op(keys=keys, values=values))
+    assert min(found.values()) > 100, found
+    # a result between the rows of q is taken as well, one over them is not
+    c = Calls(host)
+    host.clear()
+    both = T("float16", (2, 3, 2, 4, 64))
+    q = T("float16", (2, 3, 4, 64), [3 * 2 * 256, 2 * 256, 64, 1], base=both.data)
+    host.check(c.tree(q=q, y=shifted(q, 512)))
+    host.clear()
+    refused(host, c.tree(q=q, y=shifted(q, 510)), "y and q overlap")
 
 
 if __name__ == "__main__":

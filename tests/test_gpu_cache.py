@@ -241,6 +241,34 @@ def test_recorded(g):
         assert got[1].tolist() == [103, 92] and got[2].tolist() == [95, 92]
 
 
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("shape,axis", [((20, 2, 16, 3, 64), 1), ((20, 16, 2, 3, 64), 2), ((20, 16, 3, 2, 75), 3), ((20, 3, 16, 2, 128), 3), ((2, 20, 16, 3, 64), 0)])
+def test_keys_and_values_in_one_allocation(g, dtype, shape, axis):
+    """Pages that hold both: the same as of two pools, number for number, and nothing else is touched."""
+    gen = torch.Generator().manual_seed(13)
+    heads_first = shape == (20, 3, 16, 2, 128)
+    pool = torch.randn(shape, generator=gen).to(dtype).cuda()
+    one = [x.transpose(1, 2) if heads_first else x for x in pool.unbind(axis)]
+    two = [x.clone() for x in one]
+    P, R, G, D = one[0].shape
+    tables = torch.randperm(P, generator=gen)[:16].reshape(2, 8).to(torch.int32).cuda()
+    lengths, T = numbers([50, 100]), 7
+    q, k, v = (torch.randn(2, T, n, D, generator=gen).to(dtype).cuda() for n in (2 * G, G, G))
+    accepted = numbers([[0, 2, 4, 6], [1, 3, -1, 0]])
+    results = []
+    for keys, values in (one, two):
+        mass = torch.zeros(2, G, 8 * R, device="cuda")
+        g.ops.CacheAppend(keys, values, k, v, tables, lengths)
+        y = g.ops.TreeAttention(q, keys, values, tables, lengths, mass=mass)
+        longer = g.ops.CacheAccept(keys, values, tables, lengths, accepted, mass=mass)
+        shorter = g.ops.CacheEvict(keys, values, tables, longer, mass, 60, 12)
+        results.append([y, longer, shorter, mass, keys, values])
+    assert results[0][1].tolist() == [54, 102] and results[0][2].tolist() == [54, 60]
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    with pytest.raises(g.capi.ChxHipError, match="keys and values overlap"):
+        g.ops.CacheAppend(one[0], one[0], k, v, tables, lengths)
+
+
 def test_a_conversation(g):
     """The operators together: a prompt in pieces, drafted trees of which some is accepted, a cache that is cut again and again; against dense caches in 64 bits, one for each
     sequence and head.  float32, so that the choice of what stays is the same (weights further apart than their errors)."""
