@@ -735,6 +735,7 @@ __device__ __forceinline__ void load_rows(const AttentionArgs& a, const Job& j, 
         for (int c = half; c < H::kChunks; c += 2) mine[c] = chunk_of<kHalf>(at, c * 16, row_bytes, false);
 #pragma unroll
         for (int s = 0; s < H::kSteps; ++s) q[s] = mine[2 * s + half];  // (what this lane has written itself)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (before the copies that come there: they write LDS past the order of its own instructions)
     }
 }
 // They are waited for here, behind the first copies: a first use inside a loop would wait for everything that is under way, in every round of it.

@@ -587,6 +587,21 @@ def test_float16_values_next_to_the_largest(g, T):
     assert (got[..., 3] == math.inf).all() and torch.isfinite(got[..., others]).all()
 
 
+@pytest.mark.parametrize("dtype,gap", [(HALF, 1), (HALF, 3), (FLOAT, 1)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T", [1, 8, 200])
+def test_queries_at_any_alignment(g, dtype, gap, D, T):
+    """Rows that fill a kernel's size and are not at multiples of 16 bytes: the same results, number for number, as of those that are."""
+    cache = Cache(120, dtype, 2, 2, D, 16, [90, 700], T)
+    q = normal(121, (2, T, 4, D), dtype, 2.0)
+    space = torch.full((2, T, 4, D + gap), math.nan, dtype=dtype, device="cuda")
+    apart = space[..., gap:]
+    apart.copy_(q)
+    want = check_tree(g, cache, q)
+    for _ in range(4):
+        assert torch.equal(want, g.ops.TreeAttention(apart, cache.keys, cache.values, cache.tables, cache.lengths))
+
+
 # ---- an encoder's states ----------------------------------------------------------------------------
 
 def check_cross(g, q, k, v, lengths=None, scale=None, out=None):
