@@ -602,6 +602,26 @@ def test_queries_at_any_alignment(g, dtype, gap, D, T):
         assert torch.equal(want, g.ops.TreeAttention(apart, cache.keys, cache.values, cache.tables, cache.lengths))
 
 
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("D", [64, 75, 129, 256])
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_values_that_are_not_finite_at_every_size(g, dtype, D, T):
+    """Sums that are made again, in each kernel: infinite values and NaN are in their own elements alone, the others are what they are without them."""
+    cache = Cache(130, dtype, 2, 2, D, 16, [90, 700], T)
+    q = normal(131, (2, T, 4, D), dtype)
+    clean = check_tree(g, cache, q)
+    for b in range(2):
+        at = [(int(cache.tables[b, p // 16]), p % 16) for p in (10, 60)]
+        cache.values[at[0]][1, 1], cache.values[at[0]][1, 2], cache.values[at[0]][1, D - 1] = math.inf, -math.inf, math.inf
+        cache.values[at[1]][1, 2], cache.values[at[1]][1, 3] = math.inf, math.nan
+    for _ in range(2):
+        got = g.ops.TreeAttention(q, cache.keys, cache.values, cache.tables, cache.lengths)
+        assert (got[:, :, 2:, 1] == math.inf).all() and (got[:, :, 2:, D - 1] == math.inf).all() and torch.isnan(got[:, :, 2:, 2:4]).all()
+        others = torch.ones(4, D, dtype=torch.bool)
+        others[2:, 1:4] = others[2:, D - 1] = False
+        assert torch.equal(got[:, :, others], clean[:, :, others])
+
+
 # ---- an encoder's states ----------------------------------------------------------------------------
 
 def check_cross(g, q, k, v, lengths=None, scale=None, out=None):
