@@ -1183,8 +1183,9 @@ __global__ __launch_bounds__((Mass<kHalf, kSize>::kThreads)) void attention_mass
 }
 
 // The same of many rows: a work-group has the keys of a few blocks of places in LDS, and its wavefronts go over the rows, every fourth 32 of them, with scores as in the first pass: a lane has one row, whose
-// m + log2(l) is one number, and adds up the places' weights over its rows in registers; lanes and wavefronts are added at the end, in one order.  Bound by the exponentials, one to a score: 2 x 2048 tokens over up to 4000 places, 32 heads over 8 of 128 elements, float16,
-// 185 us (by places, whose lanes read each row's number from LDS, 608).
+// m + log2(l) is one number, and adds up the places' weights over its rows in registers; lanes and wavefronts are added at the end, in one order.  2 x 2048 tokens over up to 4000 places, 32 heads over 8 of 128 elements, float16,
+// 188 us (by places, whose lanes read each row's number from LDS, 608).  Bound by vector and matrix instructions, which take turns: by counters (a launch of 206 us) the vector units are busy for 51 % of the time (5.4 instructions to a
+// score; its exponential alone 16 %) and the matrix units for 32 %, with up to two wavefronts to a SIMD, which wait 19 % of their time, for the next rows of q among others.  float32, 2 x 512 tokens: 295 us, matrix units busy for 60 %.
 template <bool kHalf, int kSize, int kBlocks>
 struct MassRows {
     static constexpr int kWaves = 4, kPlaces = 32 * kBlocks;

@@ -302,7 +302,8 @@ __device__ __forceinline__ int32_t before_wave(const int32_t* of_waves, int wave
 
 // A head's places that stay: the threshold of the `best` largest of n weights by three histograms of 11, 11 and 10 bits, of equal ones the lower places; then the
 // list of moves, places that go in front of best and places that stay behind it, both in ascending order.  One work-group to a head; bound by its instructions where sequences are long (32,768 places: four passes
-// over LDS, and one that fills it), by its barriers where they are short.  128 heads of 2080 places, 2048 to stay: 9.5 us; 32 of 32768, 8192 to stay: 22.
+// over LDS, and one that fills it), by its barriers where they are short.  128 heads of 2080 places, 2048 to stay: 9.5 us; 32 of 32768, 8192 to stay, 28 (22 where nearly none move).  Tables that LDS has no room for: a weight at a time from memory, in each pass; 65536 places,
+// 1 head 95 us, 32 heads 103.
 template <bool kInLds>
 __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
     extern __shared__ u32x4 choose_lds[];
@@ -463,7 +464,8 @@ __global__ __launch_bounds__(1024) void cache_choose_kernel(MoveArgs a) {
 
 // The moves of a head's list, then the latest places behind them, `recent` of them from length - recent to keep - recent: those may overlap themselves, so they go in
 // ascending pieces, each read before it is written.  blockIdx as for cache_accept_kernel.  Bound by the look-ups and rows that wait for each other: 16 sequences of 8 heads of 128 elements, float16, cut from
-// 2080 to 2048 places, 256 recent: 11 us (37 MB); 4 from 32768 to 8192, 1024 recent: 14.5 (39 MB).
+// 2080 to 2048 places, 256 recent: 11 us (37 MB); 4 from 32768 to 8192, 1024 recent: 100 (220 MB, 2.2 TB/s: 160 work-groups, each with a slice's whole list behind each other), and 14.5 (39 MB) where most of
+// what has weight lies in front already, as after an earlier cut.
 template <typename Unit, int kThreads>
 __global__ __launch_bounds__(kThreads) void cache_evict_kernel(MoveArgs a) {
     constexpr int kAtOnce = 4;

@@ -545,7 +545,8 @@ int chx_hip_cache_append(
  *   q, y    [B, T, H, D], H a multiple of G, any strides; y overlaps nothing
  *   counts  int32 [B]: how many tokens a sequence has (numbers outside 0 to T as the nearer); NULL: T.  The others' results are 0
  *   scale   above 0
- *   mass    NULL, or gets the weights of each place, over all tokens and the heads that share its own: added for places below lengths[b], set for the tokens' own
+ *   mass    NULL, or gets the weights of each place, over all tokens and the heads that share its own: added for places below lengths[b], set for the tokens' own (drafted tokens that
+ *           are not accepted later have added theirs too; a call without mass leaves the numbers of its tokens' places as they were)
  * Products are of the operands as they are, sums float32; float16 weights are rounded to float16 before they are multiplied with values (2^-11 of each, as much as the result's own
  * rounding is).  A place whose weight rounds to 0 adds nothing, whatever it holds; a token that sees nothing, or has no score above -inf, has a result of 0; one with a score that is NaN or inf has NaN.
  * (Scores go as powers of 2: from 2e38 on, of either sign, they count as infinite.)  Values may be as large as their type holds: a sum of weights and float32 values that float32 does not hold, which
