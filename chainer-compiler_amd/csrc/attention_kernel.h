@@ -606,7 +606,10 @@ struct Runs {
 template <typename H, int kCount, typename R>
 __device__ __forceinline__ void copy_runs(const From& f, const R& runs, uint32_t lds, int32_t first) {
     constexpr int kRows = 64 / H::kChunks;
-    const int lane = threadIdx.x & 63;
+    int32_t lane = threadIdx.x & 63;
+    // (Where a row is one copy and a wavefront has many, what differs from one to the next is made where it is used.  Made ahead it is 16 registers, and the kernel for few rows of 256 elements, which has none
+    // left, kept 21 in memory: a token of 8 sequences of up to 4000 places, 32 heads over 8, 226 us, so 177.)
+    if constexpr (H::kRow > 512 && kCount > 8) asm volatile("" : "+v"(lane));
     auto all = [&](auto simple) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kCount; ++j) {

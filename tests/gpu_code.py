@@ -6,7 +6,8 @@ import subprocess
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIBRARY = os.path.join(ROOT, "chainer-compiler_amd", "lib", "libchx_hip.so")
-OBJDUMP = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "llvm-objdump")
+TOOLS = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin")
+OBJDUMP, READELF = os.path.join(TOOLS, "llvm-objdump"), os.path.join(TOOLS, "llvm-readelf")
 
 
 def code_objects():
@@ -22,6 +23,33 @@ def code_objects():
                 yield data[at + offset: at + offset + size]
             p += 24 + length
         at = data.find(b"__CLANG_OFFLOAD_BUNDLE__", at + 24)
+
+
+def files(containing, tmp_path):
+    """Files with the code objects that hold a symbol with this in its name."""
+    for i, data in enumerate(code_objects()):
+        if containing.encode() in data:
+            path = os.path.join(str(tmp_path), "%d.elf" % i)
+            with open(path, "wb") as f:
+                f.write(data)
+            yield path
+
+
+def resources(containing, tmp_path):
+    """{symbol of a kernel: {what its metadata says of it}} of the code objects that hold a symbol with this in its name."""
+    found = {}
+    for path in files(containing, tmp_path):
+        of = {}
+        for line in subprocess.run([READELF, "--notes", path], capture_output=True, text=True, check=True).stdout.splitlines():
+            m = re.match(r"^  (- |  )\.(\w+):\s*(\S*)", line)  # (arguments stand further in)
+            if not m:
+                continue
+            if m.group(1) == "- ":
+                of = {}
+            of[m.group(2)] = int(m.group(3)) if m.group(3).isdigit() else m.group(3)
+            if m.group(2) == "name":
+                found[m.group(3)] = of
+    return found
 
 
 class Function:
@@ -43,12 +71,7 @@ class Function:
 def functions(containing, tmp_path):
     """{symbol: Function} of the code objects that hold a symbol with this in its name."""
     found = {}
-    for i, data in enumerate(code_objects()):
-        if containing.encode() not in data:
-            continue
-        path = os.path.join(str(tmp_path), "%d.elf" % i)
-        with open(path, "wb") as f:
-            f.write(data)
+    for path in files(containing, tmp_path):
         function = None
         for line in subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", path], capture_output=True, text=True, check=True).stdout.splitlines():
             start = re.match(r"^[0-9a-f]+ <(.+)>:", line)

@@ -1,4 +1,4 @@
-"""Waits of the attention kernels, in the code that was built: what a missing one does, no run shows reliably."""
+"""Waits and registers of the attention kernels, in the code that was built: what a missing wait or a lost register does, no run shows reliably."""
 import re
 
 import pytest
@@ -47,3 +47,11 @@ def test_a_missing_wait_is_found(kernels):
     f.code = [("s_nop", "0") if op == "s_waitcnt" and "lgkmcnt(0)" in operands else (op, operands) for op, operands in kept]
     assert copies_before_reads(f)
     f.code = kept
+
+
+def test_no_kernel_keeps_registers_in_memory(tmp_path):
+    """Where registers run out the compiler moves live ones about, also inside branches that only some lanes take, where the other lanes lose theirs; so none of these kernels is over the limit."""
+    found = {name: of for name, of in gpu_code.resources("attention_places_kernel", tmp_path).items() if "attention_" in name}
+    assert len(found) > 20, sorted(found)
+    for name, of in found.items():
+        assert of["vgpr_spill_count"] == 0 and of["private_segment_fixed_size"] == 0 and of["vgpr_count"] <= 512, (name, of["vgpr_spill_count"], of["private_segment_fixed_size"])
