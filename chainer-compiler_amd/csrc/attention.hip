@@ -33,7 +33,7 @@ namespace {
 //   float32, 64 elements,   8 of 4000          103   61    37    31    38    36    42    43
 //            128 elements,  8 of 4000          171   98    60    63    67    71    81    88
 //                           2 of 20000         786   405   214   116   89    72    85    73    89
-//            192 elements, 5 of 60215, 4 heads       7189  3620  1830  1239  1172  1034  925   809
+//            192 elements, 5 of 60215, 4 heads       5770  2913  1476  998   946   832   747   659
 // One part, and no launch that joins them, where parts would be short: float16 below 1024 places, and below 2048 where whole sequences nearly fill the units.  us of 1 part / 2 / 4, 64 elements, the 252 to
 // states that all sequences have, the others of sequences from a sixteenth of this length to the whole:
 //                                              577 places      1500            4000
