@@ -11,9 +11,13 @@ def host_so(tmp_path_factory):
     return host_hip.build(tmp_path_factory.mktemp("host_hip"))
 
 
-@pytest.mark.parametrize("case", ["caches", "append", "tree", "cross", "accept", "evict", "empty", "launches", "large", "reached", "interleaved"])
+@pytest.mark.parametrize("case", ["caches", "append", "tree", "cross", "accept", "evict", "empty", "launches", "large", "reached"])
 def test_case(host_so, case):
     host_hip.run_case(host_so, __file__, case)
+
+
+def test_arrays_between_each_others_rows(host_so):
+    host_hip.run_case(host_so, __file__, "interleaved")
 
 
 def ref(t):
